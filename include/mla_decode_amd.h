@@ -40,6 +40,7 @@ extern "C" {
 /* dtypes of q / kv / out */
 #define MLA_DTYPE_BF16 0
 #define MLA_DTYPE_F16 1
+#define MLA_DTYPE_F32 2 /* mla_apply_rope only */
 
 /* status codes */
 #define MLA_OK 0
@@ -63,6 +64,7 @@ extern "C" {
 /* KV cache formats (mla_decode_args.kv_format, mla_kv_append_args.kv_format). */
 #define MLA_KV_NATIVE 0   /* latent and rope in the query dtype */
 #define MLA_KV_FP8_E4M3 1 /* latent as OCP e4m3 codes with power-of-two scales (below) */
+#define MLA_KV_FP4_E2M1 4 /* latent as OCP e2m1 codes with a scale byte per 32 dims (below) */
 
 /*
  * Decode arguments.  Strides are in elements.  The latent ("nope", dims
@@ -95,6 +97,14 @@ extern "C" {
  * e4m3(code_d) * scale_{d/128}; every scale must be a power of two (2^-126 .. 2^127), as
  * mla_kv_append writes them: the device applies it as an exponent.  The rope and the
  * queries are bf16.  With MLA_KV_NATIVE, kv_scale is unused and may be NULL.
+ *
+ * kv_format == MLA_KV_FP4_E2M1 (paged or sparse, dtype bf16): kv_nope points to bytes of two OCP e2m1
+ * codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; the even dim in the low half), 256 a token;
+ * kv_scale points to bytes, 16 a token, byte j the scale of dims 32j .. 32j+31 of token row r of page p:
+ *   (uint8_t*)kv_scale + p*kv_scale_stride_page + r*kv_scale_stride_blk + j
+ * (all strides of codes and scales in bytes, multiples of 16, the scale's token stride below 2^24, both
+ * pointers 16-byte aligned).  Latent value d is e2m1(code_d) * 2^(byte - 127), byte 1 .. 254; byte 255
+ * makes the block NaN.  Rope and queries as with fp8.
  */
 typedef struct mla_decode_args {
   int32_t batch;
@@ -130,7 +140,7 @@ typedef struct mla_decode_args {
   void* workspace;
   int64_t workspace_bytes;
 
-  int32_t kv_format;   /* MLA_KV_NATIVE or MLA_KV_FP8_E4M3 */
+  int32_t kv_format;   /* MLA_KV_NATIVE, MLA_KV_FP8_E4M3 or MLA_KV_FP4_E2M1 */
   int32_t kv_reserved; /* must be 0 */
   const float* kv_scale;
   int64_t kv_scale_stride_page, kv_scale_stride_blk;
@@ -169,6 +179,13 @@ const char* mla_last_error(void);
  * Replaces the num_sm_parts rule described in docs/num_split_design.md:53-71.
  */
 int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count);
+
+/*
+ * mla_num_parts for a cache of format kv_format: the 4-bit decode is laid out for two workgroups of 16, 32 or
+ * 64 query rows per compute unit, the other formats as mla_num_parts says.  Any schedule is decoded right;
+ * this one fills the GPU.
+ */
+int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format);
 
 /*
  * Kernel tile chosen for `rows` = s_q * heads_q query rows (dense bf16/fp16 cache): waves per
@@ -347,7 +364,10 @@ typedef struct mla_kv_append_args {
    * codes, kv_scale = power-of-two scales, kv_rope bf16); kv_new stays bf16 and each new
    * token's latent block j is stored as e4m3(x / 2^k) with 2^k the smallest power of two
    * such that max|x| over the block <= 448 * 2^k (k clamped to [-126, 127]; a zero block
-   * gets k = 0), rounded to nearest even. */
+   * gets k = 0), rounded to nearest even.  MLA_KV_FP4_E2M1: the fp4 format, kv_new bf16; the 32-dim block
+   * j is stored as e2m1(x / 2^k), 2^k the smallest power of two with max|x| <= 6 * 2^k (k >= -126; a
+   * zero block gets k = 0), rounded to nearest even, scale byte k + 127; a block that holds a NaN or an
+   * infinity gets byte 255 and codes 0. */
   int32_t kv_format;
   int32_t kv_reserved; /* must be 0 */
   float* kv_scale;
@@ -355,6 +375,115 @@ typedef struct mla_kv_append_args {
 } mla_kv_append_args;
 
 int mla_kv_append(const mla_kv_append_args* args, void* stream);
+
+/* ---- a serving step around the decode (no counterpart in the reference) ------------------- */
+
+/* A paged cache: formats, halves and strides as in mla_decode_args (codes' strides in bytes; scale strides
+ * in floats with MLA_KV_FP8_E4M3, in bytes with MLA_KV_FP4_E2M1, where `blk` is the token's).  A slot
+ * names a cached token: page * 64 + row, the ids the sparse decode takes. */
+typedef struct mla_kv_cache {
+  int32_t format;
+  int32_t dtype; /* of the tokens: bf16, or fp16 with MLA_KV_NATIVE */
+  int32_t num_blocks;
+  int32_t reserved; /* must be 0 */
+  void* nope;
+  void* rope;
+  void* scale;
+  int64_t stride_page, stride_tok;
+  int64_t rope_stride_page, rope_stride_tok;
+  int64_t scale_stride_page, scale_stride_blk;
+} mla_kv_cache;
+
+/*
+ * Rotary positions: pair i of the `dim` rotated dims of a head at position p is multiplied, as a complex
+ * number, by amp * exp(2 pi i p freqs[i]); freqs [dim / 2] (double, on the device) in turns per position.
+ * MLA_ROPE_INTERLEAVED: pair i is dims 2i, 2i + 1; MLA_ROPE_HALF: dims i, i + dim / 2.  The angle is formed
+ * and reduced in 64 bits, the product in 32, rounded once.  A negative position leaves its row unrotated.
+ */
+#define MLA_ROPE_INTERLEAVED 0
+#define MLA_ROPE_HALF 1
+typedef struct mla_rope {
+  const double* freqs;
+  int32_t dim; /* even, 2 .. 1024 */
+  int32_t layout;
+  float amp;
+  int32_t reserved;
+} mla_rope;
+
+/* x [tokens, heads, dim] -> out, dims [first, first + rope.dim) rotated and the others copied (left alone
+ * where out == x; otherwise the two may not overlap).  Strides in elements, a head's dims contiguous;
+ * heads * dim below 2^22. */
+typedef struct mla_rope_args {
+  const void* x;
+  void* out;
+  int64_t x_stride_t, x_stride_h, o_stride_t, o_stride_h;
+  const int32_t* positions; /* [tokens] */
+  int32_t tokens, heads, dim, first;
+  int32_t dtype; /* MLA_DTYPE_BF16, _F16 or _F32 */
+  int32_t reserved; /* must be 0 */
+} mla_rope_args;
+int mla_apply_rope(const mla_rope* rope, const mla_rope_args* args, void* stream);
+
+/*
+ * Append by slot map: row t of kv_new [tokens, 576] goes to cache row slots[t], its rope dims rotated by
+ * positions[t] (rope NULL: as they are), its latent stored as mla_kv_append does in the cache's format.  With
+ * q_pe [tokens, heads, 64], the queries' rope parts, each is rotated into q_rope (the rope dims of the
+ * decode's query buffer; may be q_pe itself) in the same launch.  A slot outside [0, 64 * num_blocks) names
+ * no row: nothing is written for that token, neither to the cache nor to q_rope.  No two rows may have
+ * the same slot.  Strides in elements, multiples of 8; pointers 16-byte aligned.
+ */
+typedef struct mla_append_slots_args {
+  const void* kv_new;
+  int64_t new_stride;
+  const int32_t* slots;     /* [tokens] */
+  const int32_t* positions; /* [tokens]; may be NULL without a rope */
+  const void* q_pe;         /* may be NULL */
+  void* q_rope;
+  int64_t pe_stride_t, pe_stride_h, q_stride_t, q_stride_h;
+  int32_t tokens, heads;
+} mla_append_slots_args;
+int mla_kv_append_slots(const mla_kv_cache* cache, const mla_rope* rope, const mla_append_slots_args* args, void* stream);
+
+/* Cached tokens as rows: out[t, 0..575] (the cache's dtype) = the token at slots[t], dequantised; a slot
+ * outside [0, 64 * num_blocks) gives a row of zeros.  out_stride in elements. */
+int mla_kv_gather(const mla_kv_cache* cache, const int32_t* slots, int32_t tokens, void* out, int64_t out_stride,
+                  void* stream);
+
+/*
+ * Pages, block tables and slot maps of a step, on the device.  The pool is a stack of page ids,
+ * free_pages[0 .. count) free, taken from the top.  Nothing here may run at the same time as another call
+ * on the same pool, table or lengths.
+ */
+typedef struct mla_page_pool {
+  int32_t* free_pages; /* [num_blocks] */
+  int32_t* count;      /* [1] */
+  int32_t num_blocks;
+  int32_t batch; /* 1 .. 16384 */
+  int32_t* block_table;
+  int32_t block_table_stride;
+  int32_t block_table_width;
+  int32_t* cache_seqlens; /* [batch] */
+} mla_page_pool;
+
+/*
+ * Room for new_lens[b] more tokens of every sequence b (a negative count is none).  cu_new [batch + 1]: exclusive
+ * prefix sums of the counts asked for: sequence b's new tokens are rows cu_new[b] .. of the step's packed
+ * rows.  Requests are served in order: granted[b] = 0, and nothing changes for b, if its length is negative,
+ * its table row or the `tokens` rows are too short, the page its new rows start in is no page of the pool, or
+ * the pool holds fewer pages than the requests up to b need (one that needs no page is granted even then).
+ * Otherwise granted[b] = 1, its new pages are in block_table and cache_seqlens[b] has advanced.
+ * slots [tokens], positions [tokens]: cache row and position of every row; -1 for rows not granted and rows
+ * behind the last sequence.  scratch [batch + 1] int32.
+ */
+int mla_reserve_pages(const mla_page_pool* pool, const int32_t* new_lens, int32_t tokens, int32_t* slots, int32_t* positions,
+                      int32_t* cu_new, int32_t* granted, int32_t* scratch, void* stream);
+
+/*
+ * Shortens every sequence to keep_lens[b] tokens (0: it is done; a longer or equal keep changes nothing) and
+ * returns the pages it no longer needs, so that releasing what mla_reserve_pages took restores the stack.
+ * block_table keeps its stale entries.
+ */
+int mla_release_pages(const mla_page_pool* pool, const int32_t* keep_lens, void* stream);
 
 #ifdef __cplusplus
 }

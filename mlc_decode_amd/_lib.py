@@ -18,6 +18,10 @@ MLA_SCHED_WORDS = 8
 MLA_DEFAULT_SPLIT_OVERHEAD = 3  # pages; the default schedule's per-split overhead
 MLA_KV_NATIVE = 0
 MLA_KV_FP8_E4M3 = 1
+MLA_KV_FP4_E2M1 = 4
+MLA_DTYPE_F32 = 2  # mla_apply_rope only
+MLA_ROPE_INTERLEAVED = 0
+MLA_ROPE_HALF = 1
 MLA_SPARSE_MAX_TOPK = 2048
 MLA_NOALLOC_SCRATCH_BYTES = 160 << 20  # the allocation-free decode's static scratch per GPU
 MLA_DIM_QK = 576
@@ -42,6 +46,12 @@ EXPORTED = (
     "mla_launch",
     "mla_kv_append",
     "mla_combine_absorb",
+    "mla_num_parts_for",
+    "mla_apply_rope",
+    "mla_kv_append_slots",
+    "mla_kv_gather",
+    "mla_reserve_pages",
+    "mla_release_pages",
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -133,6 +143,86 @@ class MlaKvAppendArgs(ctypes.Structure):
     ]
 
 
+class MlaKvCache(ctypes.Structure):
+    """Layout of ``mla_kv_cache`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("format", _i32),
+        ("dtype", _i32),
+        ("num_blocks", _i32),
+        ("reserved", _i32),
+        ("nope", _vp),
+        ("rope", _vp),
+        ("scale", _vp),
+        ("stride_page", _i64),
+        ("stride_tok", _i64),
+        ("rope_stride_page", _i64),
+        ("rope_stride_tok", _i64),
+        ("scale_stride_page", _i64),
+        ("scale_stride_blk", _i64),
+    ]
+
+
+class MlaRope(ctypes.Structure):
+    """Layout of ``mla_rope`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [("freqs", _vp), ("dim", _i32), ("layout", _i32), ("amp", _f32), ("reserved", _i32)]
+
+
+class MlaRopeArgs(ctypes.Structure):
+    """Layout of ``mla_rope_args`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("x", _vp),
+        ("out", _vp),
+        ("x_stride_t", _i64),
+        ("x_stride_h", _i64),
+        ("o_stride_t", _i64),
+        ("o_stride_h", _i64),
+        ("positions", _vp),
+        ("tokens", _i32),
+        ("heads", _i32),
+        ("dim", _i32),
+        ("first", _i32),
+        ("dtype", _i32),
+        ("reserved", _i32),
+    ]
+
+
+class MlaAppendSlotsArgs(ctypes.Structure):
+    """Layout of ``mla_append_slots_args`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("kv_new", _vp),
+        ("new_stride", _i64),
+        ("slots", _vp),
+        ("positions", _vp),
+        ("q_pe", _vp),
+        ("q_rope", _vp),
+        ("pe_stride_t", _i64),
+        ("pe_stride_h", _i64),
+        ("q_stride_t", _i64),
+        ("q_stride_h", _i64),
+        ("tokens", _i32),
+        ("heads", _i32),
+    ]
+
+
+class MlaPagePool(ctypes.Structure):
+    """Layout of ``mla_page_pool`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("free_pages", _vp),
+        ("count", _vp),
+        ("num_blocks", _i32),
+        ("batch", _i32),
+        ("block_table", _vp),
+        ("block_table_stride", _i32),
+        ("block_table_width", _i32),
+        ("cache_seqlens", _vp),
+    ]
+
+
 class MlaError(RuntimeError):
     """A nonzero status from the C ABI, carrying the library's message."""
 
@@ -196,6 +286,19 @@ def load() -> ctypes.CDLL:
         lib.mla_kv_append.restype = ctypes.c_int
         lib.mla_combine_absorb.argtypes = [ctypes.POINTER(MlaDecodeArgs), _vp, _vp, _vp]
         lib.mla_combine_absorb.restype = ctypes.c_int
+        lib.mla_num_parts_for.argtypes = [_i32] * 6
+        lib.mla_num_parts_for.restype = ctypes.c_int
+        lib.mla_apply_rope.argtypes = [ctypes.POINTER(MlaRope), ctypes.POINTER(MlaRopeArgs), _vp]
+        lib.mla_apply_rope.restype = ctypes.c_int
+        lib.mla_kv_append_slots.argtypes = [ctypes.POINTER(MlaKvCache), ctypes.POINTER(MlaRope),
+                                            ctypes.POINTER(MlaAppendSlotsArgs), _vp]
+        lib.mla_kv_append_slots.restype = ctypes.c_int
+        lib.mla_kv_gather.argtypes = [ctypes.POINTER(MlaKvCache), _vp, _i32, _vp, _i64, _vp]
+        lib.mla_kv_gather.restype = ctypes.c_int
+        lib.mla_reserve_pages.argtypes = [ctypes.POINTER(MlaPagePool), _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp]
+        lib.mla_reserve_pages.restype = ctypes.c_int
+        lib.mla_release_pages.argtypes = [ctypes.POINTER(MlaPagePool), _vp, _vp]
+        lib.mla_release_pages.restype = ctypes.c_int
         _lib = lib
         return lib
 

@@ -12,6 +12,9 @@
 * ``Fp8KVCache`` / ``fp8_kv_cache(num_blocks)`` / ``quantize_kv_cache(kv_cache)``: the fp8
   latent cache (OCP e4m3 codes with power-of-two scales per token and 128 dims, bf16 rope),
   accepted wherever a kv cache is, and written by ``kv_append``.
+* ``Fp4KVCache`` / ``fp4_kv_cache(num_blocks)`` / ``quantize_kv_cache(kv_cache, bits=4)``: the 4-bit
+  latent cache (OCP e2m1 codes with a power-of-two scale per token and 32 dims, bf16 rope), accepted
+  in the same places.
 
 Tensors live on the GPU; every call goes through the C ABI of ``include/mla_decode_amd.h``
 on torch's current stream.  Shapes: q ``[B, s_q, H, 576]``, kv cache ``[num_blocks, 64, 1,
@@ -32,8 +35,8 @@ from typing import NamedTuple, Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib
-from ._lib import (MLA_DIM_QK, MLA_DIM_V, MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_KV_FP8_E4M3,
-                   MLA_KV_NATIVE, MlaDecodeArgs, MlaKvAppendArgs, check)
+from ._lib import (MLA_DIM_QK, MLA_DIM_V, MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_KV_FP4_E2M1,
+                   MLA_KV_FP8_E4M3, MLA_KV_NATIVE, MlaDecodeArgs, MlaKvAppendArgs, check)
 
 _DTYPES = {torch.bfloat16: MLA_DTYPE_BF16, torch.float16: MLA_DTYPE_F16}
 
@@ -126,6 +129,14 @@ def num_parts_for(batch: int, s_q: int, heads_q: int, heads_k: int = 1, cu_count
     return n
 
 
+@functools.lru_cache(maxsize=4096)
+def _num_parts_fp4(rows: int, cu_count: int = 0) -> int:
+    n = _lib.load().mla_num_parts_for(1, 1, rows, 1, cu_count, MLA_KV_FP4_E2M1)
+    if n < 1:
+        check("mla_num_parts_for", -n)
+    return n
+
+
 def kernel_variant(rows: int) -> dict:
     """Tile of the main kernel for ``rows`` = s_q * heads query rows (``mla_variant``)."""
     w, t, st, r = (ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32())
@@ -139,7 +150,8 @@ def kernel_variant(rows: int) -> dict:
 
 def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num_heads_k: int,
                      num_parts: Optional[int] = None, fixed_overhead: int = -1,
-                     forced_splits: int = 0, topk: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+                     forced_splits: int = 0, topk: Optional[int] = None,
+                     kv_cache=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Tile schedule: ``(tile_scheduler_metadata [num_parts, 8] int32, num_splits [B+1] int32)``.
 
     ``num_heads_per_head_k`` is ``s_q * h_q // h_kv`` as in the reference's call; it picks
@@ -149,7 +161,9 @@ def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num
     smallest payload that fits, with the library's overhead ``MLA_DEFAULT_SPLIT_OVERHEAD``.
     ``forced_splits > 0`` cuts every sequence into that many near-equal page ranges instead
     (then ``num_parts = B * forced_splits``).  ``topk`` (sparse decode): every sequence is
-    scheduled as ``topk`` keys long, whatever ``cache_seqlens`` holds.
+    scheduled as ``topk`` keys long, whatever ``cache_seqlens`` holds.  ``kv_cache``: the cache the
+    schedule is for; an :class:`Fp4KVCache` is decoded by workgroups of another size, whose count the
+    default ``num_parts`` then is (any schedule is decoded right; that one fills the GPU).
     """
     _require_gpu(cache_seqlens, "cache_seqlens")
     if topk is not None:
@@ -165,7 +179,8 @@ def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num
     if forced_splits > 0:
         num_parts = batch * forced_splits
     elif num_parts is None:
-        num_parts = num_parts_for(batch, 1, num_heads_per_head_k, 1)
+        num_parts = (_num_parts_fp4(num_heads_per_head_k) if isinstance(kv_cache, Fp4KVCache)
+                     else num_parts_for(batch, 1, num_heads_per_head_k, 1))
     sched = torch.empty(num_parts, _lib.MLA_SCHED_WORDS, dtype=torch.int32, device=seqlens.device)
     splits = torch.empty(batch + 1, dtype=torch.int32, device=seqlens.device)
     check("mla_get_metadata", _lib.load().mla_get_metadata(
@@ -209,9 +224,32 @@ def fp8_kv_cache(num_blocks: int, device="cuda") -> Fp8KVCache:
                                   dtype=torch.bfloat16, device=device))
 
 
-def quantize_kv_cache(kv_cache: torch.Tensor) -> Fp8KVCache:
-    """Quantize every page of a bf16 cache ``[num_blocks, 64, 1, 576]`` to the fp8 format
+class Fp4KVCache(NamedTuple):
+    """The 4-bit latent cache: ``latent`` uint8 ``[num_blocks, 64, 256]`` OCP e2m1 codes, two a byte
+    (dim 2i in the low half of byte i), ``scale`` uint8 ``[num_blocks, 64, 16]`` (a byte s per token and
+    32 dims, 1 .. 254; 255 marks a block that held a NaN or an infinity), ``rope`` bf16
+    ``[num_blocks, 64, 64]``.  Latent value d of a token is ``e2m1(code_d) * 2**(scale[d // 32] - 127)``.
+    400 bytes a token (bf16: 1152, fp8: 656).  No counterpart in the reference.
+    """
+    latent: torch.Tensor
+    scale: torch.Tensor
+    rope: torch.Tensor
+
+
+def fp4_kv_cache(num_blocks: int, device="cuda") -> Fp4KVCache:
+    """An empty (zero) 4-bit cache of ``num_blocks`` pages; fill it with ``kv_append``."""
+    return Fp4KVCache(torch.zeros(num_blocks, _lib.MLA_PAGE_TOKENS, MLA_DIM_V // 2, dtype=torch.uint8, device=device),
+                      torch.full((num_blocks, _lib.MLA_PAGE_TOKENS, MLA_DIM_V // 32), 127, dtype=torch.uint8, device=device),
+                      torch.zeros(num_blocks, _lib.MLA_PAGE_TOKENS, MLA_DIM_QK - MLA_DIM_V,
+                                  dtype=torch.bfloat16, device=device))
+
+
+def quantize_kv_cache(kv_cache: torch.Tensor, bits: int = 8) -> Union[Fp8KVCache, Fp4KVCache]:
+    """Quantize every page of a bf16 cache ``[num_blocks, 64, 1, 576]`` to the fp8 format, or with
+    ``bits=4`` to the 4-bit one
     (on the GPU, through ``mla_kv_append``: page i is appended as one 64-token sequence)."""
+    if bits not in (4, 8):
+        raise ValueError("bits must be 8 or 4")
     _require_gpu(kv_cache, "kv_cache")
     if kv_cache.dtype != torch.bfloat16 or kv_cache.shape[-1] != MLA_DIM_QK or kv_cache.shape[1] != _lib.MLA_PAGE_TOKENS:
         raise ValueError("kv_cache must be a bf16 [num_blocks, 64, 1, 576] tensor")
@@ -219,9 +257,13 @@ def quantize_kv_cache(kv_cache: torch.Tensor) -> Fp8KVCache:
     # every code, scale and rope row is written below: no fill (three launches and a pass over the
     # cache; 138496 tokens: 65.6 -> 50.7 us)
     page, dev = _lib.MLA_PAGE_TOKENS, kv_cache.device
-    dst = Fp8KVCache(torch.empty(nb, page, MLA_DIM_V, dtype=torch.uint8, device=dev),
-                     torch.empty(nb, 4, page, dtype=torch.float32, device=dev),
-                     torch.empty(nb, page, MLA_DIM_QK - MLA_DIM_V, dtype=torch.bfloat16, device=dev))
+    rope = torch.empty(nb, page, MLA_DIM_QK - MLA_DIM_V, dtype=torch.bfloat16, device=dev)
+    if bits == 4:
+        dst = Fp4KVCache(torch.empty(nb, page, MLA_DIM_V // 2, dtype=torch.uint8, device=dev),
+                         torch.empty(nb, page, MLA_DIM_V // 32, dtype=torch.uint8, device=dev), rope)
+    else:
+        dst = Fp8KVCache(torch.empty(nb, page, MLA_DIM_V, dtype=torch.uint8, device=dev),
+                         torch.empty(nb, 4, page, dtype=torch.float32, device=dev), rope)
     table = torch.arange(nb, dtype=torch.int32, device=kv_cache.device).reshape(nb, 1)
     lens = torch.zeros(nb, dtype=torch.int32, device=kv_cache.device)
     kv_append(kv_cache.reshape(nb, _lib.MLA_PAGE_TOKENS, MLA_DIM_QK), dst, table, lens)
@@ -264,12 +306,12 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
     dtype = q.dtype
     if dtype not in _DTYPES:
         raise ValueError("q must be bfloat16 or float16")
-    fp8 = isinstance(kv_cache, Fp8KVCache)
+    fmt = _cache_format(kv_cache)
     scale, scale_ptr, scale_page, scale_blk = None, 0, 0, 0
-    if fp8:
-        latent, scale, rope = _check_fp8_cache(kv_cache)
+    if fmt != MLA_KV_NATIVE:
+        latent, scale, rope = _check_coded_cache(kv_cache)
         if dtype != torch.bfloat16:
-            raise ValueError("the fp8 cache is read with bf16 queries")
+            raise ValueError(f"the {'fp8' if fmt == MLA_KV_FP8_E4M3 else 'fp4'} cache is read with bf16 queries")
         (kv_page, kv_tok, _), (kr_page, kr_tok, _) = latent.stride(), rope.stride()
         kv_ptr, kr_ptr = latent.data_ptr(), rope.data_ptr()
         scale_ptr = scale.data_ptr()
@@ -350,7 +392,7 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
         kv_ptr, kr_ptr, kv_page, kv_tok, 0, kr_page, kr_tok, 0,
         bt_ptr, bt_stride, num_parts, seqlens.data_ptr() if seqlens is not None else 0, sched.data_ptr(),
         splits.data_ptr(), out.data_ptr(), os_b, os_s, os_h, lse.data_ptr(), ws_ptr, ws_bytes,
-        MLA_KV_FP8_E4M3 if fp8 else MLA_KV_NATIVE, 0, scale_ptr, scale_page, scale_blk,
+        fmt, 0, scale_ptr, scale_page, scale_blk,
         idx_ptr, idx_stride, topk, bt_width, 0, status.data_ptr() if status is not None else 0))
     keep = (q, latent, rope, scale, block_table, seqlens, sched, splits, out, lse, ws, indices, status)
     return a, out, lse, keep
@@ -466,7 +508,7 @@ def mla_decode_with_kvcache(q: torch.Tensor, kv_cache, block_table: torch.Tensor
         if num_splits is not None and forced < 1:
             raise ValueError("num_splits must be >= 1")
         sched, splits = get_mla_metadata(cache_seqlens, q.shape[1] * q.shape[2], 1,
-                                         forced_splits=forced)
+                                         forced_splits=forced, kv_cache=kv_cache)
         if forced == 1:
             return _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal,
                            out, lse, status=status, single_split=True)
@@ -510,10 +552,11 @@ def kv_append(kv_new: torch.Tensor, kv_cache, block_table: torch.Tensor,
     Returns the filled C argument struct (for re-launching through the C ABI directly).
     """
     _require_gpu(kv_new, "kv_new")
-    fp8 = isinstance(kv_cache, Fp8KVCache)
+    fmt = _cache_format(kv_cache)
+    coded = fmt != MLA_KV_NATIVE
     rope_offset = 0
-    if fp8:
-        latent, scale, rope = _check_fp8_cache(kv_cache)
+    if coded:
+        latent, scale, rope = _check_coded_cache(kv_cache)
     elif isinstance(kv_cache, (tuple, list)):
         latent, rope = _split_kv(kv_cache)
     else:  # one tensor: the rope half starts 512 elements into each row
@@ -527,13 +570,13 @@ def kv_append(kv_new: torch.Tensor, kv_cache, block_table: torch.Tensor,
         kv_new = kv_new[:, :, 0]
     if kv_new.dim() != 3 or kv_new.shape[-1] != MLA_DIM_QK:
         raise ValueError("kv_new must be [B, n_new, 576]")
-    if fp8:
+    if coded:
         if kv_new.dtype != torch.bfloat16:
-            raise ValueError("the fp8 cache takes bf16 tokens")
+            raise ValueError(f"the {'fp8' if fmt == MLA_KV_FP8_E4M3 else 'fp4'} cache takes bf16 tokens")
     elif kv_new.dtype not in _DTYPES or latent.dtype != kv_new.dtype or rope.dtype != kv_new.dtype:
         raise ValueError("kv_new and the cache must share one 16-bit dtype (bf16 or fp16)")
     B, n_new = kv_new.shape[0], kv_new.shape[1]
-    if not fp8 and (latent.dim() != 4 or latent.shape[1] != _lib.MLA_PAGE_TOKENS or latent.shape[2] != 1):
+    if not coded and (latent.dim() != 4 or latent.shape[1] != _lib.MLA_PAGE_TOKENS or latent.shape[2] != 1):
         raise ValueError("kv_cache must be [num_blocks, 64, 1, 576] (or a latent / rope pair)")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError("block_table must be [B, max_pages] int32")
@@ -546,7 +589,7 @@ def kv_append(kv_new: torch.Tensor, kv_cache, block_table: torch.Tensor,
     for t, name in ((latent, "kv_cache"), (block_table, "block_table"), (cache_seqlens, "cache_seqlens")):
         _require_gpu(t, name)
     (new_b, new_t, _), (kv_page, kv_tok), (kr_page, kr_tok) = kv_new.stride(), latent.stride()[:2], rope.stride()[:2]
-    scale_args = (MLA_KV_FP8_E4M3, 0, scale.data_ptr(), *scale.stride()[:2]) if fp8 else (MLA_KV_NATIVE, 0, 0, 0, 0)
+    scale_args = (fmt, 0, scale.data_ptr(), *scale.stride()[:2]) if coded else (fmt, 0, 0, 0, 0)
     a = MlaKvAppendArgs.from_buffer_copy(_APPEND_ARGS.pack(
         B, n_new, _DTYPES[kv_new.dtype], latent.shape[0], kv_new.data_ptr(), new_b, new_t,
         latent.data_ptr(), rope.data_ptr() + rope_offset, kv_page, kv_tok, kr_page, kr_tok,
@@ -555,6 +598,31 @@ def kv_append(kv_new: torch.Tensor, kv_cache, block_table: torch.Tensor,
         status.data_ptr() if status is not None else 0, *scale_args))
     check("mla_kv_append", _lib.load().mla_kv_append(ctypes.byref(a), _stream_ptr(kv_new.device)))
     return a
+
+
+def _cache_format(kv_cache) -> int:
+    if isinstance(kv_cache, Fp8KVCache):
+        return MLA_KV_FP8_E4M3
+    return MLA_KV_FP4_E2M1 if isinstance(kv_cache, Fp4KVCache) else MLA_KV_NATIVE
+
+
+def _check_coded_cache(c):
+    """(latent, scale, rope) of an fp8 or 4-bit cache, checked."""
+    return _check_fp8_cache(c) if isinstance(c, Fp8KVCache) else _check_fp4_cache(c)
+
+
+def _check_fp4_cache(c: Fp4KVCache):
+    latent, scale, rope = c
+    for t, n in ((latent, "fp4 latent"), (scale, "fp4 scale"), (rope, "fp4 rope")):
+        _require_gpu(t, n)
+    nb, page = latent.shape[0], _lib.MLA_PAGE_TOKENS
+    if latent.dtype != torch.uint8 or latent.shape != (nb, page, MLA_DIM_V // 2) or latent.stride(-1) != 1:
+        raise ValueError("fp4 latent must be a uint8 [num_blocks, 64, 256] tensor")
+    if scale.dtype != torch.uint8 or scale.shape != (nb, page, MLA_DIM_V // 32) or scale.stride(-1) != 1:
+        raise ValueError("fp4 scale must be a uint8 [num_blocks, 64, 16] tensor")
+    if rope.dtype != torch.bfloat16 or rope.shape != (nb, page, MLA_DIM_QK - MLA_DIM_V) or rope.stride(-1) != 1:
+        raise ValueError("fp4 rope must be a bf16 [num_blocks, 64, 64] tensor")
+    return latent, scale, rope
 
 
 def _check_fp8_cache(c: Fp8KVCache):

@@ -4,7 +4,8 @@
 of ``include/mla_decode_amd.h`` into a shared library that ``mlc_decode_amd._lib`` loads with
 ctypes.  Runs without a GPU (hipcc cross-compiles).  ``csrc/mla_decode_ws.hip`` (the dense
 wave-split kernel) is compiled with LLVM's iterative ILP machine scheduler, every other
-translation unit with the default one.
+translation unit (``mla_fp4.hip``: the decode over the 4-bit cache; ``mla_serving.hip``: rotary
+positions, appends, gather, pages) with the default one.
 """
 from __future__ import annotations
 
@@ -24,6 +25,8 @@ LIB_PATH = os.path.join(LIB_DIR, "libmla_decode_amd.so")
 SOURCES = [
     (os.path.join(CSRC, "mla_decode.hip"), []),
     (os.path.join(CSRC, "mla_decode_ws.hip"), ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"]),
+    (os.path.join(CSRC, "mla_fp4.hip"), []),
+    (os.path.join(CSRC, "mla_serving.hip"), []),
 ]
 # bench.py's MFMA-rate and shader-clock probe (a measurement helper, not the decode's ABI)
 PROBE_PATH = os.path.join(LIB_DIR, "libmla_probe.so")

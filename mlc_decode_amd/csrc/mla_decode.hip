@@ -38,7 +38,9 @@
 
 #include "mla_decode_amd.h"
 #include "mla_dispatch.h"
+#include "mla_fp4.h"
 #include "mla_sched.h"
+#include "mla_serving.h"
 
 namespace mla {
 
@@ -3931,6 +3933,18 @@ hipError_t launch_main_dt(const Variant& v, const mla::KParams& kp, int head_blo
   return launch_main<DT, 4, 2, 3, false>(kp, head_blocks, st);
 }
 
+bool known_format(int32_t f) { return f == MLA_KV_NATIVE || f == MLA_KV_FP8_E4M3 || f == MLA_KV_FP4_E2M1; }
+
+// The 4-bit cache's latent and scale strides (bytes): lanes read 16-byte pieces of a row's codes, and a
+// token's 16 scale bytes at once; a row's offset in its page is formed in 32 bits.
+int validate_fp4(int64_t page, int64_t tok, const void* scale, int64_t scale_page, int64_t scale_tok) {
+  if (page % 16 || tok % 16) return fail(MLA_ERR_INVALID, "fp4 latent strides must be multiples of 16 bytes");
+  if (!scale || !aligned(scale, 16) || scale_page < 0 || scale_tok < 0 || scale_page % 16 || scale_tok % 16)
+    return fail(MLA_ERR_INVALID, "kv_scale must be 16-byte aligned with non-negative strides, multiples of 16 bytes");
+  if (scale_tok >= (int64_t(1) << 24)) return fail(MLA_ERR_UNSUPPORTED, "kv_scale token strides must be below 2^24 bytes");
+  return MLA_OK;
+}
+
 int validate(const mla_decode_args* a, int64_t* need_ws) {
   if (a == nullptr) return fail(MLA_ERR_INVALID, "args is NULL");
   if (a->batch < 1 || a->s_q < 1 || a->heads_q < 1)
@@ -3974,8 +3988,8 @@ int validate(const mla_decode_args* a, int64_t* need_ws) {
       a->o_stride_b < 0 || a->o_stride_s < 0 || a->o_stride_h < 0)
     return fail(MLA_ERR_INVALID, "out must be 8-byte aligned with strides multiples of 4 elements");
   if (a->num_parts < 1) return fail(MLA_ERR_INVALID, "num_parts must be >= 1");
-  if ((a->kv_format != MLA_KV_NATIVE && a->kv_format != MLA_KV_FP8_E4M3) || a->kv_reserved != 0)
-    return fail(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE or MLA_KV_FP8_E4M3 (kv_reserved 0)");
+  if (!known_format(a->kv_format) || a->kv_reserved != 0)
+    return fail(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE, MLA_KV_FP8_E4M3 or MLA_KV_FP4_E2M1 (kv_reserved 0)");
   if (a->table_reserved != 0) return fail(MLA_ERR_INVALID, "table_reserved must be 0");
   if (a->status != nullptr && !aligned(a->status, 4)) return fail(MLA_ERR_INVALID, "status must be 4-byte aligned");
   if (a->indices) {
@@ -3995,6 +4009,12 @@ int validate(const mla_decode_args* a, int64_t* need_ws) {
     if (!a->kv_scale || !aligned(a->kv_scale, 16) || a->kv_scale_stride_page < 0 ||
         a->kv_scale_stride_blk < 0 || a->kv_scale_stride_page % 4 || a->kv_scale_stride_blk % 4)
       return fail(MLA_ERR_INVALID, "kv_scale must be 16-byte aligned with non-negative strides, multiples of 4 floats");
+  }
+  if (a->kv_format == MLA_KV_FP4_E2M1) {
+    if (a->dtype != MLA_DTYPE_BF16) return fail(MLA_ERR_UNSUPPORTED, "the fp4 cache is read with bf16 queries");
+    if (!a->block_table && !a->indices) return fail(MLA_ERR_UNSUPPORTED, "the fp4 cache is paged only");
+    const int rc = validate_fp4(a->kv_stride_page, a->kv_stride_tok, a->kv_scale, a->kv_scale_stride_page, a->kv_scale_stride_blk);
+    if (rc != MLA_OK) return rc;
   }
   *need_ws = mla_workspace_bytes(a->batch, a->s_q, a->heads_q, a->num_parts);
   if (a->workspace == nullptr || a->workspace_bytes < *need_ws)
@@ -4051,6 +4071,32 @@ mla::KParams make_params(const mla_decode_args* a) {
   return k;
 }
 
+mla4::DecodeParams make_params_fp4(const mla_decode_args* a, const mla::KParams& k) {
+  mla4::DecodeParams d{};
+  d.q_nope = k.q_nope; d.q_rope = k.q_rope;
+  d.q_sb = k.q_sb; d.q_ss = k.q_ss; d.q_sh = k.q_sh;
+  d.qr_sb = k.qr_sb; d.qr_ss = k.qr_ss; d.qr_sh = k.qr_sh;
+  d.codes = (const uint8_t*)a->kv_nope;
+  d.scale = (const uint8_t*)a->kv_scale;
+  d.rope = k.kv_rope;
+  d.c_sp = k.kv_sp; d.c_st = k.kv_st;
+  d.s_sp = a->kv_scale_stride_page; d.s_st = a->kv_scale_stride_blk;
+  d.r_sp = k.kr_sp; d.r_st = k.kr_st;
+  d.block_table = k.block_table;
+  d.bt_stride = k.bt_stride; d.bt_width = k.bt_width; d.num_blocks = k.num_blocks;
+  d.status = k.status;
+  d.seqlens = k.seqlens;
+  d.splits = k.splits;
+  d.indices = k.indices; d.idx_stride = k.idx_stride; d.topk = k.topk; d.pool_tokens = k.pool_tokens;
+  d.out = k.out;
+  d.o_sb = k.o_sb; d.o_ss = k.o_ss; d.o_sh = k.o_sh;
+  d.lse = k.lse;
+  d.ws_lse = k.ws_lse; d.ws_scale = k.ws_scale; d.ws_o = k.ws_o;
+  d.batch = k.batch; d.s_q = k.s_q; d.heads = k.heads; d.rows = k.rows; d.causal = k.causal;
+  d.scale_log2 = k.scale_log2;
+  return d;
+}
+
 // Partials are the decode workspace's scaled fp16 rows (SCALED), the caller's fp32 rows of
 // mla_merge_partials, or the unscaled 16-bit rows of mla_launch (PT = uint16_t).
 // Many splits per sequence on average: a small grid of long merges, which the combine kernel's
@@ -4105,6 +4151,8 @@ int launch_combine(const mla::KParams& k, const PT* part_o, int dtype, int copy_
 
 }  // namespace
 
+int mla_srv::set_error(int code, const std::string& msg) { return fail(code, msg); }
+
 extern "C" {
 
 int mla_version(void) { return MLA_DECODE_AMD_VERSION; }
@@ -4135,6 +4183,21 @@ int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, 
   const int cus = cu_count > 0 ? cu_count : cu_count_current();
   int parts = cus * wgs_per_cu(v) / head_blocks;
   return parts < 1 ? 1 : parts;
+}
+
+int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format) {
+  if (!known_format(kv_format)) {
+    fail(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE, MLA_KV_FP8_E4M3 or MLA_KV_FP4_E2M1");
+    return -MLA_ERR_INVALID;
+  }
+  const int parts = mla_num_parts(batch, s_q, heads_q, heads_k, cu_count);
+  if (parts < 0 || kv_format != MLA_KV_FP4_E2M1) return parts;
+  const int64_t rows = (int64_t)s_q * heads_q;
+  const int R = mla4::rows_per_workgroup(rows < 65536 ? (int)rows : 65536);
+  const int64_t row_blocks = (rows + R - 1) / R;
+  const int cus = cu_count > 0 ? cu_count : cu_count_current();
+  const int64_t n = (int64_t)cus * mla4::kWorkgroupsPerCu / row_blocks;
+  return n < 1 ? 1 : (int)n;
 }
 
 int mla_get_metadata_host(const int32_t* cache_seqlens, int32_t batch, int32_t num_parts,
@@ -4240,6 +4303,11 @@ int mla_splitkv_fwd(const mla_decode_args* args, void* stream) {
   const int rc = validate(args, &need);
   if (rc != MLA_OK) return rc;
   const mla::KParams kp = make_params(args);
+  if (args->kv_format == MLA_KV_FP4_E2M1) {
+    const hipError_t e = mla4::launch_decode(make_params_fp4(args, kp), kp.sched, kp.num_parts, (hipStream_t)stream);
+    if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("decode launch failed: ") + hipGetErrorString(e));
+    return MLA_OK;
+  }
   const Variant v = pick_variant(kp.rows);
   const int R = v.rows();
   const int head_blocks = (kp.rows + R - 1) / R;
@@ -4426,8 +4494,13 @@ int mla_kv_append(const mla_kv_append_args* a, void* stream) {
     if (v < 0 || v % 8) return fail(MLA_ERR_INVALID, "strides must be non-negative multiples of 8 elements");
   if (a->block_table_stride < 1 || a->max_pages < 1 || a->num_blocks < 1)
     return fail(MLA_ERR_INVALID, "block_table_stride, max_pages and num_blocks must be >= 1");
-  if ((a->kv_format != MLA_KV_NATIVE && a->kv_format != MLA_KV_FP8_E4M3) || a->kv_reserved != 0)
-    return fail(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE or MLA_KV_FP8_E4M3 (kv_reserved 0)");
+  if (!known_format(a->kv_format) || a->kv_reserved != 0)
+    return fail(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE, MLA_KV_FP8_E4M3 or MLA_KV_FP4_E2M1 (kv_reserved 0)");
+  if (a->kv_format == MLA_KV_FP4_E2M1) {
+    if (a->dtype != MLA_DTYPE_BF16) return fail(MLA_ERR_UNSUPPORTED, "the fp4 cache takes bf16 tokens");
+    const int rc = validate_fp4(a->kv_stride_page, a->kv_stride_tok, a->kv_scale, a->kv_scale_stride_page, a->kv_scale_stride_blk);
+    return rc != MLA_OK ? rc : mla_srv::append_fp4(a, (hipStream_t)stream);
+  }
   const bool kv8 = a->kv_format == MLA_KV_FP8_E4M3;
   if (kv8) {
     if (a->dtype != MLA_DTYPE_BF16) return fail(MLA_ERR_UNSUPPORTED, "the fp8 cache takes bf16 tokens");
