@@ -7,9 +7,8 @@
 //
 // A workgroup of four waves owns one schedule part for 16 * RT query rows and walks it in stages of T
 // tokens; two workgroups share a CU, so one's matrix work covers the other's loads and barriers.
-//  1. Codes go from HBM into registers, a lane holding 32 dims of one token: that is the A operand of the
-//     block-scaled 16x16x128 MFMA as it stands, the scale byte its scale.  Nothing is converted for the QK
-//     product.  The queries are split once per segment into two e4m3 parts, q = hi + lo: a bf16 has eight
+//  1. A lane holds 32 dims of one token as codes: that is the A operand of the block-scaled 16x16x128 MFMA as it
+//     stands, the scale byte its scale.  Nothing is converted for the QK product.  The queries are split once per segment into two e4m3 parts, q = hi + lo: a bf16 has eight
 //     significant bits, each part holds four (see split_query for what is left).  The rope dims take the
 //     bf16 MFMA.
 //  2. The V operand needs tokens along k, and its scales vary along k, which the block-scaled MFMA does not
@@ -52,6 +51,20 @@ typedef __bf16 bf16x8 __attribute__((__vector_size__(8 * sizeof(__bf16))));
 // LDS hand-off between the waves: own LDS accesses done, then the barrier.  Loads from HBM stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// One wave's copy from HBM into LDS, 16 (or 4) bytes a lane: lane l's bytes land at lds + 16 l (4 l).  Inline asm,
+// so that the compiler, which takes the builtin for an LDS store, does not wait for every copy in flight before
+// it reads LDS; copies_landed() is the wait.  M0 is written without a save: nothing else here reads it.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy16(const void* lane_addr, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(const void* lane_addr, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ float xor16(float v, bool sum) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
@@ -61,6 +74,18 @@ __device__ __forceinline__ float xor32(float v, bool sum) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   const float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
   return sum ? a + b : fmaxf(a, b);
+}
+// The lane id.  FRESH: formed where it is called and not before, so that addresses derived from it are recomputed
+// where they are used.  Hoisted out of the stage loop they take some forty registers that the 64-row form
+// does not have, and a spilled address is reloaded behind every copy in flight (vmcnt is in order): 64 x 128
+// heads x 4096 tokens 177 us with those reloads, 112 without.  The 16-row form has the registers (128 ragged
+// sequences: 64.5 us with FRESH, 60 without).
+template <bool FRESH>
+__device__ __forceinline__ int lane_id() {
+  if constexpr (!FRESH) return threadIdx.x & 63;
+  int l;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+  return l;
 }
 // over the four lane groups that hold one row
 __device__ __forceinline__ float row_max(float v) { return xor32(xor16(v, false), false); }
@@ -81,12 +106,20 @@ __device__ __forceinline__ f32x4 mfma_bf16(i32x4 a, i32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 // 16 tokens x 16 rows x 128 dims: A e2m1 (lane (g, i): dims 32g .. 32g+31 of token i), B e4m3 (lane (g, i):
-// dims 16g .. +15 and 64 + 16g .. +15 of row i); the scale of dims 32g .. 32g+31 is byte C of lane group g's
-// word, of either operand.
-template <int C>
+// dims 16g .. +15 and 64 + 16g .. +15 of row i); the scale of dims 32g .. 32g+31 is byte CA (CB) of lane
+// group g's word.
+template <int CA, int CB>
 __device__ __forceinline__ f32x4 mfma_scaled(i32x4 a, i32x8 b, f32x4 c, int scale_a, int scale_b) {
   const i32x8 a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b, c, 4, 0, C, scale_a, C, scale_b);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b, c, 4, 0, CA, scale_a, CB, scale_b);
+}
+// chunk C of a score tile: the code scales in a word a chunk (low byte), or all in `packed`
+template <int C, bool WORDS>
+__device__ __forceinline__ f32x4 score(const i32x4 (&k)[4], const i32x8 (&q)[4], f32x4 acc, const i32x4& words, int packed, int scale_q) {
+  if constexpr (WORDS)
+    return mfma_scaled<0, C>(k[C], q[C], acc, words[C], scale_q);
+  else
+    return mfma_scaled<C, C>(k[C], q[C], acc, packed, scale_q);
 }
 
 // V in LDS: token t of a tile of 16 is a row of 1 KiB; its 16-byte chunk k sits at slot k ^ swz(t) of the
@@ -154,26 +187,30 @@ __device__ __forceinline__ QuerySplit split_query(const i32x4 (&v)[4], int g, in
   return r;
 }
 
-// RT row tiles of 16 rows.  RT == 1: stages of 64 tokens, wave w takes token tile w from its loads to its
-// scores.  RT > 1: stages of 32 tokens, whose codes every wave reads from LDS; wave w loads and converts
-// half of the dims of token tile w % 2, and scores row tile w % RT against kTiles token tiles.
+// RT row tiles of 16 rows.  RT == 1: stages of 64 tokens, wave w takes token tile w from its loads, in registers,
+// to its scores.  RT > 1: stages of 32 tokens, copied into one of two LDS buffers in fragment order (the
+// copies of a stage are in flight during the one before), from which every wave scores; wave w converts half
+// of the dims of token tile w % 2 and scores row tile w % RT against kTiles token tiles.
 template <int RT>
 struct Shape {
   static constexpr int T = RT == 1 ? 64 : 32;
   static constexpr int kTokTiles = T / 16;
   static constexpr int kTiles = RT * kTokTiles / 4;  // score tiles per wave
   static constexpr int kShare = 4 / RT;              // waves that share a row tile
-  static constexpr int kChunks = RT == 1 ? 4 : 2;    // 128-dim chunks a wave loads of its tokens
-  static constexpr int kRopes = RT == 1 ? 2 : 1;     // 32-dim rope fragments a wave loads
+  static constexpr int kChunks = RT == 1 ? 4 : 2;    // 128-dim chunks a wave converts of its tokens
 };
 
-// A stage's loads of one lane.
-template <int RT>
+// RT == 1: a stage's loads of one lane.
 struct Stage {
-  i32x4 code[Shape<RT>::kChunks];
-  i32x4 rope[Shape<RT>::kRopes];
-  i32x4 scale;  // the token's bytes of the chunks loaded (RT > 1: eight of them)
+  i32x4 code[4];
+  i32x4 rope[2];
+  i32x4 scale;
 };
+
+// RT > 1: a stage in LDS: per token tile four 1 KiB code fragments and two of rope, then the tokens' scale bytes.
+constexpr int kRawTile = 6 * 1024;
+constexpr int kRawScale = 2 * kRawTile;
+constexpr int kRawStage = kRawScale + 512;
 
 template <int RT, bool SPARSE>
 __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const int32_t* __restrict__ sched, int row_blocks,
@@ -183,9 +220,7 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
   constexpr bool kRaw = RT > 1;
   __shared__ __attribute__((aligned(1024))) uint8_t v_sh[T * 1024];
   __shared__ __attribute__((aligned(16))) uint8_t p_sh[RT * T * 32];  // [row tile][32 tokens][lane][16 bytes]
-  __shared__ __attribute__((aligned(16))) uint8_t code_sh[kRaw ? Sh::kTokTiles * 4096 : 16];
-  __shared__ __attribute__((aligned(16))) uint8_t rope_sh[kRaw ? Sh::kTokTiles * 2048 : 16];
-  __shared__ uint32_t kscale_sh[kRaw ? Sh::kTokTiles * 64 : 1];
+  __shared__ __attribute__((aligned(16))) uint8_t raw_sh[kRaw ? 2 * kRawStage : 16];
   __shared__ float max_sh[4][16];
   __shared__ float alpha_sh[RT][16];
   __shared__ int moved_sh[4];  // row tile's reference moved in this stage
@@ -206,8 +241,6 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
     }
   }
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int g = lane >> 4, li = lane & 15;
   const int rt_own = wave % RT;                               // the row tile this wave scores
   const int tt_load = RT == 1 ? wave : (wave & 1);            // the token tile it loads
   const int tt_own = (wave / RT) * Sh::kTiles;                // the first token tile it scores
@@ -216,13 +249,7 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 
   uint8_t LDS_AS* const v_lds = (uint8_t LDS_AS*)v_sh;
   uint8_t LDS_AS* const p_lds = (uint8_t LDS_AS*)p_sh;
-  uint8_t LDS_AS* const code_lds = (uint8_t LDS_AS*)code_sh;
-  uint8_t LDS_AS* const rope_lds = (uint8_t LDS_AS*)rope_sh;
-  // V writes: token li of tile tt_load, chunk 4g + i of a 256-byte window; V^T reads: token 4g + li/4, dims
-  // 128 * wave + 16d + 4 * (li % 4), the window's chunk 2d + (li/2) % 2
-  const int v_write = tt_load * 16384 + li * 1024;
-  const int rv = 4 * g + (li >> 2);
-  const int v_read = rv * 1024 + wave * 256 + ((((li >> 1) & 1) ^ swz(rv)) << 4) + ((li & 1) << 3);
+  uint8_t LDS_AS* const raw_lds = (uint8_t LDS_AS*)raw_sh;
 
   const int32_t* rec = sched + (int64_t)part * kSchedWords;
   int b = rec[0], page = rec[1], split = rec[4];
@@ -256,52 +283,74 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
     auto page_ids = [&](int first) __attribute__((always_inline)) {
       pbase = first;
       const int last = p.bt_width - 1;
-      const int i = first + lane < last ? first + lane : last;
+      const int at = first + lane_id<(RT > 1)>();
+      const int i = at < last ? at : last;
       const int v = p.block_table[(int64_t)b * p.bt_stride + i];
       bt_lane = v < 0 ? 0 : (v >= p.num_blocks ? p.num_blocks - 1 : v);
     };
     if (!SPARSE && nst > 0) page_ids(page);
 
-    auto load_stage = [&](int k, Stage<RT>& s) __attribute__((always_inline)) {
-      const int t = k * T + 16 * tt_load + li;  // the lane's token in the segment
-      const uint8_t *cp, *sp;
-      const uint16_t* rp;
+    // where token t of the segment is
+    struct Row {
+      const uint8_t* codes;
+      const uint8_t* scale;
+      const uint8_t* rope;
+    };
+    auto row_of = [&](int t) __attribute__((always_inline)) {
+      int64_t pg;
+      int row;
       if constexpr (SPARSE) {
         const int n = tok1 - tok0;
         const int id = idx_sh[t < n ? t : n - 1];
         const int64_t at = id >= 0 && id < p.pool_tokens ? id : 0;
-        cp = p.codes + (at >> 6) * p.c_sp + (at & 63) * p.c_st;
-        sp = p.scale + (at >> 6) * p.s_sp + (at & 63) * p.s_st;
-        rp = p.rope + (at >> 6) * p.r_sp + (at & 63) * p.r_st;
+        pg = at >> 6;
+        row = (int)(at & 63);
       } else {
-        const int pidx = page + k * T / kPageTokens;
+        const int pidx = page + __builtin_amdgcn_readfirstlane(t) / kPageTokens;  // a stage lies in one page
         if (pidx - pbase >= 64) page_ids(pidx);  // uniform
-        const int64_t pg = __builtin_amdgcn_readlane(bt_lane, pidx - pbase);
-        const int row = t & 63;
-        cp = p.codes + pg * p.c_sp + (uint32_t)(row * (int)p.c_st);
-        sp = p.scale + pg * p.s_sp + (uint32_t)(row * (int)p.s_st);
-        rp = p.rope + pg * p.r_sp + (uint32_t)(row * (int)p.r_st);
+        pg = __builtin_amdgcn_readlane(bt_lane, pidx - pbase);
+        row = t & 63;
       }
+      return Row{p.codes + pg * p.c_sp + (uint32_t)(row * (int)p.c_st), p.scale + pg * p.s_sp + (uint32_t)(row * (int)p.s_st),
+                 (const uint8_t*)(p.rope + pg * p.r_sp + (uint32_t)(row * (int)p.r_st))};
+    };
+    auto load_stage = [&](int k, Stage& s) __attribute__((always_inline)) {  // RT == 1
+      const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
+      const Row r = row_of(k * T + 16 * tt_load + li);
 #pragma unroll
-      for (int c = 0; c < Sh::kChunks; ++c) s.code[c] = *(const i32x4*)(cp + 64 * (c_load + c) + 16 * g);
-      if constexpr (RT == 1) {
-        s.scale = *(const i32x4*)sp;
-      } else {
-        const i32x2 v = *(const i32x2*)(sp + 4 * c_load);
-        s.scale = i32x4{v[0], v[1], 0, 0};
+      for (int c = 0; c < 4; ++c) s.code[c] = *(const i32x4*)(r.codes + 64 * c + 16 * g);
+      s.scale = *(const i32x4*)r.scale;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) s.rope[j] = *(const i32x4*)(r.rope + 64 * j + 16 * g);
+    };
+    auto copy_stage = [&](int k) __attribute__((always_inline)) {  // RT > 1
+      const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
+      const Row r = row_of(k * T + 16 * tt_load + li);
+      const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)raw_lds + (k & 1) * kRawStage);
+      const uint32_t tile = base + tt_load * kRawTile;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) copy16(r.codes + 64 * (c_load + c) + 16 * g, tile + 1024 * (c_load + c));
+      copy16(r.rope + 64 * (wave >> 1) + 16 * g, tile + 1024 * (4 + (wave >> 1)));
+      if (wave < 2) {  // uniform: a dword of scales a lane, four lanes a token
+        const Row w = row_of(k * T + 16 * wave + (lane >> 2));
+        copy4(w.scale + 4 * (lane & 3), base + kRawScale + 256 * wave);
       }
-#pragma unroll
-      for (int j = 0; j < Sh::kRopes; ++j) s.rope[j] = *(const i32x4*)(rp + 32 * (RT == 1 ? j : wave >> 1) + 8 * g);
     };
 
-    Stage<RT> nxt;
-    if (nst > 0) load_stage(0, nxt);
+    Stage nxt;
+    if (nst > 0) {
+      if constexpr (kRaw)
+        copy_stage(0);
+      else
+        load_stage(0, nxt);
+    }
 
     // ---- queries of row tile rt_own; rows past the last re-load it, and are never written
     i32x8 qh[4], ql[4];
     i32x4 qr[2];
     int qs_hi = 0, qtok;
     {
+      const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       int row = row0 + 16 * rt_own + li;
       row = row < p.rows ? row : p.rows - 1;
       qtok = row / p.heads;
@@ -333,86 +382,96 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 
 #pragma unroll 1
     for (int k = 0; k < nst; ++k) {
-      Stage<RT> cur = nxt;
-      if (RT == 1) load_stage(k + 1 < nst ? k + 1 : k, nxt);
+      Stage cur;
+      const uint8_t LDS_AS* const raw = raw_lds + (k & 1) * kRawStage;
+      if constexpr (kRaw) {
+        copies_landed();
+        lds_barrier();  // the stage is in LDS; V, P and the other buffer are free
+        if (k + 1 < nst) copy_stage(k + 1);
+      } else {
+        cur = nxt;
+        load_stage(k + 1 < nst ? k + 1 : k, nxt);
+      }
       const int tok_k = tok0 + k * T;
+      const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       // ---- 1. the wave's tokens to bf16 in LDS.  Tokens that do not exist become zeros: their weight is
       // zero, and what their rows hold must not make 0 * NaN of it.
+      int ks_own = 0;  // RT == 1: the scale bytes of blocks g, 4 + g, 8 + g, 12 + g
       {
-        uint32_t bytes = 0;  // RT == 1: the scale bytes of blocks g, 4 + g, 8 + g, 12 + g
+        i32x4 code[Sh::kChunks], sc;
+        if constexpr (kRaw) {
 #pragma unroll
-        for (int c = 0; c < Sh::kChunks; ++c) bytes |= (((uint32_t)cur.scale[c] >> (8 * g)) & 0xFF) << (8 * c);
-        if constexpr (kRaw) {  // the fragments for everyone's scores, as they came
-          uint8_t LDS_AS* dst = code_lds + (tt_load * 4 + c_load) * 1024 + lane * 16;
-#pragma unroll
-          for (int c = 0; c < Sh::kChunks; ++c) *(i32x4 LDS_AS*)(dst + 1024 * c) = cur.code[c];
-          *(i32x4 LDS_AS*)(rope_lds + (tt_load * 2 + (wave >> 1)) * 1024 + lane * 16) = cur.rope[0];
-          ((uint16_t LDS_AS*)(uint32_t LDS_AS*)kscale_sh)[(tt_load * 64 + lane) * 2 + (wave >> 1)] = (uint16_t)bytes;
-        }
-        uint32_t vbytes = bytes;
-        i32x4 code[Sh::kChunks];
-#pragma unroll
-        for (int c = 0; c < Sh::kChunks; ++c) code[c] = cur.code[c];
-        bool gone = false;
-        const int t = tok_k + 16 * tt_load + li;
-        if constexpr (SPARSE) {
-          const int i = t - tok0, n = tok1 - tok0;
-          const int id = idx_sh[i < n ? i : n - 1];
-          gone = i >= n || id < 0 || id >= p.pool_tokens;
+          for (int c = 0; c < 2; ++c) code[c] = *(const i32x4 LDS_AS*)(raw + tt_load * kRawTile + (c_load + c) * 1024 + lane * 16);
+          const i32x2 v = *(const i32x2 LDS_AS*)(raw + kRawScale + (tt_load * 16 + li) * 16 + 4 * c_load);
+          sc = i32x4{v[0], v[1], 0, 0};
         } else {
-          gone = t >= L;
+#pragma unroll
+          for (int c = 0; c < Sh::kChunks; ++c) code[c] = cur.code[c];
+          sc = cur.scale;
+        }
+        uint32_t byte[Sh::kChunks];
+#pragma unroll
+        for (int c = 0; c < Sh::kChunks; ++c) byte[c] = ((uint32_t)sc[c] >> (8 * g)) & 0xFF;
+        if constexpr (!kRaw) {
+#pragma unroll
+          for (int c = 0; c < Sh::kChunks; ++c) ks_own |= byte[c] << (8 * c);
         }
         if (SPARSE || tok_k + T > L) {  // uniform
-          vbytes = gone ? 0x7F7F7F7Fu : vbytes;
+          const int t = tok_k + 16 * tt_load + li;
+          bool gone = t >= L;
+          if constexpr (SPARSE) {
+            const int i = t - tok0, n = tok1 - tok0;
+            const int id = idx_sh[i < n ? i : n - 1];
+            gone = i >= n || id < 0 || id >= p.pool_tokens;
+          }
 #pragma unroll
-          for (int c = 0; c < Sh::kChunks; ++c)
+          for (int c = 0; c < Sh::kChunks; ++c) {
+            byte[c] = gone ? 127 : byte[c];
 #pragma unroll
             for (int j = 0; j < 4; ++j) code[c][j] = gone ? 0 : code[c][j];
+          }
         }
 #pragma unroll
         for (int c = 0; c < Sh::kChunks; ++c) {
-          const float sc = __uint_as_float(((vbytes >> (8 * c)) & 0xFF) << 23);
-          uint8_t LDS_AS* dst = v_lds + v_write + 256 * (c_load + c);
+          const float f = __uint_as_float(byte[c] << 23);
+          // token li of tile tt_load, chunk 4g + i of the 256-byte window
+          const int at = tt_load * 16384 + li * 1024 + (((4 * g) ^ swz(li)) << 4);
+          uint8_t LDS_AS* dst = v_lds + 256 * (c_load + c);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) *(i32x4 LDS_AS*)(dst + (((4 * g + i) ^ swz(li)) << 4)) = widen8(code[c][i], sc);
+          for (int i = 0; i < 4; ++i) *(i32x4 LDS_AS*)(dst + (at ^ (16 * i))) = widen8(code[c][i], f);
         }
-        if constexpr (RT == 1) cur.scale[0] = (int)bytes;
-      }
-      if constexpr (kRaw) {
-        load_stage(k + 1 < nst ? k + 1 : k, nxt);
-        lds_barrier();
       }
       // ---- 2. scores of the wave's tiles
       f32x4 s[Sh::kTiles];
 #pragma unroll
       for (int i = 0; i < Sh::kTiles; ++i) {
-        i32x4 kc[4], kr[2];
-        int ks;
+        const uint8_t LDS_AS* const tile = raw + (tt_own + i) * kRawTile + lane * 16;
+        i32x4 kc[4], kr[2], ks;
         if constexpr (kRaw) {
-          const int tt = tt_own + i;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) kc[c] = *(const i32x4 LDS_AS*)(code_lds + (tt * 4 + c) * 1024 + lane * 16);
+          for (int c = 0; c < 4; ++c) kc[c] = *(const i32x4 LDS_AS*)(tile + 1024 * c);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) kr[j] = *(const i32x4 LDS_AS*)(rope_lds + (tt * 2 + j) * 1024 + lane * 16);
-          ks = (int)kscale_sh[tt * 64 + lane];
+          for (int j = 0; j < 2; ++j) kr[j] = *(const i32x4 LDS_AS*)(tile + 1024 * (4 + j));
+          ks = *(const i32x4 LDS_AS*)(raw + kRawScale + ((tt_own + i) * 16 + li) * 16);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ks[c] = (int)((uint32_t)ks[c] >> (8 * g));  // the MFMA takes the low byte
         } else {
 #pragma unroll
           for (int c = 0; c < 4; ++c) kc[c] = cur.code[c];
           kr[0] = cur.rope[0];
-          kr[1] = cur.rope[Sh::kRopes - 1];
-          ks = cur.scale[0];
+          kr[1] = cur.rope[1];
         }
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, l = a;
         a = mfma_bf16(kr[0], qr[0], a);
-        l = mfma_scaled<0>(kc[0], ql[0], l, ks, qs_lo);
+        l = score<0, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
         a = mfma_bf16(kr[1], qr[1], a);
-        l = mfma_scaled<1>(kc[1], ql[1], l, ks, qs_lo);
-        a = mfma_scaled<0>(kc[0], qh[0], a, ks, qs_hi);
-        l = mfma_scaled<2>(kc[2], ql[2], l, ks, qs_lo);
-        a = mfma_scaled<1>(kc[1], qh[1], a, ks, qs_hi);
-        l = mfma_scaled<3>(kc[3], ql[3], l, ks, qs_lo);
-        a = mfma_scaled<2>(kc[2], qh[2], a, ks, qs_hi);
-        a = mfma_scaled<3>(kc[3], qh[3], a, ks, qs_hi);
+        l = score<1, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
+        a = score<0, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
+        l = score<2, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
+        a = score<1, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
+        l = score<3, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
+        a = score<2, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
+        a = score<3, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
         s[i] = (a + l) * p.scale_log2;
       }
       const bool ragged = tok_k + T > tok1 || tok_k + T > lim_min;
@@ -478,11 +537,14 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
           for (int d = 0; d < 8; ++d) o[d][r] *= al;
         }
       }
+      // V^T reads: token 4g + li/4, dims 128 * wave + 16d + 4 * (li % 4): the window's chunk 2d + (li/2) % 2
+      const int ln = lane_id<(RT > 1)>(), rv = 4 * (ln >> 4) + ((ln & 15) >> 2);
+      const int v_read = rv * 1024 + wave * 256 + ((((ln >> 1) & 1) ^ swz(rv)) << 4) + ((ln & 1) << 3);
 #pragma unroll
       for (int ks = 0; ks < T / 32; ++ks) {
         i32x4 pb[RT];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) pb[r] = *(const i32x4 LDS_AS*)(p_lds + ((r * (T / 32) + ks) * 64 + lane) * 16);
+        for (int r = 0; r < RT; ++r) pb[r] = *(const i32x4 LDS_AS*)(p_lds + ((r * (T / 32) + ks) * 64 + ln) * 16);
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
           const uint8_t LDS_AS* src = v_lds + (v_read ^ (32 * d)) + ks * 32768;
@@ -493,10 +555,12 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
           for (int r = 0; r < RT; ++r) o[d][r] = mfma_bf16(va, pb[r], o[d][r]);
         }
       }
-      lds_barrier();  // V, P and the words of this stage are free
+      if constexpr (!kRaw) lds_barrier();  // V, P and the words of this stage are free
     }
+    if constexpr (kRaw) lds_barrier();  // the raw buffers are free for the next segment
 
     // ---- the rows' sums from the waves that scored them
+    const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
     l_rnd = row_sum(l_rnd);
     l_exact = row_sum(l_exact);
     sum_sh[wave][0][li] = l_rnd;
