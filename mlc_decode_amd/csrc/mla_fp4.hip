@@ -113,13 +113,12 @@ __device__ __forceinline__ f32x4 mfma_scaled(i32x4 a, i32x8 b, f32x4 c, int scal
   const i32x8 a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b, c, 4, 0, CA, scale_a, CB, scale_b);
 }
-// chunk C of a score tile: the code scales in a word a chunk (low byte), or all in `packed`
-template <int C, bool WORDS>
-__device__ __forceinline__ f32x4 score(const i32x4 (&k)[4], const i32x8 (&q)[4], f32x4 acc, const i32x4& words, int packed, int scale_q) {
-  if constexpr (WORDS)
-    return mfma_scaled<0, C>(k[C], q[C], acc, words[C], scale_q);
-  else
-    return mfma_scaled<C, C>(k[C], q[C], acc, packed, scale_q);
+// chunk C of a score tile, the codes' scales in the low byte
+__device__ __forceinline__ f32x4 score(int c, i32x4 k, const i32x8 (&q)[4], f32x4 acc, int scale_k, int scale_q) {
+  return c == 0   ? mfma_scaled<0, 0>(k, q[0], acc, scale_k, scale_q)
+         : c == 1 ? mfma_scaled<0, 1>(k, q[1], acc, scale_k, scale_q)
+         : c == 2 ? mfma_scaled<0, 2>(k, q[2], acc, scale_k, scale_q)
+                  : mfma_scaled<0, 3>(k, q[3], acc, scale_k, scale_q);
 }
 
 // V in LDS: token t of a tile of 16 is a row of 1 KiB; its 16-byte chunk k sits at slot k ^ swz(t) of the
@@ -212,19 +211,32 @@ constexpr int kRawTile = 6 * 1024;
 constexpr int kRawScale = 2 * kRawTile;
 constexpr int kRawStage = kRawScale + 512;
 
+// The kernel's DecodeParams argument, read where it is used: as ordinary arguments they are all loaded at the start and
+// kept, which is more scalar registers than there are, and the spilled ones live in vector registers.
+typedef const DecodeParams __attribute__((address_space(4))) ArgParams;
+constexpr int kArgOffset = 16;  // behind sched, row_blocks and num_parts
+__device__ __forceinline__ ArgParams& params_here() {
+  auto a = (const char __attribute__((address_space(4)))*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(ArgParams*)(a + kArgOffset);
+}
+
 template <int RT, bool SPARSE>
 __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const int32_t* __restrict__ sched, int row_blocks,
-                                                                       int num_parts, DecodeParams p) {
+                                                                       int num_parts, DecodeParams) {
+  static_assert(alignof(DecodeParams) == 8 && kArgOffset % 8 == 0, "the struct's place among the arguments");
   using Sh = Shape<RT>;
   constexpr int T = Sh::T;
   constexpr bool kRaw = RT > 1;
   __shared__ __attribute__((aligned(1024))) uint8_t v_sh[T * 1024];
   __shared__ __attribute__((aligned(16))) uint8_t p_sh[RT * T * 32];  // [row tile][32 tokens][lane][16 bytes]
   __shared__ __attribute__((aligned(16))) uint8_t raw_sh[kRaw ? 2 * kRawStage : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t qr_sh[kRaw ? 4 * 2048 : 16];  // the waves' rope queries, in operand order
   __shared__ float max_sh[4][16];
   __shared__ float alpha_sh[RT][16];
-  __shared__ int moved_sh[4];  // row tile's reference moved in this stage
+  __shared__ __attribute__((aligned(4))) uint8_t moved_sh[4];  // row tile's reference moved in this stage
   __shared__ float sum_sh[4][2][16];
+  __shared__ int lim_sh[4][16];
   __shared__ int32_t idx_sh[SPARSE ? MLA_SPARSE_MAX_TOPK : 1];
 
   // Workgroups go to the eight XCDs in turn: the row blocks of a part, which read the same pages, take
@@ -255,9 +267,11 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
   int b = rec[0], page = rec[1], split = rec[4];
   const int end_b = rec[2], end_page = rec[3];
 
+  const int batch = params_here().batch;
 #pragma unroll 1
-  for (; b < p.batch; ++b, page = 0, split = 0) {
+  for (; b < batch; ++b, page = 0, split = 0) {
     if (!(b < end_b || (b == end_b && page < end_page))) break;
+    ArgParams& p = params_here();
     int L = SPARSE ? p.topk : p.seqlens[b];
     L = L > 0 ? L : 0;
     if (!SPARSE && L > (int64_t)p.bt_width * kPageTokens) {  // uniform: cut to the table
@@ -270,25 +284,20 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
     const int tok0 = page * kPageTokens;                                            // the segment's tokens
     const int tok1 = stop * kPageTokens < L ? stop * kPageTokens : L;
     const int nst = tok1 > tok0 ? (tok1 - tok0 + T - 1) / T : 0;
-    const int slot0 = p.splits[b];
-    const bool single = p.splits[b + 1] - slot0 == 1;
 
     if constexpr (SPARSE) {
       for (int i = threadIdx.x; i < tok1 - tok0; i += 256) idx_sh[i] = p.indices[(int64_t)b * p.idx_stride + tok0 + i];
       lds_barrier();
     }
 
-    // ---- page ids: lane i holds that of page pbase + i, clamped into the pool
-    int pbase = page, bt_lane = 0;
-    auto page_ids = [&](int first) __attribute__((always_inline)) {
-      pbase = first;
-      const int last = p.bt_width - 1;
-      const int at = first + lane_id<(RT > 1)>();
-      const int i = at < last ? at : last;
-      const int v = p.block_table[(int64_t)b * p.bt_stride + i];
-      bt_lane = v < 0 ? 0 : (v >= p.num_blocks ? p.num_blocks - 1 : v);
+    // ---- the page of stage k, clamped into the pool; read by a scalar load a stage before it is used
+    auto page_of = [&](int k) __attribute__((always_inline)) {
+      if constexpr (SPARSE) return 0;
+      const int at = page + k * T / kPageTokens, last = p.bt_width - 1;
+      const auto table = (const int32_t __attribute__((address_space(4)))*)p.block_table;
+      const int v = table[(int64_t)b * p.bt_stride + (at < last ? at : last)];
+      return v < 0 ? 0 : (v >= p.num_blocks ? p.num_blocks - 1 : v);
     };
-    if (!SPARSE && nst > 0) page_ids(page);
 
     // where token t of the segment is
     struct Row {
@@ -296,53 +305,50 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       const uint8_t* scale;
       const uint8_t* rope;
     };
-    auto row_of = [&](int t) __attribute__((always_inline)) {
-      int64_t pg;
-      int row;
+    auto row_of = [&](int t, int64_t pg) __attribute__((always_inline)) {
+      int row = t & 63;
       if constexpr (SPARSE) {
         const int n = tok1 - tok0;
         const int id = idx_sh[t < n ? t : n - 1];
         const int64_t at = id >= 0 && id < p.pool_tokens ? id : 0;
         pg = at >> 6;
         row = (int)(at & 63);
-      } else {
-        const int pidx = page + __builtin_amdgcn_readfirstlane(t) / kPageTokens;  // a stage lies in one page
-        if (pidx - pbase >= 64) page_ids(pidx);  // uniform
-        pg = __builtin_amdgcn_readlane(bt_lane, pidx - pbase);
-        row = t & 63;
       }
       return Row{p.codes + pg * p.c_sp + (uint32_t)(row * (int)p.c_st), p.scale + pg * p.s_sp + (uint32_t)(row * (int)p.s_st),
                  (const uint8_t*)(p.rope + pg * p.r_sp + (uint32_t)(row * (int)p.r_st))};
     };
-    auto load_stage = [&](int k, Stage& s) __attribute__((always_inline)) {  // RT == 1
+    auto load_stage = [&](int k, int pg, Stage& s) __attribute__((always_inline)) {  // RT == 1
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
-      const Row r = row_of(k * T + 16 * tt_load + li);
+      const Row r = row_of(k * T + 16 * tt_load + li, pg);
 #pragma unroll
       for (int c = 0; c < 4; ++c) s.code[c] = *(const i32x4*)(r.codes + 64 * c + 16 * g);
       s.scale = *(const i32x4*)r.scale;
 #pragma unroll
       for (int j = 0; j < 2; ++j) s.rope[j] = *(const i32x4*)(r.rope + 64 * j + 16 * g);
     };
-    auto copy_stage = [&](int k) __attribute__((always_inline)) {  // RT > 1
+    auto copy_stage = [&](int k, int pg) __attribute__((always_inline)) {  // RT > 1
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
-      const Row r = row_of(k * T + 16 * tt_load + li);
+      const Row r = row_of(k * T + 16 * tt_load + li, pg);
       const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)raw_lds + (k & 1) * kRawStage);
       const uint32_t tile = base + tt_load * kRawTile;
 #pragma unroll
       for (int c = 0; c < 2; ++c) copy16(r.codes + 64 * (c_load + c) + 16 * g, tile + 1024 * (c_load + c));
       copy16(r.rope + 64 * (wave >> 1) + 16 * g, tile + 1024 * (4 + (wave >> 1)));
       if (wave < 2) {  // uniform: a dword of scales a lane, four lanes a token
-        const Row w = row_of(k * T + 16 * wave + (lane >> 2));
+        const Row w = row_of(k * T + 16 * wave + (lane >> 2), pg);
         copy4(w.scale + 4 * (lane & 3), base + kRawScale + 256 * wave);
       }
     };
 
     Stage nxt;
+    int pg_next = 0;
     if (nst > 0) {
+      const int pg = page_of(0);
+      pg_next = page_of(nst > 1 ? 1 : 0);
       if constexpr (kRaw)
-        copy_stage(0);
+        copy_stage(0, pg);
       else
-        load_stage(0, nxt);
+        load_stage(0, pg, nxt);
     }
 
     // ---- queries of row tile rt_own; rows past the last re-load it, and are never written
@@ -367,10 +373,15 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
         qs_hi |= r.scale << (8 * c);
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) qr[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
+      for (int j = 0; j < 2; ++j) {
+        qr[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
+        if constexpr (kRaw) *(i32x4 LDS_AS*)((uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + lane * 16) = qr[j];
+      }
     }
     const int qs_lo = qs_hi - 0x0A0A0A0A;  // every byte is 11 at least
-    const int lim = L - (p.causal ? p.s_q - 1 - qtok : 0);  // this lane's row sees tokens below it
+    // used here once: the wait for them is not left to the stage loop
+    if constexpr (!kRaw) asm volatile("" : "+v"(qr[0]), "+v"(qr[1]));
+    lim_sh[wave][lane_id<(RT > 1)>() & 15] = L - (p.causal ? p.s_q - 1 - qtok : 0);  // the row sees tokens below it
     const int lim_min = L - (p.causal ? p.s_q - 1 : 0);     // every row sees those below it
 
     f32x4 o[8][RT];
@@ -379,6 +390,7 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 #pragma unroll
       for (int r = 0; r < RT; ++r) o[d][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_ref = -INFINITY, l_rnd = 0.f, l_exact = 0.f;
+    const float scale_log2 = p.scale_log2;
 
 #pragma unroll 1
     for (int k = 0; k < nst; ++k) {
@@ -387,95 +399,121 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       if constexpr (kRaw) {
         copies_landed();
         lds_barrier();  // the stage is in LDS; V, P and the other buffer are free
-        if (k + 1 < nst) copy_stage(k + 1);
+        if (k + 1 < nst) copy_stage(k + 1, pg_next);
       } else {
         cur = nxt;
-        load_stage(k + 1 < nst ? k + 1 : k, nxt);
+        if (k + 1 < nst) load_stage(k + 1, pg_next, nxt);
       }
+      pg_next = page_of(k + 2 < nst ? k + 2 : nst - 1);
       const int tok_k = tok0 + k * T;
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       // ---- 1. the wave's tokens to bf16 in LDS.  Tokens that do not exist become zeros: their weight is
       // zero, and what their rows hold must not make 0 * NaN of it.
-      int ks_own = 0;  // RT == 1: the scale bytes of blocks g, 4 + g, 8 + g, 12 + g
-      {
-        i32x4 code[Sh::kChunks], sc;
-        if constexpr (kRaw) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) code[c] = *(const i32x4 LDS_AS*)(raw + tt_load * kRawTile + (c_load + c) * 1024 + lane * 16);
-          const i32x2 v = *(const i32x2 LDS_AS*)(raw + kRawScale + (tt_load * 16 + li) * 16 + 4 * c_load);
-          sc = i32x4{v[0], v[1], 0, 0};
-        } else {
-#pragma unroll
-          for (int c = 0; c < Sh::kChunks; ++c) code[c] = cur.code[c];
-          sc = cur.scale;
-        }
-        uint32_t byte[Sh::kChunks];
-#pragma unroll
-        for (int c = 0; c < Sh::kChunks; ++c) byte[c] = ((uint32_t)sc[c] >> (8 * g)) & 0xFF;
-        if constexpr (!kRaw) {
-#pragma unroll
-          for (int c = 0; c < Sh::kChunks; ++c) ks_own |= byte[c] << (8 * c);
-        }
-        if (SPARSE || tok_k + T > L) {  // uniform
-          const int t = tok_k + 16 * tt_load + li;
-          bool gone = t >= L;
-          if constexpr (SPARSE) {
-            const int i = t - tok0, n = tok1 - tok0;
-            const int id = idx_sh[i < n ? i : n - 1];
-            gone = i >= n || id < 0 || id >= p.pool_tokens;
-          }
-#pragma unroll
-          for (int c = 0; c < Sh::kChunks; ++c) {
-            byte[c] = gone ? 127 : byte[c];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) code[c][j] = gone ? 0 : code[c][j];
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < Sh::kChunks; ++c) {
-          const float f = __uint_as_float(byte[c] << 23);
-          // token li of tile tt_load, chunk 4g + i of the 256-byte window
-          const int at = tt_load * 16384 + li * 1024 + (((4 * g) ^ swz(li)) << 4);
-          uint8_t LDS_AS* dst = v_lds + 256 * (c_load + c);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) *(i32x4 LDS_AS*)(dst + (at ^ (16 * i))) = widen8(code[c][i], f);
+      const bool cut = SPARSE || tok_k + T > L;  // uniform
+      bool gone = false;
+      if (cut) {
+        const int t = tok_k + 16 * tt_load + li;
+        gone = t >= L;
+        if constexpr (SPARSE) {
+          const int i = t - tok0, n = tok1 - tok0;
+          const int id = idx_sh[i < n ? i : n - 1];
+          gone = i >= n || id < 0 || id >= p.pool_tokens;
         }
       }
+      i32x4 code;  // chunk c of the token (c_load + c of its 128-dim chunks)
+      float scale = 0.f;
+      auto code_in = [&](int c) __attribute__((always_inline)) {
+        uint32_t w;
+        if constexpr (kRaw) {
+          code = *(const i32x4 LDS_AS*)(raw + tt_load * kRawTile + (c_load + c) * 1024 + lane * 16);
+          w = *(const uint32_t LDS_AS*)(raw + kRawScale + (tt_load * 16 + li) * 16 + 4 * (c_load + c));
+        } else {
+          code = cur.code[c];
+          w = (uint32_t)cur.scale[c];
+        }
+        scale = __uint_as_float(((w >> (8 * g)) & 0xFF) << 23);
+        if (cut) {  // uniform
+          scale = gone ? 1.f : scale;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) code[j] = gone ? 0 : code[j];
+        }
+      };
+      // word i of a chunk: 8 dims of token li of tile tt_load, chunk 4g + i of a 256-byte window
+      const int v_at = tt_load * 16384 + li * 1024 + (((4 * g) ^ swz(li)) << 4);
+      auto widen_word = [&](int c, int i) __attribute__((always_inline)) {
+        *(i32x4 LDS_AS*)(v_lds + 256 * (c_load + c) + (v_at ^ (16 * i))) = widen8(code[i], scale);
+      };
       // ---- 2. scores of the wave's tiles
       f32x4 s[Sh::kTiles];
+      if constexpr (kRaw) {
+        // Two rope steps, then four of 128 dims; a step's fragments are read during the step before, and the
+        // conversions of the wave's own tokens fill the gaps between the MFMAs.
+        i32x4 kf[2][Sh::kTiles], qf[2];
+        uint32_t ks[2][Sh::kTiles];  // the token's four scale bytes of the step's chunk
+        const uint8_t LDS_AS* const tile = raw + tt_own * kRawTile + lane * 16;
+        auto read_step = [&](int st) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < Sh::kTiles; ++i) {
-        const uint8_t LDS_AS* const tile = raw + (tt_own + i) * kRawTile + lane * 16;
-        i32x4 kc[4], kr[2], ks;
-        if constexpr (kRaw) {
+          for (int i = 0; i < Sh::kTiles; ++i)
+          {
+            kf[st & 1][i] = *(const i32x4 LDS_AS*)(tile + i * kRawTile + 1024 * (st < 2 ? 4 + st : st - 2));
+            if (st >= 2) ks[st & 1][i] = *(const uint32_t LDS_AS*)(raw + kRawScale + ((tt_own + i) * 16 + li) * 16 + 4 * (st - 2));
+          }
+        };
 #pragma unroll
-          for (int c = 0; c < 4; ++c) kc[c] = *(const i32x4 LDS_AS*)(tile + 1024 * c);
+        for (int j = 0; j < 2; ++j) qf[j] = *(const i32x4 LDS_AS*)((const uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + lane * 16);
+        read_step(0);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) kr[j] = *(const i32x4 LDS_AS*)(tile + 1024 * (4 + j));
-          ks = *(const i32x4 LDS_AS*)(raw + kRawScale + ((tt_own + i) * 16 + li) * 16);
+        for (int i = 0; i < Sh::kTiles; ++i) {
+          s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
 #pragma unroll
-          for (int c = 0; c < 4; ++c) ks[c] = (int)((uint32_t)ks[c] >> (8 * g));  // the MFMA takes the low byte
-        } else {
+        for (int st = 0; st < 6; ++st) {
+          if (st < 5) read_step(st + 1);
+          if (st == 1) code_in(0);
+          if (st < 2) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) kc[c] = cur.code[c];
-          kr[0] = cur.rope[0];
-          kr[1] = cur.rope[1];
+            for (int i = 0; i < Sh::kTiles; ++i) s[i] = mfma_bf16(kf[st & 1][i], qf[st], s[i]);
+          } else {
+            int sc[Sh::kTiles];
+#pragma unroll
+            for (int i = 0; i < Sh::kTiles; ++i) sc[i] = (int)(ks[st & 1][i] >> (8 * g));  // the low byte counts
+#pragma unroll
+            for (int i = 0; i < Sh::kTiles; ++i) s[i] = score(st - 2, kf[st & 1][i], qh, s[i], sc[i], qs_hi);
+#pragma unroll
+            for (int i = 0; i < Sh::kTiles; ++i) s[i] = score(st - 2, kf[st & 1][i], ql, s[i], sc[i], qs_lo);
+            widen_word((st - 2) >> 1, 2 * (st & 1));
+            widen_word((st - 2) >> 1, 2 * (st & 1) + 1);
+            if (st == 3) code_in(1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int i = 0; i < Sh::kTiles; ++i) s[i] *= scale_log2;
+      } else {
+        int ks_own = 0;  // the scale bytes of blocks g, 4 + g, 8 + g, 12 + g
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          ks_own |= (int)((((uint32_t)cur.scale[c] >> (8 * g)) & 0xFF) << (8 * c));
+          code_in(c);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) widen_word(c, i);
         }
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, l = a;
-        a = mfma_bf16(kr[0], qr[0], a);
-        l = score<0, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
-        a = mfma_bf16(kr[1], qr[1], a);
-        l = score<1, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
-        a = score<0, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
-        l = score<2, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
-        a = score<1, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
-        l = score<3, kRaw>(kc, ql, l, ks, ks_own, qs_lo);
-        a = score<2, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
-        a = score<3, kRaw>(kc, qh, a, ks, ks_own, qs_hi);
-        s[i] = (a + l) * p.scale_log2;
+        a = mfma_bf16(cur.rope[0], qr[0], a);
+        l = mfma_scaled<0, 0>(cur.code[0], ql[0], l, ks_own, qs_lo);
+        a = mfma_bf16(cur.rope[1], qr[1], a);
+        l = mfma_scaled<1, 1>(cur.code[1], ql[1], l, ks_own, qs_lo);
+        a = mfma_scaled<0, 0>(cur.code[0], qh[0], a, ks_own, qs_hi);
+        l = mfma_scaled<2, 2>(cur.code[2], ql[2], l, ks_own, qs_lo);
+        a = mfma_scaled<1, 1>(cur.code[1], qh[1], a, ks_own, qs_hi);
+        l = mfma_scaled<3, 3>(cur.code[3], ql[3], l, ks_own, qs_lo);
+        a = mfma_scaled<2, 2>(cur.code[2], qh[2], a, ks_own, qs_hi);
+        a = mfma_scaled<3, 3>(cur.code[3], qh[3], a, ks_own, qs_hi);
+        s[0] = (a + l) * scale_log2;
       }
       const bool ragged = tok_k + T > tok1 || tok_k + T > lim_min;
       if (SPARSE || ragged) {  // uniform
+        const int lim = lim_sh[wave][li];
 #pragma unroll
         for (int i = 0; i < Sh::kTiles; ++i)
 #pragma unroll
@@ -529,31 +567,40 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       }
       lds_barrier();
       // ---- 4. output dims 128 * wave .. + 127 of all rows
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        if (__builtin_amdgcn_readfirstlane(moved_sh[r])) {  // uniform
-          const float al = alpha_sh[r][li];
-#pragma unroll
-          for (int d = 0; d < 8; ++d) o[d][r] *= al;
-        }
-      }
       // V^T reads: token 4g + li/4, dims 128 * wave + 16d + 4 * (li % 4): the window's chunk 2d + (li/2) % 2
       const int ln = lane_id<(RT > 1)>(), rv = 4 * (ln >> 4) + ((ln & 15) >> 2);
       const int v_read = rv * 1024 + wave * 256 + ((((ln >> 1) & 1) ^ swz(rv)) << 4) + ((ln & 1) << 3);
+      auto read_v = [&](int ks, int d) __attribute__((always_inline)) {
+        const uint8_t LDS_AS* src = v_lds + (v_read ^ (32 * d)) + ks * 32768;
+        const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)src));
+        const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(src + 16384)));
+        return i32x4{lo[0], lo[1], hi[0], hi[1]};
+      };
+      const uint32_t moves = *(const uint32_t LDS_AS*)(const uint8_t LDS_AS*)moved_sh;  // a byte a row tile
+      i32x4 pb[T / 32][RT], va[3];
 #pragma unroll
-      for (int ks = 0; ks < T / 32; ++ks) {
-        i32x4 pb[RT];
+      for (int ks = 0; ks < T / 32; ++ks)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) pb[r] = *(const i32x4 LDS_AS*)(p_lds + ((r * (T / 32) + ks) * 64 + ln) * 16);
+        for (int r = 0; r < RT; ++r) pb[ks][r] = *(const i32x4 LDS_AS*)(p_lds + ((r * (T / 32) + ks) * 64 + ln) * 16);
+      va[0] = read_v(0, 0);
+      va[1] = read_v(0, 1);
+      const uint32_t any = __builtin_amdgcn_readfirstlane(moves);
+      if (any & (0xFFFFFFFFu >> (32 - 8 * RT))) {  // uniform, rare
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const uint8_t LDS_AS* src = v_lds + (v_read ^ (32 * d)) + ks * 32768;
-          const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)src));
-          const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(src + 16384)));
-          const i32x4 va = {lo[0], lo[1], hi[0], hi[1]};
+        for (int r = 0; r < RT; ++r) {
+          if ((any >> (8 * r)) & 0xFF) {  // uniform
+            const float al = alpha_sh[r][ln & 15];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) o[d][r] = mfma_bf16(va, pb[r], o[d][r]);
+            for (int d = 0; d < 8; ++d) o[d][r] *= al;
+          }
         }
+      }
+#pragma unroll
+      for (int n = 0; n < T / 4; ++n) {  // (ks, d) = (n / 8, n % 8), two V^T fragments ahead
+        if (n + 2 < T / 4) va[(n + 2) % 3] = read_v((n + 2) / 8, (n + 2) % 8);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) o[n % 8][r] = mfma_bf16(va[n % 3], pb[n / 8][r], o[n % 8][r]);
+        __builtin_amdgcn_sched_barrier(0);
       }
       if constexpr (!kRaw) lds_barrier();  // V, P and the words of this stage are free
     }
@@ -561,6 +608,9 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 
     // ---- the rows' sums from the waves that scored them
     const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
+    ArgParams& e = params_here();
+    const int slot0 = e.splits[b];
+    const bool single = e.splits[b + 1] - slot0 == 1;
     l_rnd = row_sum(l_rnd);
     l_exact = row_sum(l_exact);
     sum_sh[wave][0][li] = l_rnd;
@@ -575,12 +625,12 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       // decodes do; its partials carry the NaN, which the merge turns into the same.
       const float lse2 = x == 0.f ? -INFINITY : m_ref + __log2f(x);
       const int row = row0 + 16 * rt_own + li;
-      if (row < p.rows && g == 0) {
+      if (row < e.rows && g == 0) {
         if (single) {
-          const int sq = row / p.heads, h = row - sq * p.heads;
-          if (p.lse != nullptr) p.lse[((int64_t)b * p.heads + h) * p.s_q + sq] = x > 0.f ? lse2 * kLn2 : -INFINITY;
+          const int sq = row / e.heads, h = row - sq * e.heads;
+          if (e.lse != nullptr) e.lse[((int64_t)b * e.heads + h) * e.s_q + sq] = x > 0.f ? lse2 * kLn2 : -INFINITY;
         } else {
-          p.ws_lse[slot * p.rows + row] = lse2;
+          e.ws_lse[slot * e.rows + row] = lse2;
         }
       }
     }
@@ -592,9 +642,9 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int row = row0 + 16 * r + li;
       if (single) {
-        if (row < p.rows) {
-          const int sq = row / p.heads, h = row - sq * p.heads;
-          uint16_t* dst = p.out + ((int64_t)b * p.o_sb + (int64_t)sq * p.o_ss + (int64_t)h * p.o_sh) + 128 * wave + 4 * g;
+        if (row < e.rows) {
+          const int sq = row / e.heads, h = row - sq * e.heads;
+          uint16_t* dst = e.out + ((int64_t)b * e.o_sb + (int64_t)sq * e.o_ss + (int64_t)h * e.o_sh) + 128 * wave + 4 * g;
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
             const f32x4 v = o[d][r] * inv;
@@ -608,16 +658,16 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 #pragma unroll
           for (int j = 0; j < 4; ++j) am = fmaxf(am, fabsf(o[d][r][j]));
         am = row_max(am * inv);
-        int e = 15 - __builtin_amdgcn_frexp_expf(am);
-        e = e < 127 ? e : 127;
-        if (row < p.rows) {
-          uint16_t* dst = p.ws_o + (slot * p.rows + row) * kDV + 128 * wave + 4 * g;
+        int ex = 15 - __builtin_amdgcn_frexp_expf(am);
+        ex = ex < 127 ? ex : 127;
+        if (row < e.rows) {
+          uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 128 * wave + 4 * g;
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
-            const f32x4 v = (o[d][r] * inv) * exp2i(e);
+            const f32x4 v = (o[d][r] * inv) * exp2i(ex);
             *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_f16(v[0], v[1]), (int)pack_f16(v[2], v[3])};
           }
-          if (g == 0) p.ws_scale[(slot * p.rows + row) * 4 + wave] = exp2i(-e);
+          if (g == 0) e.ws_scale[(slot * e.rows + row) * 4 + wave] = exp2i(-ex);
         }
       }
     }
