@@ -122,9 +122,10 @@ __device__ __forceinline__ f32x4 score(int c, i32x4 k, const i32x8 (&q)[4], f32x
 }
 
 // V in LDS: token t of a tile of 16 is a row of 1 KiB; its 16-byte chunk k sits at slot k ^ swz(t) of the
-// 256-byte window it is in, which keeps the conversions' 16-byte writes (16 tokens, one chunk) and the
-// transposed reads (16 tokens, 32 bytes) free of bank conflicts.
-__device__ __forceinline__ int swz(int t) { return ((t & 7) << 1) | ((t >> 3) & 1); }
+// 256-byte window it is in.  The conversions' 16-byte writes go eight lanes (tokens, one chunk) at a time over
+// 128 bytes, so swz's low three bits tell eight tokens apart; the transposed reads go 32 lanes (eight tokens, 32
+// bytes) at a time over 256, so its high three bits do too.  (A swizzle for the reads alone wrote at half rate.)
+__device__ __forceinline__ int swz(int t) { return ((t & 3) << 1) | ((t >> 2) & 1) * 9; }
 
 // Eight codes (one dword) to bf16 times 2^(byte - 127), the byte given as the exponent of a float.
 __device__ __forceinline__ i32x4 widen8(int w, float scale) {
