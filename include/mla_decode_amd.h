@@ -182,8 +182,8 @@ int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, 
 
 /*
  * mla_num_parts for a cache of format kv_format: the 4-bit decode is laid out for two workgroups of 16, 32 or
- * 64 query rows per compute unit, the other formats as mla_num_parts says.  Any schedule is decoded right;
- * this one fills the GPU.
+ * 64 query rows per compute unit, or one of 128, the other formats as mla_num_parts says.  Any schedule is
+ * decoded right; this one fills the GPU.
  */
 int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format);
 

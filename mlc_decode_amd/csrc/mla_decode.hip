@@ -4193,10 +4193,11 @@ int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads
   const int parts = mla_num_parts(batch, s_q, heads_q, heads_k, cu_count);
   if (parts < 0 || kv_format != MLA_KV_FP4_E2M1) return parts;
   const int64_t rows = (int64_t)s_q * heads_q;
-  const int R = mla4::rows_per_workgroup(rows < 65536 ? (int)rows : 65536);
+  const int r = rows < 65536 ? (int)rows : 65536;
+  const int R = mla4::rows_per_workgroup(r);
   const int64_t row_blocks = (rows + R - 1) / R;
   const int cus = cu_count > 0 ? cu_count : cu_count_current();
-  const int64_t n = (int64_t)cus * mla4::kWorkgroupsPerCu / row_blocks;
+  const int64_t n = (int64_t)cus * mla4::workgroups_per_cu(r) / row_blocks;
   return n < 1 ? 1 : (int)n;
 }
 

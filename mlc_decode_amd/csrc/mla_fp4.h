@@ -34,7 +34,7 @@ struct DecodeParams {
 
 // Query rows per workgroup for `rows` = s_q * heads rows, and workgroups per compute unit.
 int rows_per_workgroup(int rows);
-constexpr int kWorkgroupsPerCu = 2;
+int workgroups_per_cu(int rows);
 
 hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st);
 

@@ -21,6 +21,7 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "mla_decode_amd.h"
 #include "mla_fp4.h"
@@ -222,8 +223,133 @@ __device__ __forceinline__ ArgParams& params_here() {
   return *(ArgParams*)(a + kArgOffset);
 }
 
+// Workgroups go to the eight XCDs in turn: the row blocks of a part, which read the same pages, take
+// consecutive turns on one XCD and find them in its L2.
+__device__ __forceinline__ void place_workgroup(int row_blocks, int num_parts, int& part, int& rb) {
+  part = blockIdx.x;
+  rb = 0;
+  if (row_blocks > 1) {
+    if ((num_parts & 7) == 0) {
+      const int turn = blockIdx.x >> 3;
+      rb = turn % row_blocks;
+      part = (turn / row_blocks) * 8 + (blockIdx.x & 7);
+    } else {
+      rb = blockIdx.x % row_blocks;
+      part = blockIdx.x / row_blocks;
+    }
+  }
+}
+
+// The tokens [tok0, tok1) of sequence b that a part takes from `page` on, L the sequence's length.
+struct Segment {
+  int L, tok0, tok1;
+};
+template <bool SPARSE>
+__device__ __forceinline__ Segment segment_of(ArgParams& p, int b, int page, int end_b, int end_page) {
+  int L = SPARSE ? p.topk : p.seqlens[b];
+  L = L > 0 ? L : 0;
+  if (!SPARSE && L > (int64_t)p.bt_width * kPageTokens) {  // uniform: cut to the table
+    L = p.bt_width * kPageTokens;
+    if (p.status != nullptr) *p.status = 1;
+  }
+  const int np = pages_of(L);
+  int stop = b == end_b ? end_page : np;
+  stop = stop < np ? stop : np;
+  return Segment{L, page * kPageTokens, stop * kPageTokens < L ? stop * kPageTokens : L};
+}
+
+// The page id in column `at` of sequence b's table row, clamped into the pool: a scalar load.
+template <bool SPARSE>
+__device__ __forceinline__ int page_at(ArgParams& p, int b, int at) {
+  if constexpr (SPARSE) return 0;
+  const int last = p.bt_width - 1;
+  const auto table = (const int32_t __attribute__((address_space(4)))*)p.block_table;
+  const int v = table[(int64_t)b * p.bt_stride + (at < last ? at : last)];
+  return v < 0 ? 0 : (v >= p.num_blocks ? p.num_blocks - 1 : v);
+}
+
+// Where token t of a segment is: row t % 64 of page pg, or the pool token that the segment's index list idx[0 .. n)
+// names (an index that names none, and a t past the list, read a token that is masked later).
+struct Row {
+  const uint8_t* codes;
+  const uint8_t* scale;
+  const uint8_t* rope;
+};
+template <bool SPARSE>
+__device__ __forceinline__ Row row_at(ArgParams& p, int t, int64_t pg, const int32_t* idx, int n) {
+  int row = t & 63;
+  if constexpr (SPARSE) {
+    const int id = idx[t < n ? t : n - 1];
+    const int64_t at = id >= 0 && id < p.pool_tokens ? id : 0;
+    pg = at >> 6;
+    row = (int)(at & 63);
+  }
+  return Row{p.codes + pg * p.c_sp + (uint32_t)(row * (int)p.c_st), p.scale + pg * p.s_sp + (uint32_t)(row * (int)p.s_st),
+             (const uint8_t*)(p.rope + pg * p.r_sp + (uint32_t)(row * (int)p.r_st))};
+}
+// Whether token t of a segment of n names no key (t < n, sparse), or is past the segment.
+template <bool SPARSE>
+__device__ __forceinline__ bool no_key(ArgParams& p, int t, const int32_t* idx, int n) {
+  if constexpr (SPARSE) {
+    const int id = idx[t < n ? t : n - 1];
+    return t >= n || id < 0 || id >= p.pool_tokens;
+  }
+  return t >= n;
+}
+
+// The power of two that brings a chunk of a split's partial with this largest value into [2^14, 2^15).
+__device__ __forceinline__ int part_exp(float amax) {
+  const int e = 15 - __builtin_amdgcn_frexp_expf(amax);
+  return e < 127 ? e : 127;
+}
+// A row's lse from its reference m (log2) and the sum x of its weights; a row without a key has x = 0.  A NaN row (a NaN
+// block, or a NaN in its query) reports lse -inf beside its NaN output, as the 16-bit and fp8 decodes do; its
+// partials carry the NaN, which the merge turns into the same.
+__device__ __forceinline__ void write_lse(ArgParams& p, int b, int row, int g, int64_t slot, bool single, float m, float x) {
+  if (row >= p.rows || g != 0) return;
+  const float lse2 = x == 0.f ? -INFINITY : m + __log2f(x);
+  if (single) {
+    const int sq = row / p.heads, h = row - sq * p.heads;
+    if (p.lse != nullptr) p.lse[((int64_t)b * p.heads + h) * p.s_q + sq] = x > 0.f ? lse2 * kLn2 : -INFINITY;
+  } else {
+    p.ws_lse[slot * p.rows + row] = lse2;
+  }
+}
+
+// The queries of a lane's row (rows past the last load the last, and are never written).
+struct Query {
+  i32x8 hi[4], lo[4];
+  i32x4 rope[2];
+  int scale_hi, scale_lo;  // a byte a chunk
+  int lim;                 // the row sees tokens below it
+};
+__device__ __forceinline__ Query load_query(ArgParams& p, int b, int row, int L, int lane) {
+  Query q;
+  const int g = lane >> 4, li = lane & 15;
+  row = row < p.rows ? row : p.rows - 1;
+  const int tok = row / p.heads;
+  const int h = row - tok * p.heads;
+  const uint16_t* qn = p.q_nope + ((int64_t)b * p.q_sb + (int64_t)tok * p.q_ss + (int64_t)h * p.q_sh);
+  const uint16_t* qp = p.q_rope + ((int64_t)b * p.qr_sb + (int64_t)tok * p.qr_ss + (int64_t)h * p.qr_sh);
+  q.scale_hi = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint16_t* src = qn + 128 * c + 16 * g;
+    const i32x4 v[4] = {*(const i32x4*)src, *(const i32x4*)(src + 8), *(const i32x4*)(src + 64), *(const i32x4*)(src + 72)};
+    const QuerySplit r = split_query(v, g, li);
+    q.hi[c] = r.hi;
+    q.lo[c] = r.lo;
+    q.scale_hi |= r.scale << (8 * c);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) q.rope[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
+  q.scale_lo = q.scale_hi - 0x0A0A0A0A;  // every byte is 11 at least
+  q.lim = L - (p.causal ? p.s_q - 1 - tok : 0);
+  return q;
+}
+
 template <int RT, bool SPARSE>
-__global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const int32_t* __restrict__ sched, int row_blocks,
+__global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restrict__ sched, int row_blocks,
                                                                        int num_parts, DecodeParams) {
   static_assert(alignof(DecodeParams) == 8 && kArgOffset % 8 == 0, "the struct's place among the arguments");
   using Sh = Shape<RT>;
@@ -240,19 +366,8 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
   __shared__ int lim_sh[4][16];
   __shared__ int32_t idx_sh[SPARSE ? MLA_SPARSE_MAX_TOPK : 1];
 
-  // Workgroups go to the eight XCDs in turn: the row blocks of a part, which read the same pages, take
-  // consecutive turns on one XCD and find them in its L2.
-  int part = blockIdx.x, rb = 0;
-  if (row_blocks > 1) {
-    if ((num_parts & 7) == 0) {
-      const int turn = blockIdx.x >> 3;
-      rb = turn % row_blocks;
-      part = (turn / row_blocks) * 8 + (blockIdx.x & 7);
-    } else {
-      rb = blockIdx.x % row_blocks;
-      part = blockIdx.x / row_blocks;
-    }
-  }
+  int part, rb;
+  place_workgroup(row_blocks, num_parts, part, rb);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rt_own = wave % RT;                               // the row tile this wave scores
   const int tt_load = RT == 1 ? wave : (wave & 1);            // the token tile it loads
@@ -273,17 +388,8 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
   for (; b < batch; ++b, page = 0, split = 0) {
     if (!(b < end_b || (b == end_b && page < end_page))) break;
     ArgParams& p = params_here();
-    int L = SPARSE ? p.topk : p.seqlens[b];
-    L = L > 0 ? L : 0;
-    if (!SPARSE && L > (int64_t)p.bt_width * kPageTokens) {  // uniform: cut to the table
-      L = p.bt_width * kPageTokens;
-      if (p.status != nullptr) *p.status = 1;
-    }
-    const int np = pages_of(L);
-    int stop = b == end_b ? end_page : np;
-    stop = stop < np ? stop : np;
-    const int tok0 = page * kPageTokens;                                            // the segment's tokens
-    const int tok1 = stop * kPageTokens < L ? stop * kPageTokens : L;
+    const Segment seg = segment_of<SPARSE>(p, b, page, end_b, end_page);
+    const int L = seg.L, tok0 = seg.tok0, tok1 = seg.tok1;
     const int nst = tok1 > tok0 ? (tok1 - tok0 + T - 1) / T : 0;
 
     if constexpr (SPARSE) {
@@ -291,33 +397,8 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       lds_barrier();
     }
 
-    // ---- the page of stage k, clamped into the pool; read by a scalar load a stage before it is used
-    auto page_of = [&](int k) __attribute__((always_inline)) {
-      if constexpr (SPARSE) return 0;
-      const int at = page + k * T / kPageTokens, last = p.bt_width - 1;
-      const auto table = (const int32_t __attribute__((address_space(4)))*)p.block_table;
-      const int v = table[(int64_t)b * p.bt_stride + (at < last ? at : last)];
-      return v < 0 ? 0 : (v >= p.num_blocks ? p.num_blocks - 1 : v);
-    };
-
-    // where token t of the segment is
-    struct Row {
-      const uint8_t* codes;
-      const uint8_t* scale;
-      const uint8_t* rope;
-    };
-    auto row_of = [&](int t, int64_t pg) __attribute__((always_inline)) {
-      int row = t & 63;
-      if constexpr (SPARSE) {
-        const int n = tok1 - tok0;
-        const int id = idx_sh[t < n ? t : n - 1];
-        const int64_t at = id >= 0 && id < p.pool_tokens ? id : 0;
-        pg = at >> 6;
-        row = (int)(at & 63);
-      }
-      return Row{p.codes + pg * p.c_sp + (uint32_t)(row * (int)p.c_st), p.scale + pg * p.s_sp + (uint32_t)(row * (int)p.s_st),
-                 (const uint8_t*)(p.rope + pg * p.r_sp + (uint32_t)(row * (int)p.r_st))};
-    };
+    auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
+    auto row_of = [&](int t, int pg) __attribute__((always_inline)) { return row_at<SPARSE>(p, t, pg, idx_sh, tok1 - tok0); };
     auto load_stage = [&](int k, int pg, Stage& s) __attribute__((always_inline)) {  // RT == 1
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       const Row r = row_of(k * T + 16 * tt_load + li, pg);
@@ -352,37 +433,15 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
         load_stage(0, pg, nxt);
     }
 
-    // ---- queries of row tile rt_own; rows past the last re-load it, and are never written
-    i32x8 qh[4], ql[4];
-    i32x4 qr[2];
-    int qs_hi = 0, qtok;
-    {
-      const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
-      int row = row0 + 16 * rt_own + li;
-      row = row < p.rows ? row : p.rows - 1;
-      qtok = row / p.heads;
-      const int h = row - qtok * p.heads;
-      const uint16_t* qn = p.q_nope + ((int64_t)b * p.q_sb + (int64_t)qtok * p.q_ss + (int64_t)h * p.q_sh);
-      const uint16_t* qp = p.q_rope + ((int64_t)b * p.qr_sb + (int64_t)qtok * p.qr_ss + (int64_t)h * p.qr_sh);
+    const int ql_lane = lane_id<(RT > 1)>();
+    Query q = load_query(p, b, row0 + 16 * rt_own + (ql_lane & 15), L, ql_lane);
+    if constexpr (kRaw) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint16_t* src = qn + 128 * c + 16 * g;
-        const i32x4 v[4] = {*(const i32x4*)src, *(const i32x4*)(src + 8), *(const i32x4*)(src + 64), *(const i32x4*)(src + 72)};
-        const QuerySplit r = split_query(v, g, li);
-        qh[c] = r.hi;
-        ql[c] = r.lo;
-        qs_hi |= r.scale << (8 * c);
-      }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        qr[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
-        if constexpr (kRaw) *(i32x4 LDS_AS*)((uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + lane * 16) = qr[j];
-      }
+      for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)((uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + ql_lane * 16) = q.rope[j];
+    } else {  // used here once: the wait for them is not left to the stage loop
+      asm volatile("" : "+v"(q.rope[0]), "+v"(q.rope[1]));
     }
-    const int qs_lo = qs_hi - 0x0A0A0A0A;  // every byte is 11 at least
-    // used here once: the wait for them is not left to the stage loop
-    if constexpr (!kRaw) asm volatile("" : "+v"(qr[0]), "+v"(qr[1]));
-    lim_sh[wave][lane_id<(RT > 1)>() & 15] = L - (p.causal ? p.s_q - 1 - qtok : 0);  // the row sees tokens below it
+    lim_sh[wave][ql_lane & 15] = q.lim;
     const int lim_min = L - (p.causal ? p.s_q - 1 : 0);     // every row sees those below it
 
     f32x4 o[8][RT];
@@ -410,17 +469,8 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       // ---- 1. the wave's tokens to bf16 in LDS.  Tokens that do not exist become zeros: their weight is
       // zero, and what their rows hold must not make 0 * NaN of it.
-      const bool cut = SPARSE || tok_k + T > L;  // uniform
-      bool gone = false;
-      if (cut) {
-        const int t = tok_k + 16 * tt_load + li;
-        gone = t >= L;
-        if constexpr (SPARSE) {
-          const int i = t - tok0, n = tok1 - tok0;
-          const int id = idx_sh[i < n ? i : n - 1];
-          gone = i >= n || id < 0 || id >= p.pool_tokens;
-        }
-      }
+      const bool cut = SPARSE || tok_k + T > tok1;  // uniform
+      const bool gone = cut && no_key<SPARSE>(p, tok_k + 16 * tt_load + li - tok0, idx_sh, tok1 - tok0);
       i32x4 code;  // chunk c of the token (c_load + c of its 128-dim chunks)
       float scale = 0.f;
       auto code_in = [&](int c) __attribute__((always_inline)) {
@@ -479,9 +529,9 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 #pragma unroll
             for (int i = 0; i < Sh::kTiles; ++i) sc[i] = (int)(ks[st & 1][i] >> (8 * g));  // the low byte counts
 #pragma unroll
-            for (int i = 0; i < Sh::kTiles; ++i) s[i] = score(st - 2, kf[st & 1][i], qh, s[i], sc[i], qs_hi);
+            for (int i = 0; i < Sh::kTiles; ++i) s[i] = score(st - 2, kf[st & 1][i], q.hi, s[i], sc[i], q.scale_hi);
 #pragma unroll
-            for (int i = 0; i < Sh::kTiles; ++i) s[i] = score(st - 2, kf[st & 1][i], ql, s[i], sc[i], qs_lo);
+            for (int i = 0; i < Sh::kTiles; ++i) s[i] = score(st - 2, kf[st & 1][i], q.lo, s[i], sc[i], q.scale_lo);
             widen_word((st - 2) >> 1, 2 * (st & 1));
             widen_word((st - 2) >> 1, 2 * (st & 1) + 1);
             if (st == 3) code_in(1);
@@ -500,16 +550,16 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
           for (int i = 0; i < 4; ++i) widen_word(c, i);
         }
         f32x4 a = {0.f, 0.f, 0.f, 0.f}, l = a;
-        a = mfma_bf16(cur.rope[0], qr[0], a);
-        l = mfma_scaled<0, 0>(cur.code[0], ql[0], l, ks_own, qs_lo);
-        a = mfma_bf16(cur.rope[1], qr[1], a);
-        l = mfma_scaled<1, 1>(cur.code[1], ql[1], l, ks_own, qs_lo);
-        a = mfma_scaled<0, 0>(cur.code[0], qh[0], a, ks_own, qs_hi);
-        l = mfma_scaled<2, 2>(cur.code[2], ql[2], l, ks_own, qs_lo);
-        a = mfma_scaled<1, 1>(cur.code[1], qh[1], a, ks_own, qs_hi);
-        l = mfma_scaled<3, 3>(cur.code[3], ql[3], l, ks_own, qs_lo);
-        a = mfma_scaled<2, 2>(cur.code[2], qh[2], a, ks_own, qs_hi);
-        a = mfma_scaled<3, 3>(cur.code[3], qh[3], a, ks_own, qs_hi);
+        a = mfma_bf16(cur.rope[0], q.rope[0], a);
+        l = mfma_scaled<0, 0>(cur.code[0], q.lo[0], l, ks_own, q.scale_lo);
+        a = mfma_bf16(cur.rope[1], q.rope[1], a);
+        l = mfma_scaled<1, 1>(cur.code[1], q.lo[1], l, ks_own, q.scale_lo);
+        a = mfma_scaled<0, 0>(cur.code[0], q.hi[0], a, ks_own, q.scale_hi);
+        l = mfma_scaled<2, 2>(cur.code[2], q.lo[2], l, ks_own, q.scale_lo);
+        a = mfma_scaled<1, 1>(cur.code[1], q.hi[1], a, ks_own, q.scale_hi);
+        l = mfma_scaled<3, 3>(cur.code[3], q.lo[3], l, ks_own, q.scale_lo);
+        a = mfma_scaled<2, 2>(cur.code[2], q.hi[2], a, ks_own, q.scale_hi);
+        a = mfma_scaled<3, 3>(cur.code[3], q.hi[3], a, ks_own, q.scale_hi);
         s[0] = (a + l) * scale_log2;
       }
       const bool ragged = tok_k + T > tok1 || tok_k + T > lim_min;
@@ -520,11 +570,7 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int t = tok_k + 16 * (tt_own + i) + 4 * g + j;
-            bool see = t < tok1 && t < lim;
-            if constexpr (SPARSE) {
-              const int id = idx_sh[t < tok1 ? t - tok0 : 0];
-              see = t < tok1 && id >= 0 && id < p.pool_tokens;
-            }
+            const bool see = t < lim && !no_key<SPARSE>(p, t - tok0, idx_sh, tok1 - tok0);
             s[i][j] = see ? s[i][j] : -INFINITY;
           }
       }
@@ -622,18 +668,7 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
       float x = 0.f;
 #pragma unroll
       for (int w = 0; w < Sh::kShare; ++w) x += sum_sh[w * RT + rt_own][1][li];
-      // A NaN row (a NaN block, or one in its query) reports lse -inf beside its NaN output, as the 16-bit and fp8
-      // decodes do; its partials carry the NaN, which the merge turns into the same.
-      const float lse2 = x == 0.f ? -INFINITY : m_ref + __log2f(x);
-      const int row = row0 + 16 * rt_own + li;
-      if (row < e.rows && g == 0) {
-        if (single) {
-          const int sq = row / e.heads, h = row - sq * e.heads;
-          if (e.lse != nullptr) e.lse[((int64_t)b * e.heads + h) * e.s_q + sq] = x > 0.f ? lse2 * kLn2 : -INFINITY;
-        } else {
-          e.ws_lse[slot * e.rows + row] = lse2;
-        }
-      }
+      write_lse(e, b, row0 + 16 * rt_own + li, g, slot, single, m_ref, x);
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -659,8 +694,7 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
 #pragma unroll
           for (int j = 0; j < 4; ++j) am = fmaxf(am, fabsf(o[d][r][j]));
         am = row_max(am * inv);
-        int ex = 15 - __builtin_amdgcn_frexp_expf(am);
-        ex = ex < 127 ? ex : 127;
+        const int ex = part_exp(am);
         if (row < e.rows) {
           uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 128 * wave + 4 * g;
 #pragma unroll
@@ -676,7 +710,309 @@ __global__ __launch_bounds__(256, kWorkgroupsPerCu) void mla_fp4_kernel(const in
   }
 }
 
-int rows_per_workgroup(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+// 128 query rows: eight waves of one workgroup per CU, wave w scoring row tile w against both token tiles of a
+// 32-token stage and accumulating output dims 64w .. 64w + 63 of all rows.  One barrier a stage: while a
+// wave scores stage k and converts its share of V, P^T and V of stage k - 1 lie in the other half of two
+// buffers, and their product is interleaved with the softmax of stage k, so that the matrix unit works
+// through it.  V is converted once for 128 rows.  (Two 64-row workgroups a CU, which hide one's softmax
+// behind the other only by chance: 64 x 128 heads x 4096 tokens 97 us against 86 here, 32 x 2 x 128 x 16384 303 against 256.)
+template <bool SPARSE>
+__global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __restrict__ sched, int row_blocks, int num_parts,
+                                                              DecodeParams) {
+  constexpr int T = 32, RT = 8, W = 8;
+  __shared__ __attribute__((aligned(1024))) uint8_t v_sh[2][T * 1024];
+  __shared__ __attribute__((aligned(16))) uint8_t p_sh[2][RT * 1024];  // [row tile][lane][16 bytes]
+  __shared__ __attribute__((aligned(16))) uint8_t raw_sh[2 * kRawStage];
+  __shared__ __attribute__((aligned(16))) uint8_t qr_sh[W * 2048];  // the waves' rope queries, in operand order
+  __shared__ float alpha_sh[2][RT][16];
+  __shared__ __attribute__((aligned(8))) uint8_t moved_sh[2][RT];  // row tile's reference moved in the stage
+  __shared__ float sum_sh[RT][16];
+  __shared__ float amax_sh[W][RT][16];
+  __shared__ int lim_sh[W][16];
+  __shared__ int32_t idx_sh[SPARSE ? MLA_SPARSE_MAX_TOPK : 1];
+
+  int part, rb;
+  place_workgroup(row_blocks, num_parts, part, rb);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tt_load = wave & 1, c_load = wave >> 1;  // the token tile and 128-dim chunk it copies and converts
+  const int row0 = rb * 16 * RT;
+  uint8_t LDS_AS* const v_lds = (uint8_t LDS_AS*)&v_sh[0][0];
+  uint8_t LDS_AS* const p_lds = (uint8_t LDS_AS*)&p_sh[0][0];
+  uint8_t LDS_AS* const raw_lds = (uint8_t LDS_AS*)raw_sh;
+  uint8_t LDS_AS* const qr_lds = (uint8_t LDS_AS*)qr_sh + wave * 2048;
+
+  const int32_t* rec = sched + (int64_t)part * kSchedWords;
+  int b = rec[0], page = rec[1], split = rec[4];
+  const int end_b = rec[2], end_page = rec[3];
+  const int batch = params_here().batch;
+#pragma unroll 1
+  for (; b < batch; ++b, page = 0, split = 0) {
+    if (!(b < end_b || (b == end_b && page < end_page))) break;
+    ArgParams& p = params_here();
+    const Segment seg = segment_of<SPARSE>(p, b, page, end_b, end_page);
+    const int tok0 = seg.tok0, tok1 = seg.tok1;
+    const int nst = tok1 > tok0 ? (tok1 - tok0 + T - 1) / T : 0;
+    if constexpr (SPARSE) {
+      for (int i = threadIdx.x; i < tok1 - tok0; i += 64 * W) idx_sh[i] = p.indices[(int64_t)b * p.idx_stride + tok0 + i];
+      lds_barrier();
+    }
+    auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
+    // waves 0 .. 7 a code fragment each, 0 .. 3 one of rope, 4 and 5 a tile's scale bytes
+    auto copy_stage = [&](int k, int pg) __attribute__((always_inline)) {
+      const int lane = lane_id<true>(), g = lane >> 4, li = lane & 15;
+      const Row r = row_at<SPARSE>(p, k * T + 16 * tt_load + li, pg, idx_sh, tok1 - tok0);
+      const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)raw_lds + (k & 1) * kRawStage);
+      const uint32_t tile = base + tt_load * kRawTile;
+      copy16(r.codes + 64 * c_load + 16 * g, tile + 1024 * c_load);
+      if (wave < 4) copy16(r.rope + 64 * (wave >> 1) + 16 * g, tile + 1024 * (4 + (wave >> 1)));  // uniform
+      if ((wave >> 1) == 2) {  // uniform: a dword of scales a lane, four lanes a token
+        const Row w = row_at<SPARSE>(p, k * T + 16 * tt_load + (lane >> 2), pg, idx_sh, tok1 - tok0);
+        copy4(w.scale + 4 * (lane & 3), base + kRawScale + 256 * tt_load);
+      }
+    };
+    int pg_next = 0;
+    if (nst > 0) {
+      const int pg = page_of(0);
+      pg_next = page_of(nst > 1 ? 1 : 0);
+      copy_stage(0, pg);
+    }
+    i32x8 qh[4], ql[4];
+    int qs_hi, qs_lo;
+    {
+      const int lane = lane_id<true>();
+      const Query q = load_query(p, b, row0 + 16 * wave + (lane & 15), seg.L, lane);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) qh[c] = q.hi[c], ql[c] = q.lo[c];
+      qs_hi = q.scale_hi;
+      qs_lo = q.scale_lo;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)(qr_lds + j * 1024 + lane * 16) = q.rope[j];
+      lim_sh[wave][lane & 15] = q.lim;
+    }
+    const int lim_min = seg.L - (p.causal ? p.s_q - 1 : 0);  // every row sees the tokens below it
+    const float scale_log2 = p.scale_log2;
+
+    f32x4 o[4][RT];
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) o[d][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_ref = -INFINITY, l_rnd = 0.f, l_exact = 0.f;
+
+    // ---- S^T of stage k for row tile `wave`, and this wave's share of V of stage k
+    auto scores = [&](int k, f32x4 (&s)[2]) __attribute__((always_inline)) {
+      const int lane = lane_id<true>(), g = lane >> 4, li = lane & 15;
+      const uint8_t LDS_AS* const raw = raw_lds + (k & 1) * kRawStage;
+      const uint8_t LDS_AS* const frag = raw + lane * 16;
+      const uint8_t LDS_AS* const word = raw + kRawScale + li * 16;
+      const int t0 = k * T;  // in the segment
+      i32x4 kf[2][2], qf[2], code;
+      uint32_t ks[2][2];
+      float scale = 0.f;
+      auto read_step = [&](int st) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          kf[st & 1][i] = *(const i32x4 LDS_AS*)(frag + i * kRawTile + 1024 * (st < 2 ? 4 + st : st - 2));
+          if (st >= 2) ks[st & 1][i] = *(const uint32_t LDS_AS*)(word + i * 256 + 4 * (st - 2));
+        }
+      };
+#pragma unroll
+      for (int j = 0; j < 2; ++j) qf[j] = *(const i32x4 LDS_AS*)(qr_lds + j * 1024 + lane * 16);
+      read_step(0);
+      s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int v_at = (k & 1) * (T * 1024) + tt_load * 16384 + c_load * 256 + li * 1024 + (((4 * g) ^ swz(li)) << 4);
+#pragma unroll
+      for (int st = 0; st < 6; ++st) {
+        if (st < 5) read_step(st + 1);
+        if (st == 1) {
+          code = *(const i32x4 LDS_AS*)(frag + tt_load * kRawTile + c_load * 1024);
+          const uint32_t w = *(const uint32_t LDS_AS*)(word + tt_load * 256 + 4 * c_load);
+          scale = __uint_as_float(((w >> (8 * g)) & 0xFF) << 23);
+          if (SPARSE || tok0 + t0 + T > tok1) {  // uniform: tokens that do not exist become zeros
+            const bool gone = no_key<SPARSE>(p, t0 + 16 * tt_load + li, idx_sh, tok1 - tok0);
+            scale = gone ? 1.f : scale;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) code[j] = gone ? 0 : code[j];
+          }
+        }
+        if (st < 2) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i] = mfma_bf16(kf[st & 1][i], qf[st], s[i]);
+        } else {
+          int sc[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) sc[i] = (int)(ks[st & 1][i] >> (8 * g));  // the low byte counts
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i] = score(st - 2, kf[st & 1][i], qh, s[i], sc[i], qs_hi);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i] = score(st - 2, kf[st & 1][i], ql, s[i], sc[i], qs_lo);
+          *(i32x4 LDS_AS*)(v_lds + (v_at ^ (16 * (st - 2)))) = widen8(code[st - 2], scale);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[i] *= scale_log2;
+      if (SPARSE || tok0 + t0 + T > tok1 || tok0 + t0 + T > lim_min) {  // uniform
+        const int lim = lim_sh[wave][li];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int t = t0 + 16 * i + 4 * g + j;
+            s[i][j] = tok0 + t < lim && !no_key<SPARSE>(p, t, idx_sh, tok1 - tok0) ? s[i][j] : -INFINITY;
+          }
+      }
+    };
+
+    // ---- softmax of stage k (SOFT) in six pieces between the products P V of stage k - 1 (PV).  The reference
+    // moves without a branch: where it stays, alpha is exactly one.
+    auto weigh = [&](auto soft, auto pv, int k, f32x4 (&s)[2]) __attribute__((always_inline)) {
+      constexpr bool SOFT = decltype(soft)::value, PV = decltype(pv)::value;
+      const int ln = lane_id<true>(), was = (k & 1) ^ 1;
+      i32x4 va[4], pb[2];
+      if constexpr (PV) {
+        const i32x2 moves = *(const i32x2 LDS_AS*)(const uint8_t LDS_AS*)&moved_sh[was][0];
+        pb[0] = *(const i32x4 LDS_AS*)(p_lds + was * (RT * 1024) + ln * 16);
+        const int rv = 4 * (ln >> 4) + ((ln & 15) >> 2);
+        const int at = was * (T * 1024) + rv * 1024 + (wave >> 1) * 256 + (((8 * (wave & 1) + ((ln >> 1) & 1)) ^ swz(rv)) << 4) + ((ln & 1) << 3);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const uint8_t LDS_AS* src = v_lds + (at ^ (32 * d));
+          const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)src));
+          const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(src + 16384)));
+          va[d] = i32x4{lo[0], lo[1], hi[0], hi[1]};
+        }
+        const uint32_t m0 = __builtin_amdgcn_readfirstlane(moves[0]), m1 = __builtin_amdgcn_readfirstlane(moves[1]);
+        if (m0 | m1) {  // uniform, rare
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            if (((r < 4 ? m0 : m1) >> (8 * (r & 3))) & 0xFF) {  // uniform
+              const float al = alpha_sh[was][r][ln & 15];
+#pragma unroll
+              for (int d = 0; d < 4; ++d) o[d][r] *= al;
+            }
+          }
+        }
+      }
+      float top = 0.f, base = 0.f, alpha = 1.f, e[8];
+      bool moved = false;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        if constexpr (PV) {
+          if (r + 1 < RT) pb[(r + 1) & 1] = *(const i32x4 LDS_AS*)(p_lds + (was * RT + r + 1) * 1024 + ln * 16);
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d][r] = mfma_bf16(va[d], pb[r & 1], o[d][r]);
+        }
+        if constexpr (SOFT) {
+          if (r == 0) {
+            top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
+            top = xor16(top, false);
+          } else if (r == 1) {
+            top = xor32(top, false);
+          } else if (r == 2) {
+            const float m_old = m_ref;
+            m_ref = top > m_ref + kSlack ? top : m_ref;
+            moved = __builtin_amdgcn_ballot_w64(m_ref != m_old) != 0;
+            base = m_ref == -INFINITY ? 0.f : m_ref;
+            alpha = __builtin_amdgcn_exp2f((m_old == m_ref ? base : m_old) - base);
+          } else if (r == 3 || r == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[4 * (r - 3) + j] = __builtin_amdgcn_exp2f(s[r - 3][j] - base);
+          } else if (r == 5) {
+            const i32x4 w = {(int)pack_bf16(e[0], e[1]), (int)pack_bf16(e[2], e[3]), (int)pack_bf16(e[4], e[5]), (int)pack_bf16(e[6], e[7])};
+            *(i32x4 LDS_AS*)(p_lds + ((k & 1) * RT + wave) * 1024 + ln * 16) = w;
+            alpha_sh[k & 1][wave][ln & 15] = alpha;
+            moved_sh[k & 1][wave] = moved;
+            l_rnd *= alpha;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) l_rnd = sum2_bf16((uint32_t)w[j], l_rnd);
+          } else if (r == 6) {
+            l_exact = l_exact * alpha + ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+
+    f32x4 s[2];
+    auto next_stage = [&](int k) __attribute__((always_inline)) {
+      copies_landed();
+      lds_barrier();  // stage k is in LDS, P and V of stage k - 1 are; their buffers of stage k - 2 are free
+      if (k + 1 < nst) copy_stage(k + 1, pg_next);
+      pg_next = page_of(k + 2 < nst ? k + 2 : nst - 1);
+      scores(k, s);
+    };
+    if (nst > 0) {
+      next_stage(0);
+      weigh(yes, no, 0, s);
+#pragma unroll 1
+      for (int k = 1; k < nst; ++k) {
+        next_stage(k);
+        weigh(yes, yes, k, s);
+      }
+    }
+    const int lane = lane_id<true>(), g = lane >> 4, li = lane & 15;
+    const float l = row_sum(l_rnd), x = row_sum(l_exact);
+    sum_sh[wave][li] = l;
+    lds_barrier();
+    if (nst > 0) weigh(no, yes, nst, s);
+
+    // ---- lse of row tile `wave`, and the output dims of all
+    ArgParams& e = params_here();
+    const int slot0 = e.splits[b];
+    const bool single = e.splits[b + 1] - slot0 == 1;
+    const int64_t slot = (int64_t)slot0 + split;
+    write_lse(e, b, row0 + 16 * wave + li, g, slot, single, m_ref, x);
+    if (single) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float sum = sum_sh[r][li], inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int row = row0 + 16 * r + li;
+        if (row < e.rows) {
+          const int sq = row / e.heads, h = row - sq * e.heads;
+          uint16_t* dst = e.out + ((int64_t)b * e.o_sb + (int64_t)sq * e.o_ss + (int64_t)h * e.o_sh) + 64 * wave + 4 * g;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const f32x4 v = o[d][r] * inv;
+            *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3])};
+          }
+        }
+      }
+    } else {  // scaled fp16; a chunk of 128 dims is two waves' work
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float am = 0.f;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) am = fmaxf(am, fabsf(o[d][r][j]));
+        amax_sh[wave][r][li] = row_max(am);
+      }
+      lds_barrier();
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const float sum = sum_sh[r][li], inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int ex = part_exp(fmaxf(amax_sh[wave][r][li], amax_sh[wave ^ 1][r][li]) * inv);
+        const int row = row0 + 16 * r + li;
+        if (row < e.rows) {
+          uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 64 * wave + 4 * g;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) {
+            const f32x4 v = (o[d][r] * inv) * exp2i(ex);
+            *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_f16(v[0], v[1]), (int)pack_f16(v[2], v[3])};
+          }
+          if (g == 0 && (wave & 1) == 0) e.ws_scale[(slot * e.rows + row) * 4 + (wave >> 1)] = exp2i(-ex);
+        }
+      }
+    }
+    lds_barrier();  // the sums are read before the next segment's
+  }
+}
+
+int rows_per_workgroup(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+int workgroups_per_cu(int rows) { return rows_per_workgroup(rows) == 128 ? 1 : 2; }
 
 template <int RT>
 static hipError_t launch_rt(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st) {
@@ -689,11 +1025,22 @@ static hipError_t launch_rt(const DecodeParams& p, const int32_t* sched, int num
   return hipGetLastError();
 }
 
+static hipError_t launch_wide(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st) {
+  const int row_blocks = (p.rows + 127) / 128;
+  const dim3 grid((uint32_t)num_parts * (uint32_t)row_blocks);
+  if (p.indices != nullptr)
+    hipLaunchKernelGGL(mla_fp4_wide_kernel<true>, grid, dim3(512), 0, st, sched, row_blocks, num_parts, p);
+  else
+    hipLaunchKernelGGL(mla_fp4_wide_kernel<false>, grid, dim3(512), 0, st, sched, row_blocks, num_parts, p);
+  return hipGetLastError();
+}
+
 hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st) {
   switch (rows_per_workgroup(p.rows)) {
     case 16: return launch_rt<1>(p, sched, num_parts, st);
     case 32: return launch_rt<2>(p, sched, num_parts, st);
-    default: return launch_rt<4>(p, sched, num_parts, st);
+    case 64: return launch_rt<4>(p, sched, num_parts, st);
+    default: return launch_wide(p, sched, num_parts, st);
   }
 }
 

@@ -85,8 +85,8 @@ def test_append_refuses_bad_fp4_args(lib, changes, code, needle):
 
 
 def test_num_parts_by_format(lib):
-    for rows, blocks in ((16, 1), (32, 1), (33, 1), (64, 1), (128, 2), (256, 4), (65536, 1024)):
-        assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 4) == max(1, 512 // blocks)
+    for rows, want in ((16, 512), (32, 512), (33, 512), (64, 512), (65, 256), (128, 256), (129, 128), (65536, 1)):
+        assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 4) == want
         assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 0) == lib.mla_num_parts(4, 1, rows, 1, 256)
     assert lib.mla_num_parts_for(4, 1, 16, 1, 256, 2) == -1 and b"kv_format" in lib.mla_last_error()
     assert lib.mla_num_parts_for(0, 1, 16, 1, 256, 4) == -1
