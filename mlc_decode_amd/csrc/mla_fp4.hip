@@ -60,6 +60,12 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 __device__ __forceinline__ void copy16(const void* lane_addr, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
 }
+__device__ __forceinline__ void copy16(uint64_t base, uint32_t lane_off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void copy4(uint64_t base, uint32_t lane_off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
+}
 __device__ __forceinline__ void copy4(const void* lane_addr, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
 }
@@ -87,6 +93,17 @@ __device__ __forceinline__ int lane_id() {
   int l;
   asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
   return l;
+}
+// The maximum without fmaxf's canonicalising of each operand (scores are no signalling NaNs; a quiet one is passed over).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
 }
 // over the four lane groups that hold one row
 __device__ __forceinline__ float row_max(float v) { return xor32(xor16(v, false), false); }
@@ -122,6 +139,14 @@ __device__ __forceinline__ f32x4 score(int c, i32x4 k, const i32x8 (&q)[4], f32x
                   : mfma_scaled<0, 3>(k, q[3], acc, scale_k, scale_q);
 }
 
+// the same with the scales of the four chunks in one word
+__device__ __forceinline__ f32x4 score_packed(int c, i32x4 k, const i32x8 (&q)[4], f32x4 acc, int scale_k, int scale_q) {
+  return c == 0   ? mfma_scaled<0, 0>(k, q[0], acc, scale_k, scale_q)
+         : c == 1 ? mfma_scaled<1, 1>(k, q[1], acc, scale_k, scale_q)
+         : c == 2 ? mfma_scaled<2, 2>(k, q[2], acc, scale_k, scale_q)
+                  : mfma_scaled<3, 3>(k, q[3], acc, scale_k, scale_q);
+}
+
 // V in LDS: token t of a tile of 16 is a row of 1 KiB; its 16-byte chunk k sits at slot k ^ swz(t) of the
 // 256-byte window it is in.  The conversions' 16-byte writes go eight lanes (tokens, one chunk) at a time over
 // 128 bytes, so swz's low three bits tell eight tokens apart; the transposed reads go 32 lanes (eight tokens, 32
@@ -136,7 +161,7 @@ __device__ __forceinline__ i32x4 widen8(int w, float scale) {
                __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
 }
 
-// One row's queries of a lane for one 128-dim chunk (v: eight dwords of bf16 pairs, dims 16g .. +15 and
+// One row's queries of a lane for one 128-dim chunk (v: four times eight bf16, the B operand's k = 16g .. +15 and
 // 64 + 16g .. +15) as two e4m3 parts.  Per block of 32 dims, hi = q / 2^k rounded to e4m3 with the block's
 // amax in [2, 4) * 2^k: e4m3 then steps by 2^-9 at least, and a product with a code (up to twelve halves)
 // needs at most 13 bits.  The MFMA adds groups of eight products in a window of about that width below the
@@ -287,6 +312,21 @@ __device__ __forceinline__ Row row_at(ArgParams& p, int t, int64_t pg, const int
   return Row{p.codes + pg * p.c_sp + (uint32_t)(row * (int)p.c_st), p.scale + pg * p.s_sp + (uint32_t)(row * (int)p.s_st),
              (const uint8_t*)(p.rope + pg * p.r_sp + (uint32_t)(row * (int)p.r_st))};
 }
+// The segment's index list into LDS; whether any of it names no key (holes: a word a wave).  Every wave passes here.
+__device__ __forceinline__ bool load_indices(ArgParams& p, int b, int tok0, int n, int threads, int32_t* idx, int* holes) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  bool none = false;
+  for (int i = threadIdx.x; i < n; i += threads) {
+    const int id = p.indices[(int64_t)b * p.idx_stride + tok0 + i];
+    idx[i] = id;
+    none |= id < 0 || id >= p.pool_tokens;
+  }
+  holes[wave] = __builtin_amdgcn_ballot_w64(none) != 0;
+  lds_barrier();
+  int any = 0;
+  for (int w = 0; w < threads / 64; ++w) any |= holes[w];
+  return __builtin_amdgcn_readfirstlane(any) != 0;
+}
 // Whether token t of a segment of n names no key (t < n, sparse), or is past the segment.
 template <bool SPARSE>
 __device__ __forceinline__ bool no_key(ArgParams& p, int t, const int32_t* idx, int n) {
@@ -323,6 +363,9 @@ struct Query {
   int scale_hi, scale_lo;  // a byte a chunk
   int lim;                 // the row sees tokens below it
 };
+// Chunk c is dims 128c .. 128c + 127, or with SPREAD 32c .. 32c + 31 of each 128: lane group g of the codes then holds
+// block 4g + c, whose scale byte is byte c of the token's dword g.
+template <bool SPREAD>
 __device__ __forceinline__ Query load_query(ArgParams& p, int b, int row, int L, int lane) {
   Query q;
   const int g = lane >> 4, li = lane & 15;
@@ -334,8 +377,9 @@ __device__ __forceinline__ Query load_query(ArgParams& p, int b, int row, int L,
   q.scale_hi = 0;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    const uint16_t* src = qn + 128 * c + 16 * g;
-    const i32x4 v[4] = {*(const i32x4*)src, *(const i32x4*)(src + 8), *(const i32x4*)(src + 64), *(const i32x4*)(src + 72)};
+    const uint16_t* src = qn + (SPREAD ? 128 * (g >> 1) + 32 * c + 16 * (g & 1) : 128 * c + 16 * g);
+    constexpr int kHalf = SPREAD ? 256 : 64;
+    const i32x4 v[4] = {*(const i32x4*)src, *(const i32x4*)(src + 8), *(const i32x4*)(src + kHalf), *(const i32x4*)(src + kHalf + 8)};
     const QuerySplit r = split_query(v, g, li);
     q.hi[c] = r.hi;
     q.lo[c] = r.lo;
@@ -365,6 +409,7 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
   __shared__ float sum_sh[4][2][16];
   __shared__ int lim_sh[4][16];
   __shared__ int32_t idx_sh[SPARSE ? MLA_SPARSE_MAX_TOPK : 1];
+  __shared__ int holes_sh[4];
 
   int part, rb;
   place_workgroup(row_blocks, num_parts, part, rb);
@@ -392,10 +437,8 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
     const int L = seg.L, tok0 = seg.tok0, tok1 = seg.tok1;
     const int nst = tok1 > tok0 ? (tok1 - tok0 + T - 1) / T : 0;
 
-    if constexpr (SPARSE) {
-      for (int i = threadIdx.x; i < tok1 - tok0; i += 256) idx_sh[i] = p.indices[(int64_t)b * p.idx_stride + tok0 + i];
-      lds_barrier();
-    }
+    bool holes = false;
+    if constexpr (SPARSE) holes = load_indices(p, b, tok0, tok1 - tok0, 256, idx_sh, holes_sh);
 
     auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
     auto row_of = [&](int t, int pg) __attribute__((always_inline)) { return row_at<SPARSE>(p, t, pg, idx_sh, tok1 - tok0); };
@@ -434,7 +477,7 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
     }
 
     const int ql_lane = lane_id<(RT > 1)>();
-    Query q = load_query(p, b, row0 + 16 * rt_own + (ql_lane & 15), L, ql_lane);
+    Query q = load_query<false>(p, b, row0 + 16 * rt_own + (ql_lane & 15), L, ql_lane);
     if constexpr (kRaw) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)((uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + ql_lane * 16) = q.rope[j];
@@ -469,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       // ---- 1. the wave's tokens to bf16 in LDS.  Tokens that do not exist become zeros: their weight is
       // zero, and what their rows hold must not make 0 * NaN of it.
-      const bool cut = SPARSE || tok_k + T > tok1;  // uniform
+      const bool cut = holes || tok_k + T > tok1;  // uniform
       const bool gone = cut && no_key<SPARSE>(p, tok_k + 16 * tt_load + li - tok0, idx_sh, tok1 - tok0);
       i32x4 code;  // chunk c of the token (c_load + c of its 128-dim chunks)
       float scale = 0.f;
@@ -563,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
         s[0] = (a + l) * scale_log2;
       }
       const bool ragged = tok_k + T > tok1 || tok_k + T > lim_min;
-      if (SPARSE || ragged) {  // uniform
+      if (holes || ragged) {  // uniform
         const int lim = lim_sh[wave][li];
 #pragma unroll
         for (int i = 0; i < Sh::kTiles; ++i)
@@ -713,33 +756,56 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
 // 128 query rows: eight waves of one workgroup per CU, wave w scoring row tile w against both token tiles of a
 // 32-token stage and accumulating output dims 64w .. 64w + 63 of all rows.  One barrier a stage: while a
 // wave scores stage k and converts its share of V, P^T and V of stage k - 1 lie in the other half of two
-// buffers, and their product is interleaved with the softmax of stage k, so that the matrix unit works
-// through it.  V is converted once for 128 rows.  (Two 64-row workgroups a CU, which hide one's softmax
-// behind the other only by chance: 64 x 128 heads x 4096 tokens 97 us against 86 here, 32 x 2 x 128 x 16384 303 against 256.)
+// buffers, and their product is interleaved with the softmax of stage k.  V is converted once for 128 rows.
+// (Two 64-row workgroups a CU: 64 x 128 heads x 4096 tokens 97 us, 32 x 2 x 128 x 16384 303; the first form of this
+// kernel, which formed every address anew, 88 and 263, this one 82 and 240, all on one card.)
+// What bounds it is instruction issue: a SIMD's MFMA time and the vector instructions beyond two per MFMA add up
+// (measured: two waves of one bf16 MFMA and 2, 4, 8 additions a step take 18.5, 26, 37 cycles a step), so the loop
+// keeps its lane addresses, takes buffer halves as constants (two stages a turn) and page addresses as scalars.
+//
+// A stage in LDS (kRawStage bytes): per token tile the codes as [lane group g][token][16-byte piece c ^ (token / 2 % 4)]
+// of the 64 bytes that hold blocks 4g .. 4g + 3 (the copies read whole 64 bytes, the fragment reads of one c
+// are free of bank conflicts), two rope fragments, then the tokens' scale bytes.
 template <bool SPARSE>
 __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __restrict__ sched, int row_blocks, int num_parts,
                                                               DecodeParams) {
   constexpr int T = 32, RT = 8, W = 8;
   __shared__ __attribute__((aligned(1024))) uint8_t v_sh[2][T * 1024];
   __shared__ __attribute__((aligned(16))) uint8_t p_sh[2][RT * 1024];  // [row tile][lane][16 bytes]
-  __shared__ __attribute__((aligned(16))) uint8_t raw_sh[2 * kRawStage];
+  __shared__ __attribute__((aligned(16))) uint8_t raw_sh[2][kRawStage];
   __shared__ __attribute__((aligned(16))) uint8_t qr_sh[W * 2048];  // the waves' rope queries, in operand order
   __shared__ float alpha_sh[2][RT][16];
-  __shared__ __attribute__((aligned(8))) uint8_t moved_sh[2][RT];  // row tile's reference moved in the stage
+  __shared__ int moved_sh[2][RT];  // stage in which the row tile's reference last moved, by its parity
+  __shared__ int any_sh[2];        // and any row tile's
   __shared__ float sum_sh[RT][16];
   __shared__ float amax_sh[W][RT][16];
   __shared__ int lim_sh[W][16];
   __shared__ int32_t idx_sh[SPARSE ? MLA_SPARSE_MAX_TOPK : 1];
+  __shared__ int holes_sh[W];
 
   int part, rb;
   place_workgroup(row_blocks, num_parts, part, rb);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int tt_load = wave & 1, c_load = wave >> 1;  // the token tile and 128-dim chunk it copies and converts
+  const int tt_load = wave & 1, g_load = wave >> 1;  // the token tile and lane group's 128 dims it copies
   const int row0 = rb * 16 * RT;
-  uint8_t LDS_AS* const v_lds = (uint8_t LDS_AS*)&v_sh[0][0];
-  uint8_t LDS_AS* const p_lds = (uint8_t LDS_AS*)&p_sh[0][0];
-  uint8_t LDS_AS* const raw_lds = (uint8_t LDS_AS*)raw_sh;
-  uint8_t LDS_AS* const qr_lds = (uint8_t LDS_AS*)qr_sh + wave * 2048;
+  const auto lds_at = [](const void* a) { return (uint32_t)(uintptr_t)(const uint8_t LDS_AS*)a; };
+  const auto at_lds = [](uint32_t a) { return (uint8_t LDS_AS*)a; };
+  const uint32_t raw_base = __builtin_amdgcn_readfirstlane(lds_at(raw_sh));
+
+  // lane addresses in LDS that live through the kernel
+  const int lane0 = threadIdx.x & 63, g0 = lane0 >> 4, li0 = lane0 & 15;
+  const uint32_t frag_at = lds_at(raw_sh) + g0 * 1024 + li0 * 64 + (((li0 >> 1) & 3) << 4);  // chunk 0; chunk c: ^ 16c
+  const uint32_t word_at = lds_at(raw_sh) + kRawScale + li0 * 16 + 4 * g0;
+  // V writes: token li of tile wave / 4, dims 128g + 32 (wave % 4) .. + 31: the chunk of this wave's conversion
+  const int tt_conv = wave >> 2, c_conv = wave & 3;
+  const uint32_t vw_base = lds_at(v_sh) + tt_conv * 16384;
+  const auto v_write = [&](int lane) {
+    return vw_base + (lane & 15) * 1024 + (lane >> 4) * 256 + (((4 * c_conv) ^ swz(lane & 15)) << 4);
+  };
+  const uint32_t vw_kept = v_write(lane0);
+  // V^T reads: token 4g + li/4, dims 64 * wave + 16d + 4 * (li % 4)
+  const int rv = 4 * g0 + (li0 >> 2);
+  const uint32_t vr_at = lds_at(v_sh) + rv * 1024 + (wave >> 1) * 256 + (((8 * (wave & 1) + ((li0 >> 1) & 1)) ^ swz(rv)) << 4) + ((li0 & 1) << 3);
 
   const int32_t* rec = sched + (int64_t)part * kSchedWords;
   int b = rec[0], page = rec[1], split = rec[4];
@@ -752,41 +818,74 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
     const Segment seg = segment_of<SPARSE>(p, b, page, end_b, end_page);
     const int tok0 = seg.tok0, tok1 = seg.tok1;
     const int nst = tok1 > tok0 ? (tok1 - tok0 + T - 1) / T : 0;
-    if constexpr (SPARSE) {
-      for (int i = threadIdx.x; i < tok1 - tok0; i += 64 * W) idx_sh[i] = p.indices[(int64_t)b * p.idx_stride + tok0 + i];
-      lds_barrier();
-    }
-    auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
-    // waves 0 .. 7 a code fragment each, 0 .. 3 one of rope, 4 and 5 a tile's scale bytes
-    auto copy_stage = [&](int k, int pg) __attribute__((always_inline)) {
-      const int lane = lane_id<true>(), g = lane >> 4, li = lane & 15;
-      const Row r = row_at<SPARSE>(p, k * T + 16 * tt_load + li, pg, idx_sh, tok1 - tok0);
-      const uint32_t base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)raw_lds + (k & 1) * kRawStage);
-      const uint32_t tile = base + tt_load * kRawTile;
-      copy16(r.codes + 64 * c_load + 16 * g, tile + 1024 * c_load);
-      if (wave < 4) copy16(r.rope + 64 * (wave >> 1) + 16 * g, tile + 1024 * (4 + (wave >> 1)));  // uniform
-      if ((wave >> 1) == 2) {  // uniform: a dword of scales a lane, four lanes a token
-        const Row w = row_at<SPARSE>(p, k * T + 16 * tt_load + (lane >> 2), pg, idx_sh, tok1 - tok0);
-        copy4(w.scale + 4 * (lane & 3), base + kRawScale + 256 * tt_load);
+    if (threadIdx.x < 2) any_sh[threadIdx.x] = -1;
+    if (threadIdx.x < 2 * RT) moved_sh[0][threadIdx.x] = -1;
+    bool holes = false;
+    if constexpr (SPARSE) holes = load_indices(p, b, tok0, tok1 - tok0, 64 * W, idx_sh, holes_sh);
+    // What the copies of every stage need, held in scalar registers: read from the arguments in the loop, each stage
+    // waited for scalar loads.  A wave's second copy is of rope (waves 0 .. 3) or of scales (4, 5).
+    uint64_t codes = (uint64_t)p.codes, second = wave < 4 ? (uint64_t)p.rope : (uint64_t)p.scale;
+    int64_t c_sp = p.c_sp, second_sp = wave < 4 ? 2 * p.r_sp : p.s_sp;
+    int c_st = (int)p.c_st, second_st = wave < 4 ? 2 * (int)p.r_st : (int)p.s_st;
+    uint64_t table = SPARSE ? 0 : (uint64_t)(p.block_table + (int64_t)b * p.bt_stride);
+    int last_col = p.bt_width - 1, last_page = p.num_blocks - 1;
+    asm volatile("" : "+s"(codes), "+s"(second), "+s"(c_sp), "+s"(second_sp), "+s"(c_st), "+s"(second_st), "+s"(table), "+s"(last_col), "+s"(last_page));
+    // Lane i holds the id of the segment's page `held` + i, clamped into the pool.
+    int held = 0, ids = 0;
+    auto hold_ids = [&](int first) __attribute__((always_inline)) {
+      if constexpr (!SPARSE) {
+        held = first;
+        const int at = page + first + lane_id<true>();
+        const int v = ((const int32_t*)table)[at < last_col ? at : last_col];
+        ids = v < 0 ? 0 : (v < last_page ? v : last_page);
       }
     };
-    int pg_next = 0;
+    auto page_of = [&](int k) __attribute__((always_inline)) {
+      if constexpr (SPARSE) return 0;
+      const int at = k * T / kPageTokens;
+      if (at - held >= 64) hold_ids(at);  // uniform
+      return __builtin_amdgcn_readlane(ids, at - held);
+    };
+    // each wave a KiB of codes, waves 0 .. 3 a rope fragment, 4 and 5 a tile's scale bytes
+    auto copy_stage = [&](int k, int pg) __attribute__((always_inline)) {
+      const int lane = lane_id<true>();
+      const uint32_t base = raw_base + (k & 1) * kRawStage, tile = base + tt_load * kRawTile;
+      // codes: four lanes a token, its 16-byte piece (lane % 4) ^ (token / 2 % 4)
+      const int t4 = lane >> 2, piece = 64 * g_load + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
+      const int rope_at = 64 * (wave >> 1) + 16 * (lane >> 4), li = lane & 15;
+      if constexpr (SPARSE) {
+        const Row r = row_at<true>(p, k * T + 16 * tt_load + t4, 0, idx_sh, tok1 - tok0);
+        copy16(r.codes + piece, tile + 1024 * g_load);
+        if (wave < 4) {  // uniform
+          const Row q = row_at<true>(p, k * T + 16 * tt_load + li, 0, idx_sh, tok1 - tok0);
+          copy16(q.rope + rope_at, tile + 1024 * (4 + (wave >> 1)));
+        } else if (wave < 6) {
+          copy4(r.scale + 4 * (lane & 3), base + kRawScale + 256 * tt_load);
+        }
+      } else {
+        const int row = (k * T & (kPageTokens - 1)) + 16 * tt_load;  // of the tile's first token
+        copy16(codes + (int64_t)pg * c_sp + (int64_t)(row * c_st), (uint32_t)(t4 * c_st + piece), tile + 1024 * g_load);
+        const uint64_t from = second + (int64_t)pg * second_sp + (int64_t)(row * second_st);
+        if (wave < 4)  // uniform
+          copy16(from, (uint32_t)(li * second_st + rope_at), tile + 1024 * (4 + (wave >> 1)));
+        else if (wave < 6)
+          copy4(from, (uint32_t)(t4 * second_st + 4 * (lane & 3)), base + kRawScale + 256 * tt_load);
+      }
+    };
     if (nst > 0) {
-      const int pg = page_of(0);
-      pg_next = page_of(nst > 1 ? 1 : 0);
-      copy_stage(0, pg);
+      hold_ids(0);
+      copy_stage(0, page_of(0));
     }
     i32x8 qh[4], ql[4];
-    int qs_hi, qs_lo;
+    int qs_hi;
     {
       const int lane = lane_id<true>();
-      const Query q = load_query(p, b, row0 + 16 * wave + (lane & 15), seg.L, lane);
+      const Query q = load_query<true>(p, b, row0 + 16 * wave + (lane & 15), seg.L, lane);
 #pragma unroll
       for (int c = 0; c < 4; ++c) qh[c] = q.hi[c], ql[c] = q.lo[c];
       qs_hi = q.scale_hi;
-      qs_lo = q.scale_lo;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)(qr_lds + j * 1024 + lane * 16) = q.rope[j];
+      for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)at_lds(lds_at(qr_sh) + wave * 2048 + j * 1024 + lane * 16) = q.rope[j];
       lim_sh[wave][lane & 15] = q.lim;
     }
     const int lim_min = seg.L - (p.causal ? p.s_q - 1 : 0);  // every row sees the tokens below it
@@ -799,37 +898,37 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
       for (int r = 0; r < RT; ++r) o[d][r] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_ref = -INFINITY, l_rnd = 0.f, l_exact = 0.f;
 
-    // ---- S^T of stage k for row tile `wave`, and this wave's share of V of stage k
-    auto scores = [&](int k, f32x4 (&s)[2]) __attribute__((always_inline)) {
-      const int lane = lane_id<true>(), g = lane >> 4, li = lane & 15;
-      const uint8_t LDS_AS* const raw = raw_lds + (k & 1) * kRawStage;
-      const uint8_t LDS_AS* const frag = raw + lane * 16;
-      const uint8_t LDS_AS* const word = raw + kRawScale + li * 16;
+    // ---- q . k of stage k (in buffer `buf`) for row tile `wave`, and this wave's share of V of stage k
+    auto scores = [&](int k, auto buf, f32x4 (&s)[2]) __attribute__((always_inline)) {
+      constexpr int B = decltype(buf)::value;
       const int t0 = k * T;  // in the segment
+      const uint32_t lane16 = 16 * lane_id<true>();
+      int qs_lo;  // formed here: one register less to keep
+      asm volatile("v_add_u32 %0, 0xf5f5f5f6, %1" : "=v"(qs_lo) : "v"(qs_hi));
+      // (the sparse form, with more addresses of copies, has no register for it)
+      const uint32_t vw_at = SPARSE ? v_write(lane_id<true>()) : vw_kept;
       i32x4 kf[2][2], qf[2], code;
-      uint32_t ks[2][2];
+      int ks[2];
       float scale = 0.f;
       auto read_step = [&](int st) __attribute__((always_inline)) {
+        const uint32_t at = st < 2 ? raw_base + lane16 + 1024 * (4 + st) : (frag_at ^ (16 * (st < 2 ? 0 : st - 2)));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          kf[st & 1][i] = *(const i32x4 LDS_AS*)(frag + i * kRawTile + 1024 * (st < 2 ? 4 + st : st - 2));
-          if (st >= 2) ks[st & 1][i] = *(const uint32_t LDS_AS*)(word + i * 256 + 4 * (st - 2));
-        }
+        for (int i = 0; i < 2; ++i) kf[st & 1][i] = *(const i32x4 LDS_AS*)at_lds(at + B * kRawStage + i * kRawTile);
       };
 #pragma unroll
-      for (int j = 0; j < 2; ++j) qf[j] = *(const i32x4 LDS_AS*)(qr_lds + j * 1024 + lane * 16);
+      for (int j = 0; j < 2; ++j) qf[j] = *(const i32x4 LDS_AS*)at_lds(lds_at(qr_sh) + wave * 2048 + j * 1024 + lane16);
       read_step(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ks[i] = *(const int LDS_AS*)at_lds(word_at + B * kRawStage + i * 256);
       s[0] = s[1] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int v_at = (k & 1) * (T * 1024) + tt_load * 16384 + c_load * 256 + li * 1024 + (((4 * g) ^ swz(li)) << 4);
 #pragma unroll
       for (int st = 0; st < 6; ++st) {
         if (st < 5) read_step(st + 1);
         if (st == 1) {
-          code = *(const i32x4 LDS_AS*)(frag + tt_load * kRawTile + c_load * 1024);
-          const uint32_t w = *(const uint32_t LDS_AS*)(word + tt_load * 256 + 4 * c_load);
-          scale = __uint_as_float(((w >> (8 * g)) & 0xFF) << 23);
-          if (SPARSE || tok0 + t0 + T > tok1) {  // uniform: tokens that do not exist become zeros
-            const bool gone = no_key<SPARSE>(p, t0 + 16 * tt_load + li, idx_sh, tok1 - tok0);
+          code = *(const i32x4 LDS_AS*)at_lds((frag_at ^ (16 * c_conv)) + B * kRawStage + tt_conv * kRawTile);
+          scale = __uint_as_float((((uint32_t)(tt_conv ? ks[1] : ks[0]) >> (8 * c_conv)) & 0xFF) << 23);
+          if (holes || tok0 + t0 + T > tok1) {  // uniform: tokens that do not exist become zeros
+            const bool gone = no_key<SPARSE>(p, t0 + 16 * tt_conv + (lane_id<true>() & 15), idx_sh, tok1 - tok0);
             scale = gone ? 1.f : scale;
 #pragma unroll
             for (int j = 0; j < 4; ++j) code[j] = gone ? 0 : code[j];
@@ -839,55 +938,48 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
 #pragma unroll
           for (int i = 0; i < 2; ++i) s[i] = mfma_bf16(kf[st & 1][i], qf[st], s[i]);
         } else {
-          int sc[2];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) sc[i] = (int)(ks[st & 1][i] >> (8 * g));  // the low byte counts
+          for (int i = 0; i < 2; ++i) s[i] = score_packed(st - 2, kf[st & 1][i], qh, s[i], ks[i], qs_hi);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) s[i] = score(st - 2, kf[st & 1][i], qh, s[i], sc[i], qs_hi);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) s[i] = score(st - 2, kf[st & 1][i], ql, s[i], sc[i], qs_lo);
-          *(i32x4 LDS_AS*)(v_lds + (v_at ^ (16 * (st - 2)))) = widen8(code[st - 2], scale);
+          for (int i = 0; i < 2; ++i) s[i] = score_packed(st - 2, kf[st & 1][i], ql, s[i], ks[i], qs_lo);
+          *(i32x4 LDS_AS*)at_lds((vw_at ^ (16 * (st - 2))) + B * (T * 1024)) = widen8(code[st - 2], scale);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) s[i] *= scale_log2;
-      if (SPARSE || tok0 + t0 + T > tok1 || tok0 + t0 + T > lim_min) {  // uniform
-        const int lim = lim_sh[wave][li];
+      if (holes || tok0 + t0 + T > tok1 || tok0 + t0 + T > lim_min) {  // uniform
+        const int lane = lane_id<true>(), lim = lim_sh[wave][lane & 15];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int t = t0 + 16 * i + 4 * g + j;
+            const int t = t0 + 16 * i + 4 * (lane >> 4) + j;
             s[i][j] = tok0 + t < lim && !no_key<SPARSE>(p, t, idx_sh, tok1 - tok0) ? s[i][j] : -INFINITY;
           }
       }
     };
 
-    // ---- softmax of stage k (SOFT) in six pieces between the products P V of stage k - 1 (PV).  The reference
-    // moves without a branch: where it stays, alpha is exactly one.
-    auto weigh = [&](auto soft, auto pv, int k, f32x4 (&s)[2]) __attribute__((always_inline)) {
+    // ---- softmax of stage k (SOFT; P to buffer `buf`) in pieces between the products P V of stage k - 1 (PV; from
+    // byte offsets p_was and v_was of the buffers).  Where the reference stays, alpha is exactly one.
+    auto weigh = [&](auto soft, auto pv, auto buf, int k, uint32_t p_was, uint32_t v_was, int was, f32x4 (&s)[2]) __attribute__((always_inline)) {
       constexpr bool SOFT = decltype(soft)::value, PV = decltype(pv)::value;
-      const int ln = lane_id<true>(), was = (k & 1) ^ 1;
+      constexpr int B = decltype(buf)::value;
+      const uint32_t lane16 = 16 * lane_id<true>();
       i32x4 va[4], pb[2];
       if constexpr (PV) {
-        const i32x2 moves = *(const i32x2 LDS_AS*)(const uint8_t LDS_AS*)&moved_sh[was][0];
-        pb[0] = *(const i32x4 LDS_AS*)(p_lds + was * (RT * 1024) + ln * 16);
-        const int rv = 4 * (ln >> 4) + ((ln & 15) >> 2);
-        const int at = was * (T * 1024) + rv * 1024 + (wave >> 1) * 256 + (((8 * (wave & 1) + ((ln >> 1) & 1)) ^ swz(rv)) << 4) + ((ln & 1) << 3);
+        const int any = *(const int LDS_AS*)at_lds(lds_at(&any_sh[0]) + 4 * was);
+        pb[0] = *(const i32x4 LDS_AS*)at_lds(lds_at(p_sh) + lane16 + p_was);
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const uint8_t LDS_AS* src = v_lds + (at ^ (32 * d));
-          const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)src));
-          const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(src + 16384)));
+          const uint32_t at = (vr_at ^ (32 * d)) + v_was;
+          const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)at_lds(at)));
+          const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)at_lds(at + 16384)));
           va[d] = i32x4{lo[0], lo[1], hi[0], hi[1]};
         }
-        const uint32_t m0 = __builtin_amdgcn_readfirstlane(moves[0]), m1 = __builtin_amdgcn_readfirstlane(moves[1]);
-        if (m0 | m1) {  // uniform, rare
+        if (__builtin_amdgcn_readfirstlane(any) == k - 1) {  // uniform, rare
 #pragma unroll
           for (int r = 0; r < RT; ++r) {
-            if (((r < 4 ? m0 : m1) >> (8 * (r & 3))) & 0xFF) {  // uniform
-              const float al = alpha_sh[was][r][ln & 15];
+            if (__builtin_amdgcn_readfirstlane(moved_sh[was][r]) == k - 1) {  // uniform
+              const float al = alpha_sh[was][r][lane_id<true>() & 15];
 #pragma unroll
               for (int d = 0; d < 4; ++d) o[d][r] *= al;
             }
@@ -899,35 +991,41 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         if constexpr (PV) {
-          if (r + 1 < RT) pb[(r + 1) & 1] = *(const i32x4 LDS_AS*)(p_lds + (was * RT + r + 1) * 1024 + ln * 16);
+          if (r + 1 < RT) pb[(r + 1) & 1] = *(const i32x4 LDS_AS*)at_lds(lds_at(p_sh) + lane16 + p_was + (r + 1) * 1024);
 #pragma unroll
           for (int d = 0; d < 4; ++d) o[d][r] = mfma_bf16(va[d], pb[r & 1], o[d][r]);
         }
         if constexpr (SOFT) {
           if (r == 0) {
-            top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])), fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-            top = xor16(top, false);
+            top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max2(s[1][2], s[1][3]));
+            const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = max2(__uint_as_float(x[0]), __uint_as_float(x[1]));
           } else if (r == 1) {
-            top = xor32(top, false);
+            const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = max2(__uint_as_float(x[0]), __uint_as_float(x[1])) * scale_log2;
           } else if (r == 2) {
             const float m_old = m_ref;
             m_ref = top > m_ref + kSlack ? top : m_ref;
             moved = __builtin_amdgcn_ballot_w64(m_ref != m_old) != 0;
             base = m_ref == -INFINITY ? 0.f : m_ref;
-            alpha = __builtin_amdgcn_exp2f((m_old == m_ref ? base : m_old) - base);
+            if (moved) {  // uniform
+              alpha = __builtin_amdgcn_exp2f((m_old == m_ref ? base : m_old) - base);
+              l_rnd *= alpha;
+              l_exact *= alpha;
+              alpha_sh[B][wave][lane_id<true>() & 15] = alpha;
+              moved_sh[B][wave] = k;
+              any_sh[B] = k;
+            }
           } else if (r == 3 || r == 4) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[4 * (r - 3) + j] = __builtin_amdgcn_exp2f(s[r - 3][j] - base);
+            for (int j = 0; j < 4; ++j) e[4 * (r - 3) + j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r - 3][j], scale_log2, -base));
           } else if (r == 5) {
             const i32x4 w = {(int)pack_bf16(e[0], e[1]), (int)pack_bf16(e[2], e[3]), (int)pack_bf16(e[4], e[5]), (int)pack_bf16(e[6], e[7])};
-            *(i32x4 LDS_AS*)(p_lds + ((k & 1) * RT + wave) * 1024 + ln * 16) = w;
-            alpha_sh[k & 1][wave][ln & 15] = alpha;
-            moved_sh[k & 1][wave] = moved;
-            l_rnd *= alpha;
+            *(i32x4 LDS_AS*)at_lds(lds_at(p_sh) + lane16 + (B * RT + wave) * 1024) = w;
 #pragma unroll
             for (int j = 0; j < 4; ++j) l_rnd = sum2_bf16((uint32_t)w[j], l_rnd);
           } else if (r == 6) {
-            l_exact = l_exact * alpha + ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+            l_exact += ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
           }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -937,27 +1035,34 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
     constexpr std::false_type no{};
 
     f32x4 s[2];
-    auto next_stage = [&](int k) __attribute__((always_inline)) {
+    auto next_stage = [&](int k, auto buf) __attribute__((always_inline)) {
       copies_landed();
       lds_barrier();  // stage k is in LDS, P and V of stage k - 1 are; their buffers of stage k - 2 are free
-      if (k + 1 < nst) copy_stage(k + 1, pg_next);
-      pg_next = page_of(k + 2 < nst ? k + 2 : nst - 1);
-      scores(k, s);
+      if (k + 1 < nst) copy_stage(k + 1, page_of(k + 1));
+      scores(k, buf, s);
     };
     if (nst > 0) {
-      next_stage(0);
-      weigh(yes, no, 0, s);
+      constexpr std::integral_constant<int, 0> even{};
+      constexpr std::integral_constant<int, 1> odd{};
+      next_stage(0, even);
+      weigh(yes, no, even, 0, 0, 0, 0, s);
 #pragma unroll 1
-      for (int k = 1; k < nst; ++k) {
-        next_stage(k);
-        weigh(yes, yes, k, s);
+      for (int k = 1; k < nst; k += 2) {
+        next_stage(k, odd);
+        weigh(yes, yes, odd, k, 0, 0, 0, s);
+        if (k + 1 == nst) break;
+        next_stage(k + 1, even);
+        weigh(yes, yes, even, k + 1, RT * 1024, T * 1024, 1, s);
       }
     }
     const int lane = lane_id<true>(), g = lane >> 4, li = lane & 15;
     const float l = row_sum(l_rnd), x = row_sum(l_exact);
     sum_sh[wave][li] = l;
     lds_barrier();
-    if (nst > 0) weigh(no, yes, nst, s);
+    if (nst > 0) {
+      const int was = (nst - 1) & 1;
+      weigh(no, yes, std::integral_constant<int, 0>{}, nst, was * (RT * 1024), was * (T * 1024), was, s);
+    }
 
     // ---- lse of row tile `wave`, and the output dims of all
     ArgParams& e = params_here();
