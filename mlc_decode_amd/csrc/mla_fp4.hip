@@ -365,30 +365,81 @@ struct Query {
 };
 // Chunk c is dims 128c .. 128c + 127, or with SPREAD 32c .. 32c + 31 of each 128: lane group g of the codes then holds
 // block 4g + c, whose scale byte is byte c of the token's dword g.
-template <bool SPREAD>
-__device__ __forceinline__ Query load_query(ArgParams& p, int b, int row, int L, int lane) {
-  Query q;
-  const int g = lane >> 4, li = lane & 15;
+template <int N>
+struct QueryLoads {  // N chunks
+  i32x4 v[N][4];
+  i32x4 rope[2];
+  int tok;
+};
+template <bool SPREAD, int N>
+__device__ __forceinline__ QueryLoads<N> load_query(ArgParams& p, int b, int row, int lane, int c0) {
+  QueryLoads<N> q;
+  const int g = lane >> 4;
   row = row < p.rows ? row : p.rows - 1;
-  const int tok = row / p.heads;
-  const int h = row - tok * p.heads;
-  const uint16_t* qn = p.q_nope + ((int64_t)b * p.q_sb + (int64_t)tok * p.q_ss + (int64_t)h * p.q_sh);
-  const uint16_t* qp = p.q_rope + ((int64_t)b * p.qr_sb + (int64_t)tok * p.qr_ss + (int64_t)h * p.qr_sh);
-  q.scale_hi = 0;
+  q.tok = row / p.heads;
+  const int h = row - q.tok * p.heads;
+  const uint16_t* qn = p.q_nope + ((int64_t)b * p.q_sb + (int64_t)q.tok * p.q_ss + (int64_t)h * p.q_sh);
+  const uint16_t* qp = p.q_rope + ((int64_t)b * p.qr_sb + (int64_t)q.tok * p.qr_ss + (int64_t)h * p.qr_sh);
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const uint16_t* src = qn + (SPREAD ? 128 * (g >> 1) + 32 * c + 16 * (g & 1) : 128 * c + 16 * g);
+  for (int c = 0; c < N; ++c) {
+    const uint16_t* src = qn + (SPREAD ? 128 * (g >> 1) + 32 * c + 16 * (g & 1) : 128 * (c0 + c) + 16 * g);
     constexpr int kHalf = SPREAD ? 256 : 64;
-    const i32x4 v[4] = {*(const i32x4*)src, *(const i32x4*)(src + 8), *(const i32x4*)(src + kHalf), *(const i32x4*)(src + kHalf + 8)};
-    const QuerySplit r = split_query(v, g, li);
-    q.hi[c] = r.hi;
-    q.lo[c] = r.lo;
-    q.scale_hi |= r.scale << (8 * c);
+    q.v[c][0] = *(const i32x4*)src;
+    q.v[c][1] = *(const i32x4*)(src + 8);
+    q.v[c][2] = *(const i32x4*)(src + kHalf);
+    q.v[c][3] = *(const i32x4*)(src + kHalf + 8);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) q.rope[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
+  if constexpr (N < 4) __builtin_amdgcn_sched_barrier(0);
+  return q;
+}
+// The queries from all their chunks, or, where 4 / N waves score row tile rt of RT, from chunks c0 .. c0 + N - 1 of
+// each: they exchange them through LDS (16 KiB and 256 bytes a row tile; every wave passes here).  Splitting is 220
+// instructions a chunk: shared by four waves, and with the loads issued before the segment's length and page are
+// known, a segment of 16 rows starts 3.6 us earlier (7.2 to 3.6; 128 ragged sequences x 16 heads 60 to 52 us).
+template <int N, int RT>
+__device__ __forceinline__ Query query_of(ArgParams& p, const QueryLoads<N>& ld, int L, int lane, int rt, int c0, uint8_t LDS_AS* lds,
+                                          uint8_t LDS_AS* lds_scale) {
+  Query q;
+  if constexpr (N == 4) {
+    q.scale_hi = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const QuerySplit r = split_query(ld.v[c], lane >> 4, lane & 15);
+      q.hi[c] = r.hi;
+      q.lo[c] = r.lo;
+      q.scale_hi |= r.scale << (8 * c);
+    }
+  } else {
+    static_assert(N == RT, "the waves of a row tile share its four chunks");
+    uint8_t LDS_AS* const at = lds + rt * 16384 + lane * 16;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const QuerySplit r = split_query(ld.v[n], lane >> 4, lane & 15);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        *(i32x4 LDS_AS*)(at + (c0 + n) * 4096 + j * 1024) = i32x4{r.hi[4 * j], r.hi[4 * j + 1], r.hi[4 * j + 2], r.hi[4 * j + 3]};
+        *(i32x4 LDS_AS*)(at + (c0 + n) * 4096 + 2048 + j * 1024) = i32x4{r.lo[4 * j], r.lo[4 * j + 1], r.lo[4 * j + 2], r.lo[4 * j + 3]};
+      }
+      lds_scale[rt * 256 + lane * 4 + c0 + n] = (uint8_t)r.scale;
+    }
+    lds_barrier();
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const i32x4 h = *(const i32x4 LDS_AS*)(at + c * 4096 + j * 1024), l = *(const i32x4 LDS_AS*)(at + c * 4096 + 2048 + j * 1024);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.hi[c][4 * j + i] = h[i], q.lo[c][4 * j + i] = l[i];
+      }
+    q.scale_hi = *(const int LDS_AS*)(lds_scale + rt * 256 + lane * 4);
+    lds_barrier();  // read before the stages' V takes the place
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) q.rope[j] = ld.rope[j];
   q.scale_lo = q.scale_hi - 0x0A0A0A0A;  // every byte is 11 at least
-  q.lim = L - (p.causal ? p.s_q - 1 - tok : 0);
+  q.lim = L - (p.causal ? p.s_q - 1 - ld.tok : 0);
   return q;
 }
 
@@ -403,6 +454,7 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
   __shared__ __attribute__((aligned(16))) uint8_t p_sh[RT * T * 32];  // [row tile][32 tokens][lane][16 bytes]
   __shared__ __attribute__((aligned(16))) uint8_t raw_sh[kRaw ? 2 * kRawStage : 16];
   __shared__ __attribute__((aligned(16))) uint8_t qr_sh[kRaw ? 4 * 2048 : 16];  // the waves' rope queries, in operand order
+  __shared__ __attribute__((aligned(4))) uint8_t qs_sh[RT < 4 ? 256 * RT : 4];  // scale bytes of the shared queries
   __shared__ float max_sh[4][16];
   __shared__ float alpha_sh[RT][16];
   __shared__ __attribute__((aligned(4))) uint8_t moved_sh[4];  // row tile's reference moved in this stage
@@ -418,6 +470,7 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
   const int tt_load = RT == 1 ? wave : (wave & 1);            // the token tile it loads
   const int tt_own = (wave / RT) * Sh::kTiles;                // the first token tile it scores
   const int c_load = RT == 1 ? 0 : 2 * (wave >> 1);           // the first 128-dim chunk it loads
+  const int c_query = (wave / RT) * RT;                       // the first query chunk it splits for its row tile
   const int row0 = rb * 16 * RT;
 
   uint8_t LDS_AS* const v_lds = (uint8_t LDS_AS*)v_sh;
@@ -433,6 +486,14 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
   for (; b < batch; ++b, page = 0, split = 0) {
     if (!(b < end_b || (b == end_b && page < end_page))) break;
     ArgParams& p = params_here();
+    auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
+    const int ql_lane = lane_id<(RT > 1)>();
+    QueryLoads<RT> q_in;
+    auto load_q = [&]() __attribute__((always_inline)) {
+      q_in = load_query<false, RT>(p, b, row0 + 16 * rt_own + (ql_lane & 15), ql_lane, c_query);
+    };
+    if constexpr (RT < 4) load_q();  // four chunks, held over the first copies, spill
+    const int pg_first = page_of(0);
     const Segment seg = segment_of<SPARSE>(p, b, page, end_b, end_page);
     const int L = seg.L, tok0 = seg.tok0, tok1 = seg.tok1;
     const int nst = tok1 > tok0 ? (tok1 - tok0 + T - 1) / T : 0;
@@ -440,7 +501,6 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
     bool holes = false;
     if constexpr (SPARSE) holes = load_indices(p, b, tok0, tok1 - tok0, 256, idx_sh, holes_sh);
 
-    auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
     auto row_of = [&](int t, int pg) __attribute__((always_inline)) { return row_at<SPARSE>(p, t, pg, idx_sh, tok1 - tok0); };
     auto load_stage = [&](int k, int pg, Stage& s) __attribute__((always_inline)) {  // RT == 1
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
@@ -468,16 +528,15 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
     Stage nxt;
     int pg_next = 0;
     if (nst > 0) {
-      const int pg = page_of(0);
-      pg_next = page_of(nst > 1 ? 1 : 0);
       if constexpr (kRaw)
-        copy_stage(0, pg);
+        copy_stage(0, pg_first);
       else
-        load_stage(0, pg, nxt);
+        load_stage(0, pg_first, nxt);
+      pg_next = page_of(nst > 1 ? 1 : 0);
     }
 
-    const int ql_lane = lane_id<(RT > 1)>();
-    Query q = load_query<false>(p, b, row0 + 16 * rt_own + (ql_lane & 15), L, ql_lane);
+    if constexpr (RT == 4) load_q();
+    Query q = query_of<RT, RT>(p, q_in, L, ql_lane, rt_own, c_query, v_lds, (uint8_t LDS_AS*)qs_sh);
     if constexpr (kRaw) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)((uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + ql_lane * 16) = q.rope[j];
@@ -880,7 +939,8 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
     int qs_hi;
     {
       const int lane = lane_id<true>();
-      const Query q = load_query<true>(p, b, row0 + 16 * wave + (lane & 15), seg.L, lane);
+      const QueryLoads<4> q_in = load_query<true, 4>(p, b, row0 + 16 * wave + (lane & 15), lane, 0);
+      const Query q = query_of<4, RT>(p, q_in, seg.L, lane, wave, 0, nullptr, nullptr);
 #pragma unroll
       for (int c = 0; c < 4; ++c) qh[c] = q.hi[c], ql[c] = q.lo[c];
       qs_hi = q.scale_hi;
