@@ -342,6 +342,13 @@ __device__ __forceinline__ int part_exp(float amax) {
   const int e = 15 - __builtin_amdgcn_frexp_expf(amax);
   return e < 127 ? e : 127;
 }
+// Dims 16d + 4g .. + 3 (a) and 16(d + 1) + 4g .. + 3 (b) of a row, held by lane groups g, to dst: odd and even groups
+// exchange, so that a lane stores 16 bytes and the row's four lanes a whole 64.
+__device__ __forceinline__ void store_dims(uint16_t* dst, int d, int g, i32x2 a, i32x2 b) {
+  const auto x = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), y = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  typedef i32x4 __attribute__((aligned(8))) unaligned_t;
+  *(unaligned_t*)(dst + 16 * (d + (g & 1)) + 8 * (g >> 1)) = i32x4{(int)x[0], (int)y[0], (int)x[1], (int)y[1]};
+}
 // A row's lse from its reference m (log2) and the sum x of its weights; a row without a key has x = 0.  A NaN row (a NaN
 // block, or a NaN in its query) reports lse -inf beside its NaN output, as the 16-bit and fp8 decodes do; its
 // partials carry the NaN, which the merge turns into the same.
@@ -782,11 +789,12 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
       if (single) {
         if (row < e.rows) {
           const int sq = row / e.heads, h = row - sq * e.heads;
-          uint16_t* dst = e.out + ((int64_t)b * e.o_sb + (int64_t)sq * e.o_ss + (int64_t)h * e.o_sh) + 128 * wave + 4 * g;
+          uint16_t* dst = e.out + ((int64_t)b * e.o_sb + (int64_t)sq * e.o_ss + (int64_t)h * e.o_sh) + 128 * wave;
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const f32x4 v = o[d][r] * inv;
-            *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3])};
+          for (int d = 0; d < 8; d += 2) {
+            const f32x4 v = o[d][r] * inv, w = o[d + 1][r] * inv;
+            store_dims(dst, d, g, i32x2{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3])},
+                       i32x2{(int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])});
           }
         }
       } else {  // scaled fp16, as every split's partial (the wave's 128 dims are one chunk)
@@ -798,11 +806,12 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
         am = row_max(am * inv);
         const int ex = part_exp(am);
         if (row < e.rows) {
-          uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 128 * wave + 4 * g;
+          uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 128 * wave;
 #pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const f32x4 v = (o[d][r] * inv) * exp2i(ex);
-            *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_f16(v[0], v[1]), (int)pack_f16(v[2], v[3])};
+          for (int d = 0; d < 8; d += 2) {
+            const f32x4 v = (o[d][r] * inv) * exp2i(ex), w = (o[d + 1][r] * inv) * exp2i(ex);
+            store_dims(dst, d, g, i32x2{(int)pack_f16(v[0], v[1]), (int)pack_f16(v[2], v[3])},
+                       i32x2{(int)pack_f16(w[0], w[1]), (int)pack_f16(w[2], w[3])});
           }
           if (g == 0) e.ws_scale[(slot * e.rows + row) * 4 + wave] = exp2i(-ex);
         }
@@ -1137,11 +1146,12 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
         const int row = row0 + 16 * r + li;
         if (row < e.rows) {
           const int sq = row / e.heads, h = row - sq * e.heads;
-          uint16_t* dst = e.out + ((int64_t)b * e.o_sb + (int64_t)sq * e.o_ss + (int64_t)h * e.o_sh) + 64 * wave + 4 * g;
+          uint16_t* dst = e.out + ((int64_t)b * e.o_sb + (int64_t)sq * e.o_ss + (int64_t)h * e.o_sh) + 64 * wave;
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const f32x4 v = o[d][r] * inv;
-            *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3])};
+          for (int d = 0; d < 4; d += 2) {
+            const f32x4 v = o[d][r] * inv, w = o[d + 1][r] * inv;
+            store_dims(dst, d, g, i32x2{(int)pack_bf16(v[0], v[1]), (int)pack_bf16(v[2], v[3])},
+                       i32x2{(int)pack_bf16(w[0], w[1]), (int)pack_bf16(w[2], w[3])});
           }
         }
       }
@@ -1162,11 +1172,12 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
         const int ex = part_exp(fmaxf(amax_sh[wave][r][li], amax_sh[wave ^ 1][r][li]) * inv);
         const int row = row0 + 16 * r + li;
         if (row < e.rows) {
-          uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 64 * wave + 4 * g;
+          uint16_t* dst = e.ws_o + (slot * e.rows + row) * kDV + 64 * wave;
 #pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const f32x4 v = (o[d][r] * inv) * exp2i(ex);
-            *(i32x2*)(dst + 16 * d) = i32x2{(int)pack_f16(v[0], v[1]), (int)pack_f16(v[2], v[3])};
+          for (int d = 0; d < 4; d += 2) {
+            const f32x4 v = (o[d][r] * inv) * exp2i(ex), w = (o[d + 1][r] * inv) * exp2i(ex);
+            store_dims(dst, d, g, i32x2{(int)pack_f16(v[0], v[1]), (int)pack_f16(v[2], v[3])},
+                       i32x2{(int)pack_f16(w[0], w[1]), (int)pack_f16(w[2], w[3])});
           }
           if (g == 0 && (wave & 1) == 0) e.ws_scale[(slot * e.rows + row) * 4 + (wave >> 1)] = exp2i(-ex);
         }
