@@ -105,6 +105,29 @@ __device__ __forceinline__ void rotate(float& a, float& b, f32x2 cs) {
   a = x;
 }
 
+// Item `i` of [tokens][heads][items] as (t, h, it), in steps of 256 items without a division.
+struct Walk {
+  int t, h, it;
+  int items, heads, step_t, step_h, step_it;
+  __device__ __forceinline__ Walk(int i, int items_, int heads_) : items(items_), heads(heads_) {
+    const int th = i / items;
+    it = i - th * items;
+    t = th / heads;
+    h = th - t * heads;
+    const int s = 256 / items;
+    step_it = 256 - s * items;
+    step_t = s / heads;
+    step_h = s - step_t * heads;
+  }
+  __device__ __forceinline__ void step() {
+    it += step_it;
+    h += step_h;
+    t += step_t;
+    if (it >= items) it -= items, ++h;
+    if (h >= heads) h -= heads, ++t;
+  }
+};
+
 struct RopeParams {
   const uint8_t* x;
   uint8_t* out;
@@ -144,47 +167,67 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
   const bool in_place = p.out == p.x;
   const int items = rot_items + (in_place ? 0 : lead + tail);
   const int total = nt * nh * items;
-  for (int i = threadIdx.x; i < total; i += 256) {
-    const int th = i / items, it = i - th * items;
-    const int t = th / nh, h = h0 + th - t * nh;
-    const uint8_t* src = p.x + (int64_t)(t0 + t) * p.x_st + (int64_t)h * p.x_sh;
-    uint8_t* dst = p.out + (int64_t)(t0 + t) * p.o_st + (int64_t)h * p.o_sh;
-    if (it < rot_items) {
-      const f32x2* c = cs + t * pairs;
-      if constexpr (VEC) {
-        if (p.half) {
-          const int a = (p.first + it * W) * E::kBytes, b = a + pairs * E::kBytes;
-          float x[W], y[W];
-          unpack<E>(*(const i32x4*)(src + a), x);
-          unpack<E>(*(const i32x4*)(src + b), y);
+  Walk at(threadIdx.x, items, nh);
+  if constexpr (VEC) {
+    constexpr int U = 2;  // a thread's chunks in flight
+#pragma unroll 1
+    for (int i = threadIdx.x; i < total; i += 256 * U) {
+      i32x4 v[U], w[U];
+      uint8_t* dst[U];
+      int pair[U];  // the chunk's first pair among its tile's, -1: a chunk that is copied
 #pragma unroll
-          for (int j = 0; j < W; ++j) rotate(x[j], y[j], c[it * W + j]);
-          *(i32x4*)(dst + a) = pack<E>(x);
-          *(i32x4*)(dst + b) = pack<E>(y);
-        } else {
-          const int a = (p.first + it * W) * E::kBytes;
-          float x[W];
-          unpack<E>(*(const i32x4*)(src + a), x);
-#pragma unroll
-          for (int j = 0; j < W / 2; ++j) rotate(x[2 * j], x[2 * j + 1], c[it * (W / 2) + j]);
-          *(i32x4*)(dst + a) = pack<E>(x);
+      for (int u = 0; u < U; ++u) {
+        if (i + 256 * u < total) {
+          const bool turns = at.it < rot_items;
+          const int c = at.it - rot_items;
+          const int a = (turns ? p.first + at.it * W : c < lead ? c * W : p.first + p.rot + (c - lead) * W) * E::kBytes;
+          const uint8_t* src = p.x + (int64_t)(t0 + at.t) * p.x_st + (int64_t)(h0 + at.h) * p.x_sh + a;
+          dst[u] = p.out + (int64_t)(t0 + at.t) * p.o_st + (int64_t)(h0 + at.h) * p.o_sh + a;
+          pair[u] = turns ? at.t * pairs + at.it * (p.half ? W : W / 2) : -1;
+          v[u] = *(const i32x4*)src;
+          if (p.half && turns) w[u] = *(const i32x4*)(src + pairs * E::kBytes);
         }
-      } else {
-        const int a = (p.first + (p.half ? it : 2 * it)) * E::kBytes, b = a + (p.half ? pairs : 1) * E::kBytes;
+        at.step();
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i + 256 * u >= total) break;
+        if (pair[u] >= 0) {
+          const f32x2* c = cs + pair[u];
+          float x[W], y[W];
+          unpack<E>(v[u], x);
+          if (p.half) {
+            unpack<E>(w[u], y);
+#pragma unroll
+            for (int j = 0; j < W; ++j) rotate(x[j], y[j], c[j]);
+            *(i32x4*)(dst[u] + pairs * E::kBytes) = pack<E>(y);
+          } else {
+#pragma unroll
+            for (int j = 0; j < W / 2; ++j) rotate(x[2 * j], x[2 * j + 1], c[j]);
+          }
+          v[u] = pack<E>(x);
+        }
+        *(i32x4*)dst[u] = v[u];
+      }
+    }
+  } else {
+    for (int i = threadIdx.x; i < total; i += 256, at.step()) {
+      const uint8_t* src = p.x + (int64_t)(t0 + at.t) * p.x_st + (int64_t)(h0 + at.h) * p.x_sh;
+      uint8_t* dst = p.out + (int64_t)(t0 + at.t) * p.o_st + (int64_t)(h0 + at.h) * p.o_sh;
+      if (at.it < rot_items) {
+        const int a = (p.first + (p.half ? at.it : 2 * at.it)) * E::kBytes, b = a + (p.half ? pairs : 1) * E::kBytes;
         float x = E::get(src + a), y = E::get(src + b);
-        rotate(x, y, c[it]);
+        rotate(x, y, cs[at.t * pairs + at.it]);
         E::put(dst + a, x);
         E::put(dst + b, y);
+      } else {
+        const int c = at.it - rot_items;
+        const int a = (c < lead ? c : p.first + p.rot + (c - lead)) * E::kBytes;
+        if constexpr (E::kBytes == 4)
+          *(uint32_t*)(dst + a) = *(const uint32_t*)(src + a);
+        else
+          *(uint16_t*)(dst + a) = *(const uint16_t*)(src + a);
       }
-    } else {
-      const int c = it - rot_items;
-      const int a = (c < lead ? c * W : p.first + p.rot + (c - lead) * W) * E::kBytes;
-      if constexpr (VEC)
-        *(i32x4*)(dst + a) = *(const i32x4*)(src + a);
-      else if constexpr (E::kBytes == 4)
-        *(uint32_t*)(dst + a) = *(const uint32_t*)(src + a);
-      else
-        *(uint16_t*)(dst + a) = *(const uint16_t*)(src + a);
     }
   }
 }
@@ -278,57 +321,89 @@ constexpr int kAppendTile = 8;
 template <class E>
 __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
   __shared__ f32x2 cs[kAppendTile][32];
+  __shared__ int32_t slot_sh[kAppendTile];  // -1: names no row
   const int t0 = blockIdx.x * p.tile;
   const int nt = p.tokens - t0 < p.tile ? p.tokens - t0 : p.tile;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (threadIdx.x < nt) {
+    const int slot = p.slots[t0 + threadIdx.x];
+    slot_sh[threadIdx.x] = slot >= 0 && slot < p.cache.tokens ? slot : -1;
+  }
   if (p.freqs != nullptr) {
     const int t = threadIdx.x >> 5;
     if (t < nt) {
       const int pos = p.positions[t0 + t];
       cs[t][threadIdx.x & 31] = pos < 0 ? f32x2{1.f, 0.f} : turn(pos, p.freqs[threadIdx.x & 31], p.amp);
     }
-    __syncthreads();
   }
-  for (int t = wave; t < nt; t += 4) {  // uniform
-    const int64_t slot = p.slots[t0 + t];
-    if (slot < 0 || slot >= p.cache.tokens) continue;
-    const uint8_t* src = p.kv_new + (int64_t)(t0 + t) * p.n_st;
+  // a wave's tokens, loaded together, whatever their slots
+  i32x4 v[kAppendTile / 4];
+  float x[kAppendTile / 4], y[kAppendTile / 4];
+  const int rope_a = (p.half ? lane : 2 * lane) * 2, rope_b = rope_a + (p.half ? 64 : 2);  // a rope pair per lane < 32
+#pragma unroll
+  for (int u = 0; u < kAppendTile / 4; ++u) {
+    const int t = wave + 4 * u;
+    if (t < nt) {  // uniform
+      const uint8_t* src = p.kv_new + (int64_t)(t0 + t) * p.n_st;
+      v[u] = *(const i32x4*)(src + 16 * lane);
+      if (lane < 32) x[u] = E::get(src + 2 * kDV + rope_a), y[u] = E::get(src + 2 * kDV + rope_b);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kAppendTile / 4; ++u) {
+    const int t = wave + 4 * u;
+    if (t >= nt) break;  // uniform
+    const int64_t slot = __builtin_amdgcn_readfirstlane(slot_sh[t]);
+    if (slot < 0) continue;
     const int64_t page = slot / kPage;
     const int row = (int)(slot % kPage);
-    const i32x4 v = *(const i32x4*)(src + 16 * lane);
-    if (lane < 32) {  // a rope pair per lane
-      const int a = (p.half ? lane : 2 * lane) * 2, b = a + (p.half ? 64 : 2);
-      float x = E::get(src + 2 * kDV + a), y = E::get(src + 2 * kDV + b);
-      if (p.freqs != nullptr) rotate(x, y, cs[t][lane]);
+    if (lane < 32) {
+      if (p.freqs != nullptr) rotate(x[u], y[u], cs[t][lane]);
       uint8_t* dst = p.cache.rope + page * p.cache.rp + row * p.cache.rt;
-      E::put(dst + a, x);
-      E::put(dst + b, y);
+      E::put(dst + rope_a, x[u]);
+      E::put(dst + rope_b, y[u]);
     }
-    put_latent(p.cache, page, row, lane, v);
+    put_latent(p.cache, page, row, lane, v[u]);
   }
   if (p.q_pe == nullptr) return;
   const int per_head = p.half ? 4 : 8;
   const int total = nt * p.heads * per_head;
-  // the waves after the tokens' own start first
-  for (int i = (threadIdx.x + 256 - 64 * (nt & 3)) & 255; i < total; i += 256) {
-    const int th = i / per_head, c = i & (per_head - 1);
-    const int t = th / p.heads, h = th - t * p.heads;
-    const int64_t slot = p.slots[t0 + t];
-    if (slot < 0 || slot >= p.cache.tokens) continue;
-    const uint8_t* src = p.q_pe + (int64_t)(t0 + t) * p.pe_st + (int64_t)h * p.pe_sh + 16 * c;
-    uint8_t* dst = p.q + (int64_t)(t0 + t) * p.q_st + (int64_t)h * p.q_sh + 16 * c;
-    float x[8], y[8];
-    unpack<E>(*(const i32x4*)src, x);
-    if (p.half) {
-      unpack<E>(*(const i32x4*)(src + 64), y);
+  constexpr int U = 2;  // a thread's chunks in flight
+  const int first = (threadIdx.x + 256 - 64 * (nt & 3)) & 255;  // the waves after the tokens' own start first
+  Walk at(first, per_head, p.heads);
+#pragma unroll 1
+  for (int i = first; i < total; i += 256 * U) {
+    i32x4 a[U], b[U];
+    uint8_t* dst[U];
+    const f32x2* turns[U];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) rotate(x[j], y[j], cs[t][8 * c + j]);
-      *(i32x4*)dst = pack<E>(x);
-      *(i32x4*)(dst + 64) = pack<E>(y);
-    } else {
+    for (int u = 0; u < U; ++u) {
+      turns[u] = nullptr;
+      if (i + 256 * u < total && slot_sh[at.t] >= 0) {
+        const uint8_t* src = p.q_pe + (int64_t)(t0 + at.t) * p.pe_st + (int64_t)at.h * p.pe_sh + 16 * at.it;
+        dst[u] = p.q + (int64_t)(t0 + at.t) * p.q_st + (int64_t)at.h * p.q_sh + 16 * at.it;
+        turns[u] = &cs[at.t][(p.half ? 8 : 4) * at.it];
+        a[u] = *(const i32x4*)src;
+        if (p.half) b[u] = *(const i32x4*)(src + 64);
+      }
+      at.step();
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) rotate(x[2 * j], x[2 * j + 1], cs[t][4 * c + j]);
-      *(i32x4*)dst = pack<E>(x);
+    for (int u = 0; u < U; ++u) {
+      if (turns[u] == nullptr) continue;
+      float x[8], y[8];
+      unpack<E>(a[u], x);
+      if (p.half) {
+        unpack<E>(b[u], y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rotate(x[j], y[j], turns[u][j]);
+        *(i32x4*)(dst[u] + 64) = pack<E>(y);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) rotate(x[2 * j], x[2 * j + 1], turns[u][j]);
+      }
+      *(i32x4*)dst[u] = pack<E>(x);
     }
   }
 }
