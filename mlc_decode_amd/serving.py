@@ -45,30 +45,32 @@ for _s, _c in ((_CACHE, MlaKvCache), (_ROPE, MlaRope), (_ROPE_ARGS, MlaRopeArgs)
     assert _s.size == ctypes.sizeof(_c)
 
 
-class _on:
-    """The tensors' device made current around a launch, where it is not already."""
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
-    def __init__(self, device: torch.device):
-        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(name: str, fn, device: torch.device, *args) -> None:
+    """``fn(*args, stream)`` with the tensors' device current; an error status raised."""
+    if device.index == _current_device():
+        status = fn(*args, _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream_ptr(device))
+    if status:
+        check(name, status)
 
 
 def _require(t: torch.Tensor, name: str, device: Optional[torch.device] = None) -> None:
-    _require_gpu(t, name)
-    if device is not None and t.device != device:
+    at = t.get_device()  # -1: not on a GPU
+    if at < 0:
+        _require_gpu(t, name)
+    if device is not None and at != device.index:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
 
 
 def _require_int32(t: torch.Tensor, name: str, n: int, device: torch.device) -> None:
-    _require(t, name, device)
-    if t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous():
+    if t.get_device() != device.index:
+        _require(t, name, device)
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous [{n}] int32 tensor")
 
 
@@ -138,7 +140,7 @@ def rope_plan(dim: int = _ROPE_DIM, base: float = 10000.0, layout: str = "interl
 def _rope_struct(rope: Rope, device: torch.device) -> MlaRope:
     freqs, layout, amp = rope
     _require(freqs, "rope.freqs", device)
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or freqs.numel() < 1 or not freqs.is_contiguous():
+    if freqs.dtype is not torch.float64 or freqs.dim() != 1 or freqs.numel() < 1 or not freqs.is_contiguous():
         raise ValueError("rope.freqs must be a contiguous 1-D float64 tensor")
     if layout not in _LAYOUTS:
         raise ValueError("rope.layout must be 'interleaved' or 'half'")
@@ -150,6 +152,10 @@ def _rope_struct(rope: Rope, device: torch.device) -> MlaRope:
 
 def _rows(x: torch.Tensor):
     """``(tokens, heads, token stride, head stride)`` of ``[..., H, D]``: the leading dims as one."""
+    if x.dim() == 3:
+        tokens, heads, _ = x.shape
+        stride, head_stride, _ = x.stride()
+        return tokens, heads, stride if tokens > 1 else 0, head_stride if heads > 1 else 0
     tokens, stride = 1, 0
     for n, s in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):
         if n == 1:
@@ -188,7 +194,8 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, first: Opti
         first = D - r.dim
     if not 0 <= first <= D - r.dim:
         raise ValueError("the rotated dims [first, first + dim) must lie in the head")
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty(x.shape, dtype=x.dtype, device=device)
     else:
         _require(out, "out", device)
@@ -196,19 +203,22 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, first: Opti
             raise ValueError("out must have x's shape and dtype")
     if x.numel() == 0:
         return out
-    xr, orr = _rows(x), _rows(out)
+    xr = _rows(x)
+    if xr is not None:
+        tokens, heads, x_t, x_h = xr
+        orr = (tokens, heads, heads * D, D) if fresh else _rows(out)
     if xr is None or orr is None or (D > 1 and (x.stride(-1) != 1 or out.stride(-1) != 1)):
         raise ValueError("x and out must have unit stride in their last dim and token dims one stride apart")
-    (tokens, heads, x_t, x_h), (_, _, o_t, o_h) = xr, orr
-    if (tokens > 1 and o_t < D) or (heads > 1 and o_h < D):
-        raise ValueError("out's rows overlap")
+    o_t, o_h = orr[2:]
     x_ptr, o_ptr = x.data_ptr(), out.data_ptr()
-    if not _apart_or_same(x_ptr, (x_t, x_h), o_ptr, (o_t, o_h), (tokens, heads), D, x.element_size()):
-        raise ValueError("out overlaps x without being x")
+    if not fresh:
+        if (tokens > 1 and o_t < D) or (heads > 1 and o_h < D):
+            raise ValueError("out's rows overlap")
+        if not _apart_or_same(x_ptr, (x_t, x_h), o_ptr, (o_t, o_h), (tokens, heads), D, x.element_size()):
+            raise ValueError("out overlaps x without being x")
     a = MlaRopeArgs.from_buffer_copy(_ROPE_ARGS.pack(
         x_ptr, o_ptr, x_t, x_h, o_t, o_h, positions.data_ptr(), tokens, heads, D, first, _DTYPES[x.dtype], 0))
-    with _on(device):
-        check("mla_apply_rope", _lib.load().mla_apply_rope(ctypes.byref(r), ctypes.byref(a), _stream_ptr(device)))
+    _launch("mla_apply_rope", _lib.load().mla_apply_rope, device, ctypes.byref(r), ctypes.byref(a))
     return out
 
 
@@ -217,8 +227,8 @@ def _apart_or_same(x_ptr: int, xs, o_ptr: int, os, counts, width: int, es: int) 
     not meet: apart, or parts of the same wider rows (``w[..., :a]`` and ``w[..., a:]``)."""
     if x_ptr == o_ptr:
         return xs == os
-    end = lambda ptr, st: ptr + es * (sum((n - 1) * s for n, s in zip(counts, st)) + width)  # noqa: E731
-    if x_ptr >= end(o_ptr, os) or o_ptr >= end(x_ptr, xs):
+    t, h = counts[0] - 1, counts[1] - 1
+    if x_ptr >= o_ptr + es * (t * os[0] + h * os[1] + width) or o_ptr >= x_ptr + es * (t * xs[0] + h * xs[1] + width):
         return True
     steps = [s for s, n in zip(xs, counts) if n > 1]
     d = abs(x_ptr - o_ptr)
@@ -305,20 +315,18 @@ def kv_append_slots(kv_new: torch.Tensor, kv_cache, slots: torch.Tensor, positio
             raise ValueError(f"q_pe must be a [T, H, {_ROPE_DIM}] tensor in the cache's dtype with unit stride in its heads")
         if q.shape != (T, heads, MLA_DIM_QK) or q.dtype != dtype or (q.numel() and q.stride(2) != 1):
             raise ValueError(f"q must be a [T, H, {MLA_DIM_QK}] tensor like q_pe with unit stride in its heads")
-        stride = lambda t: (t.stride(0) if T > 1 else 0, t.stride(1) if heads > 1 else 0)  # noqa: E731
-        pe_at, q_at = stride(q_pe), stride(q)
-        if (T > 1 and q_at[0] < MLA_DIM_QK) or (heads > 1 and q_at[1] < MLA_DIM_QK):
+        (_, _, pe_t, pe_h), (_, _, q_t, q_h) = _rows(q_pe), _rows(q)
+        if (T > 1 and q_t < MLA_DIM_QK) or (heads > 1 and q_h < MLA_DIM_QK):
             raise ValueError("q's rows overlap")
-        q_ptr = q.data_ptr() + 2 * MLA_DIM_V
-        if T * heads and not _apart_or_same(q_pe.data_ptr(), pe_at, q_ptr, q_at, (T, heads), _ROPE_DIM, 2):
+        pe_ptr, q_ptr = q_pe.data_ptr(), q.data_ptr() + 2 * MLA_DIM_V
+        if T * heads and not _apart_or_same(pe_ptr, (pe_t, pe_h), q_ptr, (q_t, q_h), (T, heads), _ROPE_DIM, 2):
             raise ValueError("q's rope dims overlap q_pe without being it")
-        q_args = (q_pe.data_ptr(), q_ptr, *pe_at, *q_at)
+        q_args = (pe_ptr, q_ptr, pe_t, pe_h, q_t, q_h)
     a = MlaAppendSlotsArgs.from_buffer_copy(_APPEND.pack(
         kv_new.data_ptr(), kv_new.stride(0) if T > 1 else 0, slots.data_ptr(),
         positions.data_ptr() if positions is not None else 0, *q_args, T, heads))
-    with _on(device):
-        check("mla_kv_append_slots", _lib.load().mla_kv_append_slots(
-            ctypes.byref(c), ctypes.byref(r) if r is not None else None, ctypes.byref(a), _stream_ptr(device)))
+    _launch("mla_kv_append_slots", _lib.load().mla_kv_append_slots, device, ctypes.byref(c),
+            ctypes.byref(r) if r is not None else None, ctypes.byref(a))
 
 
 def kv_gather(kv_cache, slots: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -335,9 +343,8 @@ def kv_gather(kv_cache, slots: torch.Tensor, out: Optional[torch.Tensor] = None)
         _require(out, "out", device)
         if out.shape != (T, MLA_DIM_QK) or out.dtype != dtype or out.stride(1) != 1:
             raise ValueError(f"out must be a [T, {MLA_DIM_QK}] tensor in the cache's dtype with unit stride in its rows")
-    with _on(device):
-        check("mla_kv_gather", _lib.load().mla_kv_gather(
-            ctypes.byref(c), slots.data_ptr(), T, out.data_ptr(), out.stride(0) if T > 1 else MLA_DIM_QK, _stream_ptr(device)))
+    _launch("mla_kv_gather", _lib.load().mla_kv_gather, device, ctypes.byref(c), slots.data_ptr(), T, out.data_ptr(),
+            out.stride(0) if T > 1 else MLA_DIM_QK)
     return out
 
 
@@ -372,20 +379,24 @@ def page_pool(num_blocks: int, device="cuda") -> PagePool:
 def _pool_struct(pool: PagePool, block_table: torch.Tensor, cache_seqlens: torch.Tensor):
     _require(block_table, "block_table")
     device = block_table.device
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
         raise ValueError("block_table must be a [B, P] int32 tensor with unit column stride")
-    B, P = block_table.shape
-    if P < 1 or (B > 1 and block_table.stride(0) < P):
+    (B, P), (stride, unit) = block_table.shape, block_table.stride()
+    if P > 1 and unit != 1:
+        raise ValueError("block_table must be a [B, P] int32 tensor with unit column stride")
+    if P < 1 or (B > 1 and stride < P):
         raise ValueError("block_table must have columns, and rows that do not overlap")
     _require_int32(cache_seqlens, "cache_seqlens", B, device)
-    _require_int32(pool.free_pages, "pool.free_pages", pool.free_pages.numel(), device)
-    _require_int32(pool.count, "pool.count", 1, device)
-    stride = block_table.stride(0) if B > 1 else P
+    free, count = pool
+    pages = free.numel()
+    _require_int32(free, "pool.free_pages", pages, device)
+    _require_int32(count, "pool.count", 1, device)
+    if B <= 1:
+        stride = P
     if stride >= 2 ** 31:
         raise ValueError("block_table's row stride must be below 2^31")
     s = MlaPagePool.from_buffer_copy(_POOL.pack(
-        pool.free_pages.data_ptr(), pool.count.data_ptr(), pool.free_pages.numel(), B, block_table.data_ptr(), stride, P,
-        cache_seqlens.data_ptr()))
+        free.data_ptr(), count.data_ptr(), pages, B, block_table.data_ptr(), stride, P, cache_seqlens.data_ptr()))
     return s, B, device
 
 
@@ -406,12 +417,12 @@ def reserve_pages(pool: PagePool, block_table: torch.Tensor, cache_seqlens: torc
     if not 0 <= num_tokens < 2 ** 31:
         raise ValueError("num_tokens must be in [0, 2^31)")
     buf = torch.empty(2 * num_tokens + 3 * B + 2, dtype=torch.int32, device=device)
-    slots, positions, cu_new, granted, scratch = buf.split((num_tokens, num_tokens, B + 1, B, B + 1))
-    with _on(device):
-        check("mla_reserve_pages", _lib.load().mla_reserve_pages(
-            ctypes.byref(s), new_lens.data_ptr(), num_tokens, slots.data_ptr(), positions.data_ptr(), cu_new.data_ptr(),
-            granted.data_ptr(), scratch.data_ptr(), _stream_ptr(device)))
-    return Reservation(slots, positions, cu_new, granted)
+    slots = buf.data_ptr()
+    positions, cu_new = slots + 4 * num_tokens, slots + 8 * num_tokens
+    granted, scratch = cu_new + 4 * (B + 1), cu_new + 4 * (2 * B + 1)
+    _launch("mla_reserve_pages", _lib.load().mla_reserve_pages, device, ctypes.byref(s), new_lens.data_ptr(), num_tokens, slots,
+            positions, cu_new, granted, scratch)
+    return Reservation(*buf.split_with_sizes((num_tokens, num_tokens, B + 1, B, B + 1))[:4])
 
 
 def release_pages(pool: PagePool, block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_lens: torch.Tensor) -> None:
@@ -420,5 +431,4 @@ def release_pages(pool: PagePool, block_table: torch.Tensor, cache_seqlens: torc
     came: releasing what ``reserve_pages`` took restores the stack.  ``block_table`` keeps stale entries."""
     s, B, device = _pool_struct(pool, block_table, cache_seqlens)
     _require_int32(keep_lens, "keep_lens", B, device)
-    with _on(device):
-        check("mla_release_pages", _lib.load().mla_release_pages(ctypes.byref(s), keep_lens.data_ptr(), _stream_ptr(device)))
+    _launch("mla_release_pages", _lib.load().mla_release_pages, device, ctypes.byref(s), keep_lens.data_ptr())
