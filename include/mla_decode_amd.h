@@ -181,11 +181,14 @@ const char* mla_last_error(void);
 int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count);
 
 /*
- * mla_num_parts for a cache of format kv_format: the 4-bit decode is laid out for two workgroups of 16, 32 or
- * 64 query rows per compute unit, or one of 128, the other formats as mla_num_parts says.  Any schedule is
- * decoded right; this one fills the GPU.
+ * mla_num_parts for a cache of format kv_format: the 4-bit decode is laid out for two workgroups of 16 (at
+ * most 32 rows) or 64 query rows per compute unit, or one of 128, the other formats as mla_num_parts says.
+ * max_pages, where not 0: the batch has at most so many pages to read (batch * the block table's width, or
+ * batch * ceil(topk / 64)); few pages are decoded in workgroups of 16 rows for any row count, if the
+ * schedule has that many parts or fewer.  Any schedule is decoded right; this one fills the GPU.
  */
-int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format);
+int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format,
+                      int64_t max_pages);
 
 /*
  * Kernel tile chosen for `rows` = s_q * heads_q query rows (dense bf16/fp16 cache): waves per

@@ -286,7 +286,7 @@ def load() -> ctypes.CDLL:
         lib.mla_kv_append.restype = ctypes.c_int
         lib.mla_combine_absorb.argtypes = [ctypes.POINTER(MlaDecodeArgs), _vp, _vp, _vp]
         lib.mla_combine_absorb.restype = ctypes.c_int
-        lib.mla_num_parts_for.argtypes = [_i32] * 6
+        lib.mla_num_parts_for.argtypes = [_i32] * 6 + [ctypes.c_int64]
         lib.mla_num_parts_for.restype = ctypes.c_int
         lib.mla_apply_rope.argtypes = [ctypes.POINTER(MlaRope), ctypes.POINTER(MlaRopeArgs), _vp]
         lib.mla_apply_rope.restype = ctypes.c_int

@@ -130,8 +130,8 @@ def num_parts_for(batch: int, s_q: int, heads_q: int, heads_k: int = 1, cu_count
 
 
 @functools.lru_cache(maxsize=4096)
-def _num_parts_fp4(rows: int, cu_count: int = 0) -> int:
-    n = _lib.load().mla_num_parts_for(1, 1, rows, 1, cu_count, MLA_KV_FP4_E2M1)
+def _num_parts_fp4(rows: int, max_pages: int, cu_count: int = 0) -> int:
+    n = _lib.load().mla_num_parts_for(1, 1, rows, 1, cu_count, MLA_KV_FP4_E2M1, max_pages)
     if n < 1:
         check("mla_num_parts_for", -n)
     return n
@@ -151,7 +151,7 @@ def kernel_variant(rows: int) -> dict:
 def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num_heads_k: int,
                      num_parts: Optional[int] = None, fixed_overhead: int = -1,
                      forced_splits: int = 0, topk: Optional[int] = None,
-                     kv_cache=None) -> Tuple[torch.Tensor, torch.Tensor]:
+                     kv_cache=None, max_seqlen: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Tile schedule: ``(tile_scheduler_metadata [num_parts, 8] int32, num_splits [B+1] int32)``.
 
     ``num_heads_per_head_k`` is ``s_q * h_q // h_kv`` as in the reference's call; it picks
@@ -164,6 +164,8 @@ def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num
     scheduled as ``topk`` keys long, whatever ``cache_seqlens`` holds.  ``kv_cache``: the cache the
     schedule is for; an :class:`Fp4KVCache` is decoded by workgroups of another size, whose count the
     default ``num_parts`` then is (any schedule is decoded right; that one fills the GPU).
+    ``max_seqlen``: no sequence is longer, as far as the host knows (``64 * block_table.shape[1]``, say); a 4-bit
+    cache's schedule is then made for the decode's form for few pages, where they are few.
     """
     _require_gpu(cache_seqlens, "cache_seqlens")
     if topk is not None:
@@ -179,8 +181,14 @@ def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num
     if forced_splits > 0:
         num_parts = batch * forced_splits
     elif num_parts is None:
-        num_parts = (_num_parts_fp4(num_heads_per_head_k) if isinstance(kv_cache, Fp4KVCache)
-                     else num_parts_for(batch, 1, num_heads_per_head_k, 1))
+        if isinstance(kv_cache, Fp4KVCache):
+            longest = topk if topk is not None else max_seqlen
+            if longest is not None and longest < 0:
+                raise ValueError("max_seqlen must be at least 0")
+            pages = 0 if longest is None else batch * max(-(-int(longest) // _lib.MLA_PAGE_TOKENS), 1)
+            num_parts = _num_parts_fp4(num_heads_per_head_k, pages)
+        else:
+            num_parts = num_parts_for(batch, 1, num_heads_per_head_k, 1)
     sched = torch.empty(num_parts, _lib.MLA_SCHED_WORDS, dtype=torch.int32, device=seqlens.device)
     splits = torch.empty(batch + 1, dtype=torch.int32, device=seqlens.device)
     check("mla_get_metadata", _lib.load().mla_get_metadata(
@@ -507,8 +515,9 @@ def mla_decode_with_kvcache(q: torch.Tensor, kv_cache, block_table: torch.Tensor
         forced = int(num_splits) if num_splits is not None else 0
         if num_splits is not None and forced < 1:
             raise ValueError("num_splits must be >= 1")
+        longest = _lib.MLA_PAGE_TOKENS * block_table.shape[1] if block_table is not None and block_table.dim() == 2 else None
         sched, splits = get_mla_metadata(cache_seqlens, q.shape[1] * q.shape[2], 1,
-                                         forced_splits=forced, kv_cache=kv_cache)
+                                         forced_splits=forced, kv_cache=kv_cache, max_seqlen=longest)
         if forced == 1:
             return _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal,
                            out, lse, status=status, single_split=True)

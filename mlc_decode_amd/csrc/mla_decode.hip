@@ -4185,19 +4185,24 @@ int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, 
   return parts < 1 ? 1 : parts;
 }
 
-int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format) {
+int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format,
+                      int64_t max_pages) {
   if (!known_format(kv_format)) {
     fail(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE, MLA_KV_FP8_E4M3 or MLA_KV_FP4_E2M1");
+    return -MLA_ERR_INVALID;
+  }
+  if (max_pages < 0) {
+    fail(MLA_ERR_INVALID, "max_pages must be >= 0");
     return -MLA_ERR_INVALID;
   }
   const int parts = mla_num_parts(batch, s_q, heads_q, heads_k, cu_count);
   if (parts < 0 || kv_format != MLA_KV_FP4_E2M1) return parts;
   const int64_t rows = (int64_t)s_q * heads_q;
-  const int r = rows < 65536 ? (int)rows : 65536;
-  const int R = mla4::rows_per_workgroup(r);
+  const int64_t tiles = (rows + 15) / 16;
+  const int R = max_pages > 0 && max_pages <= mla4::kFewPages / tiles ? 16 : mla4::rows_per_workgroup(rows);
   const int64_t row_blocks = (rows + R - 1) / R;
   const int cus = cu_count > 0 ? cu_count : cu_count_current();
-  const int64_t n = (int64_t)cus * mla4::workgroups_per_cu(r) / row_blocks;
+  const int64_t n = (int64_t)cus * mla4::workgroups_per_cu(R) / row_blocks;
   return n < 1 ? 1 : (int)n;
 }
 
@@ -4305,7 +4310,7 @@ int mla_splitkv_fwd(const mla_decode_args* args, void* stream) {
   if (rc != MLA_OK) return rc;
   const mla::KParams kp = make_params(args);
   if (args->kv_format == MLA_KV_FP4_E2M1) {
-    const hipError_t e = mla4::launch_decode(make_params_fp4(args, kp), kp.sched, kp.num_parts, (hipStream_t)stream);
+    const hipError_t e = mla4::launch_decode(make_params_fp4(args, kp), kp.sched, kp.num_parts, cu_count_current(), (hipStream_t)stream);
     if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("decode launch failed: ") + hipGetErrorString(e));
     return MLA_OK;
   }

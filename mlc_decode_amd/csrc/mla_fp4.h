@@ -32,10 +32,12 @@ struct DecodeParams {
   float scale_log2;
 };
 
-// Query rows per workgroup for `rows` = s_q * heads rows, and workgroups per compute unit.
-int rows_per_workgroup(int rows);
-int workgroups_per_cu(int rows);
+// Query rows of a workgroup for `rows` = s_q * heads rows, and workgroups of R rows per compute unit.
+int rows_per_workgroup(int64_t rows);
+int workgroups_per_cu(int R);
+// Row tiles of 16 times pages up to which workgroups of 16 rows are the faster ones for any row count.
+constexpr int64_t kFewPages = 6144;
 
-hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st);
+hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_parts, int cus, hipStream_t st);
 
 }  // namespace mla4

@@ -1187,8 +1187,13 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
   }
 }
 
-int rows_per_workgroup(int rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
-int workgroups_per_cu(int rows) { return rows_per_workgroup(rows) == 128 ? 1 : 2; }
+// The schedule's parts are laid out for this many rows a workgroup.  Measured (us; 64 sequences x 4096 tokens, one
+// token a sequence), with workgroups of 16, 64 and 128 rows:
+//   heads   16: 27.7, 47.9, 63.1     32: 42.6, 50.6, 65.9     33: 61.6, 51.4, 66.8     64: 73.6, 56.7, 69.8
+//           72: 94.2, 86.0, 70.2    128: 134,  90.2, 76.7    256: 263,  158,  128
+// (32 rows a workgroup took 42.7 at 32 heads, 67.2 at 33 and 69.7 at 64: nowhere ahead, and is not kept.)
+int rows_per_workgroup(int64_t rows) { return rows <= 32 ? 16 : rows <= 64 ? 64 : 128; }
+int workgroups_per_cu(int R) { return R == 128 ? 1 : 2; }
 
 template <int RT>
 static hipError_t launch_rt(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st) {
@@ -1211,13 +1216,20 @@ static hipError_t launch_wide(const DecodeParams& p, const int32_t* sched, int n
   return hipGetLastError();
 }
 
-hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_parts, hipStream_t st) {
-  switch (rows_per_workgroup(p.rows)) {
-    case 16: return launch_rt<1>(p, sched, num_parts, st);
-    case 32: return launch_rt<2>(p, sched, num_parts, st);
-    case 64: return launch_rt<4>(p, sched, num_parts, st);
-    default: return launch_wide(p, sched, num_parts, st);
-  }
+hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_parts, int cus, hipStream_t st) {
+  // Few pages: a part is one or two pages, and what a workgroup does before and after them counts, which is least
+  // with 16 rows.  Measured (us, one token a sequence; 16 rows and the form for many pages, each with its schedule):
+  //   128 heads: 1 sequence x 64 pages 15.0, 25.3    32 x 11 pages 23.4, 30.9    64 x 11 30.7, 36.7    64 x 22 52.5, 45.7
+  //    64 heads: 1 x 64 12.0, 17.3    64 x 11 22.9, 29.9    64 x 22 32.8, 36.4      192 heads: 64 x 11 54.9, 44.0
+  // Only with a schedule made for it: 16 rows with the other form's parts are more splits to merge than they save
+  // (128 heads, 32 x 11 pages: 35.0).
+  const int64_t pages = (int64_t)p.batch * (p.indices != nullptr ? pages_of(p.topk) : p.bt_width);
+  const int64_t tiles = (p.rows + 15) / 16;
+  const bool few = pages <= kFewPages / tiles && num_parts * tiles <= 2 * cus;
+  const int R = few ? 16 : rows_per_workgroup(p.rows);
+  if (R == 16) return launch_rt<1>(p, sched, num_parts, st);
+  if (R == 64) return launch_rt<4>(p, sched, num_parts, st);
+  return launch_wide(p, sched, num_parts, st);
 }
 
 }  // namespace mla4

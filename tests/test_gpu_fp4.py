@@ -179,12 +179,26 @@ def problem(seed, lens, H, s_q, sigma=1.0, spare=1, poison=True):
     return q, to_gpu(codes, byte, rope), table, torch.tensor(lens, dtype=torch.int32), exactkv
 
 
+FEW = 6144  # table columns times row tiles of 16 up to which the decode takes workgroups of 16 rows
+
+
+def table_for(table, rows, few):
+    """The table as it is (few pages), or with columns behind it that make the decode take its forms for many."""
+    tiles = (rows + 15) // 16
+    if few:
+        assert table.numel() * tiles <= FEW
+        return table
+    return torch.nn.functional.pad(table, (0, FEW // (tiles * table.shape[0]) + 1))
+
+
 LENS = [0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 700]
 
 
 @pytest.mark.parametrize("H,s_q", [(1, 1), (8, 1), (16, 1), (17, 1), (32, 1), (40, 1), (64, 1), (100, 1), (128, 1), (16, 2), (5, 3), (64, 2), (128, 2), (40, 4)])
-def test_decode_rows(gpu, H, s_q):
+@pytest.mark.parametrize("few", [False, True])
+def test_decode_rows(gpu, H, s_q, few):
     q, cache, table, lens, kv = problem(H * 8 + s_q, LENS, H, s_q)
+    table = table_for(table, H * s_q, few)
     d = (q.cuda(), cache, table.cuda(), lens.cuda())
     say(f"decode H={H} s_q={s_q}")
     for splits in (None, 1, 3):
@@ -194,19 +208,23 @@ def test_decode_rows(gpu, H, s_q):
 
 
 @pytest.mark.parametrize("H", [16, 32, 128])
-def test_decode_without_mask_and_scales(gpu, H):
+@pytest.mark.parametrize("few", [False, True])
+def test_decode_without_mask_and_scales(gpu, H, few):
     q, cache, table, lens, kv = problem(7, [5, 200, 64], H, 2, sigma=3.0)
+    table = table_for(table, 2 * H, few)
     say(f"decode no mask H={H}")
     out, lse = mla_decode_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), causal=False)
     torch.cuda.synchronize()
     assert_decode(out, lse, q, kv, table, lens, False, f"no mask H={H}")
 
 
-@pytest.mark.parametrize("H", [16, 24, 128])
+@pytest.mark.parametrize("H", [16, 24, 64, 128])
 @pytest.mark.parametrize("parts", [1, 2, 7, 64])
-def test_decode_schedules(gpu, H, parts):
+@pytest.mark.parametrize("few", [False, True])
+def test_decode_schedules(gpu, H, parts, few):
     """Any schedule: parts that span sequences, sequences that span parts, parts with nothing to do."""
     q, cache, table, lens, kv = problem(50 + H, [300, 1, 0, 2000, 64, 65], H, 1)
+    table = table_for(table, H, few)
     say(f"decode parts={parts} H={H}")
     ld = lens.cuda()
     sched, splits = get_mla_metadata(ld, H, 1, num_parts=parts)
@@ -272,12 +290,14 @@ def test_decode_cut_at_the_table_and_foreign_pages(gpu):
     assert_decode(out, lse, q, kv, short, lens, False, "cut")
 
 
-@pytest.mark.parametrize("H", [16, 128])
-def test_decode_far_pages(gpu, H):
+@pytest.mark.parametrize("H", [16, 64, 128])
+@pytest.mark.parametrize("few", [False, True])
+def test_decode_far_pages(gpu, H, few):
     """Pages past 4 GiB from the pool's start."""
     nb, gap = 72, 1 << 26
     buf = torch.empty(nb * gap, dtype=torch.uint8, device="cuda")
     q, cache, table, lens, kv = problem(33, [200, 64 * 60 + 3], H, 1, spare=nb - 65)
+    table = table_for(table, H, few)
     far = buf.as_strided((nb, 64, 256), (gap, 256, 1))
     far.copy_(cache.latent)
     sc = buf.as_strided((nb, 64, 16), (gap, 16, 1), 1 << 20)
@@ -302,7 +322,8 @@ def test_decode_nan_block_stays_with_its_sequence(gpu):
 
 @pytest.mark.parametrize("H", [16, 32, 64, 128])
 @pytest.mark.parametrize("topk", [1, 63, 64, 200, 2048])
-def test_sparse(gpu, H, topk):
+@pytest.mark.parametrize("parts", [None, 512])  # 512: more than the form for few pages is taken with
+def test_sparse(gpu, H, topk, parts):
     g = torch.Generator().manual_seed(topk + H)
     nb, B = 40, 3
     kv = torch.randn(nb, 64, 1, 576, generator=g).to(torch.bfloat16)
@@ -314,10 +335,29 @@ def test_sparse(gpu, H, topk):
     q = torch.randn(B, 1, H, 576, generator=g).to(torch.bfloat16)
     cache = to_gpu(codes, byte, rope)
     say(f"sparse H={H} topk={topk}")
-    sched, splits = get_mla_metadata(torch.zeros(B, dtype=torch.int32, device="cuda"), H, 1, topk=topk, kv_cache=cache)
+    sched, splits = get_mla_metadata(torch.zeros(B, dtype=torch.int32, device="cuda"), H, 1, parts, topk=topk, kv_cache=cache)
     out, lse = flash_mla_with_kvcache(q.cuda(), cache, None, None, 512, sched, splits, indices=idx.cuda().unsqueeze(1))
     torch.cuda.synchronize()
     assert_decode(out, lse, q, F4.dequantize_pages(codes, byte, rope), None, None, False, f"sparse H={H} topk={topk}", indices=idx)
+
+
+@pytest.mark.parametrize("H", [33, 128, 200])
+def test_schedule_for_few_pages(gpu, H):
+    """A schedule made with the longest length a host knows has fewer parts, and decodes the same."""
+    q, cache, table, lens, kv = problem(H, [0, 1, 700, 64], H, 1)
+    ld = lens.cuda()
+    say(f"few pages H={H}")
+    out = []
+    for longest in (None, 64 * table.shape[1]):
+        sched, splits = get_mla_metadata(ld, H, 1, kv_cache=cache, max_seqlen=longest)
+        o, lse = flash_mla_with_kvcache(q.cuda(), cache, table.cuda(), ld, 512, sched, splits)
+        torch.cuda.synchronize()
+        assert_decode(o, lse, q, kv, table, lens, False, f"few pages H={H} {longest}")
+        out.append(sched.shape[0] * ((H + 15) // 16))
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    assert out[1] <= 2 * cus < out[0]
+    with pytest.raises(ValueError, match="max_seqlen"):
+        get_mla_metadata(ld, H, 1, kv_cache=cache, max_seqlen=-1)
 
 
 def test_absorbed_and_noalloc_agree_with_the_decode(gpu):
@@ -343,9 +383,11 @@ def test_absorbed_and_noalloc_agree_with_the_decode(gpu):
     assert ((v.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * mag).all()
 
 
-def test_same_result_on_another_stream_and_twice(gpu):
+@pytest.mark.parametrize("few", [False, True])
+def test_same_result_on_another_stream_and_twice(gpu, few):
     H = 128
     q, cache, table, lens, _ = problem(6, [1000, 300, 64, 5], H, 1)
+    table = table_for(table, H, few)
     d = (q.cuda(), cache, table.cuda(), lens.cuda())
     say("two streams")
     out, lse = mla_decode_with_kvcache(*d)

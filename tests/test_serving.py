@@ -85,11 +85,15 @@ def test_append_refuses_bad_fp4_args(lib, changes, code, needle):
 
 
 def test_num_parts_by_format(lib):
-    for rows, want in ((16, 512), (32, 512), (33, 512), (64, 512), (65, 256), (128, 256), (129, 128), (65536, 1)):
-        assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 4) == want
-        assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 0) == lib.mla_num_parts(4, 1, rows, 1, 256)
-    assert lib.mla_num_parts_for(4, 1, 16, 1, 256, 2) == -1 and b"kv_format" in lib.mla_last_error()
-    assert lib.mla_num_parts_for(0, 1, 16, 1, 256, 4) == -1
+    for rows, want in ((16, 512), (17, 256), (32, 256), (33, 512), (64, 512), (65, 256), (128, 256), (129, 128), (65536, 1)):
+        for pages in (0, 65536, 2 ** 40):
+            assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 4, pages) == want
+            assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 0, pages) == lib.mla_num_parts(4, 1, rows, 1, 256)
+    for rows, pages, want in ((64, 1536, 128), (64, 1537, 512), (128, 768, 64), (128, 769, 256), (8192, 8, 1), (1, 6144, 512)):
+        assert lib.mla_num_parts_for(4, 1, rows, 1, 256, 4, pages) == want  # few pages: 512 workgroups of 16 rows
+    assert lib.mla_num_parts_for(4, 1, 16, 1, 256, 2, 0) == -1 and b"kv_format" in lib.mla_last_error()
+    assert lib.mla_num_parts_for(4, 1, 16, 1, 256, 4, -1) == -1 and b"max_pages" in lib.mla_last_error()
+    assert lib.mla_num_parts_for(0, 1, 16, 1, 256, 4, 0) == -1
 
 
 @pytest.mark.parametrize("fmt,changes,code,needle", [
