@@ -5,17 +5,23 @@
 // in bf16: 400 bytes.  Math, schedule, splits and partials are those of mla_decode.hip:
 //   S = sm_scale * [q_nope|q_rope] . [latent|rope]^T,  O = softmax(S) . latent,  lse = log sum exp S.
 //
-// A workgroup of four waves owns one schedule part for 16 * RT query rows and walks it in stages of T
-// tokens; two workgroups share a CU, so one's matrix work covers the other's loads and barriers.
+// Three forms, by query rows and pages (see launch_decode): 16 and 64 rows in workgroups of four waves, two to a CU
+// (one's matrix work covers the other's loads and barriers), and 128 rows in one of eight.  A workgroup owns one
+// schedule part for its rows and walks it in stages of T tokens.
 //  1. A lane holds 32 dims of one token as codes: that is the A operand of the block-scaled 16x16x128 MFMA as it
-//     stands, the scale byte its scale.  Nothing is converted for the QK product.  The queries are split once per segment into two e4m3 parts, q = hi + lo: a bf16 has eight
-//     significant bits, each part holds four (see split_query for what is left).  The rope dims take the
-//     bf16 MFMA.
+//     stands, the scale byte its scale.  Nothing is converted for the QK product.  The queries are split once per
+//     segment into two e4m3 parts, q = hi + lo: a bf16 has eight significant bits, each part holds four (see
+//     split_query for what is left).  The rope dims take the bf16 MFMA.
 //  2. The V operand needs tokens along k, and its scales vary along k, which the block-scaled MFMA does not
 //     take: each wave converts its tokens' codes to bf16 (exact: two significant bits and a power of two)
 //     and writes them to LDS, where transposed reads form V^T.
 //  3. S^T tiles (token, row) are held by the wave that owns a row tile's token tiles; P^T goes through LDS in
-//     operand order to all four waves, each of which accumulates 128 of the 512 output dims.
+//     operand order, rounded to bf16 (the PV operand's type; the sum that divides the output is of the rounded
+//     weights, so that the rounding cancels in it), to all waves, each of which accumulates its share of the
+//     512 output dims in fp32.
+// What bounds them (one token a sequence unless said): 16 rows, 128 ragged sequences, 213 MB: 46 us in the main kernel,
+// 4.65 TB/s, a large copy's rate, 52 with the merge.  128 rows: instruction issue (see mla_fp4_wide_kernel): 64 x 4096
+// tokens x 128 heads 79 us with the merge, 32 x 16384 x 2 x 128 233 us, 1.25 PFLOP/s of bf16 products.
 // The running row maximum moves only when a score passes it by more than 2^kSlack (P then stays far from
 // overflow in bf16 and fp32), so the output is rescaled rarely and exactly.
 #include <hip/hip_runtime.h>

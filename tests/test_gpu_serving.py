@@ -72,6 +72,9 @@ ROPE_CASES = [
     (3, 1, 1024, 1024, 0, "half", torch.bfloat16, None),
     (2, 1, 1030, 1022, 8, "interleaved", torch.bfloat16, None),
     (4097, 2, 64, 64, 0, "half", torch.bfloat16, "yarn"),
+    (8195, 3, 96, 64, 16, "half", torch.bfloat16, None),        # eight tokens a workgroup, chunks beside the rotated ones
+    (8195, 3, 96, 64, 16, "interleaved", torch.float32, "ntk"),
+    (8195, 2, 71, 8, 1, "half", torch.float16, None),           # and one value at a time
 ]
 
 
