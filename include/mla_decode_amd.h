@@ -185,7 +185,8 @@ int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, 
  * most 32 rows) or 64 query rows per compute unit, or one of 128, the other formats as mla_num_parts says.
  * max_pages, where not 0: the batch has at most so many pages to read (batch * the block table's width, or
  * batch * ceil(topk / 64)); few pages are decoded in workgroups of 16 rows for any row count, if the
- * schedule has that many parts or fewer.  Any schedule is decoded right; this one fills the GPU.
+ * schedule has that many parts or fewer (or no sequence has more than one page).  Any schedule is decoded
+ * right; this one fills the GPU.
  */
 int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format,
                       int64_t max_pages);

@@ -8,10 +8,12 @@
 // Three forms, by query rows and pages (see launch_decode): 16 and 64 rows in workgroups of four waves, two to a CU
 // (one's matrix work covers the other's loads and barriers), and 128 rows in one of eight.  A workgroup owns one
 // schedule part for its rows and walks it in stages of T tokens.
-//  1. A lane holds 32 dims of one token as codes: that is the A operand of the block-scaled 16x16x128 MFMA as it
-//     stands, the scale byte its scale.  Nothing is converted for the QK product.  The queries are split once per
-//     segment into two e4m3 parts, q = hi + lo: a bf16 has eight significant bits, each part holds four (see
-//     split_query for what is left).  The rope dims take the bf16 MFMA.
+//  1. 64 and 128 rows: a lane holds 32 dims of one token as codes: that is the A operand of the block-scaled
+//     16x16x128 MFMA as it stands, the scale byte its scale.  Nothing is converted for the QK product, whose tokens
+//     every wave scores.  The queries are split once per segment into two e4m3 parts, q = hi + lo: a bf16 has eight
+//     significant bits, each part holds four (see split_query for what is left).  The rope dims take the bf16 MFMA.
+//     16 rows: a wave scores the tokens that it converts for V (2.), so QK takes those bf16 words: the same MFMA
+//     clocks, exact products, and a score's relative error is 6e-8 instead of 1e-6.
 //  2. The V operand needs tokens along k, and its scales vary along k, which the block-scaled MFMA does not
 //     take: each wave converts its tokens' codes to bf16 (exact: two significant bits and a power of two)
 //     and writes them to LDS, where transposed reads form V^T.
@@ -376,83 +378,63 @@ struct Query {
   int scale_hi, scale_lo;  // a byte a chunk
   int lim;                 // the row sees tokens below it
 };
+__device__ __forceinline__ int clamp_row(ArgParams& p, int row) { return row < p.rows ? row : p.rows - 1; }
+__device__ __forceinline__ const uint16_t* nope_of(ArgParams& p, int b, int tok, int h) {
+  return p.q_nope + ((int64_t)b * p.q_sb + (int64_t)tok * p.q_ss + (int64_t)h * p.q_sh);
+}
+__device__ __forceinline__ const uint16_t* rope_of(ArgParams& p, int b, int tok, int h) {
+  return p.q_rope + ((int64_t)b * p.qr_sb + (int64_t)tok * p.qr_ss + (int64_t)h * p.qr_sh);
+}
+__device__ __forceinline__ int limit_of(ArgParams& p, int L, int tok) { return L - (p.causal ? p.s_q - 1 - tok : 0); }
 // Chunk c is dims 128c .. 128c + 127, or with SPREAD 32c .. 32c + 31 of each 128: lane group g of the codes then holds
 // block 4g + c, whose scale byte is byte c of the token's dword g.
-template <int N>
-struct QueryLoads {  // N chunks
-  i32x4 v[N][4];
-  i32x4 rope[2];
-  int tok;
-};
-template <bool SPREAD, int N>
-__device__ __forceinline__ QueryLoads<N> load_query(ArgParams& p, int b, int row, int lane, int c0) {
-  QueryLoads<N> q;
-  const int g = lane >> 4;
-  row = row < p.rows ? row : p.rows - 1;
-  q.tok = row / p.heads;
-  const int h = row - q.tok * p.heads;
-  const uint16_t* qn = p.q_nope + ((int64_t)b * p.q_sb + (int64_t)q.tok * p.q_ss + (int64_t)h * p.q_sh);
-  const uint16_t* qp = p.q_rope + ((int64_t)b * p.qr_sb + (int64_t)q.tok * p.qr_ss + (int64_t)h * p.qr_sh);
+template <bool SPREAD>
+__device__ __forceinline__ Query load_query(ArgParams& p, int b, int row, int L, int lane) {
+  Query q;
+  const int g = lane >> 4, li = lane & 15;
+  row = clamp_row(p, row);
+  const int tok = row / p.heads, h = row - tok * p.heads;
+  const uint16_t* qn = nope_of(p, b, tok, h);
+  const uint16_t* qp = rope_of(p, b, tok, h);
+  q.scale_hi = 0;
 #pragma unroll
-  for (int c = 0; c < N; ++c) {
-    const uint16_t* src = qn + (SPREAD ? 128 * (g >> 1) + 32 * c + 16 * (g & 1) : 128 * (c0 + c) + 16 * g);
+  for (int c = 0; c < 4; ++c) {
+    const uint16_t* src = qn + (SPREAD ? 128 * (g >> 1) + 32 * c + 16 * (g & 1) : 128 * c + 16 * g);
     constexpr int kHalf = SPREAD ? 256 : 64;
-    q.v[c][0] = *(const i32x4*)src;
-    q.v[c][1] = *(const i32x4*)(src + 8);
-    q.v[c][2] = *(const i32x4*)(src + kHalf);
-    q.v[c][3] = *(const i32x4*)(src + kHalf + 8);
+    const i32x4 v[4] = {*(const i32x4*)src, *(const i32x4*)(src + 8), *(const i32x4*)(src + kHalf), *(const i32x4*)(src + kHalf + 8)};
+    const QuerySplit r = split_query(v, g, li);
+    q.hi[c] = r.hi;
+    q.lo[c] = r.lo;
+    q.scale_hi |= r.scale << (8 * c);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) q.rope[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
-  if constexpr (N < 4) __builtin_amdgcn_sched_barrier(0);
+  q.scale_lo = q.scale_hi - 0x0A0A0A0A;  // every byte is 11 at least
+  q.lim = limit_of(p, L, tok);
   return q;
 }
-// The queries from all their chunks, or, where 4 / N waves score row tile rt of RT, from chunks c0 .. c0 + N - 1 of
-// each: they exchange them through LDS (16 KiB and 256 bytes a row tile; every wave passes here).  Splitting is 220
-// instructions a chunk: shared by four waves, and with the loads issued before the segment's length and page are
-// known, a segment of 16 rows starts 3.6 us earlier (7.2 to 3.6; 128 ragged sequences x 16 heads 60 to 52 us).
-template <int N, int RT>
-__device__ __forceinline__ Query query_of(ArgParams& p, const QueryLoads<N>& ld, int L, int lane, int rt, int c0, uint8_t LDS_AS* lds,
-                                          uint8_t LDS_AS* lds_scale) {
-  Query q;
-  if constexpr (N == 4) {
-    q.scale_hi = 0;
+
+// The same in bf16, for the form whose waves score the tokens that they convert: dims 128c + 32g + 8i .. + 7 are those
+// of a token's word i of chunk c in lane group g.  All four waves need the same queries: each loads chunk `wave` and
+// they exchange them through 16 KiB of LDS (a segment starts 2.6 us earlier than with all of it loaded by each).
+struct Query16 {
+  i32x4 nope[4];
+  i32x4 rope[2];
+  int tok;
+};
+__device__ __forceinline__ Query16 load_query16(ArgParams& p, int b, int row, int lane, int wave) {
+  Query16 q;
+  const int g = lane >> 4;
+  row = clamp_row(p, row);
+  q.tok = row / p.heads;
+  const int h = row - q.tok * p.heads;
+  const uint16_t* qn = nope_of(p, b, q.tok, h);
+  const uint16_t* qp = rope_of(p, b, q.tok, h);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const QuerySplit r = split_query(ld.v[c], lane >> 4, lane & 15);
-      q.hi[c] = r.hi;
-      q.lo[c] = r.lo;
-      q.scale_hi |= r.scale << (8 * c);
-    }
-  } else {
-    static_assert(N == RT, "the waves of a row tile share its four chunks");
-    uint8_t LDS_AS* const at = lds + rt * 16384 + lane * 16;
+  for (int i = 0; i < 4; ++i) q.nope[i] = *(const i32x4*)(qn + 128 * wave + 32 * g + 8 * i);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      const QuerySplit r = split_query(ld.v[n], lane >> 4, lane & 15);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        *(i32x4 LDS_AS*)(at + (c0 + n) * 4096 + j * 1024) = i32x4{r.hi[4 * j], r.hi[4 * j + 1], r.hi[4 * j + 2], r.hi[4 * j + 3]};
-        *(i32x4 LDS_AS*)(at + (c0 + n) * 4096 + 2048 + j * 1024) = i32x4{r.lo[4 * j], r.lo[4 * j + 1], r.lo[4 * j + 2], r.lo[4 * j + 3]};
-      }
-      lds_scale[rt * 256 + lane * 4 + c0 + n] = (uint8_t)r.scale;
-    }
-    lds_barrier();
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const i32x4 h = *(const i32x4 LDS_AS*)(at + c * 4096 + j * 1024), l = *(const i32x4 LDS_AS*)(at + c * 4096 + 2048 + j * 1024);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) q.hi[c][4 * j + i] = h[i], q.lo[c][4 * j + i] = l[i];
-      }
-    q.scale_hi = *(const int LDS_AS*)(lds_scale + rt * 256 + lane * 4);
-    lds_barrier();  // read before the stages' V takes the place
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) q.rope[j] = ld.rope[j];
-  q.scale_lo = q.scale_hi - 0x0A0A0A0A;  // every byte is 11 at least
-  q.lim = L - (p.causal ? p.s_q - 1 - ld.tok : 0);
+  for (int j = 0; j < 2; ++j) q.rope[j] = *(const i32x4*)(qp + 32 * j + 8 * g);
+  __builtin_amdgcn_sched_barrier(0);
   return q;
 }
 
@@ -467,7 +449,6 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
   __shared__ __attribute__((aligned(16))) uint8_t p_sh[RT * T * 32];  // [row tile][32 tokens][lane][16 bytes]
   __shared__ __attribute__((aligned(16))) uint8_t raw_sh[kRaw ? 2 * kRawStage : 16];
   __shared__ __attribute__((aligned(16))) uint8_t qr_sh[kRaw ? 4 * 2048 : 16];  // the waves' rope queries, in operand order
-  __shared__ __attribute__((aligned(4))) uint8_t qs_sh[RT < 4 ? 256 * RT : 4];  // scale bytes of the shared queries
   __shared__ float max_sh[4][16];
   __shared__ float alpha_sh[RT][16];
   __shared__ __attribute__((aligned(4))) uint8_t moved_sh[4];  // row tile's reference moved in this stage
@@ -483,7 +464,6 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
   const int tt_load = RT == 1 ? wave : (wave & 1);            // the token tile it loads
   const int tt_own = (wave / RT) * Sh::kTiles;                // the first token tile it scores
   const int c_load = RT == 1 ? 0 : 2 * (wave >> 1);           // the first 128-dim chunk it loads
-  const int c_query = (wave / RT) * RT;                       // the first query chunk it splits for its row tile
   const int row0 = rb * 16 * RT;
 
   uint8_t LDS_AS* const v_lds = (uint8_t LDS_AS*)v_sh;
@@ -501,11 +481,12 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
     ArgParams& p = params_here();
     auto page_of = [&](int k) __attribute__((always_inline)) { return page_at<SPARSE>(p, b, page + k * T / kPageTokens); };
     const int ql_lane = lane_id<(RT > 1)>();
-    QueryLoads<RT> q_in;
-    auto load_q = [&]() __attribute__((always_inline)) {
-      q_in = load_query<false, RT>(p, b, row0 + 16 * rt_own + (ql_lane & 15), ql_lane, c_query);
-    };
-    if constexpr (RT < 4) load_q();  // four chunks, held over the first copies, spill
+    const int q_row = row0 + 16 * rt_own + (ql_lane & 15);
+    Query q;
+    Query16 q16;
+    i32x4 qn[4][4];  // RT == 1: the rows' nope queries
+    // Before the segment's length and page are known: the waits of the three overlap.
+    if constexpr (!kRaw) q16 = load_query16(p, b, q_row, ql_lane, wave);
     const int pg_first = page_of(0);
     const Segment seg = segment_of<SPARSE>(p, b, page, end_b, end_page);
     const int L = seg.L, tok0 = seg.tok0, tok1 = seg.tok1;
@@ -548,13 +529,22 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
       pg_next = page_of(nst > 1 ? 1 : 0);
     }
 
-    if constexpr (RT == 4) load_q();
-    Query q = query_of<RT, RT>(p, q_in, L, ql_lane, rt_own, c_query, v_lds, (uint8_t LDS_AS*)qs_sh);
     if constexpr (kRaw) {
+      q = load_query<false>(p, b, q_row, L, ql_lane);
 #pragma unroll
       for (int j = 0; j < 2; ++j) *(i32x4 LDS_AS*)((uint8_t LDS_AS*)qr_sh + (wave * 2 + j) * 1024 + ql_lane * 16) = q.rope[j];
-    } else {  // used here once: the wait for them is not left to the stage loop
-      asm volatile("" : "+v"(q.rope[0]), "+v"(q.rope[1]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *(i32x4 LDS_AS*)(v_lds + (4 * wave + i) * 1024 + ql_lane * 16) = q16.nope[i];
+      lds_barrier();
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qn[c][i] = *(const i32x4 LDS_AS*)(v_lds + (4 * c + i) * 1024 + ql_lane * 16);
+      lds_barrier();  // read before the stages' V takes the place
+      // used here once: the wait for them is not left to the stage loop
+      asm volatile("" : "+v"(q16.rope[0]), "+v"(q16.rope[1]));
+      q.lim = limit_of(p, L, q16.tok);
     }
     lim_sh[wave][ql_lane & 15] = q.lim;
     const int lim_min = L - (p.causal ? p.s_q - 1 : 0);     // every row sees those below it
@@ -656,25 +646,23 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
 #pragma unroll
         for (int i = 0; i < Sh::kTiles; ++i) s[i] *= scale_log2;
       } else {
-        int ks_own = 0;  // the scale bytes of blocks g, 4 + g, 8 + g, 12 + g
+        // The words that go to LDS for V are the QK operand too.
+        f32x4 a = {0.f, 0.f, 0.f, 0.f}, l = a;
+        a = mfma_bf16(cur.rope[0], q16.rope[0], a);
+        l = mfma_bf16(cur.rope[1], q16.rope[1], l);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          ks_own |= (int)((((uint32_t)cur.scale[c] >> (8 * g)) & 0xFF) << (8 * c));
           code_in(c);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) widen_word(c, i);
+          for (int i = 0; i < 4; ++i) {
+            const i32x4 w = widen8(code[i], scale);
+            *(i32x4 LDS_AS*)(v_lds + 256 * c + (v_at ^ (16 * i))) = w;
+            if (i & 1)
+              l = mfma_bf16(w, qn[c][i], l);
+            else
+              a = mfma_bf16(w, qn[c][i], a);
+          }
         }
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, l = a;
-        a = mfma_bf16(cur.rope[0], q.rope[0], a);
-        l = mfma_scaled<0, 0>(cur.code[0], q.lo[0], l, ks_own, q.scale_lo);
-        a = mfma_bf16(cur.rope[1], q.rope[1], a);
-        l = mfma_scaled<1, 1>(cur.code[1], q.lo[1], l, ks_own, q.scale_lo);
-        a = mfma_scaled<0, 0>(cur.code[0], q.hi[0], a, ks_own, q.scale_hi);
-        l = mfma_scaled<2, 2>(cur.code[2], q.lo[2], l, ks_own, q.scale_lo);
-        a = mfma_scaled<1, 1>(cur.code[1], q.hi[1], a, ks_own, q.scale_hi);
-        l = mfma_scaled<3, 3>(cur.code[3], q.lo[3], l, ks_own, q.scale_lo);
-        a = mfma_scaled<2, 2>(cur.code[2], q.hi[2], a, ks_own, q.scale_hi);
-        a = mfma_scaled<3, 3>(cur.code[3], q.hi[3], a, ks_own, q.scale_hi);
         s[0] = (a + l) * scale_log2;
       }
       const bool ragged = tok_k + T > tok1 || tok_k + T > lim_min;
@@ -954,8 +942,7 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
     int qs_hi;
     {
       const int lane = lane_id<true>();
-      const QueryLoads<4> q_in = load_query<true, 4>(p, b, row0 + 16 * wave + (lane & 15), lane, 0);
-      const Query q = query_of<4, RT>(p, q_in, seg.L, lane, wave, 0, nullptr, nullptr);
+      const Query q = load_query<true>(p, b, row0 + 16 * wave + (lane & 15), seg.L, lane);
 #pragma unroll
       for (int c = 0; c < 4; ++c) qh[c] = q.hi[c], ql[c] = q.lo[c];
       qs_hi = q.scale_hi;
@@ -1228,10 +1215,15 @@ hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_pa
   //   128 heads: 1 sequence x 64 pages 15.0, 25.3    32 x 11 pages 23.4, 30.9    64 x 11 30.7, 36.7    64 x 22 52.5, 45.7
   //    64 heads: 1 x 64 12.0, 17.3    64 x 11 22.9, 29.9    64 x 22 32.8, 36.4      192 heads: 64 x 11 54.9, 44.0
   // Only with a schedule made for it: 16 rows with the other form's parts are more splits to merge than they save
-  // (128 heads, 32 x 11 pages: 35.0).
-  const int64_t pages = (int64_t)p.batch * (p.indices != nullptr ? pages_of(p.topk) : p.bt_width);
+  // (128 heads, 32 x 11 pages: 35.0); where a sequence is one page there are no splits, and any schedule will do, for
+  // one round of workgroups, or two against the form of 128 rows: 64 sequences x 128 heads 11.0 (20.3), 64 x 256 17.9
+  // (23.2), 64 x 64 8.2 (13.7), but 256 x 64 17.9 (16.5), 256 x 128 31.8 (27.0).
+  const int most = p.indices != nullptr ? pages_of(p.topk) : p.bt_width;  // pages of a sequence
+  const int64_t pages = (int64_t)p.batch * most;
   const int64_t tiles = (p.rows + 15) / 16;
-  const bool few = pages <= kFewPages / tiles && num_parts * tiles <= 2 * cus;
+  const int64_t round = 2 * cus;
+  const bool few = pages <= kFewPages / tiles &&
+                   (num_parts * tiles <= round || (most <= 1 && pages * tiles <= (p.rows > 64 ? 2 : 1) * round));
   const int R = few ? 16 : rows_per_workgroup(p.rows);
   if (R == 16) return launch_rt<1>(p, sched, num_parts, st);
   if (R == 64) return launch_rt<4>(p, sched, num_parts, st);

@@ -341,6 +341,19 @@ def test_sparse(gpu, H, topk, parts):
     assert_decode(out, lse, q, F4.dequantize_pages(codes, byte, rope), None, None, False, f"sparse H={H} topk={topk}", indices=idx)
 
 
+@pytest.mark.parametrize("H", [33, 64, 128, 200])
+@pytest.mark.parametrize("B", [3, 70, 200])
+def test_one_page_a_sequence(gpu, H, B):
+    """One column: no splits, whatever the schedule; with many sequences the forms for more rows again."""
+    q, cache, table, lens, kv = problem(H + B, [(7 * b) % 65 for b in range(B)], H, 1)
+    ld = lens.cuda()
+    say(f"one page H={H} B={B}")
+    sched, splits = get_mla_metadata(ld, H, 1, kv_cache=cache)
+    o, lse = flash_mla_with_kvcache(q.cuda(), cache, table.cuda(), ld, 512, sched, splits)
+    torch.cuda.synchronize()
+    assert_decode(o, lse, q, kv, table, lens, False, f"one page H={H} B={B}")
+
+
 @pytest.mark.parametrize("H", [33, 128, 200])
 def test_schedule_for_few_pages(gpu, H):
     """A schedule made with the longest length a host knows has fewer parts, and decodes the same."""
