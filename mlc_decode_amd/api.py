@@ -63,6 +63,20 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _launch(name: str, fn, device: torch.device, *args) -> None:
+    """``fn(*args, stream)`` with the tensors' device current; an error status raised."""
+    if device.index == _current_device():
+        status = fn(*args, _stream_ptr(device))
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, _stream_ptr(device))
+    if status:
+        check(name, status)
+
+
 def _require_gpu(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (the decode runs only as HIP kernels)")
@@ -191,9 +205,8 @@ def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num
             num_parts = num_parts_for(batch, 1, num_heads_per_head_k, 1)
     sched = torch.empty(num_parts, _lib.MLA_SCHED_WORDS, dtype=torch.int32, device=seqlens.device)
     splits = torch.empty(batch + 1, dtype=torch.int32, device=seqlens.device)
-    check("mla_get_metadata", _lib.load().mla_get_metadata(
-        seqlens.data_ptr(), batch, num_parts, fixed_overhead, forced_splits, sched.data_ptr(),
-        splits.data_ptr(), _stream_ptr(seqlens.device)))
+    _launch("mla_get_metadata", _lib.load().mla_get_metadata, seqlens.device, seqlens.data_ptr(), batch, num_parts,
+            fixed_overhead, forced_splits, sched.data_ptr(), splits.data_ptr())
     return sched, splits
 
 
@@ -415,9 +428,9 @@ def _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, ca
                                          sm_scale, causal, out, lse, indices, status)
     lib = _lib.load()
     if single_split:
-        check("mla_splitkv_fwd", lib.mla_splitkv_fwd(ctypes.byref(a), _stream_ptr(q.device)))
+        _launch("mla_splitkv_fwd", lib.mla_splitkv_fwd, q.device, ctypes.byref(a))
     else:
-        check("mla_decode_fwd", lib.mla_decode_fwd(ctypes.byref(a), _stream_ptr(q.device)))
+        _launch("mla_decode_fwd", lib.mla_decode_fwd, q.device, ctypes.byref(a))
     del keep
     return out, lse
 
@@ -483,9 +496,8 @@ def mla_decode_absorbed(q: torch.Tensor, kv_cache, block_table: Optional[torch.T
                                          num_splits, softmax_scale, causal, None, lse, indices)
     v = torch.empty(B, s_q, H, 128, dtype=q.dtype, device=q.device)
     lib = _lib.load()
-    st = _stream_ptr(q.device)
-    check("mla_splitkv_fwd", lib.mla_splitkv_fwd(ctypes.byref(a), st))
-    check("mla_combine_absorb", lib.mla_combine_absorb(ctypes.byref(a), w_uv_blk.data_ptr(), v.data_ptr(), st))
+    _launch("mla_splitkv_fwd", lib.mla_splitkv_fwd, q.device, ctypes.byref(a))
+    _launch("mla_combine_absorb", lib.mla_combine_absorb, q.device, ctypes.byref(a), w_uv_blk.data_ptr(), v.data_ptr())
     del keep
     if w_o is None:
         return v, lse
@@ -605,7 +617,7 @@ def kv_append(kv_new: torch.Tensor, kv_cache, block_table: torch.Tensor,
         block_table.data_ptr(), block_table.stride(0) if B > 1 else min(block_table.stride(0), 2 ** 31 - 1),
         block_table.shape[1], cache_seqlens.data_ptr(),
         status.data_ptr() if status is not None else 0, *scale_args))
-    check("mla_kv_append", _lib.load().mla_kv_append(ctypes.byref(a), _stream_ptr(kv_new.device)))
+    _launch("mla_kv_append", _lib.load().mla_kv_append, kv_new.device, ctypes.byref(a))
     return a
 
 

@@ -27,7 +27,7 @@ import torch
 from . import _lib
 from ._lib import (MLA_DIM_QK, MLA_DIM_V, MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_DTYPE_F32, MLA_KV_NATIVE, MLA_ROPE_HALF,
                    MLA_ROPE_INTERLEAVED, MlaAppendSlotsArgs, MlaKvCache, MlaPagePool, MlaRope, MlaRopeArgs, check)
-from .api import _cache_format, _check_coded_cache, _require_gpu, _split_kv, _stream_ptr
+from .api import _cache_format, _check_coded_cache, _launch, _require_gpu, _split_kv
 
 _DTYPES = {torch.bfloat16: MLA_DTYPE_BF16, torch.float16: MLA_DTYPE_F16, torch.float32: MLA_DTYPE_F32}
 _LAYOUTS = {"interleaved": MLA_ROPE_INTERLEAVED, "half": MLA_ROPE_HALF}
@@ -43,20 +43,6 @@ _APPEND = struct.Struct("=Qq4Q4q2i")
 _POOL = struct.Struct("=2Q2iQ2iQ")
 for _s, _c in ((_CACHE, MlaKvCache), (_ROPE, MlaRope), (_ROPE_ARGS, MlaRopeArgs), (_APPEND, MlaAppendSlotsArgs), (_POOL, MlaPagePool)):
     assert _s.size == ctypes.sizeof(_c)
-
-
-_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-
-
-def _launch(name: str, fn, device: torch.device, *args) -> None:
-    """``fn(*args, stream)`` with the tensors' device current; an error status raised."""
-    if device.index == _current_device():
-        status = fn(*args, _stream_ptr(device))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, _stream_ptr(device))
-    if status:
-        check(name, status)
 
 
 def _require(t: torch.Tensor, name: str, device: Optional[torch.device] = None) -> None:

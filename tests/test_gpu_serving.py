@@ -527,6 +527,35 @@ def serve(kind, steps=3, capture=False):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8", "fp4"])
+def test_serving_step_makes_its_device_current(gpu, kind, monkeypatch):
+    """Every launch of a step happens with the tensors' device current, where another one was."""
+    from mlc_decode_amd import api
+    inside, streams, stream_of = [], [], api._stream_ptr
+
+    class Guard(torch.cuda.device):
+        def __enter__(self):
+            inside.append(self.idx)
+            super().__enter__()
+
+        def __exit__(self, *exc):
+            inside.pop()
+            return super().__exit__(*exc)
+
+    def stream_ptr(device):  # a launch asks for its stream inside the guard, the workspace outside
+        streams.append(list(inside))
+        return stream_of(device)
+
+    say(f"device {kind}")
+    want, _ = serve(kind, steps=1)
+    monkeypatch.setattr(api, "_current_device", lambda: 1)  # another than the tensors'
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(api, "_stream_ptr", stream_ptr)
+    got, _ = serve(kind, steps=1)
+    assert streams.count([0]) == 6  # two reservations, two appends, schedule, decode
+    assert torch.equal(got[0][0], want[0][0]) and torch.equal(got[0][1], want[0][1])
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "fp4"])
 @pytest.mark.parametrize("capture", [False, True])
 def test_serving_steps(gpu, kind, capture):
     """Reserve, rotate and append, schedule, decode.  The decode's bar (1e-2, lse 1e-3); a rope value that the kernel
