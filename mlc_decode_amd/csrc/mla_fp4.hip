@@ -222,16 +222,15 @@ __device__ __forceinline__ QuerySplit split_query(const i32x4 (&v)[4], int g, in
 }
 
 // RT row tiles of 16 rows.  RT == 1: stages of 64 tokens, wave w takes token tile w from its loads, in registers,
-// to its scores.  RT > 1: stages of 32 tokens, copied into one of two LDS buffers in fragment order (the
+// to its scores.  RT == 4: stages of 32 tokens, copied into one of two LDS buffers in fragment order (the
 // copies of a stage are in flight during the one before), from which every wave scores; wave w converts half
-// of the dims of token tile w % 2 and scores row tile w % RT against kTiles token tiles.
+// of the dims of token tile w % 2 and scores row tile w against both token tiles.
 template <int RT>
 struct Shape {
   static constexpr int T = RT == 1 ? 64 : 32;
   static constexpr int kTokTiles = T / 16;
   static constexpr int kTiles = RT * kTokTiles / 4;  // score tiles per wave
   static constexpr int kShare = 4 / RT;              // waves that share a row tile
-  static constexpr int kChunks = RT == 1 ? 4 : 2;    // 128-dim chunks a wave converts of its tokens
 };
 
 // RT == 1: a stage's loads of one lane.
@@ -241,7 +240,7 @@ struct Stage {
   i32x4 scale;
 };
 
-// RT > 1: a stage in LDS: per token tile four 1 KiB code fragments and two of rope, then the tokens' scale bytes.
+// RT == 4: a stage in LDS: per token tile four 1 KiB code fragments and two of rope, then the tokens' scale bytes.
 constexpr int kRawTile = 6 * 1024;
 constexpr int kRawScale = 2 * kRawTile;
 constexpr int kRawStage = kRawScale + 512;
@@ -820,7 +819,8 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
 // wave scores stage k and converts its share of V, P^T and V of stage k - 1 lie in the other half of two
 // buffers, and their product is interleaved with the softmax of stage k.  V is converted once for 128 rows.
 // (Two 64-row workgroups a CU: 64 x 128 heads x 4096 tokens 97 us, 32 x 2 x 128 x 16384 303; the first form of this
-// kernel, which formed every address anew, 88 and 263, this one 82 and 240, all on one card.)
+// kernel, which formed every address anew, 88 and 263, with the addresses kept 82 and 240, and with rows stored as 16
+// bytes a lane 80 and 235.)
 // What bounds it is instruction issue: a SIMD's MFMA time and the vector instructions beyond two per MFMA add up
 // (measured: two waves of one bf16 MFMA and 2, 4, 8 additions a step take 18.5, 26, 37 cycles a step), so the loop
 // keeps its lane addresses, takes buffer halves as constants (two stages a turn) and page addresses as scalars.

@@ -396,6 +396,32 @@ def test_absorbed_and_noalloc_agree_with_the_decode(gpu):
     assert ((v.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * mag).all()
 
 
+@pytest.mark.parametrize("H", [16, 64, 128])
+@pytest.mark.parametrize("few", [False, True])
+def test_two_graphs_of_one_decode(gpu, H, few):
+    """Schedule and decode captured twice on one stream (they share a workspace), replayed in turn with lengths that change in
+    place and eager decodes between: each replay is the eager call's result bit for bit."""
+    q, cache, table, lens, _ = problem(8, [1000, 300, 64, 5], H, 1, poison=False)
+    table = table_for(table, H, few).cuda()
+    qd, ld = [q.cuda(), q.flip(0).cuda()], lens.cuda()
+    say(f"two graphs H={H} few={few}")
+    eager = lambda i: mla_decode_with_kvcache(qd[i], cache, table, ld)  # noqa: E731
+    eager(0)
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            held.append(eager(i))
+    for new in ([1000, 300, 64, 5], [0, 1, 63, 64], [512, 299, 1, 0], [1000, 300, 64, 5]):
+        ld.copy_(torch.tensor(new, dtype=torch.int32))
+        for i in (0, 1):
+            graphs[i].replay()
+            out, lse = (t.clone() for t in held[i])
+            want = eager(i)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1]), f"graph {i} lens {new}"
+
+
 @pytest.mark.parametrize("few", [False, True])
 def test_same_result_on_another_stream_and_twice(gpu, few):
     H = 128
