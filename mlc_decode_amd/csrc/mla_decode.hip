@@ -249,6 +249,8 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // a save/restore: M0 is a reserved register, which clang does not preserve for a clobber, and
 // nothing else in these kernels reads it (no LDS-DMA builtins, message sends or relative
 // register moves; the generated code has no M0 reader besides these copies).
+// The copy needs one wait state after the write of M0, which the compiler adds for the builtin
+// only: the s_nop 0 in each of these helpers.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t lds_addr) {
@@ -261,6 +263,7 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t 
   const uint64_t sbase = ((uint64_t)hi << 32) | (uint64_t)lo;
   asm volatile(
       "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
       "global_load_lds_dwordx4 %0, %1 nt"
       :
       : "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
@@ -280,6 +283,7 @@ __device__ __forceinline__ void dma16_m0(uint64_t sbase, uint32_t voff, uint32_t
   if constexpr (NT) {
     asm volatile(
         "s_add_u32 m0, %2, %3\n\t"
+        "s_nop 0\n\t"
         "global_load_lds_dwordx4 %0, %1 offset:%4 nt"
         :
         : "v"(voff), "s"(sbase), "s"(lds_base), "i"(LDS_OFF - GOFF), "i"(GOFF)
@@ -287,6 +291,7 @@ __device__ __forceinline__ void dma16_m0(uint64_t sbase, uint32_t voff, uint32_t
   } else {
     asm volatile(
         "s_add_u32 m0, %2, %3\n\t"
+        "s_nop 0\n\t"
         "global_load_lds_dwordx4 %0, %1 offset:%4"
         :
         : "v"(voff), "s"(sbase), "s"(lds_base), "i"(LDS_OFF - GOFF), "i"(GOFF)
@@ -298,6 +303,7 @@ __device__ __forceinline__ void dma16_m0(uint64_t sbase, uint32_t voff, uint32_t
 __device__ __forceinline__ void dma16_lane(const void* addr, uint32_t lds_addr) {
   asm volatile(
       "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
       "global_load_lds_dwordx4 %0, off nt"
       :
       : "v"(addr), "s"(__builtin_amdgcn_readfirstlane(lds_addr))
@@ -307,6 +313,7 @@ __device__ __forceinline__ void dma16_lane(const void* addr, uint32_t lds_addr) 
 __device__ __forceinline__ void dma4_m0(uint64_t sbase, uint32_t voff, uint32_t lds_base) {
   asm volatile(
       "s_mov_b32 m0, %2\n\t"
+      "s_nop 0\n\t"
       "global_load_lds_dword %0, %1"
       :
       : "v"(voff), "s"(sbase), "s"(lds_base)
@@ -318,6 +325,7 @@ __device__ __forceinline__ void dma16_lane_m0(uint64_t addr, uint32_t lds_base) 
   static_assert(GOFF >= 0 && GOFF < 4096 && LDS_OFF - GOFF > -65536, "immediate offset range");
   asm volatile(
       "s_add_u32 m0, %1, %2\n\t"
+      "s_nop 0\n\t"
       "global_load_lds_dwordx4 %0, off offset:%3 nt"
       :
       : "v"(addr), "s"(lds_base), "i"(LDS_OFF - GOFF), "i"(GOFF)
@@ -327,6 +335,7 @@ __device__ __forceinline__ void dma16_lane_m0(uint64_t addr, uint32_t lds_base) 
 __device__ __forceinline__ void dma4_lane(const void* addr, uint32_t lds_addr) {
   asm volatile(
       "s_mov_b32 m0, %1\n\t"
+      "s_nop 0\n\t"
       "global_load_lds_dword %0, off nt"
       :
       : "v"(addr), "s"(__builtin_amdgcn_readfirstlane(lds_addr))

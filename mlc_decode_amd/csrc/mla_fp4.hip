@@ -62,20 +62,21 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 
 // One wave's copy from HBM into LDS, 16 (or 4) bytes a lane: lane l's bytes land at lds + 16 l (4 l).  Inline asm,
 // so that the compiler, which takes the builtin for an LDS store, does not wait for every copy in flight before
-// it reads LDS; copies_landed() is the wait.  M0 is written without a save: nothing else here reads it.
+// it reads LDS; copies_landed() is the wait.  M0 is written without a save: nothing else here reads it; the copy
+// needs one wait state after the write (s_nop 0), which the compiler would add for the builtin only.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy16(const void* lane_addr, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void copy16(uint64_t base, uint32_t lane_off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(uint64_t base, uint32_t lane_off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(lane_off), "s"(base), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void copy4(const void* lane_addr, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(lane_addr), "s"(lds) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 __device__ __forceinline__ void copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
