@@ -137,19 +137,29 @@ __device__ __forceinline__ f32x4 mfma32(i32x4 a, i32x4 b, f32x4 c) {
 // (256 registers) already fills the AGPR file.  Operands come straight from LDS / global
 // loads; the chain is volatile so no compiler VALU lands between its MFMAs, and
 // qk_settle() adds the wait states an MFMA result needs before a VALU may read it.
-template <int DT>
+// FRESH: an operand may be the result of a VALU instruction right before (the fp8 conversions, a
+// register back from the AGPR file), after which the MFMA needs two wait states.
+template <int DT, bool FRESH = false>
 __device__ __forceinline__ void mfma_qk_first(f32x4& acc, const i32x4& a, const i32x4& b) {
-  if constexpr (DT == MLA_DTYPE_BF16)
+  if constexpr (FRESH) {
+    static_assert(DT == MLA_DTYPE_BF16, "the fp8 cache is read with bf16 queries");
+    asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(a), "v"(b));
+  } else if constexpr (DT == MLA_DTYPE_BF16) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=&v"(acc) : "v"(a), "v"(b));
-  else
+  } else {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, 0" : "=&v"(acc) : "v"(a), "v"(b));
+  }
 }
-template <int DT>
+template <int DT, bool FRESH = false>
 __device__ __forceinline__ void mfma_qk(f32x4& acc, const i32x4& a, const i32x4& b) {
-  if constexpr (DT == MLA_DTYPE_BF16)
+  if constexpr (FRESH) {
+    static_assert(DT == MLA_DTYPE_BF16, "the fp8 cache is read with bf16 queries");
+    asm volatile("s_nop 1\n\tv_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
+  } else if constexpr (DT == MLA_DTYPE_BF16) {
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
-  else
+  } else {
     asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(acc) : "v"(a), "v"(b));
+  }
 }
 // 32 wait states after the last QK MFMA: covers the MFMA-result -> VALU-read latency and the
 // passes during which the last MFMAs still read their A/B operands.
@@ -1281,10 +1291,9 @@ void mla_splitkv_kernel(const int32_t* __restrict__ sched, KParams p) {
         };
         if constexpr (kInl8) {
           // The converted fragments are VALU results read by the (inline-asm) MFMAs, whose
-          // hazards the compiler does not see.  Fragment n+1 is converted before MFMA n issues
-          // (so an MFMA separates every conversion from its reader), and fragment n-1 is held
-          // live until MFMA n has issued (so no conversion overwrites the operands of the MFMA
-          // just issued).
+          // hazards the compiler does not see: each MFMA brings its own wait states for them.
+          // Fragment n+1 is converted before MFMA n issues, and fragment n-1 is held live until
+          // MFMA n has issued (so no conversion overwrites the operands of the MFMA just issued).
           auto k8_conv = [&](int n, const i32x4& raw) __attribute__((always_inline)) -> i32x4 {
             if ((n >> 1) < 16) {
               const int r0 = raw.x, r1 = raw.y;
@@ -1307,9 +1316,9 @@ void mla_splitkv_kernel(const int32_t* __restrict__ sched, KParams p) {
 #pragma unroll
             for (int ht = 0; ht < HT; ++ht) {
               if (n < 2)
-                mfma_qk_first<DT>(acc[ht][n & 1], c_cur, qf[ht][n >> 1]);
+                mfma_qk_first<DT, true>(acc[ht][n & 1], c_cur, qf[ht][n >> 1]);
               else
-                mfma_qk<DT>(acc[ht][n & 1], c_cur, qf[ht][n >> 1]);
+                mfma_qk<DT, true>(acc[ht][n & 1], c_cur, qf[ht][n >> 1]);
             }
             asm volatile("" ::"v"(c_prev));
             __builtin_amdgcn_sched_barrier(0);
