@@ -104,6 +104,8 @@ __device__ __forceinline__ int lane_id() {
   return l;
 }
 // The maximum without fmaxf's canonicalising of each operand (scores are no signalling NaNs; a quiet one is passed over).
+// Its operands come from ordinary vector instructions, or from MFMAs through settled(): the compiler does not see
+// what asm reads, and keeps the wait states after an MFMA for its own instructions only.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -114,6 +116,8 @@ __device__ __forceinline__ float max2(float a, float b) {
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
   return r;
 }
+// The results of the scaled MFMAs that were issued last, 12 wait states on.
+__device__ __forceinline__ void settled(f32x4 (&s)[2]) { asm volatile("s_nop 7\n\ts_nop 3" : "+v"(s[0]), "+v"(s[1])); }
 // over the four lane groups that hold one row
 __device__ __forceinline__ float row_max(float v) { return xor32(xor16(v, false), false); }
 __device__ __forceinline__ float row_sum(float v) { return xor32(xor16(v, true), true); }
@@ -1060,6 +1064,7 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
         }
         if constexpr (SOFT) {
           if (r == 0) {
+            settled(s);
             top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max2(s[1][2], s[1][3]));
             const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = max2(__uint_as_float(x[0]), __uint_as_float(x[1]));

@@ -176,7 +176,7 @@ def early(library):
     return [(rule, f"{name}+{at:x}: {what}") for name, body in library for rule, at, what in violations(body)]
 
 
-@pytest.mark.parametrize("rule", ["copy", "operand"])
+@pytest.mark.parametrize("rule", ["copy", "operand", "result"])
 def test_wait_states_of_every_kernel(early, rule):
     bad = [what for r, what in early if r == rule]
     assert not bad, f"{len(bad)} places, first:\n" + "\n".join(bad[:20])
