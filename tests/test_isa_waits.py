@@ -8,7 +8,9 @@ counts the wait states on all paths, by the numbers that the compiler itself kee
 * a scalar write of M0, then a copy into LDS: 1;
 * an MFMA's result, then a vector instruction, a store or an LDS write that reads or overwrites it: 8 for
   16x16x32 and smaller, 12 for the scaled 16x16x128, 20 for everything larger;
-* a vector instruction's result, then an MFMA that reads it: 2.
+* a vector instruction's result, then an MFMA, a lane swap or a DPP operand that reads it: 2;
+* the result of a transcendental, then any other vector instruction that reads it: 1;
+* a scalar register that a vector instruction wrote, then a load, copy or store that takes its address from it: 5.
 """
 import os
 import re
@@ -22,7 +24,9 @@ from mlc_decode_amd import build as B
 TOOL = shutil.which("llvm-objdump") or "/opt/rocm/llvm/bin/llvm-objdump"
 _LINE = re.compile(r"^\t(\S+)\s*(.*?)\s*// ([0-9A-F]+):.*?(?:<\S+?(?:\+0x([0-9a-f]+))?>)?$")
 _HEAD = re.compile(r"^([0-9a-f]+) <(\S+)>:$")
-_REG = re.compile(r"(?<![\w.])([va])(?:(\d+)\b|\[(\d+):(\d+)\])")
+_REG = re.compile(r"(?<![\w.])([vas])(?:(\d+)\b|\[(\d+):(\d+)\])")
+TRANS = ("v_exp_", "v_log_", "v_rcp_", "v_rsq_", "v_sqrt_", "v_sin_", "v_cos_")
+MEMORY = ("global_", "buffer_", "flat_", "scratch_")
 STORES = ("global_store", "buffer_store", "flat_store", "scratch_store", "ds_write", "global_atomic", "buffer_atomic", "flat_atomic")
 
 
@@ -33,7 +37,7 @@ def registers(text):
 
 
 class Instruction:
-    __slots__ = ("op", "text", "at", "target", "writes", "reads", "mfma", "valu", "m0", "copy", "states")
+    __slots__ = ("op", "text", "at", "target", "writes", "reads", "mfma", "valu", "m0", "copy", "states", "special", "base")
 
     def __init__(self, op, rest, at, target):
         self.op, self.text, self.at, self.target = op, f"{op} {rest}", at, target
@@ -43,6 +47,8 @@ class Instruction:
         self.copy = op.startswith(("global_load_lds", "buffer_load")) and ("_lds_" in op or " lds" in rest)
         self.m0 = op.startswith("s_") and first == "m0"
         self.states = int(rest, 0) + 1 if op == "s_nop" else 1
+        self.special = "swap" if op.startswith("v_permlane") else "dpp" if self.valu and "_dpp" in op else "trans" if op.startswith(TRANS) else None
+        self.base = frozenset(r for r in registers(rest) if r[0] == "s") if op.startswith(MEMORY) else frozenset()
         if self.mfma or self.valu:
             swaps = "swap" in op  # both operands are read and written
             self.writes = frozenset(registers(rest if swaps else first))
@@ -73,32 +79,41 @@ def kernels(listing):
 
 
 def advance(ins, pending, found):
-    """`pending`: wait states still missing, by ("m0",), ("mfma", register) or ("valu", register); updated in place."""
+    """`pending`: wait states still missing, by ("m0",) or (what wrote it, register); updated in place."""
+    def too_early(kind, regs, rule, verb):
+        for r in regs:
+            if (kind, r) in pending:
+                found.add((rule, ins.at, f"{ins.text}: {verb} {r[0]}{r[1]} {pending[kind, r]} wait states too early"))
+
     if pending:
         if ins.copy and ("m0",) in pending:
             found.add(("copy", ins.at, f"{ins.text}: right behind the write of m0"))
+        too_early("scalar", ins.base, "address", "takes its address from")
         if ins.mfma:
-            for r in ins.reads:
-                if ("valu", r) in pending:
-                    found.add(("operand", ins.at, f"{ins.text}: reads {r[0]}{r[1]} {pending['valu', r]} wait states too early"))
+            too_early("valu", ins.reads, "operand", "reads")
         else:
-            for r in ins.reads | ins.writes:
-                if ("mfma", r) in pending:
-                    found.add(("result", ins.at, f"{ins.text}: meets the result {r[0]}{r[1]} {pending['mfma', r]} wait states too early"))
+            too_early("mfma", ins.reads | ins.writes, "result", "meets the result")
+        if ins.special in ("swap", "dpp"):
+            too_early("valu", ins.reads, "lanes", "reads")
+        if ins.valu and ins.special != "trans":
+            too_early("trans", ins.reads, "transcendental", "reads")
         for k in list(pending):
             pending[k] -= ins.states
             if pending[k] <= 0:
                 del pending[k]
     if ins.m0:
         pending[("m0",)] = 1
-    if ins.mfma:
-        for r in ins.writes:
-            pending.pop(("valu", r), None)
-            pending[("mfma", r)] = ins.result_wait()
-    elif ins.valu:
-        for r in ins.writes:
-            pending.pop(("mfma", r), None)
-            pending[("valu", r)] = 2
+    for r in ins.writes:
+        for kind in ("mfma", "valu", "trans", "scalar"):
+            pending.pop((kind, r), None)
+        if ins.mfma:
+            pending["mfma", r] = ins.result_wait()
+        elif r[0] == "s":
+            pending["scalar", r] = 5
+        else:
+            pending["valu", r] = 2
+            if ins.special == "trans":
+                pending["trans", r] = 1
 
 
 def violations(body):
@@ -152,6 +167,12 @@ def test_rules_on_small_listings():
     assert len(run(mfma, "s_nop 5", ("s_cbranch_scc1 1", 16), "s_nop 0", "v_add_f32_e32 v9, v0, v0")) == 1  # on the taken path alone
     assert len(run("v_mov_b32_e32 v8, v20", "s_nop 0", mfma)) == 1 and not run("v_mov_b32_e32 v8, v20", "s_nop 1", mfma)
     assert len(run("v_permlane16_swap_b32 v20, v8", mfma)) == 1
+    assert len(run("v_max_f32_e32 v7, v6, v5", "v_mov_b32_e32 v8, v9", "v_permlane32_swap_b32_e32 v7, v1")) == 1
+    assert len(run("v_max_f32_e32 v7, v6, v5", "v_mov_b32_dpp v1, v7 row_ror:8")) == 1 and not run("v_max_f32_e32 v7, v6, v5", "s_nop 1", "v_mov_b32_dpp v1, v7 row_ror:8")
+    assert len(run("v_exp_f32_e32 v7, v6", "v_mul_f32_e32 v1, v7, v7")) == 1 and not run("v_exp_f32_e32 v7, v6", "v_exp_f32_e32 v8, v7")
+    assert len(run("v_readfirstlane_b32 s5, v1", "s_nop 3", "global_load_dword v1, v0, s[4:5]")) == 1
+    assert not run("v_readfirstlane_b32 s5, v1", "s_nop 4", "global_load_dword v1, v0, s[4:5]")
+    assert not run("v_readfirstlane_b32 s5, v1", "s_add_u32 s4, s5, s6", "global_load_dword v1, v0, s[2:3]")
 
 
 @pytest.fixture(scope="module")
@@ -176,7 +197,7 @@ def early(library):
     return [(rule, f"{name}+{at:x}: {what}") for name, body in library for rule, at, what in violations(body)]
 
 
-@pytest.mark.parametrize("rule", ["copy", "operand", "result"])
+@pytest.mark.parametrize("rule", ["copy", "operand", "result", "address", "lanes", "transcendental"])
 def test_wait_states_of_every_kernel(early, rule):
     bad = [what for r, what in early if r == rule]
     assert not bad, f"{len(bad)} places, first:\n" + "\n".join(bad[:20])
