@@ -39,18 +39,21 @@ struct Cache {
 // ---------------------------------------------------------------------------------------
 struct Bf16 {
   static constexpr int kBytes = 2;
-  __device__ static float get(const uint8_t* p) { return __uint_as_float((uint32_t) * (const uint16_t*)p << 16); }
-  __device__ static void put(uint8_t* p, float v) { *(__bf16*)p = (__bf16)v; }
+  typedef uint16_t bits;
+  __device__ static float value(bits b) { return __uint_as_float((uint32_t)b << 16); }
+  __device__ static bits of(float v) { return __builtin_bit_cast(bits, (__bf16)v); }
 };
 struct F16 {
   static constexpr int kBytes = 2;
-  __device__ static float get(const uint8_t* p) { return (float)*(const _Float16*)p; }
-  __device__ static void put(uint8_t* p, float v) { *(_Float16*)p = (_Float16)v; }
+  typedef uint16_t bits;
+  __device__ static float value(bits b) { return (float)__builtin_bit_cast(_Float16, b); }
+  __device__ static bits of(float v) { return __builtin_bit_cast(bits, (_Float16)v); }
 };
 struct F32 {
   static constexpr int kBytes = 4;
-  __device__ static float get(const uint8_t* p) { return *(const float*)p; }
-  __device__ static void put(uint8_t* p, float v) { *(float*)p = v; }
+  typedef uint32_t bits;
+  __device__ static float value(bits b) { return __uint_as_float(b); }
+  __device__ static bits of(float v) { return __float_as_uint(v); }
 };
 
 // 16 bytes to floats and back (8 values, or 4 of fp32)
@@ -104,6 +107,13 @@ __device__ __forceinline__ void rotate(float& a, float& b, f32x2 cs) {
   b = a * cs[1] + b * cs[0];
   a = x;
 }
+template <class E>
+__device__ __forceinline__ void rotate_bits(typename E::bits& a, typename E::bits& b, f32x2 cs) {
+  float x = E::value(a), y = E::value(b);
+  rotate(x, y, cs);
+  a = E::of(x);
+  b = E::of(y);
+}
 
 // Item `i` of [tokens][heads][items] as (t, h, it), in steps of 256 items without a division.
 struct Walk {
@@ -142,13 +152,15 @@ struct RopeParams {
 
 // 256 threads take `tile` tokens (tile * rot / 2 <= kPairs): each pair's cosine and sine once per token into LDS,
 // then every head.  VEC: 16-byte chunks; a chunk of the rotated dims holds whole pairs (interleaved), or is
-// taken together with the chunk half the rotated dims further on (half layout).
+// taken together with the chunk half the rotated dims further on (half layout).  A token without a position is copied
+// bit for bit: by a turn of zero an infinity or a NaN would spread to its pair, and -0 could become 0.
 // Bound by memory: 8191 tokens x 32 heads of 128 fp16 dims, 64 of them rotated, 23.0 us (134 MB; 24.8 with one chunk
 // a thread in flight and a division an item, 23.4 with four chunks).  128 tokens x 128 heads: 3.8 us, a launch.
-constexpr int kPairs = 512;
+constexpr int kPairs = 512, kRopeTile = 8;
 template <class E, bool VEC>
 __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
   __shared__ f32x2 cs[kPairs];
+  __shared__ bool still[kRopeTile];  // the token has no position
   const int pairs = p.rot / 2;
   const int wg = blockIdx.x / p.split, sub = blockIdx.x - wg * p.split;
   const int t0 = wg * p.tile;
@@ -156,7 +168,8 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
   for (int i = threadIdx.x; i < nt * pairs; i += 256) {
     const int t = i / pairs;
     const int pos = p.positions[t0 + t];
-    cs[i] = pos < 0 ? f32x2{1.f, 0.f} : turn(pos, p.freqs[i - t * pairs], p.amp);
+    cs[i] = turn(pos, p.freqs[i - t * pairs], p.amp);
+    still[t] = pos < 0;
   }
   __syncthreads();
   const int h0 = (int)((int64_t)p.heads * sub / p.split), h1 = (int)((int64_t)p.heads * (sub + 1) / p.split);
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
     for (int i = threadIdx.x; i < total; i += 256 * U) {
       i32x4 v[U], w[U];
       uint8_t* dst[U];
-      int pair[U];  // the chunk's first pair among its tile's, -1: a chunk that is copied
+      int pair[U];  // the chunk's first pair among its tile's, -1: a chunk that is copied, -2: with its other half
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + 256 * u < total) {
@@ -185,7 +198,7 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
           const int a = (turns ? p.first + at.it * W : c < lead ? c * W : p.first + p.rot + (c - lead) * W) * E::kBytes;
           const uint8_t* src = p.x + (int64_t)(t0 + at.t) * p.x_st + (int64_t)(h0 + at.h) * p.x_sh + a;
           dst[u] = p.out + (int64_t)(t0 + at.t) * p.o_st + (int64_t)(h0 + at.h) * p.o_sh + a;
-          pair[u] = turns ? at.t * pairs + at.it * (p.half ? W : W / 2) : -1;
+          pair[u] = !turns ? -1 : still[at.t] ? -2 : at.t * pairs + at.it * (p.half ? W : W / 2);
           v[u] = *(const i32x4*)src;
           if (p.half && turns) w[u] = *(const i32x4*)(src + pairs * E::kBytes);
         }
@@ -208,6 +221,8 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
             for (int j = 0; j < W / 2; ++j) rotate(x[2 * j], x[2 * j + 1], c[j]);
           }
           v[u] = pack<E>(x);
+        } else if (p.half && pair[u] == -2) {
+          *(i32x4*)(dst[u] + pairs * E::kBytes) = w[u];
         }
         *(i32x4*)dst[u] = v[u];
       }
@@ -218,17 +233,14 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
       uint8_t* dst = p.out + (int64_t)(t0 + at.t) * p.o_st + (int64_t)(h0 + at.h) * p.o_sh;
       if (at.it < rot_items) {
         const int a = (p.first + (p.half ? at.it : 2 * at.it)) * E::kBytes, b = a + (p.half ? pairs : 1) * E::kBytes;
-        float x = E::get(src + a), y = E::get(src + b);
-        rotate(x, y, cs[at.t * pairs + at.it]);
-        E::put(dst + a, x);
-        E::put(dst + b, y);
+        typename E::bits x = *(const typename E::bits*)(src + a), y = *(const typename E::bits*)(src + b);
+        if (!still[at.t]) rotate_bits<E>(x, y, cs[at.t * pairs + at.it]);
+        *(typename E::bits*)(dst + a) = x;
+        *(typename E::bits*)(dst + b) = y;
       } else {
         const int c = at.it - rot_items;
         const int a = (c < lead ? c : p.first + p.rot + (c - lead)) * E::kBytes;
-        if constexpr (E::kBytes == 4)
-          *(uint32_t*)(dst + a) = *(const uint32_t*)(src + a);
-        else
-          *(uint16_t*)(dst + a) = *(const uint16_t*)(src + a);
+        *(typename E::bits*)(dst + a) = *(const typename E::bits*)(src + a);
       }
     }
   }
@@ -319,13 +331,14 @@ struct AppendParams {
 
 // Workgroups of four waves take `tile` tokens: the 32 pairs' cosines and sines of each token into LDS, a
 // wave per token for its cache row, and all threads for the queries' rope dims in 16-byte chunks.  One launch for
-// the three.  Bound by memory where there is any: 76 MB of a ragged prefill (16 heads, 4-bit cache) in 15.7 us, 4.8
+// the three.  What is not rotated is copied bit for bit.  Bound by memory where there is any: 76 MB of a ragged prefill (16 heads, 4-bit cache) in 15.7 us, 4.8
 // TB/s, a large copy's rate; a decode step's 128 tokens x 64 heads 3.7 us.
 constexpr int kAppendTile = 8;
 template <class E>
 __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
   __shared__ f32x2 cs[kAppendTile][32];
   __shared__ int32_t slot_sh[kAppendTile];  // -1: names no row
+  __shared__ bool still[kAppendTile];       // the token has no position
   const int t0 = blockIdx.x * p.tile;
   const int nt = p.tokens - t0 < p.tile ? p.tokens - t0 : p.tile;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -337,12 +350,13 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
     const int t = threadIdx.x >> 5;
     if (t < nt) {
       const int pos = p.positions[t0 + t];
-      cs[t][threadIdx.x & 31] = pos < 0 ? f32x2{1.f, 0.f} : turn(pos, p.freqs[threadIdx.x & 31], p.amp);
+      cs[t][threadIdx.x & 31] = turn(pos, p.freqs[threadIdx.x & 31], p.amp);
+      still[t] = pos < 0;
     }
   }
   // a wave's tokens, loaded together, whatever their slots
   i32x4 v[kAppendTile / 4];
-  float x[kAppendTile / 4], y[kAppendTile / 4];
+  uint16_t x[kAppendTile / 4], y[kAppendTile / 4];
   const int rope_a = (p.half ? lane : 2 * lane) * 2, rope_b = rope_a + (p.half ? 64 : 2);  // a rope pair per lane < 32
 #pragma unroll
   for (int u = 0; u < kAppendTile / 4; ++u) {
@@ -350,7 +364,7 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
     if (t < nt) {  // uniform
       const uint8_t* src = p.kv_new + (int64_t)(t0 + t) * p.n_st;
       v[u] = *(const i32x4*)(src + 16 * lane);
-      if (lane < 32) x[u] = E::get(src + 2 * kDV + rope_a), y[u] = E::get(src + 2 * kDV + rope_b);
+      if (lane < 32) x[u] = *(const uint16_t*)(src + 2 * kDV + rope_a), y[u] = *(const uint16_t*)(src + 2 * kDV + rope_b);
     }
   }
   __syncthreads();
@@ -363,10 +377,10 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
     const int64_t page = slot / kPage;
     const int row = (int)(slot % kPage);
     if (lane < 32) {
-      if (p.freqs != nullptr) rotate(x[u], y[u], cs[t][lane]);
+      if (p.freqs != nullptr && !still[t]) rotate_bits<E>(x[u], y[u], cs[t][lane]);
       uint8_t* dst = p.cache.rope + page * p.cache.rp + row * p.cache.rt;
-      E::put(dst + rope_a, x[u]);
-      E::put(dst + rope_b, y[u]);
+      *(uint16_t*)(dst + rope_a) = x[u];
+      *(uint16_t*)(dst + rope_b) = y[u];
     }
     put_latent(p.cache, page, row, lane, v[u]);
   }
@@ -380,7 +394,8 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
   for (int i = first; i < total; i += 256 * U) {
     i32x4 a[U], b[U];
     uint8_t* dst[U];
-    const f32x2* turns[U];
+    const f32x2* turns[U];  // null: no row
+    bool copied[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       turns[u] = nullptr;
@@ -388,6 +403,7 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
         const uint8_t* src = p.q_pe + (int64_t)(t0 + at.t) * p.pe_st + (int64_t)at.h * p.pe_sh + 16 * at.it;
         dst[u] = p.q + (int64_t)(t0 + at.t) * p.q_st + (int64_t)at.h * p.q_sh + 16 * at.it;
         turns[u] = &cs[at.t][(p.half ? 8 : 4) * at.it];
+        copied[u] = still[at.t];
         a[u] = *(const i32x4*)src;
         if (p.half) b[u] = *(const i32x4*)(src + 64);
       }
@@ -396,6 +412,11 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (turns[u] == nullptr) continue;
+      if (copied[u]) {
+        *(i32x4*)dst[u] = a[u];
+        if (p.half) *(i32x4*)(dst[u] + 64) = b[u];
+        continue;
+      }
       float x[8], y[8];
       unpack<E>(a[u], x);
       if (p.half) {
@@ -869,7 +890,7 @@ int mla_apply_rope(const mla_rope* rope, const mla_rope_args* a, void* stream) {
   // tokens their heads are split, up to 512 workgroups: 128 tokens x 128 heads 4.8 us (7.3 without, 5.3 with 2048),
   // 16 x 128 3.3 (4.2 with 2048).
   int tile = kPairs / pairs;
-  tile = tile < 8 ? tile : 8;
+  tile = tile < kRopeTile ? tile : kRopeTile;
   while (tile > 1 && (a->tokens + tile - 1) / tile < 1024) tile >>= 1;
   const int groups = (a->tokens + tile - 1) / tile;
   int split = 1;
