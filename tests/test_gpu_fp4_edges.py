@@ -1,0 +1,144 @@
+"""GPU tests of the 4-bit cache where its decode's three forms (16, 64 and 128 rows a workgroup) could part: references that
+move, NaN blocks that some rows do not see, page ids that name no page, segments of many pages, queries with
+outliers, the largest latents, and the projections on top of it."""
+import math
+
+import pytest
+import torch
+
+from mlc_decode_amd import (flash_mla_with_kvcache, get_mla_metadata, mla_decode_absorbed, mla_decode_with_kvcache,
+                            prepare_w_uv)
+from oracle import mla_fp4_ref as F4
+from test_gpu_fp4 import SCALE, assert_decode, problem, say, table_for, to_gpu
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("H", [16, 64, 128])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_rising_and_falling_scores(gpu, H, splits):
+    """Each page's scores pass the last one's by far, so that the running reference moves with nearly every stage, for
+    every row tile; and the other way round, where it never moves again.  Rows of one tile move apart: odd
+    heads rise where even ones fall."""
+    q, cache, table, lens, _ = problem(3, [1500, 1500, 1500], H, 1)
+    codes, byte, rope = cache.latent.cpu().numpy(), cache.scale.cpu().numpy(), cache.rope.cpu()
+    q[..., 512:] = q[..., 512:].abs() + 0.5
+    q[2, :, 1::2, 512:] *= -1
+    for b in range(3):
+        for i in range(24):
+            rope[int(table[b, i])] = 0.5 * (23 - i if b == 1 else i)
+    cache = cache._replace(rope=rope.cuda())
+    table = table_for(table, H, False)
+    say(f"rising H={H} splits={splits}")
+    out, lse = mla_decode_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), num_splits=splits)
+    torch.cuda.synchronize()
+    assert_decode(out, lse, q, F4.dequantize_pages(codes, byte, rope), table, lens, True, f"rising H={H} splits={splits}")
+
+
+@pytest.mark.parametrize("H", [16, 20, 64, 128])
+@pytest.mark.parametrize("splits", [1, 2])
+def test_nan_block_in_each_form(gpu, H, splits):
+    q, cache, table, lens, kv = problem(44, [100, 100, 700], H, 1)
+    cache.scale[int(table[0, 0]), 7, 3] = 255
+    cache.scale[int(table[2, 9]), 63, 15] = 255
+    table = table_for(table, H, False)
+    say(f"NaN block H={H} splits={splits}")
+    out, lse = mla_decode_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), num_splits=splits)
+    torch.cuda.synchronize()
+    assert torch.isnan(out[::2]).all() and (lse[::2] == -math.inf).all()
+    assert_decode(out[1:2], lse[1:2], q[1:2], kv, table[1:2], lens[1:2], True, f"beside NaNs H={H}")
+
+
+@pytest.mark.parametrize("H", [16, 64, 128])
+def test_cut_at_the_table_and_foreign_pages(gpu, H):
+    """Page ids that name no page are clamped into the pool, in the first, a middle and the last page that is read."""
+    q, cache, table, lens, kv = problem(12, [640, 300, 64 * 90], H, 1, poison=False)
+    table = table_for(table, H, False).clone()
+    table[0, 0], table[0, 5], table[1, 4] = -3, 10 ** 6, 2 ** 31 - 1
+    table[2, 0], table[2, 70], table[2, 89] = 2 ** 31 - 1, -2 ** 31, kv.shape[0]
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    say(f"foreign pages H={H}")
+    for parts in (None, 1):
+        sched, splits = get_mla_metadata(lens.cuda(), H, 1, parts)
+        out, lse = flash_mla_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), 512, sched, splits, status=status)
+        torch.cuda.synchronize()
+        assert status.item() == 0
+        assert_decode(out, lse, q, kv, table, lens, False, f"foreign H={H} parts={parts}")
+    long = lens + 64 * table.shape[1]  # every sequence is cut
+    sched, splits = get_mla_metadata(long.cuda(), H, 1)
+    flash_mla_with_kvcache(q.cuda(), cache, table.cuda(), long.cuda(), 512, sched, splits, status=status)
+    torch.cuda.synchronize()
+    assert status.item() == 1
+
+
+@pytest.mark.parametrize("H", [16, 64, 128])
+def test_many_pages_in_one_segment(gpu, H):
+    """More than two wavefronts' worth of pages in one part, a ragged last one, and ids that name no page."""
+    q, cache, table, lens, kv = problem(77, [64 * 150 + 7, 64 * 129], H, 1, poison=False)
+    table = table_for(table, H, False)
+    table[0, 63], table[0, 64], table[0, 127], table[0, 128], table[1, 64] = -1, 10 ** 9, 10 ** 6, -2 ** 31, 2 ** 31 - 1
+    say(f"many pages H={H}")
+    for parts in (1, 2):
+        sched, splits = get_mla_metadata(lens.cuda(), H, 1, parts)
+        out, lse = flash_mla_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), 512, sched, splits)
+        torch.cuda.synchronize()
+        assert_decode(out, lse, q, kv, table, lens, False, f"many pages H={H} parts={parts}")
+
+
+@pytest.mark.parametrize("H", [16, 64, 128])
+@pytest.mark.parametrize("kind", ["blocks", "outliers", "tiny", "huge"])
+def test_queries_of_unequal_size(gpu, H, kind):
+    """Blocks of 32 dims that differ by up to 2^12, one dim of each block 1024 times its neighbours, queries at both ends of
+    bf16 (scores of huge ones are kept finite by a zero query elsewhere and a tiny scale)."""
+    q, cache, table, lens, kv = problem(H, [700, 64, 1], H, 1)
+    g = torch.Generator().manual_seed(5)
+    x = q.float()
+    scale = SCALE
+    if kind == "blocks":
+        x[..., :512] *= torch.exp2(-torch.randint(0, 13, x.shape[:3] + (16,), generator=g).float()).repeat_interleave(32, -1)
+    elif kind == "outliers":
+        x[..., 7:512:32] *= 1024.0
+        x /= 64.0
+    elif kind == "tiny":
+        x *= 2.0 ** -60
+    else:
+        x *= 2.0 ** 100
+        scale = SCALE * 2.0 ** -100
+    q = x.to(torch.bfloat16)
+    table = table_for(table, H, False)
+    say(f"unequal queries H={H} {kind}")
+    out, lse = mla_decode_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), sm_scale=scale)
+    torch.cuda.synchronize()
+    if kind == "huge":
+        q = (q.double() * 2.0 ** -100)  # the same scores
+    assert_decode(out, lse, q, kv, table, lens, True, f"unequal H={H} {kind}")
+
+
+@pytest.mark.parametrize("H", [16, 24, 64, 128])
+@pytest.mark.parametrize("sparse", [False, True])
+def test_absorbed(gpu, H, sparse):
+    q, cache, table, lens, _ = problem(5 + H, [400, 64, 1, 900], H, 1)
+    g = torch.Generator().manual_seed(1)
+    w = (torch.randn(H, 512, 128, generator=g) * 512 ** -0.5).to(torch.bfloat16)
+    wb = prepare_w_uv(w.cuda())
+    say(f"absorbed H={H} sparse={sparse}")
+    if sparse:
+        nb = cache.latent.shape[0]
+        cache = to_gpu(*F4.quantize_pages(torch.randn(nb, 64, 1, 576, generator=g).to(torch.bfloat16)))
+        idx = torch.randint(0, nb * 64, (4, 1, 200), generator=g, dtype=torch.int32)
+        idx[1, 0, ::3], idx[2] = -1, -1
+        meta = get_mla_metadata(torch.zeros(4, dtype=torch.int32, device="cuda"), H, 1, topk=200, kv_cache=cache)
+        out, lse = flash_mla_with_kvcache(q.cuda(), cache, None, None, 512, *meta, indices=idx.cuda())
+        v, lse2 = mla_decode_absorbed(q.cuda(), cache, None, None, *meta, wb, indices=idx.cuda())
+    else:
+        d = (q.cuda(), cache, table_for(table, H, False).cuda(), lens.cuda())
+        meta = get_mla_metadata(d[3], H, 1, kv_cache=cache)
+        out, lse = flash_mla_with_kvcache(*d, 512, *meta, causal=True)
+        v, lse2 = mla_decode_absorbed(*d, *meta, wb, causal=True)
+    torch.cuda.synchronize()
+    assert torch.equal(lse, lse2)
+    o = out.double().cpu()
+    want = torch.stack([o[:, :, h] @ w[h].double() for h in range(H)], 2)
+    mag = torch.stack([o[:, :, h].abs() @ w[h].double().abs() for h in range(H)], 2)
+    # v's own rounding (2^-8) and fp32 sums of 512 products
+    assert ((v.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * mag).all()
