@@ -104,7 +104,8 @@ extern "C" {
  *   (uint8_t*)kv_scale + p*kv_scale_stride_page + r*kv_scale_stride_blk + j
  * (all strides of codes and scales in bytes, multiples of 16, the scale's token stride below 2^24, both
  * pointers 16-byte aligned).  Latent value d is e2m1(code_d) * 2^(byte - 127), byte 1 .. 254; byte 255
- * makes the block NaN.  Rope and queries as with fp8.
+ * makes the block NaN, and with it every output of the query rows that see the token (their lse is -inf, as any NaN
+ * row's); rows that do not see it are as without it.  Rope and queries as with fp8.
  */
 typedef struct mla_decode_args {
   int32_t batch;

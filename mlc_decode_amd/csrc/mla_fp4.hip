@@ -577,11 +577,13 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
       const int tok_k = tok0 + k * T;
       const int lane = lane_id<(RT > 1)>(), g = lane >> 4, li = lane & 15;
       // ---- 1. the wave's tokens to bf16 in LDS.  Tokens that do not exist become zeros: their weight is
-      // zero, and what their rows hold must not make 0 * NaN of it.
-      const bool cut = holes || tok_k + T > tok1;  // uniform
+      // zero, and what their rows hold must not make 0 * NaN of it.  So do the NaN blocks of tokens that some
+      // rows do not see: the score of a row that sees one is NaN, and with it all of its outputs.
+      const bool cut = holes || tok_k + T > tok1 || tok_k + T > lim_min;  // uniform
       const bool gone = cut && no_key<SPARSE>(p, tok_k + 16 * tt_load + li - tok0, idx_sh, tok1 - tok0);
       i32x4 code;  // chunk c of the token (c_load + c of its 128-dim chunks)
       float scale = 0.f;
+      bool bad = false;  // one of the lane's blocks is NaN (RT == 1: QK takes the zeros too, and its score is set)
       auto code_in = [&](int c) __attribute__((always_inline)) {
         uint32_t w;
         if constexpr (kRaw) {
@@ -591,11 +593,13 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
           code = cur.code[c];
           w = (uint32_t)cur.scale[c];
         }
-        scale = __uint_as_float(((w >> (8 * g)) & 0xFF) << 23);
+        scale = __uint_as_float(((w >> (8 * g)) & 0xFF) << 23);  // byte 255 is infinity
         if (cut) {  // uniform
-          scale = gone ? 1.f : scale;
+          const bool nan = scale == INFINITY, none = gone || nan;
+          bad |= nan;
+          scale = none ? 1.f : scale;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) code[j] = gone ? 0 : code[j];
+          for (int j = 0; j < 4; ++j) code[j] = none ? 0 : code[j];
         }
       };
       // word i of a chunk: 8 dims of token li of tile tt_load, chunk 4g + i of a 256-byte window
@@ -669,15 +673,20 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
         }
         s[0] = (a + l) * scale_log2;
       }
-      const bool ragged = tok_k + T > tok1 || tok_k + T > lim_min;
-      if (holes || ragged) {  // uniform
+      if (cut) {  // uniform
         const int lim = lim_sh[wave][li];
+        uint32_t nan_tokens = 0;  // of the tile, a bit each: lane (g, li) has token li's blocks of lane group g
+        if constexpr (!kRaw) {
+          const uint64_t m = __builtin_amdgcn_ballot_w64(bad);
+          nan_tokens = (uint32_t)(m | m >> 16 | m >> 32 | m >> 48);
+        }
 #pragma unroll
         for (int i = 0; i < Sh::kTiles; ++i)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int t = tok_k + 16 * (tt_own + i) + 4 * g + j;
             const bool see = t < lim && !no_key<SPARSE>(p, t - tok0, idx_sh, tok1 - tok0);
+            if constexpr (!kRaw) s[i][j] = (nan_tokens >> (4 * g + j)) & 1 ? NAN : s[i][j];
             s[i][j] = see ? s[i][j] : -INFINITY;
           }
       }
@@ -969,6 +978,7 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
     auto scores = [&](int k, auto buf, f32x4 (&s)[2]) __attribute__((always_inline)) {
       constexpr int B = decltype(buf)::value;
       const int t0 = k * T;  // in the segment
+      const bool cut = holes || tok0 + t0 + T > tok1 || tok0 + t0 + T > lim_min;  // uniform
       const uint32_t lane16 = 16 * lane_id<true>();
       int qs_lo;  // formed here: one register less to keep
       asm volatile("v_add_u32 %0, 0xf5f5f5f6, %1" : "=v"(qs_lo) : "v"(qs_hi));
@@ -994,11 +1004,12 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
         if (st == 1) {
           code = *(const i32x4 LDS_AS*)at_lds((frag_at ^ (16 * c_conv)) + B * kRawStage + tt_conv * kRawTile);
           scale = __uint_as_float((((uint32_t)(tt_conv ? ks[1] : ks[0]) >> (8 * c_conv)) & 0xFF) << 23);
-          if (holes || tok0 + t0 + T > tok1) {  // uniform: tokens that do not exist become zeros
-            const bool gone = no_key<SPARSE>(p, t0 + 16 * tt_conv + (lane_id<true>() & 15), idx_sh, tok1 - tok0);
-            scale = gone ? 1.f : scale;
+          // uniform: tokens that do not exist become zeros, and NaN blocks where some rows do not see the token (as above)
+          if (cut) {
+            const bool none = scale == INFINITY || no_key<SPARSE>(p, t0 + 16 * tt_conv + (lane_id<true>() & 15), idx_sh, tok1 - tok0);
+            scale = none ? 1.f : scale;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) code[j] = gone ? 0 : code[j];
+            for (int j = 0; j < 4; ++j) code[j] = none ? 0 : code[j];
           }
         }
         if (st < 2) {
@@ -1013,7 +1024,7 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (holes || tok0 + t0 + T > tok1 || tok0 + t0 + T > lim_min) {  // uniform
+      if (cut) {  // uniform
         const int lane = lane_id<true>(), lim = lim_sh[wave][lane & 15];
 #pragma unroll
         for (int i = 0; i < 2; ++i)

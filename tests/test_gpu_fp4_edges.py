@@ -49,6 +49,23 @@ def test_nan_block_in_each_form(gpu, H, splits):
     assert_decode(out[1:2], lse[1:2], q[1:2], kv, table[1:2], lens[1:2], True, f"beside NaNs H={H}")
 
 
+@pytest.mark.parametrize("H,s_q", [(8, 2), (1, 3), (16, 2), (16, 4), (64, 2), (33, 4), (128, 2)])
+@pytest.mark.parametrize("splits", [None, 1, 2])
+def test_nan_block_of_a_hidden_token(gpu, H, s_q, splits):
+    """A NaN block in each sequence's last token: the last query's rows are NaN, every other row, and a row that sees no
+    token, is as without it."""
+    q, cache, table, lens, kv = problem(H + s_q, [1, 2, 64, 65, 96, 130, 800], H, s_q)
+    for b, n in enumerate(lens.tolist()):
+        cache.scale[int(table[b, (n - 1) // 64]), (n - 1) % 64, b] = 255
+    table = table_for(table, H * s_q, False)
+    say(f"hidden NaN H={H} s_q={s_q} splits={splits}")
+    out, lse = mla_decode_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda(), num_splits=splits, causal=True)
+    torch.cuda.synchronize()
+    assert torch.isnan(out[:, -1]).all() and (lse[..., -1] == -math.inf).all()
+    # without the last query the last token is seen by nobody: L - 1 tokens, s_q - 1 queries
+    assert_decode(out[:, :-1], lse[..., :-1], q[:, :-1], kv, table, lens - 1, True, f"hidden NaN H={H} s_q={s_q}")
+
+
 @pytest.mark.parametrize("H", [16, 64, 128])
 def test_cut_at_the_table_and_foreign_pages(gpu, H):
     """Page ids that name no page are clamped into the pool, in the first, a middle and the last page that is read."""
