@@ -371,8 +371,9 @@ typedef struct mla_kv_append_args {
    * such that max|x| over the block <= 448 * 2^k (k clamped to [-126, 127]; a zero block
    * gets k = 0), rounded to nearest even.  MLA_KV_FP4_E2M1: the fp4 format, kv_new bf16; the 32-dim block
    * j is stored as e2m1(x / 2^k), 2^k the smallest power of two with max|x| <= 6 * 2^k (k >= -126; a
-   * zero block gets k = 0), rounded to nearest even, scale byte k + 127; a block that holds a NaN or an
-   * infinity gets byte 255 and codes 0. */
+   * zero block gets k = 0), rounded to nearest even, scale byte k + 127; values past 1.5 * 2^127, the largest
+   * that the format and bf16 both hold, are stored as that one; a block that holds a NaN or an infinity gets byte
+   * 255 and codes 0. */
   int32_t kv_format;
   int32_t kv_reserved; /* must be 0 */
   float* kv_scale;
@@ -449,8 +450,10 @@ typedef struct mla_append_slots_args {
 } mla_append_slots_args;
 int mla_kv_append_slots(const mla_kv_cache* cache, const mla_rope* rope, const mla_append_slots_args* args, void* stream);
 
-/* Cached tokens as rows: out[t, 0..575] (the cache's dtype) = the token at slots[t], dequantised; a slot
- * outside [0, 64 * num_blocks) gives a row of zeros.  out_stride in elements. */
+/* Cached tokens as rows: out[t, 0..575] (the cache's dtype) = the token at slots[t], dequantised: exact, as a code times
+ * its power of two fits bf16, where it lies in bf16's range (an infinity beyond it; the 4-bit appends store no such
+ * value, the fp8 ones for latents of 1.9375 * 2^127 and more); a slot outside [0, 64 * num_blocks) gives a row
+ * of zeros.  out_stride in elements. */
 int mla_kv_gather(const mla_kv_cache* cache, const int32_t* slots, int32_t tokens, void* out, int64_t out_stride,
                   void* stream);
 

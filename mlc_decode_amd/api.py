@@ -250,6 +250,7 @@ class Fp4KVCache(NamedTuple):
     (dim 2i in the low half of byte i), ``scale`` uint8 ``[num_blocks, 64, 16]`` (a byte s per token and
     32 dims, 1 .. 254; 255 marks a block that held a NaN or an infinity), ``rope`` bf16
     ``[num_blocks, 64, 64]``.  Latent value d of a token is ``e2m1(code_d) * 2**(scale[d // 32] - 127)``.
+    Values past ``1.5 * 2**127``, the largest that the codes and bf16 both hold, are stored as that one.
     400 bytes a token (bf16: 1152, fp8: 656).  No counterpart in the reference.
     """
     latent: torch.Tensor

@@ -258,7 +258,9 @@ __device__ __forceinline__ int block_exp(uint32_t bits, int e, uint32_t m) {
 }
 
 // The wave's lane l holds dims 8l .. 8l+7 of the token's latent (v); written to (page, row) of the cache.
-// A 4-bit block with a NaN or an infinity in it is marked whole (scale byte 255): the format has neither.
+// A 4-bit block with a NaN or an infinity in it is marked whole (scale byte 255): the format has neither.  A value past
+// 1.5 * 2^127, the largest that e2m1 and bf16 both hold, is stored as that one: the next, 4 * 2^126, would read back
+// as an infinity.
 __device__ __forceinline__ void put_latent(const Cache& c, int64_t page, int row, int lane, i32x4 v) {
   uint8_t* dst = c.nope + page * c.sp + row * c.st;
   if (c.format == MLA_KV_NATIVE) {
@@ -284,6 +286,8 @@ __device__ __forceinline__ void put_latent(const Cache& c, int64_t page, int row
     const bool bad = top >= 0x7F80u;
     const int k = bad ? 0 : block_exp(top, 2, 0x40);
     const float sc = __uint_as_float((uint32_t)(k + 127) << 23);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_fmed3f(x[j], -0x1.8p127f, 0x1.8p127f);
     uint32_t w = 0;
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], sc, 0);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], sc, 1);

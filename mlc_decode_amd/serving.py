@@ -316,8 +316,10 @@ def kv_append_slots(kv_new: torch.Tensor, kv_cache, slots: torch.Tensor, positio
 
 
 def kv_gather(kv_cache, slots: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The cached tokens ``slots [T]`` (int32, page * 64 + row) as rows ``[T, 576]`` in the cache's dtype (bf16 for the
-    coded caches, exact: a code times its scale fits bf16).  A slot outside the cache gives a row of zeros."""
+    """The cached tokens ``slots [T]`` (int32, page * 64 + row) as rows ``[T, 576]`` in the cache's dtype.  The coded caches
+    give bf16, exactly: a code times its scale fits it, up to its range (an fp8 block whose largest latent is
+    ``1.9375 * 2**127`` or more can hold a code past it, which reads as an infinity; the 4-bit appends store none).
+    A slot outside the cache gives a row of zeros."""
     c, dtype, device = _cache_struct(kv_cache, None)
     if slots.dim() != 1:
         raise ValueError("slots must be a 1-D int32 tensor")

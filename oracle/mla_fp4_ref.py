@@ -7,6 +7,8 @@ The reference has no such cache.  This file defines the format the 4-bit append 
     to the even code, saturating at 6;
   * ``scale_byte`` -- the scale of 32 dims: 2^k as the byte k + 127, k the smallest with amax <= 6 * 2^k
     (-126 at least; 0 for zeros), byte 255 where the block holds a NaN or an infinity;
+  * ``LARGEST`` -- 1.5 * 2^127, the largest value that e2m1 codes and bf16 both hold: larger ones are stored as it
+    (the next code, 4 * 2^126 = 2^128, is no bf16 or fp32 number);
   * ``quantize_latent`` / ``dequantize_latent`` / ``dequantize_pages`` / ``append_paged_fp4`` as in
     ``mla_fp8_ref``: dim 2i of a token is the low half of byte i.
 
@@ -21,6 +23,7 @@ import torch
 LATENT, ROPE, BLOCK, PAGE = 512, 64, 32, 64
 NBLK = LATENT // BLOCK
 E2M1_MAX = 6.0
+LARGEST = 1.5 * 2.0 ** 127
 NAN_BYTE = 255
 
 
@@ -58,7 +61,7 @@ def quantize_latent(latent: torch.Tensor):
     amax = np.where(np.isfinite(x).all(-1), np.abs(x).max(-1), np.inf)
     byte = scale_byte(amax)
     bad = byte == NAN_BYTE
-    v = np.where(bad[..., None], 0.0, x) / np.exp2(np.where(bad, 0, byte.astype(np.int64) - 127))[..., None]
+    v = np.clip(np.where(bad[..., None], 0.0, x), -LARGEST, LARGEST) / np.exp2(np.where(bad, 0, byte.astype(np.int64) - 127))[..., None]
     c = np.where(bad[..., None], 0, e2m1_encode(v)).astype(np.uint8).reshape(-1, LATENT // 2, 2)
     return c[..., 0] | (c[..., 1] << 4), byte
 

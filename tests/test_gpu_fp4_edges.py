@@ -6,10 +6,10 @@ import math
 import pytest
 import torch
 
-from mlc_decode_amd import (flash_mla_with_kvcache, get_mla_metadata, mla_decode_absorbed, mla_decode_with_kvcache,
-                            prepare_w_uv)
+from mlc_decode_amd import (flash_mla_with_kvcache, get_mla_metadata, kv_gather, mla_decode_absorbed, mla_decode_with_kvcache,
+                            prepare_w_uv, quantize_kv_cache)
 from oracle import mla_fp4_ref as F4
-from test_gpu_fp4 import SCALE, assert_decode, problem, say, table_for, to_gpu
+from test_gpu_fp4 import SCALE, assert_cache, assert_decode, problem, say, table_for, to_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -129,6 +129,36 @@ def test_queries_of_unequal_size(gpu, H, kind):
     if kind == "huge":
         q = (q.double() * 2.0 ** -100)  # the same scores
     assert_decode(out, lse, q, kv, table, lens, True, f"unequal H={H} {kind}")
+
+
+def test_largest_latents(gpu):
+    """Up to the largest bf16 value: what is stored reads back finite, to the nearest value that the format and bf16 hold,
+    and a single token's decode gives it back."""
+    g = torch.Generator().manual_seed(1)
+    top = 3.3895313892515355e38
+    kv = torch.randn(3, 64, 1, 576, generator=g)
+    kv[..., 480:512] = 0.0
+    kv[0, :, 0, 480:512] = torch.linspace(0.5, 1.0, 64)[:, None] * torch.linspace(-1, 1, 32) * top
+    kv[0, 5, 0, 480:512] = top
+    kv[1, 0, 0, 480:512] = -top
+    kv = kv.to(torch.bfloat16)
+    assert torch.isfinite(kv).all()
+    say("largest latents")
+    cache = quantize_kv_cache(kv.cuda(), bits=4)
+    rows = kv_gather(cache, torch.arange(192, dtype=torch.int32, device="cuda"))
+    q = torch.randn(1, 1, 128, 576, generator=g)
+    q[..., 480:512] = 0.0
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    out, _ = mla_decode_with_kvcache(q.to(torch.bfloat16).cuda(), cache, one.reshape(1, 1), one)
+    torch.cuda.synchronize()
+    assert_cache(cache, *F4.quantize_pages(kv), "largest")
+    got, want = rows[:, 480:512].double().cpu(), kv.reshape(192, 576)[:, 480:512].double()
+    assert torch.isfinite(rows).all()
+    # e2m1 is off by at most a quarter of the value or of the smallest step of its block; what lies past the largest
+    # value, 1.5 * 2^127 (bf16 ends below 2^128), by a quarter too
+    k = torch.exp2(torch.ceil(torch.log2(want.abs().amax(-1, keepdim=True) / 6)))
+    assert ((got - want).abs() <= torch.maximum(want.abs() * 0.25, 0.25 * k)).all()
+    assert torch.equal(out[0, 0, 0].cpu().double(), rows[64, :512].cpu().double()) and (out[0, 0, :, 480:] == -1.5 * 2.0 ** 127).all()
 
 
 @pytest.mark.parametrize("H", [16, 24, 64, 128])

@@ -48,3 +48,16 @@ def test_bad_blocks_are_marked():
     codes, byte = F4.quantize_latent(x)
     v = F4.dequantize_latent(codes, byte)
     assert np.isnan(v[0, 32:64]).all() and np.isnan(v[1, 480:]).all() and np.isnan(v).sum() == 64
+
+
+def test_values_past_the_largest_are_stored_as_it():
+    top = torch.finfo(torch.bfloat16).max
+    x = torch.zeros(4, 512)
+    x[0, :4] = torch.tensor([top, -top, 1.75 * 2.0 ** 127, 2.5 * 2.0 ** 126])
+    x[1, 32:34] = torch.tensor([1.5 * 2.0 ** 127, -1.5 * 2.0 ** 127])
+    x[2, 0] = -top
+    codes, byte = F4.quantize_latent(x)
+    v = F4.dequantize_latent(codes, byte)
+    assert v[0, :4].tolist() == [1.5 * 2.0 ** 127, -1.5 * 2.0 ** 127, 1.5 * 2.0 ** 127, 2.0 ** 127]  # the tie to the even code
+    assert v[1, 32:34].tolist() == [1.5 * 2.0 ** 127, -1.5 * 2.0 ** 127] and byte[1, 1] == 125 + 127
+    assert np.isfinite(torch.from_numpy(v).to(torch.bfloat16).float().numpy()).all() and byte[0, 0] == 126 + 127
