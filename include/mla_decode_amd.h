@@ -489,7 +489,8 @@ int mla_reserve_pages(const mla_page_pool* pool, const int32_t* new_lens, int32_
 /*
  * Shortens every sequence to keep_lens[b] tokens (0: it is done; a longer or equal keep changes nothing) and
  * returns the pages it no longer needs, so that releasing what mla_reserve_pages took restores the stack.
- * block_table keeps its stale entries.
+ * block_table keeps its stale entries.  An entry outside [0, num_blocks) is no page and is not put back.  A count
+ * outside [0, num_blocks] is taken as the nearer end, here and in mla_reserve_pages.
  */
 int mla_release_pages(const mla_page_pool* pool, const int32_t* keep_lens, void* stream);
 

@@ -692,63 +692,93 @@ struct ReleaseParams {
 };
 
 // Sequence b keeps its first min(L, keep) tokens; the pages behind them go back so that the last page taken
-// comes off first again: releasing what a reservation took leaves the stack as it was.  4 to 6 us, latency.
+// comes off first again: releasing what a reservation took leaves the stack as it was.  A table entry that is no page of
+// the pool is not put back: the first pass counts those that are, and where some are not (rare) the second
+// closes the gaps with a prefix sum over the entries.
 __global__ __launch_bounds__(kChunk) void mla_release_kernel(ReleaseParams p) {
   __shared__ int64_t wsum[kChunk / 64];
-  __shared__ int64_t total_sh;
-  __shared__ int start_sh[kChunk + 1], from_sh[kChunk];
+  __shared__ int64_t sum_sh;
+  __shared__ int64_t start_sh[kChunk + 1];
+  __shared__ int from_sh[kChunk];
+  __shared__ int gaps_sh;
   const int tid = threadIdx.x;
-  const int count = *p.count;
-  auto drop_of = [&](int b, int& from, int& kept, bool& cut) {
-    int L = p.seqlens[b];
-    int keep = p.keep[b];
-    keep = keep > 0 ? keep : 0;
-    cut = L > keep;
-    kept = keep;
-    const int64_t most = (int64_t)p.width * kPage;
-    const int64_t l = L < 0 ? 0 : (L < most ? L : most);
-    from = pages_up(keep);
-    const int n = pages_up(l) - from;
-    return cut && n > 0 ? n : 0;
+  int count = *p.count;
+  count = count < 0 ? 0 : (count > p.num_blocks ? p.num_blocks : count);
+  auto is_page = [&](int page) { return page >= 0 && page < p.num_blocks; };
+  // table entry r of those that the chunk's requests drop
+  auto entry = [&](int base, int64_t r) __attribute__((always_inline)) {
+    int i = 0, j = kChunk;
+    while (j - i > 1) {
+      const int m = (i + j) >> 1;
+      if (start_sh[m] <= r) i = m; else j = m;
+    }
+    return p.block_table[(int64_t)(base + i) * p.bt_stride + from_sh[i] + (r - start_sh[i])];
   };
-  int64_t total = 0;
-  {
-    int64_t mine = 0;
-    for (int b = tid; b < p.batch; b += kChunk) {
-      int from, kept;
-      bool cut;
-      mine += drop_of(b, from, kept, cut);
-    }
-    const int64_t s = block_scan(mine, wsum);
-    if (tid == kChunk - 1) total_sh = s;
-    __syncthreads();
-    total = total_sh;
-  }
-  int64_t before = 0;
-  for (int base = 0; base < p.batch; base += kChunk) {
-    const int b = base + tid;
-    int from = 0, kept = 0, n = 0;
-    bool cut = false;
-    if (b < p.batch) n = drop_of(b, from, kept, cut);
-    const int64_t end = block_scan(n, wsum);
-    start_sh[tid] = (int)(end - n);
-    from_sh[tid] = from;
-    if (tid == kChunk - 1) start_sh[kChunk] = (int)end;
-    __syncthreads();
-    const int here = start_sh[kChunk];
-    for (int r = tid; r < here; r += kChunk) {
-      int i = 0, j = kChunk;
-      while (j - i > 1) {
-        const int m = (i + j) >> 1;
-        if (start_sh[m] <= r) i = m; else j = m;
+  if (tid == 0) gaps_sh = 0;  // ordered by the scan's barriers
+  int keep = 0;
+  bool cut = false, gaps = false;
+  int64_t dropped = 0, missing = 0, total = 0, before = 0;  // missing: of this thread's entries; before: pages put back
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+    for (int base = 0; base < p.batch; base += kChunk) {
+      if (pass == 0 || p.batch > kChunk) {  // uniform: a single chunk is kept from the first pass
+        const int b = base + tid;
+        int64_t from = 0, n = 0;
+        cut = false;
+        if (b < p.batch) {
+          const int64_t most = (int64_t)p.width * kPage;
+          const int L = p.seqlens[b];
+          keep = p.keep[b];
+          keep = keep > 0 ? keep : 0;
+          cut = L > keep;
+          from = pages_up(keep);
+          n = cut ? pages_up(L < most ? L : most) - from : 0;
+          n = n > 0 ? n : 0;
+        }
+        const int64_t end = block_scan(n, wsum);
+        start_sh[tid] = end - n;
+        from_sh[tid] = (int)from;
+        if (tid == kChunk - 1) start_sh[kChunk] = end;
+        __syncthreads();
       }
-      const int64_t at = count + total - 1 - (before + r);
-      if (at >= 0 && at < p.num_blocks)
-        p.free[at] = p.block_table[(int64_t)(base + i) * p.bt_stride + from_sh[i] + (r - start_sh[i])];
+      const int64_t here = start_sh[kChunk];
+      if (pass == 0) {
+        dropped += here;
+        for (int64_t r = tid; r < here; r += kChunk) missing += !is_page(entry(base, r));
+      } else {
+        for (int64_t r0 = 0; r0 < here; r0 += kChunk) {  // uniform
+          const int page = r0 + tid < here ? entry(base, r0 + tid) : -1;
+          int64_t rank = before + tid;
+          if (gaps) {  // uniform
+            rank = before + block_scan(is_page(page) ? 1 : 0, wsum) - 1;
+            if (tid == kChunk - 1) sum_sh = rank + 1;
+            __syncthreads();
+            before = sum_sh;
+            __syncthreads();
+          } else {
+            before += here - r0 < kChunk ? here - r0 : kChunk;
+          }
+          const int64_t at = count + total - 1 - rank;
+          if (is_page(page) && at >= 0 && at < p.num_blocks) p.free[at] = page;
+        }
+        if (cut) p.seqlens[base + tid] = keep;
+      }
+      if (p.batch > kChunk) __syncthreads();  // read before the next chunk's
     }
-    if (cut) p.seqlens[b] = kept;
-    before += here;
-    __syncthreads();
+    if (pass == 0) {
+      if (missing != 0) gaps_sh = 1;
+      __syncthreads();
+      gaps = gaps_sh != 0;
+      total = dropped;
+      if (gaps) {  // uniform
+        const int64_t all = block_scan(missing, wsum);
+        if (tid == kChunk - 1) sum_sh = all;
+        __syncthreads();
+        total -= sum_sh;
+        __syncthreads();
+      }
+    }
   }
   if (tid == 0) {
     const int64_t now = count + total;

@@ -416,7 +416,8 @@ def reserve_pages(pool: PagePool, block_table: torch.Tensor, cache_seqlens: torc
 def release_pages(pool: PagePool, block_table: torch.Tensor, cache_seqlens: torch.Tensor, keep_lens: torch.Tensor) -> None:
     """Shorten every sequence to ``keep_lens[b]`` tokens (int32 ``[B]``; 0: it is done, its length or more: nothing
     changes) and return the pages it no longer needs to ``pool``, in place.  The pages go back in the order they
-    came: releasing what ``reserve_pages`` took restores the stack.  ``block_table`` keeps stale entries."""
+    came: releasing what ``reserve_pages`` took restores the stack.  ``block_table`` keeps stale entries; one that is no
+    page of the pool is not put back."""
     s, B, device = _pool_struct(pool, block_table, cache_seqlens)
     _require_int32(keep_lens, "keep_lens", B, device)
     _launch("mla_release_pages", _lib.load().mla_release_pages, device, ctypes.byref(s), keep_lens.data_ptr())

@@ -7,7 +7,7 @@ import mlc_decode_amd as M
 from oracle import mla_fp4_ref as F4
 from oracle import mla_fp8_ref as F8
 from test_gpu_fp4 import varied_cache
-from test_gpu_serving import make_cache, say
+from test_gpu_serving import Model, assert_state, device_state, make_cache, say, state
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +106,65 @@ def test_append_by_slot_at_the_ends_of_bf16(gpu, kind, n):
         codes, scale = F8.quantize_latent(new[fin][:, :512])
         got = b.scale[:, :, :n].transpose(1, 2)[fin.cuda()].cpu()
         assert torch.equal(b.latent[:, :n][fin.cuda()].cpu(), torch.from_numpy(codes)) and torch.equal(got, torch.from_numpy(scale))
+
+
+# ---------------------------------------------------------------------------------------
+# ids that name no page
+# ---------------------------------------------------------------------------------------
+class Pool(Model):
+    """The model with what a release may put back: pages of the pool."""
+
+    def release(self, keep):
+        count = min(max(self.count, 0), self.nb)
+        back = []
+        for b, k in enumerate(keep):
+            k, L = max(k, 0), self.lens[b]
+            if L > k:
+                back += [p for p in self.table[b][-(-k // 64):min(-(-L // 64), len(self.table[b]))] if 0 <= p < self.nb]
+                self.lens[b] = k
+        for i, p in enumerate(reversed(back)):
+            self.free[count + i] = p
+        self.count = count + len(back)
+
+
+def foreign(m, rows, seed):
+    """Ids of no page into the tables of some sequences; the pages they stood for are nobody's now."""
+    g = torch.Generator().manual_seed(seed)
+    ids = [-1, m.nb, 2 ** 31 - 1, -2 ** 31, m.nb + 7]
+    for b in rows:
+        held = -(-max(m.lens[b], 0) // 64)
+        for c in range(held):
+            if torch.rand(1, generator=g).item() < 0.4:
+                m.table[b][c] = ids[(b + c) % len(ids)]
+    return m
+
+
+@pytest.mark.parametrize("B,hi,P", [(1, 300, 6), (7, 700, 12), (64, 500, 9), (1030, 200, 5), (2500, 100, 3), (40, 64 * 40, 41)])
+def test_release_gives_back_pages_of_the_pool_only(gpu, B, hi, P):
+    m, g = state(B, B, P, hi, 10)
+    m = foreign(Pool(m.free, m.count, m.table, m.lens, m.nb), range(0, B, 3), B)
+    if B > 5:
+        m.lens[2] = 64 * P + 1000  # longer than its row: what the row holds comes back
+        m.table[2] = [-1] * P
+    pool, table, lens = device_state(m)
+    say(f"release foreign B={B}")
+    for keep in ([max(0, n // 2) for n in m.lens], [0] * B):
+        M.release_pages(pool, table, lens, torch.tensor(keep, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        m.release(keep)
+        assert_state(pool, table, lens, m, f"release foreign B={B}")
+    assert all(0 <= p < m.nb for p in m.free[:m.count])
+
+
+@pytest.mark.parametrize("count", [-5, 0])
+def test_release_into_an_empty_pool(gpu, count):
+    """A count below zero holds no page, for a release as for a reservation."""
+    m, _ = state(3, 6, 8, 400, 0)
+    m = Pool(m.free, count, m.table, m.lens, m.nb)
+    pool, table, lens = device_state(m)
+    say(f"release count={count}")
+    M.release_pages(pool, table, lens, torch.zeros_like(lens))
+    torch.cuda.synchronize()
+    m.release([0] * 6)
+    assert_state(pool, table, lens, m, f"count={count}")
+    assert m.count == m.nb and sorted(m.free) == list(range(m.nb))
