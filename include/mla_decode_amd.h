@@ -481,7 +481,8 @@ typedef struct mla_page_pool {
  * the pool holds fewer pages than the requests up to b need (one that needs no page is granted even then).
  * Otherwise granted[b] = 1, its new pages are in block_table and cache_seqlens[b] has advanced.
  * slots [tokens], positions [tokens]: cache row and position of every row; -1 for rows not granted and rows
- * behind the last sequence.  scratch [batch + 1] int32.
+ * behind the last sequence.  (An id outside [0, num_blocks) that a caller put into free_pages is handed out like the
+ * others, and its rows have slot -1.)  scratch [batch + 1] int32.
  */
 int mla_reserve_pages(const mla_page_pool* pool, const int32_t* new_lens, int32_t tokens, int32_t* slots, int32_t* positions,
                       int32_t* cu_new, int32_t* granted, int32_t* scratch, void* stream);

@@ -581,7 +581,7 @@ __device__ __forceinline__ void place_row(const ReserveParams& p, int t, int b, 
       page = p.free[count - 1 - (first + col - pages_up(L))];
       if ((pos & (kPage - 1)) == 0) *cell = page;  // every new page starts with a new row
     }
-    slot = page * kPage + (pos & (kPage - 1));
+    if (page >= 0 && page < p.num_blocks) slot = page * kPage + (pos & (kPage - 1));  // else no row, and no overflow
   }
   p.slots[t] = slot;
   p.positions[t] = pos;

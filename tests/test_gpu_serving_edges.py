@@ -168,3 +168,22 @@ def test_release_into_an_empty_pool(gpu, count):
     m.release([0] * 6)
     assert_state(pool, table, lens, m, f"count={count}")
     assert m.count == m.nb and sorted(m.free) == list(range(m.nb))
+
+
+@pytest.mark.parametrize("new", [1, 300])
+def test_a_popped_id_of_no_page_names_no_row(gpu, new):
+    """A stack that its user filled with such ids: the rows on them have slot -1, never another page's slot."""
+    B, nb = 40, 500
+    free = torch.arange(nb, dtype=torch.int32)
+    bad = torch.tensor([-1, nb, 2 ** 26 + 3, 2 ** 31 - 1, -2 ** 31], dtype=torch.int32)  # 2^26 pages are 2^32 rows
+    free[1::2] = bad[torch.arange(nb // 2) % 5]
+    pool = M.PagePool(free.cuda(), torch.tensor([nb], dtype=torch.int32, device="cuda"))
+    table, lens = torch.zeros(B, 8, dtype=torch.int32, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    say(f"bad stack new={new}")
+    r = M.reserve_pages(pool, table, lens, torch.full_like(lens, new), B * new)
+    torch.cuda.synchronize()
+    assert r.granted.all()
+    page = table.cpu().long().repeat_interleave(new, 0).gather(1, (r.positions.cpu().long() // 64)[:, None])[:, 0]
+    ok = (page >= 0) & (page < nb)
+    want = torch.where(ok, page * 64 + r.positions.cpu().long() % 64, torch.full_like(page, -1))
+    assert not ok.all() and torch.equal(r.slots.cpu().long(), want)
