@@ -665,8 +665,9 @@ __global__ __launch_bounds__(kChunk) void mla_reserve_kernel(ReserveParams p) {
 }
 
 __global__ __launch_bounds__(256) void mla_slot_rows_kernel(ReserveParams p) {
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= p.tokens) return;
+  const uint32_t row = blockIdx.x * 256 + threadIdx.x;  // past 2^31 in the last workgroup of the longest map
+  if (row >= (uint32_t)p.tokens) return;
+  const int t = (int)row;
   const int count = p.first[p.batch];
   if (t >= p.cu_new[p.batch]) {
     p.slots[t] = p.positions[t] = -1;
@@ -1051,7 +1052,7 @@ int mla_reserve_pages(const mla_page_pool* pool, const int32_t* new_lens, int32_
     hipLaunchKernelGGL(mla_reserve_kernel<true>, dim3(1), dim3(kChunk), 0, st, k);
   } else {
     hipLaunchKernelGGL(mla_reserve_kernel<false>, dim3(1), dim3(kChunk), 0, st, k);
-    hipLaunchKernelGGL(mla_slot_rows_kernel, dim3((tokens + 255) / 256), dim3(256), 0, st, k);
+    hipLaunchKernelGGL(mla_slot_rows_kernel, dim3(((uint32_t)tokens + 255) / 256), dim3(256), 0, st, k);
   }
   return launched("reserve pages");
 }

@@ -187,3 +187,17 @@ def test_a_popped_id_of_no_page_names_no_row(gpu, new):
     ok = (page >= 0) & (page < nb)
     want = torch.where(ok, page * 64 + r.positions.cpu().long() % 64, torch.full_like(page, -1))
     assert not ok.all() and torch.equal(r.slots.cpu().long(), want)
+
+
+def test_the_longest_slot_map(gpu):
+    """2^31 - 1 rows: the last workgroup's row numbers pass 2^31."""
+    T = 2 ** 31 - 1
+    pool, table = M.page_pool(9), torch.zeros(3, 3, dtype=torch.int32, device="cuda")
+    lens, new = torch.tensor([0, 70, 5], dtype=torch.int32, device="cuda"), torch.tensor([100, 0, 3], dtype=torch.int32, device="cuda")
+    say("longest map")
+    r = M.reserve_pages(pool, table, lens, new, T)
+    torch.cuda.synchronize()
+    assert r.cu_new.tolist() == [0, 100, 100, 103] and r.granted.tolist() == [1, 1, 1] and lens.tolist() == [100, 70, 8]
+    assert r.positions[:104].tolist() == [*range(100), 5, 6, 7, -1] and r.slots[:101].tolist() == [*range(100), 5]
+    for m in (r.slots, r.positions):
+        assert m.shape == (T,) and (m[-(1 << 20):] == -1).all() and (m[1 << 30:(1 << 30) + 1000] == -1).all()
