@@ -418,7 +418,7 @@ typedef struct mla_rope {
 
 /* x [tokens, heads, dim] -> out, dims [first, first + rope.dim) rotated and the others copied (left alone
  * where out == x; otherwise the two may not overlap).  Strides in elements, a head's dims contiguous;
- * heads * dim below 2^22. */
+ * heads * dim below 2^22; at most (2^24 - 1) * min(8, 1024 / rope.dim) tokens. */
 typedef struct mla_rope_args {
   const void* x;
   void* out;
@@ -436,7 +436,7 @@ int mla_apply_rope(const mla_rope* rope, const mla_rope_args* args, void* stream
  * q_pe [tokens, heads, 64], the queries' rope parts, each is rotated into q_rope (the rope dims of the
  * decode's query buffer; may be q_pe itself) in the same launch.  A slot outside [0, 64 * num_blocks) names
  * no row: nothing is written for that token, neither to the cache nor to q_rope.  No two rows may have
- * the same slot.  Strides in elements, multiples of 8; pointers 16-byte aligned.
+ * the same slot.  Strides in elements, multiples of 8; pointers 16-byte aligned; at most 2^27 - 8 tokens.
  */
 typedef struct mla_append_slots_args {
   const void* kv_new;
@@ -453,7 +453,7 @@ int mla_kv_append_slots(const mla_kv_cache* cache, const mla_rope* rope, const m
 /* Cached tokens as rows: out[t, 0..575] (the cache's dtype) = the token at slots[t], dequantised: exact, as a code times
  * its power of two fits bf16, where it lies in bf16's range (an infinity beyond it; the 4-bit appends store no such
  * value, the fp8 ones for latents of 1.9375 * 2^127 and more); a slot outside [0, 64 * num_blocks) gives a row
- * of zeros.  out_stride in elements. */
+ * of zeros.  out_stride in elements; at most 2^26 - 4 tokens. */
 int mla_kv_gather(const mla_kv_cache* cache, const int32_t* slots, int32_t tokens, void* out, int64_t out_stride,
                   void* stream);
 

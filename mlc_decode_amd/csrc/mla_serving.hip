@@ -798,6 +798,14 @@ static int launched(const char* what) {
   return MLA_OK;
 }
 
+// Workgroups of `per` tokens each; 0, with the error left, where they are more than a launch takes (2^32 threads).
+static uint32_t groups_of(int64_t tokens, int per) {
+  const int64_t n = (tokens + per - 1) / per;
+  if (n < (int64_t(1) << 24)) return (uint32_t)n;
+  set_error(MLA_ERR_UNSUPPORTED, "too many tokens for one call");
+  return 0;
+}
+
 // Checks a cache descriptor and fills the kernels' form of it (strides in bytes).
 static int check_cache(const mla_kv_cache* c, Cache* k) {
   if (c->format != MLA_KV_NATIVE && c->format != MLA_KV_FP8_E4M3 && c->format != MLA_KV_FP4_E2M1)
@@ -926,13 +934,14 @@ int mla_apply_rope(const mla_rope* rope, const mla_rope_args* a, void* stream) {
   // 16 x 128 3.3 (4.2 with 2048).
   int tile = kPairs / pairs;
   tile = tile < kRopeTile ? tile : kRopeTile;
-  while (tile > 1 && (a->tokens + tile - 1) / tile < 1024) tile >>= 1;
-  const int groups = (a->tokens + tile - 1) / tile;
-  int split = 1;
-  while (groups * split < 512 && 2 * split <= a->heads) split *= 2;
+  while (tile > 1 && ((int64_t)a->tokens + tile - 1) / tile < 1024) tile >>= 1;
+  const uint32_t groups = groups_of(a->tokens, tile);
+  if (groups == 0) return MLA_ERR_UNSUPPORTED;
+  uint32_t split = 1;
+  while (groups * split < 512 && 2 * split <= (uint32_t)a->heads) split *= 2;
   k.tile = tile;
-  k.split = split;
-  const uint32_t grid = (uint32_t)groups * (uint32_t)split;
+  k.split = (int)split;
+  const uint32_t grid = groups * split;
   const hipStream_t st = (hipStream_t)stream;
   if (a->dtype == MLA_DTYPE_BF16) launch_rope<Bf16>(k, vec, grid, st);
   else if (a->dtype == MLA_DTYPE_F16) launch_rope<F16>(k, vec, grid, st);
@@ -978,9 +987,11 @@ int mla_kv_append_slots(const mla_kv_cache* cache, const mla_rope* rope, const m
   // 1024 workgroups at least: 1024 tokens x 128 heads 8.2 us, 4096 x 16 6.3 (11.7 and 7.0 with 256 at least, 8.1
   // and 8.6 with 4096)
   int tile = kAppendTile;
-  while (tile > 1 && (a->tokens + tile - 1) / tile < 1024) tile >>= 1;
+  while (tile > 1 && ((int64_t)a->tokens + tile - 1) / tile < 1024) tile >>= 1;
   k.tile = tile;
-  const dim3 grid((a->tokens + tile - 1) / tile);
+  const uint32_t groups = groups_of(a->tokens, tile);
+  if (groups == 0) return MLA_ERR_UNSUPPORTED;
+  const dim3 grid(groups);
   if (k.cache.f16)
     hipLaunchKernelGGL(mla_append_slots_kernel<F16>, grid, dim3(256), 0, (hipStream_t)stream, k);
   else
@@ -1002,7 +1013,9 @@ int mla_kv_gather(const mla_kv_cache* cache, const int32_t* slots, int32_t token
   k.out = (uint8_t*)out;
   k.o_st = out_stride * 2;
   k.tokens = tokens;
-  const dim3 grid((tokens + 3) / 4);
+  const uint32_t groups = groups_of(tokens, 4);
+  if (groups == 0) return MLA_ERR_UNSUPPORTED;
+  const dim3 grid(groups);
   const hipStream_t st = (hipStream_t)stream;
   if (cache->format == MLA_KV_NATIVE)
     hipLaunchKernelGGL(mla_gather_kernel<MLA_KV_NATIVE>, grid, dim3(256), 0, st, k);
