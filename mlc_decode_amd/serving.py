@@ -198,7 +198,7 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, first: Opti
     o_t, o_h = orr[2:]
     x_ptr, o_ptr = x.data_ptr(), out.data_ptr()
     if not fresh:
-        if (tokens > 1 and o_t < D) or (heads > 1 and o_h < D):
+        if _rows_meet((o_t, o_h), (tokens, heads), D):
             raise ValueError("out's rows overlap")
         if not _apart_or_same(x_ptr, (x_t, x_h), o_ptr, (o_t, o_h), (tokens, heads), D, x.element_size()):
             raise ValueError("out overlaps x without being x")
@@ -206,6 +206,23 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, first: Opti
         x_ptr, o_ptr, x_t, x_h, o_t, o_h, positions.data_ptr(), tokens, heads, D, first, _DTYPES[x.dtype], 0))
     _launch("mla_apply_rope", _lib.load().mla_apply_rope, device, ctypes.byref(r), ctypes.byref(a))
     return out
+
+
+def _rows_meet(strides, counts, width: int, shift: int = 0) -> bool:
+    """Whether any two of ``counts[0] * counts[1]`` rows of ``width`` elements at these strides overlap; with a ``shift``,
+    whether a row and one of the same rows that many elements on do."""
+    (s0, n0), (s1, n1) = sorted((s if n > 1 else 0, n) for s, n in zip(strides, counts))
+    if shift == 0 and ((n0 > 1 and s0 < width) or (n1 > 1 and s1 < width)):
+        return True
+    reach = 0 if s1 == 0 else min(n1 - 1, ((n0 - 1) * s0 + abs(shift) + width) // s1)
+    for k1 in range(-reach, reach + 1):  # as far as the other stride's rows reach: 0 or 1 in the usual layouts
+        at = shift + k1 * s1
+        near = 0 if s0 == 0 else -at // s0
+        for k0 in (near, near + 1):
+            k0 = min(max(k0, 1 - n0), n0 - 1)
+            if abs(at + k0 * s0) < width and (shift or k0 or k1):
+                return True
+    return False
 
 
 def _apart_or_same(x_ptr: int, xs, o_ptr: int, os, counts, width: int, es: int) -> bool:
@@ -216,9 +233,7 @@ def _apart_or_same(x_ptr: int, xs, o_ptr: int, os, counts, width: int, es: int) 
     t, h = counts[0] - 1, counts[1] - 1
     if x_ptr >= o_ptr + es * (t * os[0] + h * os[1] + width) or o_ptr >= x_ptr + es * (t * xs[0] + h * xs[1] + width):
         return True
-    steps = [s for s, n in zip(xs, counts) if n > 1]
-    d = abs(x_ptr - o_ptr)
-    return xs == os and bool(steps) and es * width <= d and d + es * width <= es * min(steps)
+    return xs == os and not _rows_meet(xs, counts, width, (o_ptr - x_ptr) // es)
 
 
 # ---------------------------------------------------------------------------------------
@@ -302,7 +317,7 @@ def kv_append_slots(kv_new: torch.Tensor, kv_cache, slots: torch.Tensor, positio
         if q.shape != (T, heads, MLA_DIM_QK) or q.dtype != dtype or (q.numel() and q.stride(2) != 1):
             raise ValueError(f"q must be a [T, H, {MLA_DIM_QK}] tensor like q_pe with unit stride in its heads")
         (_, _, pe_t, pe_h), (_, _, q_t, q_h) = _rows(q_pe), _rows(q)
-        if (T > 1 and q_t < MLA_DIM_QK) or (heads > 1 and q_h < MLA_DIM_QK):
+        if T * heads and _rows_meet((q_t, q_h), (T, heads), MLA_DIM_QK):
             raise ValueError("q's rows overlap")
         pe_ptr, q_ptr = q_pe.data_ptr(), q.data_ptr() + 2 * MLA_DIM_V
         if T * heads and not _apart_or_same(pe_ptr, (pe_t, pe_h), q_ptr, (q_t, q_h), (T, heads), _ROPE_DIM, 2):

@@ -201,3 +201,16 @@ def test_the_longest_slot_map(gpu):
     assert r.positions[:104].tolist() == [*range(100), 5, 6, 7, -1] and r.slots[:101].tolist() == [*range(100), 5]
     for m in (r.slots, r.positions):
         assert m.shape == (T,) and (m[-(1 << 20):] == -1).all() and (m[1 << 30:(1 << 30) + 1000] == -1).all()
+
+
+def test_outputs_whose_rows_share_memory_are_refused(gpu):
+    """Strides that are wide enough each, but not together."""
+    x, pos, rope = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda"), M.rope_plan()
+    buf = torch.zeros(8192, dtype=torch.bfloat16, device="cuda")
+    for strides in ((64, 64, 1), (64, 128, 1), (128, 64 + 32, 1)):
+        with pytest.raises(ValueError, match="rows overlap"):
+            M.apply_rope(x, pos, rope, out=buf.as_strided((3, 2, 64), strides))
+    M.apply_rope(x, pos, rope, out=buf.as_strided((3, 2, 64), (64, 256, 1)))  # heads apart, tokens close
+    new, cache = torch.zeros(3, 576, dtype=torch.bfloat16, device="cuda"), M.fp4_kv_cache(1)
+    with pytest.raises(ValueError, match="q's rows overlap"):
+        M.kv_append_slots(new, cache, pos, pos, rope, x, buf.as_strided((3, 2, 576), (576, 576, 1)))

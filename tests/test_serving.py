@@ -245,19 +245,3 @@ def test_overlap_rule():
     assert _apart_or_same(0, (1152, 576), 1024, (1152, 576), **same)     # parts of one row
     assert not _apart_or_same(0, (1152, 576), 1152 - 64, (1152, 576), **same)  # into the next head
     assert not _apart_or_same(0, (128, 64), 64, (128, 64), **same)
-
-
-def test_more_tokens_than_a_launch_takes_are_refused(lib):
-    """Up to the largest counts an int32 holds; the limits are those of the header."""
-    c, r = cache_desc(), rope_desc()
-    for tokens in ((1 << 26) - 3, 1 << 30, 2 ** 31 - 1):
-        assert lib.mla_kv_gather(ctypes.byref(c), BASE, tokens, BASE, 576, None) == 4 and b"too many tokens" in lib.mla_last_error()
-    a = _lib.MlaAppendSlotsArgs()
-    a.kv_new, a.new_stride, a.slots = BASE, 576, BASE
-    for a.tokens in ((1 << 27) - 7, 1 << 30, 2 ** 31 - 1):
-        assert lib.mla_kv_append_slots(ctypes.byref(c), None, ctypes.byref(a), None) == 4 and b"too many tokens" in lib.mla_last_error()
-    a = _lib.MlaRopeArgs()
-    a.x, a.out, a.positions, a.heads, a.dim = BASE, 2 * BASE, BASE, 1, 1024
-    for r.dim, per in ((64, 8), (128, 8), (256, 4), (1024, 1)):
-        for a.tokens in (((1 << 24) - 1) * per + 1, 2 ** 31 - 1):
-            assert lib.mla_apply_rope(ctypes.byref(r), ctypes.byref(a), None) == 4 and b"too many tokens" in lib.mla_last_error()
