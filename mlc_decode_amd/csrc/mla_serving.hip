@@ -107,12 +107,26 @@ __device__ __forceinline__ void rotate(float& a, float& b, f32x2 cs) {
   b = a * cs[1] + b * cs[0];
   a = x;
 }
+// A token without a position stays as it is, bit for bit (a turn of zero would spread an infinity or a NaN to its pair,
+// and make some -0 a 0): its cosines hold a signalling NaN, which no arithmetic gives.
+constexpr uint32_t kStill = 0x7F800001u;
+__device__ __forceinline__ f32x2 turn_or_still(int pos, double f, float amp) {
+  return pos < 0 ? f32x2{__uint_as_float(kStill), 0.f} : turn(pos, f, amp);
+}
+__device__ __forceinline__ bool is_still(f32x2 cs) { return __float_as_uint(cs[0]) == kStill; }
+// Whether any of the four waves' lanes set `mine`, the same for all of them; a barrier.
+__device__ __forceinline__ bool any_of_256(bool mine, int (&any_sh)[4]) {
+  any_sh[threadIdx.x >> 6] = __builtin_amdgcn_ballot_w64(mine) != 0;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(any_sh[0] | any_sh[1] | any_sh[2] | any_sh[3]) != 0;
+}
 template <class E>
 __device__ __forceinline__ void rotate_bits(typename E::bits& a, typename E::bits& b, f32x2 cs) {
   float x = E::value(a), y = E::value(b);
   rotate(x, y, cs);
-  a = E::of(x);
-  b = E::of(y);
+  const bool keep = is_still(cs);
+  a = keep ? a : E::of(x);
+  b = keep ? b : E::of(y);
 }
 
 // Item `i` of [tokens][heads][items] as (t, h, it), in steps of 256 items without a division.
@@ -152,26 +166,26 @@ struct RopeParams {
 
 // 256 threads take `tile` tokens (tile * rot / 2 <= kPairs): each pair's cosine and sine once per token into LDS,
 // then every head.  VEC: 16-byte chunks; a chunk of the rotated dims holds whole pairs (interleaved), or is
-// taken together with the chunk half the rotated dims further on (half layout).  A token without a position is copied
-// bit for bit: by a turn of zero an infinity or a NaN would spread to its pair, and -0 could become 0.
+// taken together with the chunk half the rotated dims further on (half layout).
 // Bound by memory: 8191 tokens x 32 heads of 128 fp16 dims, 64 of them rotated, 23.0 us (134 MB; 24.8 with one chunk
 // a thread in flight and a division an item, 23.4 with four chunks).  128 tokens x 128 heads: 3.8 us, a launch.
 constexpr int kPairs = 512, kRopeTile = 8;
 template <class E, bool VEC>
 __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
   __shared__ f32x2 cs[kPairs];
-  __shared__ bool still[kRopeTile];  // the token has no position
+  __shared__ int any_sh[4];
   const int pairs = p.rot / 2;
   const int wg = blockIdx.x / p.split, sub = blockIdx.x - wg * p.split;
   const int t0 = wg * p.tile;
   const int nt = p.tokens - t0 < p.tile ? p.tokens - t0 : p.tile;
+  bool mine = false;
   for (int i = threadIdx.x; i < nt * pairs; i += 256) {
     const int t = i / pairs;
     const int pos = p.positions[t0 + t];
-    cs[i] = turn(pos, p.freqs[i - t * pairs], p.amp);
-    still[t] = pos < 0;
+    cs[i] = turn_or_still(pos, p.freqs[i - t * pairs], p.amp);
+    mine |= pos < 0;
   }
-  __syncthreads();
+  const bool some_still = any_of_256(mine, any_sh);  // rare: the loop looks for them only then
   const int h0 = (int)((int64_t)p.heads * sub / p.split), h1 = (int)((int64_t)p.heads * (sub + 1) / p.split);
   const int nh = h1 - h0;
   constexpr int W = VEC ? 16 / E::kBytes : 1;  // values per item
@@ -189,7 +203,7 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
     for (int i = threadIdx.x; i < total; i += 256 * U) {
       i32x4 v[U], w[U];
       uint8_t* dst[U];
-      int pair[U];  // the chunk's first pair among its tile's, -1: a chunk that is copied, -2: with its other half
+      int pair[U];  // the chunk's first pair among its tile's, -1: a chunk that is copied
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + 256 * u < total) {
@@ -198,7 +212,7 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
           const int a = (turns ? p.first + at.it * W : c < lead ? c * W : p.first + p.rot + (c - lead) * W) * E::kBytes;
           const uint8_t* src = p.x + (int64_t)(t0 + at.t) * p.x_st + (int64_t)(h0 + at.h) * p.x_sh + a;
           dst[u] = p.out + (int64_t)(t0 + at.t) * p.o_st + (int64_t)(h0 + at.h) * p.o_sh + a;
-          pair[u] = !turns ? -1 : still[at.t] ? -2 : at.t * pairs + at.it * (p.half ? W : W / 2);
+          pair[u] = turns ? at.t * pairs + at.it * (p.half ? W : W / 2) : -1;
           v[u] = *(const i32x4*)src;
           if (p.half && turns) w[u] = *(const i32x4*)(src + pairs * E::kBytes);
         }
@@ -209,20 +223,21 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
         if (i + 256 * u >= total) break;
         if (pair[u] >= 0) {
           const f32x2* c = cs + pair[u];
-          float x[W], y[W];
-          unpack<E>(v[u], x);
-          if (p.half) {
-            unpack<E>(w[u], y);
+          if (!(some_still && is_still(c[0]))) {
+            float x[W], y[W];
+            unpack<E>(v[u], x);
+            if (p.half) {
+              unpack<E>(w[u], y);
 #pragma unroll
-            for (int j = 0; j < W; ++j) rotate(x[j], y[j], c[j]);
-            *(i32x4*)(dst[u] + pairs * E::kBytes) = pack<E>(y);
-          } else {
+              for (int j = 0; j < W; ++j) rotate(x[j], y[j], c[j]);
+              w[u] = pack<E>(y);
+            } else {
 #pragma unroll
-            for (int j = 0; j < W / 2; ++j) rotate(x[2 * j], x[2 * j + 1], c[j]);
+              for (int j = 0; j < W / 2; ++j) rotate(x[2 * j], x[2 * j + 1], c[j]);
+            }
+            v[u] = pack<E>(x);
           }
-          v[u] = pack<E>(x);
-        } else if (p.half && pair[u] == -2) {
-          *(i32x4*)(dst[u] + pairs * E::kBytes) = w[u];
+          if (p.half) *(i32x4*)(dst[u] + pairs * E::kBytes) = w[u];
         }
         *(i32x4*)dst[u] = v[u];
       }
@@ -234,7 +249,7 @@ __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
       if (at.it < rot_items) {
         const int a = (p.first + (p.half ? at.it : 2 * at.it)) * E::kBytes, b = a + (p.half ? pairs : 1) * E::kBytes;
         typename E::bits x = *(const typename E::bits*)(src + a), y = *(const typename E::bits*)(src + b);
-        if (!still[at.t]) rotate_bits<E>(x, y, cs[at.t * pairs + at.it]);
+        rotate_bits<E>(x, y, cs[at.t * pairs + at.it]);
         *(typename E::bits*)(dst + a) = x;
         *(typename E::bits*)(dst + b) = y;
       } else {
@@ -286,8 +301,10 @@ __device__ __forceinline__ void put_latent(const Cache& c, int64_t page, int row
     const bool bad = top >= 0x7F80u;
     const int k = bad ? 0 : block_exp(top, 2, 0x40);
     const float sc = __uint_as_float((uint32_t)(k + 127) << 23);
+    if (__builtin_amdgcn_ballot_w64(k > 125) != 0) {  // uniform, rare
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_fmed3f(x[j], -0x1.8p127f, 0x1.8p127f);
+      for (int j = 0; j < 8; ++j) x[j] = __builtin_amdgcn_fmed3f(x[j], -0x1.8p127f, 0x1.8p127f);
+    }
     uint32_t w = 0;
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], sc, 0);
     w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], sc, 1);
@@ -342,7 +359,7 @@ template <class E>
 __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
   __shared__ f32x2 cs[kAppendTile][32];
   __shared__ int32_t slot_sh[kAppendTile];  // -1: names no row
-  __shared__ bool still[kAppendTile];       // the token has no position
+  __shared__ int any_sh[4];
   const int t0 = blockIdx.x * p.tile;
   const int nt = p.tokens - t0 < p.tile ? p.tokens - t0 : p.tile;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -350,12 +367,13 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
     const int slot = p.slots[t0 + threadIdx.x];
     slot_sh[threadIdx.x] = slot >= 0 && slot < p.cache.tokens ? slot : -1;
   }
+  bool mine = false;
   if (p.freqs != nullptr) {
     const int t = threadIdx.x >> 5;
     if (t < nt) {
       const int pos = p.positions[t0 + t];
-      cs[t][threadIdx.x & 31] = turn(pos, p.freqs[threadIdx.x & 31], p.amp);
-      still[t] = pos < 0;
+      mine = pos < 0;
+      cs[t][threadIdx.x & 31] = turn_or_still(pos, p.freqs[threadIdx.x & 31], p.amp);
     }
   }
   // a wave's tokens, loaded together, whatever their slots
@@ -371,7 +389,7 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
       if (lane < 32) x[u] = *(const uint16_t*)(src + 2 * kDV + rope_a), y[u] = *(const uint16_t*)(src + 2 * kDV + rope_b);
     }
   }
-  __syncthreads();
+  const bool some_still = any_of_256(mine, any_sh);
 #pragma unroll
   for (int u = 0; u < kAppendTile / 4; ++u) {
     const int t = wave + 4 * u;
@@ -381,7 +399,7 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
     const int64_t page = slot / kPage;
     const int row = (int)(slot % kPage);
     if (lane < 32) {
-      if (p.freqs != nullptr && !still[t]) rotate_bits<E>(x[u], y[u], cs[t][lane]);
+      if (p.freqs != nullptr) rotate_bits<E>(x[u], y[u], cs[t][lane]);
       uint8_t* dst = p.cache.rope + page * p.cache.rp + row * p.cache.rt;
       *(uint16_t*)(dst + rope_a) = x[u];
       *(uint16_t*)(dst + rope_b) = y[u];
@@ -398,8 +416,7 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
   for (int i = first; i < total; i += 256 * U) {
     i32x4 a[U], b[U];
     uint8_t* dst[U];
-    const f32x2* turns[U];  // null: no row
-    bool copied[U];
+    const f32x2* turns[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       turns[u] = nullptr;
@@ -407,7 +424,6 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
         const uint8_t* src = p.q_pe + (int64_t)(t0 + at.t) * p.pe_st + (int64_t)at.h * p.pe_sh + 16 * at.it;
         dst[u] = p.q + (int64_t)(t0 + at.t) * p.q_st + (int64_t)at.h * p.q_sh + 16 * at.it;
         turns[u] = &cs[at.t][(p.half ? 8 : 4) * at.it];
-        copied[u] = still[at.t];
         a[u] = *(const i32x4*)src;
         if (p.half) b[u] = *(const i32x4*)(src + 64);
       }
@@ -416,7 +432,7 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (turns[u] == nullptr) continue;
-      if (copied[u]) {
+      if (some_still && is_still(turns[u][0])) {
         *(i32x4*)dst[u] = a[u];
         if (p.half) *(i32x4*)(dst[u] + 64) = b[u];
         continue;

@@ -211,11 +211,14 @@ def apply_rope(x: torch.Tensor, positions: torch.Tensor, rope: Rope, first: Opti
 def _rows_meet(strides, counts, width: int, shift: int = 0) -> bool:
     """Whether any two of ``counts[0] * counts[1]`` rows of ``width`` elements at these strides overlap; with a ``shift``,
     whether a row and one of the same rows that many elements on do."""
+    (st, sh), (t, h), d = strides, counts, abs(shift)
+    if (d == 0 or d >= width) and (h == 1 or sh >= d + width) and (t == 1 or st >= (h - 1) * sh + d + width):
+        return False  # the usual layouts: heads side by side, token after token
     (s0, n0), (s1, n1) = sorted((s if n > 1 else 0, n) for s, n in zip(strides, counts))
     if shift == 0 and ((n0 > 1 and s0 < width) or (n1 > 1 and s1 < width)):
         return True
     reach = 0 if s1 == 0 else min(n1 - 1, ((n0 - 1) * s0 + abs(shift) + width) // s1)
-    for k1 in range(-reach, reach + 1):  # as far as the other stride's rows reach: 0 or 1 in the usual layouts
+    for k1 in range(-reach, reach + 1):  # as far as the other stride's rows reach
         at = shift + k1 * s1
         near = 0 if s0 == 0 else -at // s0
         for k0 in (near, near + 1):
