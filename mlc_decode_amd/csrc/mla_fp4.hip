@@ -1075,7 +1075,11 @@ __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __r
         }
         if constexpr (SOFT) {
           if (r == 0) {
-            settled(s);
+            // With PV, four of its MFMAs and the reads before them lie between: the empty asm keeps that order.
+            if constexpr (PV)
+              asm volatile("" : "+v"(s[0]), "+v"(s[1]), "+v"(o[0][0]), "+v"(o[1][0]), "+v"(o[2][0]), "+v"(o[3][0]));
+            else
+              settled(s);
             top = max3(max3(s[0][0], s[0][1], s[0][2]), max3(s[0][3], s[1][0], s[1][1]), max2(s[1][2], s[1][3]));
             const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = max2(__uint_as_float(x[0]), __uint_as_float(x[1]));
