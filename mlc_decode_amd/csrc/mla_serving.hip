@@ -732,7 +732,7 @@ __global__ __launch_bounds__(kChunk) void mla_release_kernel(ReleaseParams p) {
     return p.block_table[(int64_t)(base + i) * p.bt_stride + from_sh[i] + (r - start_sh[i])];
   };
   if (tid == 0) gaps_sh = 0;  // ordered by the scan's barriers
-  int keep = 0;
+  int keep = 0, held[2] = {-1, -1};  // held: this thread's first entries of a single chunk
   bool cut = false, gaps = false;
   int64_t dropped = 0, missing = 0, total = 0, before = 0;  // missing: of this thread's entries; before: pages put back
 #pragma unroll 1
@@ -762,10 +762,15 @@ __global__ __launch_bounds__(kChunk) void mla_release_kernel(ReleaseParams p) {
       const int64_t here = start_sh[kChunk];
       if (pass == 0) {
         dropped += here;
-        for (int64_t r = tid; r < here; r += kChunk) missing += !is_page(entry(base, r));
+        // the first two requested together
+        if (tid < here) held[0] = entry(base, tid);
+        if (tid + kChunk < here) held[1] = entry(base, tid + kChunk);
+        missing += (tid < here && !is_page(held[0])) + (tid + kChunk < here && !is_page(held[1]));
+        for (int64_t r = tid + 2 * kChunk; r < here; r += kChunk) missing += !is_page(entry(base, r));
       } else {
         for (int64_t r0 = 0; r0 < here; r0 += kChunk) {  // uniform
-          const int page = r0 + tid < here ? entry(base, r0 + tid) : -1;
+          const bool again = p.batch <= kChunk && r0 < 2 * kChunk;  // uniform
+          const int page = r0 + tid >= here ? -1 : again ? held[r0 >= kChunk] : entry(base, r0 + tid);
           int64_t rank = before + tid;
           if (gaps) {  // uniform
             rank = before + block_scan(is_page(page) ? 1 : 0, wsum) - 1;

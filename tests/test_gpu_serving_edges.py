@@ -139,7 +139,7 @@ def foreign(m, rows, seed):
     return m
 
 
-@pytest.mark.parametrize("B,hi,P", [(1, 300, 6), (7, 700, 12), (64, 500, 9), (1030, 200, 5), (2500, 100, 3), (40, 64 * 40, 41)])
+@pytest.mark.parametrize("B,hi,P", [(1, 300, 6), (7, 700, 12), (64, 500, 9), (1000, 500, 9), (1030, 200, 5), (2500, 100, 3), (40, 64 * 40, 41)])
 def test_release_gives_back_pages_of_the_pool_only(gpu, B, hi, P):
     m, g = state(B, B, P, hi, 10)
     m = foreign(Pool(m.free, m.count, m.table, m.lens, m.nb), range(0, B, 3), B)
