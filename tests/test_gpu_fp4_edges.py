@@ -9,7 +9,8 @@ import torch
 from mlc_decode_amd import (flash_mla_with_kvcache, get_mla_metadata, kv_gather, mla_decode_absorbed, mla_decode_with_kvcache,
                             prepare_w_uv, quantize_kv_cache)
 from oracle import mla_fp4_ref as F4
-from test_gpu_fp4 import SCALE, assert_cache, assert_decode, problem, say, table_for, to_gpu
+from oracle import mla_ref as R
+from test_gpu_fp4 import SCALE, assert_cache, assert_decode, exact, problem, say, table_for, to_gpu
 
 pytestmark = pytest.mark.gpu
 
@@ -129,6 +130,27 @@ def test_queries_of_unequal_size(gpu, H, kind):
     if kind == "huge":
         q = (q.double() * 2.0 ** -100)  # the same scores
     assert_decode(out, lse, q, kv, table, lens, True, f"unequal H={H} {kind}")
+
+
+@pytest.mark.parametrize("H", [16, 64, 128])
+def test_outlier_queries_within_the_decodes_bar(gpu, H):
+    """One query dim of every 32 a thousand times its neighbours: the decode's own bar (outputs 1e-2, lse
+    1e-3), against the exact attention of the same inputs.  Above 32 rows the query is two e4m3 parts, which drop at
+    most 2^-15 of a block's largest value a: a logit is off by at most 2^-15 sum_d a_d |k_d| / 24, and by the root of
+    that sum of squares over sqrt(3) where the dropped bits are even.  Here a = 16, |k_d| about 1: 2^-15 * 16 * sqrt(512) /
+    (24 sqrt(3)) = 2.7e-4."""
+    q, cache, table, lens, kv = problem(H + 1, [900, 300, 65, 1], H, 1)
+    x = q.float() / 64.0
+    x[..., 7:512:32] *= 1024.0
+    q = x.to(torch.bfloat16)
+    table = table_for(table, H, False)
+    say(f"outliers within the bar H={H}")
+    out, lse = mla_decode_with_kvcache(q.cuda(), cache, table.cuda(), lens.cuda())
+    torch.cuda.synchronize()
+    for b, n in enumerate(lens.tolist()):
+        keys = R.gather(kv[:, :, 0], table[b], n)
+        o, l, _, _ = exact(q[b], kv, keys, [n])
+        assert (out[b].double().cpu() - o).abs().max() <= 1e-2 and (lse[b].double().cpu() - l).abs().max() <= 1e-3
 
 
 def test_largest_latents(gpu):
