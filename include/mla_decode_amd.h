@@ -184,10 +184,11 @@ int mla_num_parts(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, 
 /*
  * mla_num_parts for a cache of format kv_format: the 4-bit decode is laid out for two workgroups of 16 (at
  * most 32 rows) or 64 query rows per compute unit, or one of 128, the other formats as mla_num_parts says.
- * max_pages, where not 0: the batch has at most so many pages to read (batch * the block table's width, or
- * batch * ceil(topk / 64)); few pages are decoded in workgroups of 16 rows for any row count, if the
- * schedule has that many parts or fewer (or no sequence has more than one page).  Any schedule is decoded
- * right; this one fills the GPU.
+ * max_pages, where not 0: the batch has at most so many pages to read (batch * the longest sequence's, the block
+ * table's width if that is all that is known, or batch * ceil(topk / 64)).  For few pages the result is that of
+ * workgroups of 16 rows for any row count; the decode takes them with a schedule of exactly so many parts, and where
+ * the table's width says that the pages are few with fewer parts too (or where no sequence has more than one page).
+ * Any schedule is decoded right; this one fills the GPU.
  */
 int mla_num_parts_for(int32_t batch, int32_t s_q, int32_t heads_q, int32_t heads_k, int32_t cu_count, int32_t kv_format,
                       int64_t max_pages);

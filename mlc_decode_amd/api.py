@@ -178,8 +178,9 @@ def get_mla_metadata(cache_seqlens: torch.Tensor, num_heads_per_head_k: int, num
     scheduled as ``topk`` keys long, whatever ``cache_seqlens`` holds.  ``kv_cache``: the cache the
     schedule is for; an :class:`Fp4KVCache` is decoded by workgroups of another size, whose count the
     default ``num_parts`` then is (any schedule is decoded right; that one fills the GPU).
-    ``max_seqlen``: no sequence is longer, as far as the host knows (``64 * block_table.shape[1]``, say); a 4-bit
-    cache's schedule is then made for the decode's form for few pages, where they are few.
+    ``max_seqlen``: no sequence is longer, as far as the host knows (the table's width, ``64 * block_table.shape[1]``,
+    if it knows no better); a 4-bit cache's schedule is then made for the decode's form for few pages, where they are few,
+    and the decode takes that form, however wide its table is.
     """
     _require_gpu(cache_seqlens, "cache_seqlens")
     if topk is not None:

@@ -1243,8 +1243,12 @@ hipError_t launch_decode(const DecodeParams& p, const int32_t* sched, int num_pa
   const int64_t pages = (int64_t)p.batch * most;
   const int64_t tiles = (p.rows + 15) / 16;
   const int64_t round = 2 * cus;
-  const bool few = pages <= kFewPages / tiles &&
-                   (num_parts * tiles <= round || (most <= 1 && pages * tiles <= (p.rows > 64 ? 2 : 1) * round));
+  // A schedule of exactly as many parts as such a form's fill the GPU with was made for it, from the longest length; the
+  // table may be as wide as the longest context that is allowed.  (The other forms' parts of such a schedule fill a
+  // quarter: 32 x 11 pages x 128 heads in a table of 2048 columns 37.9, and 22.9 with 16 rows.)
+  const bool made = num_parts * tiles <= round && num_parts == round / tiles;
+  const bool few = made || (pages <= kFewPages / tiles &&
+                            (num_parts * tiles <= round || (most <= 1 && pages * tiles <= (p.rows > 64 ? 2 : 1) * round)));
   const int R = few ? 16 : rows_per_workgroup(p.rows);
   if (R == 16) return launch_rt<1>(p, sched, num_parts, st);
   if (R == 64) return launch_rt<4>(p, sched, num_parts, st);

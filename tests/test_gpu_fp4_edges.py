@@ -211,3 +211,18 @@ def test_absorbed(gpu, H, sparse):
     mag = torch.stack([o[:, :, h].abs() @ w[h].double().abs() for h in range(H)], 2)
     # v's own rounding (2^-8) and fp32 sums of 512 products
     assert ((v.double().cpu() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * mag).all()
+
+
+@pytest.mark.parametrize("H", [40, 128, 200])
+def test_a_schedule_for_few_pages_is_taken_with_a_wide_table(gpu, H):
+    """The longest length that the host knows decides, not the table's width: the same workgroups, bit for bit."""
+    q, cache, table, lens, kv = problem(H, [700, 64, 0, 333, 1], H, 1)
+    wide = torch.nn.functional.pad(table, (0, 2000))
+    ld = lens.cuda()
+    say(f"few pages, wide table H={H}")
+    meta = get_mla_metadata(ld, H, 1, kv_cache=cache, max_seqlen=700)
+    out, lse = flash_mla_with_kvcache(q.cuda(), cache, wide.cuda(), ld, 512, *meta)
+    want = flash_mla_with_kvcache(q.cuda(), cache, table.cuda(), ld, 512, *meta)
+    torch.cuda.synchronize()
+    assert_decode(out, lse, q, kv, wide, lens, False, f"wide table H={H}")
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
