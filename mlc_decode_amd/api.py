@@ -252,6 +252,8 @@ class Fp4KVCache(NamedTuple):
     32 dims, 1 .. 254; 255 marks a block that held a NaN or an infinity), ``rope`` bf16
     ``[num_blocks, 64, 64]``.  Latent value d of a token is ``e2m1(code_d) * 2**(scale[d // 32] - 127)``.
     Values past ``1.5 * 2**127``, the largest that the codes and bf16 both hold, are stored as that one.
+    Decodes of more than 32 query rows may hold a query's latent values to ``2**-15`` of the largest of their 32 dims
+    (exactly down to ``2**-7`` of it); those of up to 32 rows take them as they are.
     400 bytes a token (bf16: 1152, fp8: 656).  No counterpart in the reference.
     """
     latent: torch.Tensor

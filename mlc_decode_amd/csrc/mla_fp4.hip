@@ -21,9 +21,11 @@
 //     operand order, rounded to bf16 (the PV operand's type; the sum that divides the output is of the rounded
 //     weights, so that the rounding cancels in it), to all waves, each of which accumulates its share of the
 //     512 output dims in fp32.
-// What bounds them (one token a sequence unless said): 16 rows, 128 ragged sequences, 213 MB: 46 us in the main kernel,
-// 4.65 TB/s, a large copy's rate, 52 with the merge.  128 rows: instruction issue (see mla_fp4_wide_kernel): 64 x 4096
-// tokens x 128 heads 79 us with the merge, 32 x 16384 x 2 x 128 233 us, 1.25 PFLOP/s of bf16 products.
+// What bounds them (one token a sequence unless said): 16 rows, 128 ragged sequences, 213 MB: 44.5 us in the main
+// kernel, 4.8 TB/s, a large copy's rate, 52 with the merge.  64 rows: two barriers a stage with nothing between the
+// products but the softmax: 64 x 64 heads x 4096 tokens 57 us where bytes and operations take 28, the matrix
+// pipes busy 32% of the time.  128 rows: issue and waits (see mla_fp4_wide_kernel): 64 x 4096 tokens x 128 heads
+// 78 us with the merge, 32 x 16384 x 2 x 128 235 us, 1.24 PFLOP/s of bf16 products.
 // The running row maximum moves only when a score passes it by more than 2^kSlack (P then stays far from
 // overflow in bf16 and fp32), so the output is rescaled rarely and exactly.
 #include <hip/hip_runtime.h>
@@ -181,7 +183,10 @@ __device__ __forceinline__ i32x4 widen8(int w, float scale) {
 // largest (measured; between groups it adds as fp32), so hi's products lose nothing there, which a scale
 // that uses all of e4m3's range does not give (relative error of S, normal data: 4.6e-6 at amax 240, 1.1e-6
 // here).  lo = (q - hi) / 2^(k - 10) holds four more bits: values of the block's top seven binades are
-// exact, smaller ones off by at most 2^-15 of the amax.
+// exact, smaller ones off by at most 2^-15 of the amax a.  So beside an outlier a thousand times as large a value is
+// held to 2^-5, less than bf16's 2^-8; in a logit that is 2^-15 a |k_d|, where the outlier's own rounding to bf16 has
+// put up to 2^-8 a |k|.  Queries of 512 dims with such an outlier in every block stay within the decodes' bar of 1e-3 (lse)
+// and 1e-2 (outputs).
 struct QuerySplit {
   i32x8 hi, lo;
   int scale;  // this lane group's scale byte of hi
@@ -835,13 +840,16 @@ __global__ __launch_bounds__(256, 2) void mla_fp4_kernel(const int32_t* __restri
 // (Two 64-row workgroups a CU: 64 x 128 heads x 4096 tokens 97 us, 32 x 2 x 128 x 16384 303; the first form of this
 // kernel, which formed every address anew, 88 and 263, with the addresses kept 82 and 240, and with rows stored as 16
 // bytes a lane 80 and 235.)
-// What bounds it is instruction issue: a SIMD's MFMA time and the vector instructions beyond two per MFMA add up
-// (measured: two waves of one bf16 MFMA and 2, 4, 8 additions a step take 18.5, 26, 37 cycles a step), so the loop
-// keeps its lane addresses, takes buffer halves as constants (two stages a turn) and page addresses as scalars.
+// What bounds it is issue and waits: of the waves' cycles (64 x 4096 tokens x 128 heads) 36% wait to issue and 32% at
+// counters and barriers, which two waves a SIMD cannot cover for each other; the matrix pipes are busy 46% of the
+// time, LDS 34%, a fifth of that in bank conflicts.  A SIMD's MFMA time and the vector instructions beyond
+// two per MFMA add up (measured: two waves of one bf16 MFMA and 2, 4, 8 additions a step take 18.5, 26, 37 cycles a
+// step), so the loop keeps its lane addresses, takes buffer halves as constants (two stages a turn) and page
+// addresses as scalars.
 //
 // A stage in LDS (kRawStage bytes): per token tile the codes as [lane group g][token][16-byte piece c ^ (token / 2 % 4)]
-// of the 64 bytes that hold blocks 4g .. 4g + 3 (the copies read whole 64 bytes, the fragment reads of one c
-// are free of bank conflicts), two rope fragments, then the tokens' scale bytes.
+// of the 64 bytes that hold blocks 4g .. 4g + 3 (the copies read whole 64 bytes, and the fragment reads of one c
+// spread over the banks), two rope fragments, then the tokens' scale bytes.
 template <bool SPARSE>
 __global__ __launch_bounds__(512, 2) void mla_fp4_wide_kernel(const int32_t* __restrict__ sched, int row_blocks, int num_parts,
                                                               DecodeParams) {

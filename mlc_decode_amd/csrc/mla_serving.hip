@@ -167,8 +167,10 @@ struct RopeParams {
 // 256 threads take `tile` tokens (tile * rot / 2 <= kPairs): each pair's cosine and sine once per token into LDS,
 // then every head.  VEC: 16-byte chunks; a chunk of the rotated dims holds whole pairs (interleaved), or is
 // taken together with the chunk half the rotated dims further on (half layout).
-// Bound by memory: 8191 tokens x 32 heads of 128 fp16 dims, 64 of them rotated, 23.0 us (134 MB; 24.8 with one chunk
-// a thread in flight and a division an item, 23.4 with four chunks).  128 tokens x 128 heads: 3.8 us, a launch.
+// Bound by memory: 8191 tokens x 32 heads of 128 fp16 dims, 64 of them rotated, 23.3 us (134 MB; 24.8 with one chunk
+// a thread in flight and a division an item, 23.4 with four chunks).  128 tokens x 128 heads: 4.0 us, a launch.
+// Rows that no 16-byte chunk fits (71 dims a head) go value by value, in 2- or 4-byte accesses: 8191 x 32 heads, 75 MB,
+// 34.9 us; rows that start on odd elements have no wider ones.
 constexpr int kPairs = 512, kRopeTile = 8;
 template <class E, bool VEC>
 __global__ __launch_bounds__(256) void mla_rope_kernel(RopeParams p) {
@@ -352,8 +354,10 @@ struct AppendParams {
 
 // Workgroups of four waves take `tile` tokens: the 32 pairs' cosines and sines of each token into LDS, a
 // wave per token for its cache row, and all threads for the queries' rope dims in 16-byte chunks.  One launch for
-// the three.  What is not rotated is copied bit for bit.  Bound by memory where there is any: 76 MB of a ragged prefill (16 heads, 4-bit cache) in 15.7 us, 4.8
-// TB/s, a large copy's rate; a decode step's 128 tokens x 64 heads 3.7 us.
+// the three.  What is not rotated is copied bit for bit.  Bound by memory where there is any: 76 MB of a ragged prefill
+// (16 heads, 4-bit cache) in 16.1 us, 4.7 TB/s, a large copy's rate; 65536 tokens without queries into the 4-bit cache
+// 22.8 us (floor 21), into the fp8 one 27.5 (24.5: its scales leave four bytes a token and block).  A decode step's
+// 128 tokens x 16 heads 3.5 us.
 constexpr int kAppendTile = 8;
 template <class E>
 __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
@@ -455,7 +459,8 @@ __global__ __launch_bounds__(256) void mla_append_slots_kernel(AppendParams p) {
 
 // The 4-bit form of mla_kv_append: n_new tokens of each sequence at its length, which then advances.  One
 // workgroup per sequence, a wave per token; every wave checks all of the sequence's pages first.  What bounds it
-// is latency: the length, the table's entry, the token, one after the other.
+// is latency: the length, the table's entry, the token, one after the other: a token of each of 128 sequences 3.2 us.
+// Whole pages (a quantised cache of 138496 tokens, 215 MB) 39.5 us, 5.4 TB/s.
 struct SeqAppendParams {
   Cache cache;
   const uint8_t* kv_new;
