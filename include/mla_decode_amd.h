@@ -105,7 +105,9 @@ extern "C" {
  * (all strides of codes and scales in bytes, multiples of 16, the scale's token stride below 2^24, both
  * pointers 16-byte aligned).  Latent value d is e2m1(code_d) * 2^(byte - 127), byte 1 .. 254; byte 255
  * makes the block NaN, and with it every output of the query rows that see the token (their lse is -inf, as any NaN
- * row's); rows that do not see it are as without it.  Rope and queries as with fp8.  Above 32 query rows (s_q * heads,
+ * row's); rows that do not see it are as without it.  (With the other formats a NaN or an infinity in the latent of a
+ * causally hidden token makes its dim of every row's output NaN: the token's weight of 0 times it.)  Rope and
+ * queries as with fp8.  Above 32 query rows (s_q * heads,
  * where the pages are not few: mla_num_parts_for) the latent part of a query enters the scores as two 8-bit parts:
  * a value is exact down to 2^-7 of the largest of its 32 dims, and off by at most 2^-15 of that largest below it.
  */
