@@ -500,6 +500,67 @@ int mla_reserve_pages(const mla_page_pool* pool, const int32_t* new_lens, int32_
  */
 int mla_release_pages(const mla_page_pool* pool, const int32_t* keep_lens, void* stream);
 
+/* ---- drafted tokens: trees over a paged cache (no counterpart in the reference) ------------ */
+
+/*
+ * The plan of a step whose last tree_lens[b] (at most s_q; NULL: s_q) cached tokens are a tree of drafted ones, from
+ * each one's parent: -1 for a root, whose parent is the prefix's last token, or a lower node of the same tree.  Any other
+ * value, and a node below such a one or past tree_lens, is no node: it sees nothing and nothing sees it.
+ *   prefix_lens [batch]       cache_seqlens - tree_lens
+ *   mask [batch, s_q]         bit j of node i: j is i or an ancestor of it; 0 for no node
+ *   positions [batch, s_q]    prefix + the node's depth; -1 for no node
+ *   slots [batch, s_q]        the cache row (page * 64 + row) of token prefix + i, i < tree_lens; -1 past it, or where
+ *                             the table's row has no column or no page (a negative id) for it
+ * A sequence shorter than its tree has none of it: prefix 0, no nodes, slots -1.
+ */
+typedef struct mla_tree_plan_args {
+  const int32_t* parents; /* [batch, s_q] */
+  const int32_t* cache_seqlens;
+  const int32_t* tree_lens;
+  const int32_t* block_table;
+  int32_t block_table_stride, block_table_width;
+  int32_t batch, s_q; /* batch at most 2^20, s_q 1 .. 64 */
+  uint64_t* mask;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* prefix_lens;
+} mla_tree_plan_args;
+int mla_tree_plan(const mla_tree_plan_args* args, void* stream);
+
+/*
+ * mla_decode_fwd for trees of drafted tokens: query i of sequence b sees its first cache_seqlens[b] tokens (here the
+ * prefix's length) and token cache_seqlens[b] + j for every set bit j < s_q of mask[b, i].  Paged caches of every format,
+ * no indices, s_q at most 64, batch at most 65535; `causal` has no part in it.  The schedule is mla_get_metadata's for
+ * the prefix lengths; the workspace is mla_tree_workspace_bytes.  A bit whose token lies past the table's width names
+ * no key, and sets *status.  A row without a key gets out = 0 and lse = -inf.  What the cache rows of drafted tokens
+ * hold reaches only the query rows that see them; an infinity or a NaN in such a token's latent makes those rows' outputs
+ * NaN (lse -inf).
+ */
+int mla_tree_decode_fwd(const mla_decode_args* args, const uint64_t* mask, void* stream);
+
+/* The same followed by the absorbed value projection, as mla_splitkv_fwd and mla_combine_absorb. */
+int mla_tree_absorb_fwd(const mla_decode_args* args, const uint64_t* mask, const void* w_uv_blk, void* v, void* stream);
+
+int64_t mla_tree_workspace_bytes(int32_t batch, int32_t s_q, int32_t heads_q, int32_t num_parts);
+
+/*
+ * The drafted path that the model agrees with.  mask and prefix_lens from mla_tree_plan; tokens [batch, s_q] the drafted
+ * tokens, targets [batch, s_q] the model's choice after each node, both int32 or (wide) int64.  Node 0 is the token that
+ * the step before decided; from it the path goes on to the lowest child whose token is the target of the node before.
+ *   path [batch, s_q]   its nodes, -1 behind its end      counts [batch]      how many they are
+ *   next_tokens [batch] the target after its last node    keep_lens [batch]   prefix_lens + counts
+ * Where node 0 is no root's node the path is empty: counts 0, next token -1.
+ */
+int mla_tree_accept(const uint64_t* mask, const int32_t* prefix_lens, const void* tokens, const void* targets, int32_t wide,
+                    int32_t batch, int32_t s_q, int32_t* path, int32_t* counts, void* next_tokens, int32_t* keep_lens, void* stream);
+
+/*
+ * The path's tokens together at the front of the tree: cache row slots[b, k] takes the token of row slots[b, path[b, k]],
+ * as if all were read before any is written, bit for bit, in every cache format.  Entries below their own place k, negative
+ * or past s_q, and slots outside the cache, name nothing; no two sequences may name the same row.
+ */
+int mla_kv_keep_path(const mla_kv_cache* cache, const int32_t* slots, const int32_t* path, int32_t batch, int32_t s_q, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

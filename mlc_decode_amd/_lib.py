@@ -27,6 +27,7 @@ MLA_NOALLOC_SCRATCH_BYTES = 160 << 20  # the allocation-free decode's static scr
 MLA_DIM_QK = 576
 MLA_DIM_V = 512
 MLA_PAGE_TOKENS = 64
+MLA_TREE_MAX_NODES = 64  # drafted tokens of a sequence
 
 # Every symbol include/mla_decode_amd.h declares.
 EXPORTED = (
@@ -52,6 +53,12 @@ EXPORTED = (
     "mla_kv_gather",
     "mla_reserve_pages",
     "mla_release_pages",
+    "mla_tree_plan",
+    "mla_tree_decode_fwd",
+    "mla_tree_absorb_fwd",
+    "mla_tree_workspace_bytes",
+    "mla_tree_accept",
+    "mla_kv_keep_path",
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -223,6 +230,25 @@ class MlaPagePool(ctypes.Structure):
     ]
 
 
+class MlaTreePlanArgs(ctypes.Structure):
+    """Layout of ``mla_tree_plan_args`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("parents", _vp),
+        ("cache_seqlens", _vp),
+        ("tree_lens", _vp),
+        ("block_table", _vp),
+        ("block_table_stride", _i32),
+        ("block_table_width", _i32),
+        ("batch", _i32),
+        ("s_q", _i32),
+        ("mask", _vp),
+        ("positions", _vp),
+        ("slots", _vp),
+        ("prefix_lens", _vp),
+    ]
+
+
 class MlaError(RuntimeError):
     """A nonzero status from the C ABI, carrying the library's message."""
 
@@ -299,6 +325,18 @@ def load() -> ctypes.CDLL:
         lib.mla_reserve_pages.restype = ctypes.c_int
         lib.mla_release_pages.argtypes = [ctypes.POINTER(MlaPagePool), _vp, _vp]
         lib.mla_release_pages.restype = ctypes.c_int
+        lib.mla_tree_plan.argtypes = [ctypes.POINTER(MlaTreePlanArgs), _vp]
+        lib.mla_tree_plan.restype = ctypes.c_int
+        lib.mla_tree_decode_fwd.argtypes = [ctypes.POINTER(MlaDecodeArgs), _vp, _vp]
+        lib.mla_tree_decode_fwd.restype = ctypes.c_int
+        lib.mla_tree_absorb_fwd.argtypes = [ctypes.POINTER(MlaDecodeArgs), _vp, _vp, _vp, _vp]
+        lib.mla_tree_absorb_fwd.restype = ctypes.c_int
+        lib.mla_tree_workspace_bytes.argtypes = [_i32] * 4
+        lib.mla_tree_workspace_bytes.restype = ctypes.c_int64
+        lib.mla_tree_accept.argtypes = [_vp] * 4 + [_i32] * 3 + [_vp] * 5
+        lib.mla_tree_accept.restype = ctypes.c_int
+        lib.mla_kv_keep_path.argtypes = [ctypes.POINTER(MlaKvCache), _vp, _vp, _i32, _i32, _vp]
+        lib.mla_kv_keep_path.restype = ctypes.c_int
         _lib = lib
         return lib
 

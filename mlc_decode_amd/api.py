@@ -119,8 +119,9 @@ def _workspace(device: torch.device, stream: int, nbytes: int):
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(batch: int, s_q: int, heads: int, num_parts: int) -> int:
-    return _lib.load().mla_workspace_bytes(batch, s_q, heads, num_parts)
+def _workspace_bytes(batch: int, s_q: int, heads: int, num_parts: int, tree: bool = False) -> int:
+    lib = _lib.load()
+    return (lib.mla_tree_workspace_bytes if tree else lib.mla_workspace_bytes)(batch, s_q, heads, num_parts)
 
 
 def grown_workspace_size(current: Optional[int], need: int) -> int:
@@ -316,8 +317,9 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
                      cache_seqlens: Optional[torch.Tensor], sched: torch.Tensor, splits: torch.Tensor,
                      sm_scale: float, causal: bool, out: Optional[torch.Tensor] = None,
                      lse: Optional[torch.Tensor] = None, indices: Optional[torch.Tensor] = None,
-                     status: Optional[torch.Tensor] = None):
-    """Validate a paged decode and fill the C ``mla_decode_args`` for it.
+                     status: Optional[torch.Tensor] = None, tree: Optional["TreePlan"] = None):
+    """Validate a paged decode and fill the C ``mla_decode_args`` for it (with ``tree``: those of the tree decode,
+    whose lengths are the plan's prefix lengths).
 
     The decode reads no block-table column at or past ``block_table.shape[1]``: a sequence
     whose ``cache_seqlens`` entry exceeds ``64 * block_table.shape[1]`` is decoded over the
@@ -356,6 +358,12 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
         kv_ptr = kv_cache.data_ptr()
         kr_ptr = kv_ptr + MLA_DIM_V * 2
     B, s_q, H, _ = q.shape
+    if tree is not None:
+        if indices is not None:
+            raise ValueError("a tree decode takes no indices")
+        cache_seqlens = _check_tree(tree, B, s_q, q.device)
+        if block_table is None:
+            raise ValueError("a tree decode takes a block_table")
     if indices is not None:  # sparse: keys named by index, no page table or lengths
         _require_gpu(indices, "indices")
         if s_q != 1:
@@ -397,7 +405,7 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
     splits = splits.contiguous()
     num_parts = sched.shape[0]
     device = q.device
-    ws, ws_ptr, ws_bytes = _workspace(device, _stream_ptr(device), _workspace_bytes(B, s_q, H, num_parts))
+    ws, ws_ptr, ws_bytes = _workspace(device, _stream_ptr(device), _workspace_bytes(B, s_q, H, num_parts, tree is not None))
     q_ptr = q.data_ptr()
     if indices is not None:
         idx_ptr, idx_stride, topk = indices.data_ptr(), indices.stride(0), indices.shape[1]
@@ -419,19 +427,21 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
         splits.data_ptr(), out.data_ptr(), os_b, os_s, os_h, lse.data_ptr(), ws_ptr, ws_bytes,
         fmt, 0, scale_ptr, scale_page, scale_blk,
         idx_ptr, idx_stride, topk, bt_width, 0, status.data_ptr() if status is not None else 0))
-    keep = (q, latent, rope, scale, block_table, seqlens, sched, splits, out, lse, ws, indices, status)
+    keep = (q, latent, rope, scale, block_table, seqlens, sched, splits, out, lse, ws, indices, status, tree)
     return a, out, lse, keep
 
 
 def _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal,
-            out=None, lse=None, indices=None, status=None, single_split=False):
+            out=None, lse=None, indices=None, status=None, single_split=False, tree=None):
     """One decode through the C ABI.  ``single_split``: the schedule is known to give every
     sequence one split (forced ``num_splits = 1``), so the split-KV pass finishes every row and
-    the combine launch is skipped."""
+    the combine launch is skipped (but for a tree's, whose drafted tokens are one more split)."""
     a, out, lse, keep = make_decode_args(q, kv_cache, block_table, cache_seqlens, sched, splits,
-                                         sm_scale, causal, out, lse, indices, status)
+                                         sm_scale, causal, out, lse, indices, status, tree)
     lib = _lib.load()
-    if single_split:
+    if tree is not None:
+        _launch("mla_tree_decode_fwd", lib.mla_tree_decode_fwd, q.device, ctypes.byref(a), tree.mask.data_ptr())
+    elif single_split:
         _launch("mla_splitkv_fwd", lib.mla_splitkv_fwd, q.device, ctypes.byref(a))
     else:
         _launch("mla_decode_fwd", lib.mla_decode_fwd, q.device, ctypes.byref(a))
@@ -444,7 +454,8 @@ def flash_mla_with_kvcache(q: torch.Tensor, k_cache, block_table: torch.Tensor,
                            tile_scheduler_metadata: torch.Tensor, num_splits: torch.Tensor,
                            softmax_scale: Optional[float] = None, causal: bool = False,
                            out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                           indices: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+                           indices: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None,
+                           tree: Optional["TreePlan"] = None):
     """Paged decode with a precomputed schedule -> ``(out [B,s_q,H,512], lse [B,H,s_q])``.
 
     Same call shape as the reference's use of FlashMLA (handmade/bench_metax_flashmla.py:33-35).
@@ -456,13 +467,18 @@ def flash_mla_with_kvcache(q: torch.Tensor, k_cache, block_table: torch.Tensor,
     No block-table column at or past ``block_table.shape[1]`` is read: a longer
     ``cache_seqlens`` entry is cut to the table and sets ``status[0] = 1`` (``status``: an
     int32 device tensor the caller clears, optional).
+
+    ``tree`` (from ``tree_plan``) decodes the s_q <= 64 query tokens of a sequence as a tree of drafted tokens: each
+    sees the sequence's prefix and, of the drafted ones, its ancestors and itself, as the plan's masks say.
+    ``cache_seqlens`` is not read (the plan has the lengths) and ``causal`` has no part in it; the schedule must come
+    from ``get_mla_metadata(tree.prefix_lens, ...)``.  Every cache format; no ``indices``.
     """
     if head_dim_v != MLA_DIM_V:
         raise ValueError(f"head_dim_v must be {MLA_DIM_V}")
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** -0.5
     return _decode(q, k_cache, block_table, cache_seqlens, tile_scheduler_metadata, num_splits,
-                   softmax_scale, causal, out, lse, indices, status)
+                   softmax_scale, causal, out, lse, indices, status, tree=tree)
 
 
 def prepare_w_uv(w_uv: torch.Tensor) -> torch.Tensor:
@@ -479,7 +495,8 @@ def mla_decode_absorbed(q: torch.Tensor, kv_cache, block_table: Optional[torch.T
                         cache_seqlens: Optional[torch.Tensor], tile_scheduler_metadata: torch.Tensor,
                         num_splits: torch.Tensor, w_uv_blk: torch.Tensor, w_o: Optional[torch.Tensor] = None,
                         softmax_scale: Optional[float] = None, causal: bool = False,
-                        lse: Optional[torch.Tensor] = None, indices: Optional[torch.Tensor] = None):
+                        lse: Optional[torch.Tensor] = None, indices: Optional[torch.Tensor] = None,
+                        tree: Optional["TreePlan"] = None):
     """Decode followed by the absorbed output projection -> ``(y, lse)``.
 
     The split-KV pass runs as in ``flash_mla_with_kvcache``; its partials are merged straight
@@ -497,11 +514,15 @@ def mla_decode_absorbed(q: torch.Tensor, kv_cache, block_table: Optional[torch.T
         raise ValueError("w_uv_blk must be a contiguous [H, 16, 128, 32] tensor in q's dtype (see prepare_w_uv)")
     _require_gpu(w_uv_blk, "w_uv_blk")
     a, out, lse, keep = make_decode_args(q, kv_cache, block_table, cache_seqlens, tile_scheduler_metadata,
-                                         num_splits, softmax_scale, causal, None, lse, indices)
+                                         num_splits, softmax_scale, causal, None, lse, indices, tree=tree)
     v = torch.empty(B, s_q, H, 128, dtype=q.dtype, device=q.device)
     lib = _lib.load()
-    _launch("mla_splitkv_fwd", lib.mla_splitkv_fwd, q.device, ctypes.byref(a))
-    _launch("mla_combine_absorb", lib.mla_combine_absorb, q.device, ctypes.byref(a), w_uv_blk.data_ptr(), v.data_ptr())
+    if tree is not None:
+        _launch("mla_tree_absorb_fwd", lib.mla_tree_absorb_fwd, q.device, ctypes.byref(a), tree.mask.data_ptr(),
+                w_uv_blk.data_ptr(), v.data_ptr())
+    else:
+        _launch("mla_splitkv_fwd", lib.mla_splitkv_fwd, q.device, ctypes.byref(a))
+        _launch("mla_combine_absorb", lib.mla_combine_absorb, q.device, ctypes.byref(a), w_uv_blk.data_ptr(), v.data_ptr())
     del keep
     if w_o is None:
         return v, lse
@@ -515,13 +536,13 @@ def mla_decode_with_kvcache(q: torch.Tensor, kv_cache, block_table: torch.Tensor
                             num_splits: Union[None, int, Tuple[torch.Tensor, torch.Tensor]] = None,
                             sm_scale: Optional[float] = None, causal: bool = True,
                             out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
-                            status: Optional[torch.Tensor] = None):
+                            status: Optional[torch.Tensor] = None, tree: Optional["TreePlan"] = None):
     """Schedule + decode in one call -> ``(out, lse)``.
 
     ``num_splits``: ``None`` = balanced schedule for this GPU; an ``int`` = cut every
     sequence into that many page ranges (1 = the reference's serial baseline: one launch,
     no combine); or a ``(tile_scheduler_metadata, num_splits)`` pair from
-    :func:`get_mla_metadata`.  ``status`` as in :func:`flash_mla_with_kvcache`.
+    :func:`get_mla_metadata`.  ``status`` and ``tree`` as in :func:`flash_mla_with_kvcache`.
     """
     if sm_scale is None:
         sm_scale = MLA_DIM_QK ** -0.5
@@ -531,14 +552,16 @@ def mla_decode_with_kvcache(q: torch.Tensor, kv_cache, block_table: torch.Tensor
         forced = int(num_splits) if num_splits is not None else 0
         if num_splits is not None and forced < 1:
             raise ValueError("num_splits must be >= 1")
+        if tree is not None:
+            cache_seqlens = tree.prefix_lens
         longest = _lib.MLA_PAGE_TOKENS * block_table.shape[1] if block_table is not None and block_table.dim() == 2 else None
         sched, splits = get_mla_metadata(cache_seqlens, q.shape[1] * q.shape[2], 1,
                                          forced_splits=forced, kv_cache=kv_cache, max_seqlen=longest)
         if forced == 1:
             return _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal,
-                           out, lse, status=status, single_split=True)
+                           out, lse, status=status, single_split=True, tree=tree)
     return _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal, out, lse,
-                   status=status)
+                   status=status, tree=tree)
 
 
 def merge_partials(part_o: torch.Tensor, part_lse: torch.Tensor, num_splits: torch.Tensor,
@@ -623,6 +646,33 @@ def kv_append(kv_new: torch.Tensor, kv_cache, block_table: torch.Tensor,
         status.data_ptr() if status is not None else 0, *scale_args))
     _launch("mla_kv_append", _lib.load().mla_kv_append, kv_new.device, ctypes.byref(a))
     return a
+
+
+class TreePlan(NamedTuple):
+    """Trees of drafted tokens behind the sequences' prefixes.  ``mask [B, s_q]`` int64: bit j of row i is set where
+    drafted token i sees drafted token j; ``positions [B, s_q]`` int32, the prefix's length and the token's depth (-1: no
+    token); ``slots [B, s_q]`` int32, the cache rows of the drafted tokens (page * 64 + row; -1: none); ``prefix_lens
+    [B]`` int32.  Made by ``tree_plan``, or with masks of one's own."""
+    mask: torch.Tensor
+    positions: torch.Tensor
+    slots: torch.Tensor
+    prefix_lens: torch.Tensor
+
+
+def _check_tree(tree: TreePlan, B: int, s_q: int, device: torch.device) -> torch.Tensor:
+    """The prefix lengths of a plan for ``[B, s_q]`` query tokens, checked with its masks."""
+    mask, lens = tree.mask, tree.prefix_lens
+    if s_q > _lib.MLA_TREE_MAX_NODES:
+        raise ValueError(f"a tree decode takes s_q <= {_lib.MLA_TREE_MAX_NODES}")
+    for t, name in ((mask, "tree.mask"), (lens, "tree.prefix_lens")):
+        _require_gpu(t, name)
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, q on {device}")
+    if mask.dtype != torch.int64 or mask.shape != (B, s_q) or not mask.is_contiguous():
+        raise ValueError("tree.mask must be a contiguous int64 [B, s_q] tensor")
+    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+        raise ValueError("tree.prefix_lens must be a contiguous int32 [B] tensor")
+    return lens
 
 
 def _cache_format(kv_cache) -> int:

@@ -41,6 +41,7 @@
 #include "mla_fp4.h"
 #include "mla_sched.h"
 #include "mla_serving.h"
+#include "mla_tree.h"
 
 namespace mla {
 
@@ -3963,7 +3964,7 @@ int validate_fp4(int64_t page, int64_t tok, const void* scale, int64_t scale_pag
   return MLA_OK;
 }
 
-int validate(const mla_decode_args* a, int64_t* need_ws) {
+int validate(const mla_decode_args* a, int64_t (*bytes)(int32_t, int32_t, int32_t, int32_t) = mla_workspace_bytes) {
   if (a == nullptr) return fail(MLA_ERR_INVALID, "args is NULL");
   if (a->batch < 1 || a->s_q < 1 || a->heads_q < 1)
     return fail(MLA_ERR_INVALID, "batch, s_q and heads_q must be >= 1");
@@ -4034,11 +4035,18 @@ int validate(const mla_decode_args* a, int64_t* need_ws) {
     const int rc = validate_fp4(a->kv_stride_page, a->kv_stride_tok, a->kv_scale, a->kv_scale_stride_page, a->kv_scale_stride_blk);
     if (rc != MLA_OK) return rc;
   }
-  *need_ws = mla_workspace_bytes(a->batch, a->s_q, a->heads_q, a->num_parts);
-  if (a->workspace == nullptr || a->workspace_bytes < *need_ws)
-    return fail(MLA_ERR_WORKSPACE, "workspace missing or smaller than mla_workspace_bytes()");
+  if (a->workspace == nullptr || a->workspace_bytes < bytes(a->batch, a->s_q, a->heads_q, a->num_parts))
+    return fail(MLA_ERR_WORKSPACE, bytes == mla_workspace_bytes
+                                       ? "workspace missing or smaller than mla_workspace_bytes()"
+                                       : "workspace missing or smaller than mla_tree_workspace_bytes()");
   if (!aligned(a->workspace, 256)) return fail(MLA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   return MLA_OK;
+}
+
+void place_partials(mla::KParams* k, void* at, int64_t slots, int64_t rows) {
+  k->ws_lse = (float*)at;
+  k->ws_scale = (float*)((char*)at + ws_lse_bytes(slots, rows));
+  k->ws_o = (uint16_t*)((char*)k->ws_scale + ws_scale_bytes(slots, rows));
 }
 
 mla::KParams make_params(const mla_decode_args* a) {
@@ -4069,10 +4077,7 @@ mla::KParams make_params(const mla_decode_args* a) {
   k.o_sb = a->o_stride_b; k.o_ss = a->o_stride_s; k.o_sh = a->o_stride_h;
   k.lse = a->lse;
   const int64_t rows = (int64_t)a->s_q * a->heads_q;
-  const int64_t slots = (int64_t)a->batch + a->num_parts;
-  k.ws_lse = (float*)a->workspace;
-  k.ws_scale = (float*)((char*)a->workspace + ws_lse_bytes(slots, rows));
-  k.ws_o = (uint16_t*)((char*)k.ws_scale + ws_scale_bytes(slots, rows));
+  place_partials(&k, a->workspace, (int64_t)a->batch + a->num_parts, rows);
   k.batch = a->batch;
   k.s_q = a->s_q;
   k.heads = a->heads_q;
@@ -4165,6 +4170,116 @@ int launch_combine(const mla::KParams& k, const PT* part_o, int dtype, int copy_
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("combine launch failed: ") + hipGetErrorString(e));
   return MLA_OK;
+}
+
+// The split-KV pass of checked arguments.
+int launch_splitkv(const mla_decode_args* args, const mla::KParams& kp, hipStream_t st) {
+  if (args->kv_format == MLA_KV_FP4_E2M1) {
+    const hipError_t e = mla4::launch_decode(make_params_fp4(args, kp), kp.sched, kp.num_parts, cu_count_current(), st);
+    if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("decode launch failed: ") + hipGetErrorString(e));
+    return MLA_OK;
+  }
+  const Variant v = pick_variant(kp.rows);
+  const int R = v.rows();
+  const int head_blocks = (kp.rows + R - 1) / R;
+  const hipError_t e = args->dtype == MLA_DTYPE_BF16
+                           ? launch_main_dt<MLA_DTYPE_BF16>(v, kp, head_blocks, st)
+                           : launch_main_dt<MLA_DTYPE_F16>(v, kp, head_blocks, st);
+  if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("decode launch failed: ") + hipGetErrorString(e));
+  return MLA_OK;
+}
+
+int validate_absorb(const void* w_uv_blk, const void* v) {
+  if (!w_uv_blk || !v) return fail(MLA_ERR_INVALID, "w_uv_blk and v must not be NULL");
+  if (!aligned(w_uv_blk, 16)) return fail(MLA_ERR_INVALID, "w_uv_blk must be 16-byte aligned");
+  if (!aligned(v, 4)) return fail(MLA_ERR_INVALID, "v must be 4-byte aligned");
+  return MLA_OK;
+}
+
+// The merge with the value projection over checked arguments' partials.
+int launch_absorb(const mla::KParams& kp, int dtype, const void* w_uv_blk, void* v, hipStream_t st) {
+  mla::AbsorbParams a{};
+  a.ws_o = kp.ws_o;
+  a.ws_scale = kp.ws_scale;
+  a.ws_lse = kp.ws_lse;
+  a.splits = kp.splits;
+  a.out = kp.out;
+  a.o_sb = kp.o_sb; a.o_ss = kp.o_ss; a.o_sh = kp.o_sh;
+  a.w_blk = (const uint16_t*)w_uv_blk;
+  a.v = (uint16_t*)v;
+  a.lse = kp.lse;
+  a.m_rows = kp.batch * kp.s_q;
+  a.s_q = kp.s_q;
+  a.heads = kp.heads;
+  a.rows = kp.rows;
+  if (combine_is_deep(kp)) {
+    // long merges: the combine kernel's DEEP form writes the merged rows (bf16/fp16, as the
+    // fused merge rounds them into LDS) and their lse, and the projection reads every row from
+    // `out`; v is bit-identical to the fused merge's, except where the combine shares a long merge
+    // among four waves (launch_combine), whose fp32 sums have another order
+    const int rc2 = launch_combine<uint16_t, true>(kp, kp.ws_o, dtype, 0, st);
+    if (rc2 != MLA_OK) return rc2;
+    a.premerged = 1;
+  }
+  const dim3 grid(kp.heads, (a.m_rows + mla::kAbsRows - 1) / mla::kAbsRows);
+  if (dtype == MLA_DTYPE_BF16)
+    hipLaunchKernelGGL(mla::mla_combine_absorb_kernel<MLA_DTYPE_BF16>, grid, dim3(64 * mla::kAbsRows), 0, st, a);
+  else
+    hipLaunchKernelGGL(mla::mla_combine_absorb_kernel<MLA_DTYPE_F16>, grid, dim3(64 * mla::kAbsRows), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("combine-absorb launch failed: ") + hipGetErrorString(e));
+  return MLA_OK;
+}
+
+// A tree decode's workspace: the prefix sums of the splits with one more a sequence, then the partials: of
+// the schedule's splits (fewer than batch + num_parts) and of the drafted tokens.
+int64_t tree_slots(int64_t batch, int64_t num_parts) { return 2 * batch + num_parts; }
+int64_t tree_splits_bytes(int64_t batch) { return ((batch + 1) * 4 + 255) / 256 * 256; }
+
+// Checks a tree decode, runs its drafted tokens' part and the split-KV pass over the prefixes; *kp: what the merge
+// takes.  The first writes the prefix sums that tell the second of one more split, so that it writes partials also of
+// the sequences that the schedule did not cut.
+int launch_tree(const mla_decode_args* args, const uint64_t* mask, mla::KParams* kp, hipStream_t st) {
+  int rc = validate(args, mla_tree_workspace_bytes);
+  if (rc != MLA_OK) return rc;
+  if (mask == nullptr || !aligned(mask, 8)) return fail(MLA_ERR_INVALID, "mask must be 8-byte aligned and not NULL");
+  if (args->block_table == nullptr || args->indices != nullptr)
+    return fail(MLA_ERR_UNSUPPORTED, "the tree decode takes a paged cache, and no indices");
+  if (args->s_q > mla_tree::kMaxNodes) return fail(MLA_ERR_UNSUPPORTED, "the tree decode takes s_q <= 64");
+  if (args->batch > 65535) return fail(MLA_ERR_UNSUPPORTED, "the tree decode takes a batch of at most 65535");
+  mla::KParams k = make_params(args);
+  k.causal = 0;
+  const int64_t rows = k.rows;
+  int32_t* splits = (int32_t*)args->workspace;
+  place_partials(&k, (char*)args->workspace + tree_splits_bytes(k.batch), tree_slots(k.batch, k.num_parts), rows);
+  mla_tree::TreeParams t{};
+  t.q_nope = k.q_nope; t.q_rope = k.q_rope;
+  t.q_sb = k.q_sb; t.q_ss = k.q_ss; t.q_sh = k.q_sh;
+  t.qr_sb = k.qr_sb; t.qr_ss = k.qr_ss; t.qr_sh = k.qr_sh;
+  t.nope = (const uint8_t*)args->kv_nope;
+  t.rope = (const uint8_t*)args->kv_rope;
+  t.scale = (const uint8_t*)args->kv_scale;
+  const int e = args->kv_format == MLA_KV_NATIVE ? 2 : 1, c = args->kv_format == MLA_KV_FP8_E4M3 ? 4 : 1;
+  t.sp = args->kv_stride_page * e; t.st = args->kv_stride_tok * e;
+  t.rp = args->kv_rope_stride_page * 2; t.rt = args->kv_rope_stride_tok * 2;
+  t.cp = args->kv_scale_stride_page * c; t.ct = args->kv_scale_stride_blk * c;
+  t.block_table = k.block_table;
+  t.bt_stride = k.bt_stride; t.bt_width = k.bt_width; t.num_blocks = k.num_blocks;
+  t.status = k.status;
+  t.prefix = k.seqlens;
+  t.mask = mask;
+  t.splits = args->num_splits;
+  t.splits_out = splits;
+  t.ws_lse = k.ws_lse; t.ws_scale = k.ws_scale; t.ws_o = k.ws_o;
+  t.batch = k.batch; t.s_q = k.s_q; t.heads = k.heads; t.rows = k.rows;
+  t.format = args->kv_format; t.f16 = args->dtype == MLA_DTYPE_F16;
+  t.scale_log2 = k.scale_log2;
+  const hipError_t err = mla_tree::launch_drafts(t, st);
+  if (err != hipSuccess) return fail(MLA_ERR_HIP, std::string("drafted tokens launch failed: ") + hipGetErrorString(err));
+  k.splits = splits;
+  rc = launch_splitkv(args, k, st);
+  *kp = k;
+  return rc;
 }
 
 }  // namespace
@@ -4323,72 +4438,45 @@ int mla_decode_fwd_noalloc(const mla_decode_args* args, void* stream) {
 }
 
 int mla_splitkv_fwd(const mla_decode_args* args, void* stream) {
-  int64_t need = 0;
-  const int rc = validate(args, &need);
+  const int rc = validate(args);
   if (rc != MLA_OK) return rc;
-  const mla::KParams kp = make_params(args);
-  if (args->kv_format == MLA_KV_FP4_E2M1) {
-    const hipError_t e = mla4::launch_decode(make_params_fp4(args, kp), kp.sched, kp.num_parts, cu_count_current(), (hipStream_t)stream);
-    if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("decode launch failed: ") + hipGetErrorString(e));
-    return MLA_OK;
-  }
-  const Variant v = pick_variant(kp.rows);
-  const int R = v.rows();
-  const int head_blocks = (kp.rows + R - 1) / R;
-  const hipError_t e = args->dtype == MLA_DTYPE_BF16
-                           ? launch_main_dt<MLA_DTYPE_BF16>(v, kp, head_blocks, (hipStream_t)stream)
-                           : launch_main_dt<MLA_DTYPE_F16>(v, kp, head_blocks, (hipStream_t)stream);
-  if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("decode launch failed: ") + hipGetErrorString(e));
-  return MLA_OK;
+  return launch_splitkv(args, make_params(args), (hipStream_t)stream);
 }
 
 int mla_combine_fwd(const mla_decode_args* args, void* stream) {
-  int64_t need = 0;
-  const int rc = validate(args, &need);
+  const int rc = validate(args);
   if (rc != MLA_OK) return rc;
   const mla::KParams kp = make_params(args);
   return launch_combine<uint16_t, true>(kp, kp.ws_o, args->dtype, 0, (hipStream_t)stream);
 }
 
 int mla_combine_absorb(const mla_decode_args* args, const void* w_uv_blk, void* v, void* stream) {
-  int64_t need = 0;
-  const int rc = validate(args, &need);
+  int rc = validate(args);
+  if (rc == MLA_OK) rc = validate_absorb(w_uv_blk, v);
   if (rc != MLA_OK) return rc;
-  if (!w_uv_blk || !v) return fail(MLA_ERR_INVALID, "w_uv_blk and v must not be NULL");
-  if (!aligned(w_uv_blk, 16)) return fail(MLA_ERR_INVALID, "w_uv_blk must be 16-byte aligned");
-  if (!aligned(v, 4)) return fail(MLA_ERR_INVALID, "v must be 4-byte aligned");
-  const mla::KParams kp = make_params(args);
-  mla::AbsorbParams a{};
-  a.ws_o = kp.ws_o;
-  a.ws_scale = kp.ws_scale;
-  a.ws_lse = kp.ws_lse;
-  a.splits = kp.splits;
-  a.out = kp.out;
-  a.o_sb = kp.o_sb; a.o_ss = kp.o_ss; a.o_sh = kp.o_sh;
-  a.w_blk = (const uint16_t*)w_uv_blk;
-  a.v = (uint16_t*)v;
-  a.lse = kp.lse;
-  a.m_rows = kp.batch * kp.s_q;
-  a.s_q = kp.s_q;
-  a.heads = kp.heads;
-  a.rows = kp.rows;
-  if (combine_is_deep(kp)) {
-    // long merges: the combine kernel's DEEP form writes the merged rows (bf16/fp16, as the
-    // fused merge rounds them into LDS) and their lse, and the projection reads every row from
-    // `out`; v is bit-identical to the fused merge's, except where the combine shares a long merge
-    // among four waves (launch_combine), whose fp32 sums have another order
-    const int rc2 = launch_combine<uint16_t, true>(kp, kp.ws_o, args->dtype, 0, (hipStream_t)stream);
-    if (rc2 != MLA_OK) return rc2;
-    a.premerged = 1;
-  }
-  const dim3 grid(kp.heads, (a.m_rows + mla::kAbsRows - 1) / mla::kAbsRows);
-  if (args->dtype == MLA_DTYPE_BF16)
-    hipLaunchKernelGGL(mla::mla_combine_absorb_kernel<MLA_DTYPE_BF16>, grid, dim3(64 * mla::kAbsRows), 0, (hipStream_t)stream, a);
-  else
-    hipLaunchKernelGGL(mla::mla_combine_absorb_kernel<MLA_DTYPE_F16>, grid, dim3(64 * mla::kAbsRows), 0, (hipStream_t)stream, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return fail(MLA_ERR_HIP, std::string("combine-absorb launch failed: ") + hipGetErrorString(e));
-  return MLA_OK;
+  return launch_absorb(make_params(args), args->dtype, w_uv_blk, v, (hipStream_t)stream);
+}
+
+int64_t mla_tree_workspace_bytes(int32_t batch, int32_t s_q, int32_t heads_q, int32_t num_parts) {
+  if (batch < 1 || s_q < 1 || heads_q < 1 || num_parts < 1) return 0;
+  const int64_t rows = (int64_t)s_q * heads_q;
+  const int64_t slots = tree_slots(batch, num_parts);
+  return tree_splits_bytes(batch) + ws_lse_bytes(slots, rows) + ws_scale_bytes(slots, rows) + slots * rows * mla::kDV * 2;
+}
+
+int mla_tree_decode_fwd(const mla_decode_args* args, const uint64_t* mask, void* stream) {
+  mla::KParams kp;
+  const int rc = launch_tree(args, mask, &kp, (hipStream_t)stream);
+  if (rc != MLA_OK) return rc;
+  return launch_combine<uint16_t, true>(kp, kp.ws_o, args->dtype, 0, (hipStream_t)stream);
+}
+
+int mla_tree_absorb_fwd(const mla_decode_args* args, const uint64_t* mask, const void* w_uv_blk, void* v, void* stream) {
+  mla::KParams kp;
+  int rc = validate_absorb(w_uv_blk, v);
+  if (rc == MLA_OK) rc = launch_tree(args, mask, &kp, (hipStream_t)stream);
+  if (rc != MLA_OK) return rc;
+  return launch_absorb(kp, args->dtype, w_uv_blk, v, (hipStream_t)stream);
 }
 
 int mla_merge_partials(const float* part_o, const float* part_lse, const int32_t* num_splits,

@@ -1,4 +1,4 @@
-// mla_serving.h -- what mla_decode.hip and mla_serving.hip share (host code).
+// mla_serving.h -- what the translation units share (host code).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <string>
@@ -9,6 +9,20 @@ namespace mla_srv {
 
 // Leaves `msg` for mla_last_error() on this thread and returns `code`.
 int set_error(int code, const std::string& msg);
+
+// A paged cache as the kernels take it.
+struct Cache {
+  int32_t format;
+  int32_t f16;  // native: fp16 (else bf16)
+  int64_t tokens;
+  uint8_t* nope;
+  uint8_t* rope;
+  uint8_t* scale;
+  int64_t sp, st, rp, rt, cp, ct;  // page and token (fp8 scale: block) strides in bytes
+};
+
+// Checks a cache descriptor and fills the kernels' form of it (strides in bytes).
+int check_cache(const mla_kv_cache* c, Cache* k);
 
 // mla_kv_append into the 4-bit cache, its other arguments checked.
 int append_fp4(const mla_kv_append_args* a, hipStream_t st);

@@ -24,16 +24,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-struct Cache {
-  int32_t format;
-  int32_t f16;  // native: fp16 (else bf16)
-  int64_t tokens;
-  uint8_t* nope;
-  uint8_t* rope;
-  uint8_t* scale;
-  int64_t sp, st, rp, rt, cp, ct;  // page and token (fp8 scale: block) strides in bytes
-};
-
 // ---------------------------------------------------------------------------------------
 // values of the three element types
 // ---------------------------------------------------------------------------------------
@@ -832,8 +822,7 @@ static uint32_t groups_of(int64_t tokens, int per) {
   return 0;
 }
 
-// Checks a cache descriptor and fills the kernels' form of it (strides in bytes).
-static int check_cache(const mla_kv_cache* c, Cache* k) {
+int check_cache(const mla_kv_cache* c, Cache* k) {
   if (c->format != MLA_KV_NATIVE && c->format != MLA_KV_FP8_E4M3 && c->format != MLA_KV_FP4_E2M1)
     return set_error(MLA_ERR_INVALID, "kv_format must be MLA_KV_NATIVE, MLA_KV_FP8_E4M3 or MLA_KV_FP4_E2M1");
   if (c->dtype != MLA_DTYPE_BF16 && c->dtype != MLA_DTYPE_F16)
