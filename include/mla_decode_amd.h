@@ -538,7 +538,14 @@ int mla_tree_plan(const mla_tree_plan_args* args, void* stream);
  */
 int mla_tree_decode_fwd(const mla_decode_args* args, const uint64_t* mask, void* stream);
 
-/* The same followed by the absorbed value projection, as mla_splitkv_fwd and mla_combine_absorb. */
+/*
+ * Whether such a decode makes every page of the prefixes a split of its own (1; the table is narrow and the rows are few)
+ * instead of following the schedule (0).  It then does not read tile_sched and num_splits, which need not be computed.
+ */
+int mla_tree_takes_pages(int32_t batch, int32_t s_q, int32_t heads_q, int32_t num_parts, int32_t kv_format,
+                         int32_t block_table_width);
+
+/* mla_tree_decode_fwd followed by the absorbed value projection, as mla_splitkv_fwd and mla_combine_absorb. */
 int mla_tree_absorb_fwd(const mla_decode_args* args, const uint64_t* mask, const void* w_uv_blk, void* v, void* stream);
 
 int64_t mla_tree_workspace_bytes(int32_t batch, int32_t s_q, int32_t heads_q, int32_t num_parts);

@@ -57,6 +57,7 @@ EXPORTED = (
     "mla_tree_decode_fwd",
     "mla_tree_absorb_fwd",
     "mla_tree_workspace_bytes",
+    "mla_tree_takes_pages",
     "mla_tree_accept",
     "mla_kv_keep_path",
 )
@@ -333,6 +334,8 @@ def load() -> ctypes.CDLL:
         lib.mla_tree_absorb_fwd.restype = ctypes.c_int
         lib.mla_tree_workspace_bytes.argtypes = [_i32] * 4
         lib.mla_tree_workspace_bytes.restype = ctypes.c_int64
+        lib.mla_tree_takes_pages.argtypes = [_i32] * 6
+        lib.mla_tree_takes_pages.restype = ctypes.c_int
         lib.mla_tree_accept.argtypes = [_vp] * 4 + [_i32] * 3 + [_vp] * 5
         lib.mla_tree_accept.restype = ctypes.c_int
         lib.mla_kv_keep_path.argtypes = [ctypes.POINTER(MlaKvCache), _vp, _vp, _i32, _i32, _vp]

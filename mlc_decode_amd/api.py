@@ -152,6 +152,16 @@ def _num_parts_fp4(rows: int, max_pages: int, cu_count: int = 0) -> int:
     return n
 
 
+@functools.lru_cache(maxsize=4096)
+def _tree_without_schedule(batch: int, s_q: int, heads: int, fmt: int, width: int) -> Optional[int]:
+    """The parts of a schedule that a tree decode over a table of ``width`` columns would not read, or None."""
+    if batch < 1:
+        return None
+    rows = s_q * heads
+    parts = _num_parts_fp4(rows, batch * width) if fmt == MLA_KV_FP4_E2M1 else num_parts_for(batch, 1, rows, 1)
+    return parts if _lib.load().mla_tree_takes_pages(batch, s_q, heads, parts, fmt, width) else None
+
+
 def kernel_variant(rows: int) -> dict:
     """Tile of the main kernel for ``rows`` = s_q * heads query rows (``mla_variant``)."""
     w, t, st, r = (ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32())
@@ -555,8 +565,15 @@ def mla_decode_with_kvcache(q: torch.Tensor, kv_cache, block_table: torch.Tensor
         if tree is not None:
             cache_seqlens = tree.prefix_lens
         longest = _lib.MLA_PAGE_TOKENS * block_table.shape[1] if block_table is not None and block_table.dim() == 2 else None
-        sched, splits = get_mla_metadata(cache_seqlens, q.shape[1] * q.shape[2], 1,
-                                         forced_splits=forced, kv_cache=kv_cache, max_seqlen=longest)
+        sched = None
+        if tree is not None and not forced and longest is not None:
+            sched = _tree_without_schedule(q.shape[0], q.shape[1], q.shape[2], _cache_format(kv_cache), block_table.shape[1])
+        if sched is None:
+            sched, splits = get_mla_metadata(cache_seqlens, q.shape[1] * q.shape[2], 1,
+                                             forced_splits=forced, kv_cache=kv_cache, max_seqlen=longest)
+        else:  # of that many parts, and not read
+            sched = torch.empty(sched, _lib.MLA_SCHED_WORDS, dtype=torch.int32, device=q.device)
+            splits = torch.empty(q.shape[0] + 1, dtype=torch.int32, device=q.device)
         if forced == 1:
             return _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal,
                            out, lse, status=status, single_split=True, tree=tree)

@@ -3114,22 +3114,25 @@ __device__ __forceinline__ float merge_row16(const uint16_t* __restrict__ ws_o, 
 constexpr int kDeepSplits = 256;
 constexpr int kDeepMaxRows = 16384;  // kDeepSplits * kDeepMaxRows KiB = 2^32 bytes
 constexpr int kQueue = 32;
-constexpr int kDeepLds = (kDeepSplits + kQueue) * 4;  // kw
+// A tree decode has one more split a sequence than a schedule: one long sequence in 256 parts has 257.  Its merges have
+// room for them in an instantiation of their own (as whole rows: one sequence of 16384 tokens, 128 rows, the decode 57 us).
+constexpr int kTreeSplits = kDeepSplits + 64;
+constexpr int kTreeMaxRows = 12288;  // kTreeSplits * kTreeMaxRows KiB < 2^32 bytes
 constexpr int kShareSplits = 64;  // longer rows are shared by a workgroup's waves (see launch_combine)
 // Splits lo .. hi - 1 only, with the weights of a merge of all n: the waves of a workgroup that
 // share a quarter row take consecutive ranges of its splits, and their sums are added.
-template <int DT, bool SCALED>
+template <int DT, bool SCALED, int CAP = kDeepSplits>
 __device__ __forceinline__ float merge_many_splits(const uint16_t* __restrict__ ws_o, const float* __restrict__ ws_scale,
                                                    const float* __restrict__ ws_lse, int base, int n, int rows,
                                                    int row, int q, int lane, char* smem, int lo, int hi,
                                                    float (&acc)[2]) {
-  static_assert(kDeepSplits % 64 == 0 && kQueue <= 63 && kQueue % 4 == 0 && kQueue <= 64, "queue shape");
+  static_assert(CAP % 64 == 0 && kQueue <= 63 && kQueue % 4 == 0 && kQueue <= 64, "queue shape");
   constexpr int LDT = SCALED ? MLA_DTYPE_F16 : DT;
-  constexpr int kL = kDeepSplits / 64;
+  constexpr int kL = CAP / 64;
   float* kw = (float*)smem;
   // split k's quarter row: a uniform base plus the lane's 4 bytes.  Offsets are 32-bit: the host
-  // takes this path only for rows <= kDeepMaxRows, so the last split's offset, at most
-  // (kDeepSplits - 1) * rows KiB, stays below 2^32 (a surplus load's offset may wrap, to an
+  // takes this path only for rows <= kDeepMaxRows (for CAP = kDeepSplits), so the last split's offset, at most
+  // (CAP - 1) * rows KiB, stays below 2^32 (a surplus load's offset may wrap, to an
   // earlier split of the same row, and is consumed as zeros)
   const char* row0 = (const char*)(ws_o + ((int64_t)base * rows + row) * kDV + 128 * q);
   const uint32_t split_bytes = (uint32_t)rows * kDV * 2;
@@ -3177,7 +3180,7 @@ __device__ __forceinline__ float merge_many_splits(const uint16_t* __restrict__ 
     if (k < n && lse2 != -INFINITY) w = fast_exp2(lv[c] - lse2);
     kw[k] = SCALED ? w * sc[c] : w;
   }
-  if (lane < kQueue) kw[kDeepSplits + lane] = 0.f;
+  if (lane < kQueue) kw[CAP + lane] = 0.f;
   __builtin_amdgcn_wave_barrier();
 
   acc[0] = acc[1] = 0.f;
@@ -3219,7 +3222,7 @@ __device__ __forceinline__ float merge_many_splits(const uint16_t* __restrict__ 
 // grid.z = 4, the quarter of the row the workgroup merges when the row has kFewSplits < n <=
 // kDeepSplits splits (merge_many_splits); other rows are merged whole by the first wave of quarter
 // 0.  Otherwise four waves per workgroup, for large batches of rows with few splits each.
-template <int DT, typename PT, bool SCALED, int DEEP = 0>
+template <int DT, typename PT, bool SCALED, int DEEP = 0, int CAP = kDeepSplits>
 __global__ __launch_bounds__(DEEP ? 64 * DEEP : 256) void mla_combine_kernel(const PT* __restrict__ ws_o,
                                                           const float* __restrict__ ws_scale,
                                                           const float* __restrict__ ws_lse,
@@ -3230,7 +3233,7 @@ __global__ __launch_bounds__(DEEP ? 64 * DEEP : 256) void mla_combine_kernel(con
                                                           float* __restrict__ lse_out,
                                                           int copy_single) {
   constexpr int W = DEEP ? 1 : 4;  // rows per workgroup
-  __shared__ __attribute__((aligned(16))) char smem[DEEP ? DEEP * kDeepLds : W * 64 * 4];
+  __shared__ __attribute__((aligned(16))) char smem[DEEP ? DEEP * (CAP + kQueue) * 4 : W * 64 * 4];
   __shared__ float sum_sh[DEEP > 1 ? DEEP : 1][2][64];
   float* w_sh = (float*)smem + (DEEP ? 0 : 64 * (threadIdx.x >> 6));  // the wave's 64 weights (merge_splits_wave)
   const int b = blockIdx.x;
@@ -3250,7 +3253,7 @@ __global__ __launch_bounds__(DEEP ? 64 * DEEP : 256) void mla_combine_kernel(con
   float* lse_dst = lse_out != nullptr ? lse_out + ((int64_t)b * heads + h) * s_q + s : nullptr;
   if constexpr (DEEP > 0 && std::is_same<PT, uint16_t>::value) {
     const int q = blockIdx.z;
-    if (n > kFewSplits && n <= kDeepSplits) {  // uniform
+    if (n > kFewSplits && n <= CAP) {  // uniform
       float acc2[2];
       const bool share = DEEP > 1 && n > kShareSplits;  // uniform
       const int wave_u = DEEP == 1 ? 0 : __builtin_amdgcn_readfirstlane(wave);
@@ -3258,8 +3261,8 @@ __global__ __launch_bounds__(DEEP ? 64 * DEEP : 256) void mla_combine_kernel(con
       const int per = share ? ((n + 4 * DEEP - 1) / (4 * DEEP)) * 4 : n;  // whole fours: the weights are read so
       const int lo = wave_u * per;
       const int hi = lo + per < n ? lo + per : n;
-      const float lse2 = merge_many_splits<DT, SCALED>(ws_o, ws_scale, ws_lse, base, n, rows, row, q, lane,
-                                                       smem + wave_u * kDeepLds, lo, hi, acc2);
+      const float lse2 = merge_many_splits<DT, SCALED, CAP>(ws_o, ws_scale, ws_lse, base, n, rows, row, q, lane,
+                                                       smem + wave_u * (CAP + kQueue) * 4, lo, hi, acc2);
       if (share) {
         sum_sh[wave][0][lane] = acc2[0];
         sum_sh[wave][1][lane] = acc2[1];
@@ -4136,7 +4139,7 @@ int64_t pages_bound(const mla::KParams& k) {
   return mla::contiguous_pages_bound(k.kv_sb, k.kv_st);
 }
 
-template <typename PT, bool SCALED = false>
+template <typename PT, bool SCALED = false, int CAP = mla::kDeepSplits>
 int launch_combine(const mla::KParams& k, const PT* part_o, int dtype, int copy_single, hipStream_t st) {
   // Four waves share a quarter row's splits where its merge is long (more than 64) and every quarter
   // row has a CU to itself.  Combine in the call's kernel trace, one -> four waves: 16 rows x 256
@@ -4151,7 +4154,7 @@ int launch_combine(const mla::KParams& k, const PT* part_o, int dtype, int copy_
   const int W = deep ? 1 : 4;
   const dim3 grid(k.batch, (k.rows + W - 1) / W, deep ? 4 : 1);
 #define MLA_COMBINE(D, DP)                                                                                     \
-  hipLaunchKernelGGL((mla::mla_combine_kernel<D, PT, SCALED, DP>), grid, dim3(DP ? 64 * DP : 256), 0, st, part_o, \
+  hipLaunchKernelGGL((mla::mla_combine_kernel<D, PT, SCALED, DP, CAP>), grid, dim3(DP ? 64 * DP : 256), 0, st, part_o, \
                      k.ws_scale, k.ws_lse, k.splits, k.rows, k.heads, k.s_q, k.out, k.o_sb, k.o_ss, k.o_sh, k.lse, \
                      copy_single)
 #define MLA_COMBINE_DT(D)                      \
@@ -4189,6 +4192,12 @@ int launch_splitkv(const mla_decode_args* args, const mla::KParams& kp, hipStrea
   return MLA_OK;
 }
 
+// The merge of a tree decode: the combine, with room for a split more than schedules have parts.
+int launch_tree_combine(const mla::KParams& k, int dtype, hipStream_t st) {
+  return k.rows <= mla::kTreeMaxRows ? launch_combine<uint16_t, true, mla::kTreeSplits>(k, k.ws_o, dtype, 0, st)
+                                     : launch_combine<uint16_t, true>(k, k.ws_o, dtype, 0, st);
+}
+
 int validate_absorb(const void* w_uv_blk, const void* v) {
   if (!w_uv_blk || !v) return fail(MLA_ERR_INVALID, "w_uv_blk and v must not be NULL");
   if (!aligned(w_uv_blk, 16)) return fail(MLA_ERR_INVALID, "w_uv_blk must be 16-byte aligned");
@@ -4197,7 +4206,7 @@ int validate_absorb(const void* w_uv_blk, const void* v) {
 }
 
 // The merge with the value projection over checked arguments' partials.
-int launch_absorb(const mla::KParams& kp, int dtype, const void* w_uv_blk, void* v, hipStream_t st) {
+int launch_absorb(const mla::KParams& kp, int dtype, const void* w_uv_blk, void* v, bool tree, hipStream_t st) {
   mla::AbsorbParams a{};
   a.ws_o = kp.ws_o;
   a.ws_scale = kp.ws_scale;
@@ -4217,7 +4226,7 @@ int launch_absorb(const mla::KParams& kp, int dtype, const void* w_uv_blk, void*
     // fused merge rounds them into LDS) and their lse, and the projection reads every row from
     // `out`; v is bit-identical to the fused merge's, except where the combine shares a long merge
     // among four waves (launch_combine), whose fp32 sums have another order
-    const int rc2 = launch_combine<uint16_t, true>(kp, kp.ws_o, dtype, 0, st);
+    const int rc2 = tree ? launch_tree_combine(kp, dtype, st) : launch_combine<uint16_t, true>(kp, kp.ws_o, dtype, 0, st);
     if (rc2 != MLA_OK) return rc2;
     a.premerged = 1;
   }
@@ -4236,9 +4245,9 @@ int launch_absorb(const mla::KParams& kp, int dtype, const void* w_uv_blk, void*
 int64_t tree_slots(int64_t batch, int64_t num_parts) { return 2 * batch + num_parts; }
 int64_t tree_splits_bytes(int64_t batch) { return ((batch + 1) * 4 + 255) / 256 * 256; }
 
-// Checks a tree decode, runs its drafted tokens' part and the split-KV pass over the prefixes; *kp: what the merge
-// takes.  The first writes the prefix sums that tell the second of one more split, so that it writes partials also of
-// the sequences that the schedule did not cut.
+// Checks a tree decode, runs its drafted tokens' part and the split-KV pass over the prefixes (or, where their pages
+// are few, both in one launch); *kp: what the merge takes.  The first writes the prefix sums that tell the second of one
+// more split, so that it writes partials also of the sequences that the schedule did not cut.
 int launch_tree(const mla_decode_args* args, const uint64_t* mask, mla::KParams* kp, hipStream_t st) {
   int rc = validate(args, mla_tree_workspace_bytes);
   if (rc != MLA_OK) return rc;
@@ -4274,10 +4283,11 @@ int launch_tree(const mla_decode_args* args, const uint64_t* mask, mla::KParams*
   t.batch = k.batch; t.s_q = k.s_q; t.heads = k.heads; t.rows = k.rows;
   t.format = args->kv_format; t.f16 = args->dtype == MLA_DTYPE_F16;
   t.scale_log2 = k.scale_log2;
-  const hipError_t err = mla_tree::launch_drafts(t, st);
+  t.pages = mla_tree::takes_pages(k.batch, rows, args->kv_format, k.bt_width, tree_slots(k.batch, k.num_parts), cu_count_current());
+  const hipError_t err = mla_tree::launch_tiles(t, cu_count_current(), st);
   if (err != hipSuccess) return fail(MLA_ERR_HIP, std::string("drafted tokens launch failed: ") + hipGetErrorString(err));
   k.splits = splits;
-  rc = launch_splitkv(args, k, st);
+  if (!t.pages) rc = launch_splitkv(args, k, st);
   *kp = k;
   return rc;
 }
@@ -4454,7 +4464,7 @@ int mla_combine_absorb(const mla_decode_args* args, const void* w_uv_blk, void* 
   int rc = validate(args);
   if (rc == MLA_OK) rc = validate_absorb(w_uv_blk, v);
   if (rc != MLA_OK) return rc;
-  return launch_absorb(make_params(args), args->dtype, w_uv_blk, v, (hipStream_t)stream);
+  return launch_absorb(make_params(args), args->dtype, w_uv_blk, v, false, (hipStream_t)stream);
 }
 
 int64_t mla_tree_workspace_bytes(int32_t batch, int32_t s_q, int32_t heads_q, int32_t num_parts) {
@@ -4464,11 +4474,18 @@ int64_t mla_tree_workspace_bytes(int32_t batch, int32_t s_q, int32_t heads_q, in
   return tree_splits_bytes(batch) + ws_lse_bytes(slots, rows) + ws_scale_bytes(slots, rows) + slots * rows * mla::kDV * 2;
 }
 
+int mla_tree_takes_pages(int32_t batch, int32_t s_q, int32_t heads_q, int32_t num_parts, int32_t kv_format,
+                         int32_t block_table_width) {
+  if (batch < 1 || s_q < 1 || heads_q < 1 || num_parts < 1 || block_table_width < 1 || !known_format(kv_format)) return 0;
+  return mla_tree::takes_pages(batch, (int64_t)s_q * heads_q, kv_format, block_table_width, tree_slots(batch, num_parts),
+                               cu_count_current());
+}
+
 int mla_tree_decode_fwd(const mla_decode_args* args, const uint64_t* mask, void* stream) {
   mla::KParams kp;
   const int rc = launch_tree(args, mask, &kp, (hipStream_t)stream);
   if (rc != MLA_OK) return rc;
-  return launch_combine<uint16_t, true>(kp, kp.ws_o, args->dtype, 0, (hipStream_t)stream);
+  return launch_tree_combine(kp, args->dtype, (hipStream_t)stream);
 }
 
 int mla_tree_absorb_fwd(const mla_decode_args* args, const uint64_t* mask, const void* w_uv_blk, void* v, void* stream) {
@@ -4476,7 +4493,7 @@ int mla_tree_absorb_fwd(const mla_decode_args* args, const uint64_t* mask, const
   int rc = validate_absorb(w_uv_blk, v);
   if (rc == MLA_OK) rc = launch_tree(args, mask, &kp, (hipStream_t)stream);
   if (rc != MLA_OK) return rc;
-  return launch_absorb(kp, args->dtype, w_uv_blk, v, (hipStream_t)stream);
+  return launch_absorb(kp, args->dtype, w_uv_blk, v, true, (hipStream_t)stream);
 }
 
 int mla_merge_partials(const float* part_o, const float* part_lse, const int32_t* num_splits,

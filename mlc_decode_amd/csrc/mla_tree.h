@@ -28,9 +28,11 @@ struct TreeParams {
   uint16_t* ws_o;
   int32_t batch, s_q, heads, rows;
   int32_t format, f16;
+  int32_t pages;     // nonzero: the prefixes' pages too, each a split (splits is not read)
   float scale_log2;
 };
 
-hipError_t launch_drafts(const TreeParams& p, hipStream_t st);
+bool takes_pages(int64_t batch, int64_t rows, int format, int64_t bt_width, int64_t slots, int cus);
+hipError_t launch_tiles(const TreeParams& p, int cus, hipStream_t st);
 
 }  // namespace mla_tree

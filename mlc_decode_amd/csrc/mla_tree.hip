@@ -19,7 +19,6 @@ namespace mla_tree {
 constexpr int kPage = MLA_PAGE_TOKENS;
 constexpr int kDV = MLA_DIM_V;
 constexpr int kKSteps = MLA_DIM_QK / 32;
-constexpr int kDimTiles = kDV / 16;
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -83,218 +82,468 @@ __device__ __forceinline__ bool non_finite(i32x4 v) {
   return bad;
 }
 
-// Eight latent values (dims 8 lane ..) of a cached token as 16-bit words; coded caches widen to bf16, exactly.
+// ---------------------------------------------------------------------------------------
+// one tile of keys
+// ---------------------------------------------------------------------------------------
+// A workgroup scores rows of a sequence against one tile of up to 64 keys, its drafted tokens or a page of its prefix,
+// and leaves a partial: S^T = K Q^T (16x16x32 MFMA), softmax over the visible keys, O^T = V^T P^T with V^T from
+// transposed LDS reads.  All keys are in the tile, so the softmax is one pass.  P is rounded to 16 bits (the operand's
+// type) and the sum that divides the output is of the rounded weights, so that the rounding cancels in it.
+//
+// Tokens and queries are read row by row, a wave's lanes side by side, and become operands through LDS.  Loaded in operand
+// order, 16 rows a quarter wave, each load took the address unit 64 cycles instead of 16: 36 of them 4.2 us.
+//
+// A drafted token that a row does not see must not reach it, whatever its cache row holds (it may never have been
+// written): a weight of 0 times an infinity or a NaN is a NaN.  A token whose latent holds one is zeroed in part,
+// remembered, and the rows that do see it become NaN.
+constexpr int kPitch = 2 * MLA_DIM_QK + 16;  // bytes of a row in LDS: 16 rows start on 16 different groups of 4 banks
+constexpr int kTileBytes = 16 * kPitch;      // 16 rows
+
+// What a lane holds of a wave's share of the tokens, 16 bytes a load whatever the format: of one token 8 dims, of
+// two 16 (e4m3) or of four 32 (e2m1).
 template <int FMT>
-__device__ __forceinline__ i32x4 latent8(const TreeParams& p, int64_t page, int row, int lane) {
-  const uint8_t* src = p.nope + page * p.sp + row * p.st;
-  if constexpr (FMT == MLA_KV_NATIVE) {
-    return *(const i32x4*)(src + 16 * lane);
-  } else if constexpr (FMT == MLA_KV_FP8_E4M3) {
-    const i32x2 w = *(const i32x2*)(src + 8 * lane);
-    const float sc = *(const float*)(p.scale + page * p.cp + (lane >> 4) * p.ct + 4 * row);
-    const int a = w[0], b = w[1];
+struct Lanes {
+  static constexpr int kTokens = FMT == MLA_KV_NATIVE ? 1 : FMT == MLA_KV_FP8_E4M3 ? 2 : 4;  // of a load
+  static constexpr int kLanes = 64 / kTokens;                                               // of a token
+};
+// 8 u .. 8 u + 7 of the dims that a lane holds; coded caches widen to bf16, exactly.
+template <int FMT>
+__device__ __forceinline__ i32x4 widen8(i32x4 raw, float sc, int u) {
+  if constexpr (FMT == MLA_KV_FP8_E4M3) {
+    const int a = raw[2 * u], b = raw[2 * u + 1];
     return i32x4{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, false)),
                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, true)),
                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, false)),
                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, true))};
-  } else {
-    const int w = *(const int*)(src + 4 * lane);
-    const float sc = __uint_as_float((uint32_t)p.scale[page * p.cp + row * p.ct + (lane >> 2)] << 23);
+  } else if constexpr (FMT == MLA_KV_FP4_E2M1) {
+    const int w = raw[u];
     return i32x4{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 0)),
                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 1)),
                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 2)),
                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, sc, 3))};
+  } else {
+    return raw;
   }
 }
 
-// ---------------------------------------------------------------------------------------
-// the drafted tokens' split
-// ---------------------------------------------------------------------------------------
-// For 64 rows of a sequence, a wave 16 of them: S^T = K Q^T over the drafted tokens (16x16x32 MFMA, K rows from LDS,
-// queries in registers), softmax over the row's visible ones, O^T = V^T P^T.  All keys are in one tile (32 KT of
-// them), so the softmax is one pass and P^T never leaves the registers: the S^T accumulators of two token tiles, packed
-// to 16 bits, are the B operand of PV in the k order of the transposed V reads.  P is rounded to 16 bits (the operand's
-// type) and the sum that divides the output is of the rounded weights, so that the rounding cancels in it.
-//
-// A drafted token that a row does not see must not reach it, whatever its cache row holds (it may never have been
-// written): a weight of 0 times an infinity or a NaN is a NaN.  A chunk that holds one is zeroed in LDS, the token is
-// remembered, and rows that do see it become NaN.
-constexpr int kPitch = 2 * MLA_DIM_QK + 16;  // bytes of a token in LDS: 16 rows start on 16 different groups of 4 banks
+// A prefix's splits where every page is one: an empty prefix has an empty one (the merge passes over sequences of one split).
+__device__ __forceinline__ int page_splits(int tokens) { return tokens > 0 ? (tokens + kPage - 1) / kPage : 1; }
 
-template <int FMT, bool F16, int KT>
-__global__ __launch_bounds__(256, 2) void mla_tree_kernel(TreeParams p) {
-  constexpr int kTok = 32 * KT;
-  __shared__ __attribute__((aligned(16))) uint8_t kv_sh[kTok * kPitch];
-  __shared__ unsigned long long bad_sh;
-  const int b = blockIdx.y;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int g = lane >> 4, li = lane & 15;
-  const int last = p.splits[b + 1] + b;  // the sequence's last slot, with one more split for it and those before it
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    if (b == 0) p.splits_out[0] = p.splits[0];
-    p.splits_out[b + 1] = last + 1;
-  }
-  if (threadIdx.x == 0) bad_sh = 0;
-  int prefix = p.prefix[b];
-  prefix = prefix > 0 ? prefix : 0;
-  // drafted tokens that the table's row has room for, and the one or two pages that they lie in
-  const int64_t room = (int64_t)p.bt_width * kPage - prefix;
-  const int held = room < 0 ? 0 : room < p.s_q ? (int)room : p.s_q;
-  const int at = prefix & (kPage - 1);
-  int pages[2];
+// The tile of a workgroup; grid (row blocks, tiles, batch): tile 0 is the drafted tokens; with `pages`, tile 1 + i is page
+// i of the prefix.
+struct Tile {
+  bool drafts;
+  int held;       // keys
+  int at;         // the first one's row in the first page
+  int pages[2];   // 64 keys lie in one page or two
+  uint64_t known; // bits of the keys
+  int prefix_raw, prefix, cap;
+};
+// False where the sequence has no such tile.
+__device__ __forceinline__ bool find_tile(const TreeParams& p, int b, int tile, Tile& t) {
+  t.drafts = tile == 0;
+  t.cap = p.bt_width * kPage;
+  const int raw = p.prefix[b];
+  t.prefix_raw = raw > 0 ? raw : 0;
+  t.prefix = t.prefix_raw < t.cap ? t.prefix_raw : t.cap;
+  if (!t.drafts && tile > page_splits(t.prefix)) return false;
+  const int64_t room = (int64_t)t.cap - t.prefix_raw;  // of the table's row, for drafted tokens
+  t.at = t.drafts ? t.prefix_raw & (kPage - 1) : 0;
+  t.held = !t.drafts ? min(t.prefix - (tile - 1) * kPage, kPage) : room < 0 ? 0 : room < p.s_q ? (int)room : p.s_q;
+  t.known = t.held >= 64 ? ~0ull : (1ull << t.held) - 1;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    int col = prefix / kPage + i;
+    int col = (t.drafts ? t.prefix_raw / kPage : tile - 1) + i;
     col = col < p.bt_width ? col : p.bt_width - 1;
     const int id = p.block_table[(int64_t)b * p.bt_stride + col];
-    pages[i] = id < 0 ? 0 : id < p.num_blocks ? id : p.num_blocks - 1;
+    t.pages[i] = id < 0 ? 0 : id < p.num_blocks ? id : p.num_blocks - 1;
   }
+  return true;
+}
 
-  // queries (B operand): lane (g, i) holds dims 32 kk + 8 g .. +7 of row i
-  const int row_raw = blockIdx.x * 64 + 16 * wave + li;
-  const int row = row_raw < p.rows ? row_raw : p.rows - 1;
-  const int s = row / p.heads, h = row - s * p.heads;
-  const uint16_t* qn = p.q_nope + (b * p.q_sb + s * p.q_ss + h * p.q_sh) + 8 * g;
-  const uint16_t* qr = p.q_rope + (b * p.qr_sb + s * p.qr_ss + h * p.qr_sh) + 8 * g;
+// The tile's slot; the drafted tokens' workgroup also writes what the merge (and the split-KV pass) are told.
+__device__ __forceinline__ int find_slot(const TreeParams& p, int b, int tile, const Tile& t, int lane) {
+  int slot;
+  if (p.pages) {  // uniform: every page a split, in order, then the drafted tokens
+    int before = 0;
+    for (int i = lane; i < b; i += 64) {
+      const int n = p.prefix[i];
+      before += 1 + page_splits(n < t.cap ? n : t.cap);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d);
+    slot = __builtin_amdgcn_readfirstlane(before) + (t.drafts ? page_splits(t.prefix) : tile - 1);
+  } else {
+    slot = p.splits[b + 1] + b;  // one more split for this sequence and each before it
+  }
+  if (t.drafts && blockIdx.x == 0 && threadIdx.x == 0) {
+    if (b == 0) p.splits_out[0] = p.pages ? 0 : p.splits[0];
+    p.splits_out[b + 1] = slot + 1;
+    if (p.pages && t.prefix_raw > t.cap && p.status != nullptr) *p.status = 1;
+  }
+  return slot;
+}
+
+// N tokens first, first + 1, .. of the tile (rows past its keys as zeros): their latents, the coded ones' scales, and the
+// rope dims, 8 tokens a register.
+template <int FMT, int N>
+struct Share {
+  static constexpr int kLoads = N / Lanes<FMT>::kTokens;
+  i32x4 v[kLoads], r[N / 8];
+  float sc[FMT == MLA_KV_NATIVE ? 1 : kLoads];
+};
+template <int FMT, int N>
+__device__ __forceinline__ void load_tokens(const TreeParams& p, const Tile& t, int first, int lane, Share<FMT, N>& x) {
+  constexpr int kTokens = Lanes<FMT>::kTokens, kLanes = Lanes<FMT>::kLanes;
+#pragma unroll
+  for (int i = 0; i < N / kTokens; ++i) {
+    const int j = first + kTokens * i + (kTokens > 1 ? lane / kLanes : 0);  // 16-bit caches: uniform
+    x.v[i] = i32x4{0, 0, 0, 0};
+    if constexpr (FMT != MLA_KV_NATIVE) x.sc[i] = 1.f;
+    if (j < t.held) {
+      const int64_t page = t.at + j < kPage ? t.pages[0] : t.pages[1];
+      const int row = (t.at + j) & (kPage - 1), piece = lane % kLanes;
+      x.v[i] = *(const i32x4*)(p.nope + page * p.sp + row * p.st + 16 * piece);
+      if constexpr (FMT == MLA_KV_FP8_E4M3)
+        x.sc[i] = *(const float*)(p.scale + page * p.cp + (piece >> 3) * p.ct + 4 * row);
+      else if constexpr (FMT == MLA_KV_FP4_E2M1)
+        x.sc[i] = __uint_as_float((uint32_t)p.scale[page * p.cp + row * p.ct + piece] << 23);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) {
+    const int j = first + 8 * i + (lane >> 3);
+    x.r[i] = i32x4{0, 0, 0, 0};
+    if (j < t.held) {
+      const int64_t page = t.at + j < kPage ? t.pages[0] : t.pages[1];
+      x.r[i] = *(const i32x4*)(p.rope + page * p.rp + ((t.at + j) & (kPage - 1)) * p.rt + 16 * (lane & 7));
+    }
+  }
+}
+// The same to rows of LDS.  Of drafted tokens, what is not finite is left out; bits of such tokens come back.
+template <int FMT, bool F16, int N>
+__device__ __forceinline__ uint32_t put_tokens(uint8_t* dst, bool drafts, int lane, const Share<FMT, N>& x) {
+  constexpr int kTokens = Lanes<FMT>::kTokens, kLanes = Lanes<FMT>::kLanes;
+  uint32_t spoilt = 0;
+#pragma unroll
+  for (int i = 0; i < N / kTokens; ++i) {
+    uint8_t* row = dst + (kTokens * i + lane / kLanes) * kPitch + 16 * kTokens * (lane % kLanes);
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      i32x4 v = widen8<FMT>(x.v[i], FMT == MLA_KV_NATIVE ? 0.f : x.sc[FMT == MLA_KV_NATIVE ? 0 : i], u);
+      if (drafts) {  // uniform
+        const bool bad = non_finite<F16>(v);
+        const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
+        if (any != 0) {  // uniform, rare
+          if (bad) v = i32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < kTokens; ++w) spoilt |= (uint32_t)((any >> (w * kLanes) << (64 - kLanes)) != 0) << (kTokens * i + w);
+        }
+      }
+      *(i32x4*)(row + 16 * u) = v;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N / 8; ++i) *(i32x4*)(dst + (8 * i + (lane >> 3)) * kPitch + 2 * kDV + 16 * (lane & 7)) = x.r[i];
+  return spoilt;
+}
+// Rows first .. of the queries (past the last: the last), alike.
+template <int N>
+__device__ __forceinline__ void load_queries(const TreeParams& p, int b, int first, int lane, i32x4 (&v)[N], i32x4 (&r)[(N + 7) / 8]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int row = first + i < p.rows ? first + i : p.rows - 1;  // uniform
+    const int s = row / p.heads, h = row - s * p.heads;
+    v[i] = *(const i32x4*)(p.q_nope + (b * p.q_sb + s * p.q_ss + h * p.q_sh) + 8 * lane);
+  }
+#pragma unroll
+  for (int i = 0; i < (N + 7) / 8; ++i) {
+    const int j = first + 8 * i + ((lane >> 3) & (N < 8 ? N - 1 : 7));
+    const int row = j < p.rows ? j : p.rows - 1;
+    const int s = row / p.heads, h = row - s * p.heads;
+    r[i] = *(const i32x4*)(p.q_rope + (b * p.qr_sb + s * p.qr_ss + h * p.qr_sh) + 8 * (lane & 7));
+  }
+}
+template <int N>
+__device__ __forceinline__ void put_queries(uint8_t* dst, int lane, const i32x4 (&v)[N], const i32x4 (&r)[(N + 7) / 8]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) *(i32x4*)(dst + i * kPitch + 16 * lane) = v[i];
+#pragma unroll
+  for (int i = 0; i < (N + 7) / 8; ++i)
+    if (N >= 8 || lane < 8 * N) *(i32x4*)(dst + (8 * i + (lane >> 3)) * kPitch + 2 * kDV + 16 * (lane & 7)) = r[i];
+}
+// Fragments of 16 rows: lane (g, i) holds dims 32 kk + 8 g .. +7 of row i.
+__device__ __forceinline__ void read_fragments(const uint8_t* src, int g, int li, i32x4 (&f)[kKSteps]) {
+#pragma unroll
+  for (int kk = 0; kk < kKSteps; ++kk) f[kk] = *(const i32x4*)(src + li * kPitch + 64 * kk + 16 * g);
+}
+// V^T (A operand): transposed reads give lane (g, i) keys 4 g .. +3 and 16 + 4 g .. +3 of 32 at dim 16 d + i.
+__device__ __forceinline__ i32x4 read_vt(const uint8_t* rows32, int d, int g, int li) {
+  const uint8_t LDS_AS* a = (const uint8_t LDS_AS*)(rows32 + (4 * g + (li >> 2)) * kPitch + 32 * d + 8 * (li & 3));
+  const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)a));
+  const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(a + kTileBytes)));
+  return i32x4{lo[0], lo[1], hi[0], hi[1]};
+}
+
+__device__ __forceinline__ float largest(f32x4 v, float a) {
+  return fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), a);
+}
+// A row's divisor and lse.  A NaN in the lse makes the merged one -inf, as any NaN row's is.
+__device__ __forceinline__ void finish_row(bool spoilt, float l, float lx, float ref, float& inv, float& lse2) {
+  const float nan = __builtin_nanf("");
+  inv = spoilt ? nan : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  lse2 = spoilt ? nan : lx > 0.f ? ref + __log2f(lx) : lx == 0.f ? -INFINITY : lx;
+}
+
+// The rows of one 128-dim chunk on their way out: 16 rows of 256 bytes in LDS, 16-byte pieces swizzled by the row, so
+// that a store writes four rows' whole chunks (fragments stored directly write pieces of 32 bytes of 16 rows).
+__device__ __forceinline__ void stage_chunk(uint8_t* stage, int d, int g, int li, f32x4 x) {
+  *(i32x2*)(stage + li * 256 + (((2 * d + (g >> 1)) ^ li) << 4) + 8 * (g & 1)) =
+      i32x2{(int)pack2<true>(x[0], x[1]), (int)pack2<true>(x[2], x[3])};
+}
+__device__ __forceinline__ void store_chunk(const TreeParams& p, const uint8_t* stage, int64_t slot, int first, int chunk, int g, int li) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int r = 4 * j + g;
+    const i32x4 x = *(const i32x4*)(stage + r * 256 + ((li ^ r) << 4));
+    if (first + r < p.rows) *(i32x4*)(p.ws_o + (slot * p.rows + first + r) * kDV + 128 * chunk + 8 * li) = x;
+  }
+}
+
+// 64 rows, a wave 16 of them: few synchronisations, for many rows.  The waves read their own 16 queries and a quarter of
+// the keys; the queries become operands in the place that the keys take afterwards.
+template <int FMT, bool F16, int KT>
+__global__ __launch_bounds__(256, 2) void mla_tree_rows_kernel(TreeParams p) {
+  constexpr int kTok = 32 * KT, kShare = kTok / 4;
+  __shared__ __attribute__((aligned(16))) uint8_t kv_sh[4 * kTileBytes];
+  __shared__ uint32_t spoilt_sh[4];
+  const int b = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, li = lane & 15;
+  const int first = blockIdx.x * 64 + 16 * wave;
   i32x4 q[kKSteps];
-#pragma unroll
-  for (int kk = 0; kk < kKSteps; ++kk) q[kk] = *(const i32x4*)(kk < 16 ? qn + 32 * kk : qr + 32 * (kk - 16));
-  uint64_t mask = p.mask[(int64_t)b * p.s_q + s];
-  const uint64_t nodes = p.s_q == 64 ? ~0ull : (1ull << p.s_q) - 1;
-  const uint64_t known = held == 64 ? ~0ull : (1ull << held) - 1;
-  if ((mask & nodes & ~known) != 0 && p.status != nullptr) *p.status = 1;
-  mask &= known;
-
-  // the tokens into LDS: wave w takes tokens w, w + 4, .., a lane 8 dims of each
-  i32x4 v[kTok / 4], r[KT];
-#pragma unroll
-  for (int i = 0; i < kTok / 4; ++i) {
-    const int j = 4 * i + wave;  // uniform
-    v[i] = i32x4{0, 0, 0, 0};
-    if (j < held) v[i] = latent8<FMT>(p, at + j < kPage ? pages[0] : pages[1], (at + j) & (kPage - 1), lane);
+  Share<FMT, kShare> x;
+  Tile t;
+  {
+    i32x4 qv[16], qr[2];
+    load_queries<16>(p, b, first, lane, qv, qr);
+    if (!find_tile(p, b, blockIdx.y, t)) return;
+    load_tokens(p, t, wave * kShare, lane, x);
+    put_queries<16>(kv_sh + wave * kTileBytes, lane, qv, qr);
   }
-#pragma unroll
-  for (int i = 0; i < KT; ++i) {
-    const int j = 32 * i + 8 * wave + (lane >> 3);
-    r[i] = i32x4{0, 0, 0, 0};
-    if (j < held) {
-      const int64_t page = at + j < kPage ? pages[0] : pages[1];
-      r[i] = *(const i32x4*)(p.rope + page * p.rp + ((at + j) & (kPage - 1)) * p.rt + 16 * (lane & 7));
-    }
+  __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS runs its accesses in order
+  read_fragments(kv_sh + wave * kTileBytes, g, li, q);
+  const int row_raw = first + li;
+  const int row = row_raw < p.rows ? row_raw : p.rows - 1;
+  uint64_t mask = t.known;
+  if (t.drafts) {  // uniform
+    const uint64_t nodes = p.s_q == 64 ? ~0ull : (1ull << p.s_q) - 1;
+    mask = p.mask[(int64_t)b * p.s_q + row / p.heads];
+    if ((mask & nodes & ~t.known) != 0 && p.status != nullptr) *p.status = 1;
+    mask &= t.known;
   }
-  __syncthreads();  // bad_sh is clear
-#pragma unroll
-  for (int i = 0; i < kTok / 4; ++i) {
-    const int j = 4 * i + wave;
-    const bool bad = non_finite<F16>(v[i]);
-    if (__builtin_amdgcn_ballot_w64(bad) != 0) {  // uniform, rare
-      if (bad) v[i] = i32x4{0, 0, 0, 0};
-      if (lane == 0) atomicOr(&bad_sh, 1ull << j);
-    }
-    *(i32x4*)(kv_sh + j * kPitch + 16 * lane) = v[i];
-  }
-#pragma unroll
-  for (int i = 0; i < KT; ++i)
-    *(i32x4*)(kv_sh + (32 * i + 8 * wave + (lane >> 3)) * kPitch + 2 * kDV + 16 * (lane & 7)) = r[i];
+  const int64_t slot = find_slot(p, b, blockIdx.y, t, lane);
+  __syncthreads();  // the queries are read
+  spoilt_sh[wave] = put_tokens<FMT, F16, kShare>(kv_sh + wave * kShare * kPitch, t.drafts, lane, x);
   __syncthreads();
-  const uint64_t bad = bad_sh;
+  uint64_t spoilt = 0;
+  if (t.drafts)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) spoilt |= (uint64_t)spoilt_sh[w] << (w * kShare);
 
-  // S^T: lane (g, i) gets tokens 16 t + 4 g .. +3 of row i
+  // S^T: lane (g, i) gets keys 16 u + 4 g .. +3 of row i
   f32x4 sc[2 * KT];
 #pragma unroll
-  for (int t = 0; t < 2 * KT; ++t) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    const uint8_t* k = kv_sh + (16 * t + li) * kPitch + 16 * g;
+  for (int u = 0; u < 2 * KT; ++u) {
+    const uint8_t* k = kv_sh + (16 * u + li) * kPitch + 16 * g;
+    sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < kKSteps; ++kk) acc = mfma32<F16>(*(const i32x4*)(k + 64 * kk), q[kk], acc);
-    sc[t] = acc;
+    for (int kk = 0; kk < kKSteps; ++kk) sc[u] = mfma32<F16>(*(const i32x4*)(k + 64 * kk), q[kk], sc[u]);
   }
   float mx = -INFINITY;
 #pragma unroll
-  for (int t = 0; t < 2 * KT; ++t)
+  for (int u = 0; u < 2 * KT; ++u)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const bool seen = (mask >> (16 * t + 4 * g + i)) & 1;
-      sc[t][i] = seen ? sc[t][i] * p.scale_log2 : -INFINITY;
-      mx = fmaxf(mx, sc[t][i]);
+      const bool seen = (mask >> (16 * u + 4 * g + i)) & 1;
+      sc[u][i] = seen ? sc[u][i] * p.scale_log2 : -INFINITY;
+      mx = fmaxf(mx, sc[u][i]);
     }
   mx = group_max(mx);
   const float ref = mx == -INFINITY ? 0.f : mx;
   float l = 0.f, lx = 0.f;
-  i32x4 pb[KT];
+  i32x4 pb[KT];  // P^T as it is: the B operand in the key order of the transposed reads
 #pragma unroll
-  for (int t = 0; t < 2 * KT; ++t) {
+  for (int u = 0; u < 2 * KT; ++u) {
     float e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      e[i] = __builtin_amdgcn_exp2f(sc[t][i] - ref);
+      e[i] = __builtin_amdgcn_exp2f(sc[u][i] - ref);
       lx += e[i];
     }
     const uint32_t w0 = pack2<F16>(e[0], e[1]), w1 = pack2<F16>(e[2], e[3]);
     l += sum2<F16>(w0) + sum2<F16>(w1);
-    pb[t >> 1][2 * (t & 1)] = (int)w0;
-    pb[t >> 1][2 * (t & 1) + 1] = (int)w1;
+    pb[u >> 1][2 * (u & 1)] = (int)w0;
+    pb[u >> 1][2 * (u & 1) + 1] = (int)w1;
   }
-  l = group_sum(l);
-  lx = group_sum(lx);
-
-  // O^T: transposed reads give lane (g, i) tokens 4 g .. +3 and 16 + 4 g .. +3 of dim 16 d + i
-  f32x4 o[kDimTiles];
-  const uint8_t* vt = kv_sh + (4 * g + (li >> 2)) * kPitch + 8 * (li & 3);
+  f32x4 o[kDV / 16];
 #pragma unroll
-  for (int d = 0; d < kDimTiles; ++d) {
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int d = 0; d < kDV / 16; ++d) {
+    o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const uint8_t LDS_AS* a = (const uint8_t LDS_AS*)(vt + 32 * t * kPitch + 32 * d);
-      const i32x2 lo = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)a));
-      const i32x2 hi = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 LDS_AS*)(a + 16 * kPitch)));
-      acc = mfma32<F16>(i32x4{lo[0], lo[1], hi[0], hi[1]}, pb[t], acc);
-    }
-    o[d] = acc;
+    for (int u = 0; u < KT; ++u) o[d] = mfma32<F16>(read_vt(kv_sh + 2 * u * kTileBytes, d, g, li), pb[u], o[d]);
   }
-
-  // the partial, as the split-KV decode writes its own: fp16 rows, each 128-dim chunk times a power of two
-  const bool spoilt = (mask & bad) != 0;
-  const float inv = spoilt ? __builtin_nanf("") : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-  // a NaN here makes the merged lse -inf, as any NaN row's is
-  const float lse2 = spoilt ? __builtin_nanf("") : lx > 0.f ? mx + __log2f(lx) : lx == 0.f ? -INFINITY : lx;
-  int e[4];
+  float inv, lse2;
+  finish_row((mask & spoilt) != 0, group_sum(l), group_sum(lx), mx, inv, lse2);
+  __syncthreads();  // V is read: its place takes the rows on their way out
+  uint8_t* stage = kv_sh + wave * kTileBytes;  // 4 KiB a chunk
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     float a = 0.f;
 #pragma unroll
-    for (int d = 8 * c; d < 8 * c + 8; ++d)
-      a = fmaxf(fmaxf(fmaxf(fabsf(o[d][0]), fabsf(o[d][1])), fmaxf(fabsf(o[d][2]), fabsf(o[d][3]))), a);
-    e[c] = part_exp(group_max(a * inv));
-  }
-  if (row_raw >= p.rows) return;
-  const int64_t dst_row = (int64_t)last * p.rows + row;
-  uint16_t* dst = p.ws_o + dst_row * kDV + 4 * g;
+    for (int d = 0; d < 8; ++d) a = largest(o[8 * c + d], a);
+    const int e = part_exp(group_max(a * inv));
 #pragma unroll
-  for (int d = 0; d < kDimTiles; ++d) {
-    const f32x4 x = (o[d] * inv) * exp2i(e[d >> 3]);
-    *(i32x2*)(dst + 16 * d) = i32x2{(int)pack2<true>(x[0], x[1]), (int)pack2<true>(x[2], x[3])};
+    for (int d = 0; d < 8; ++d) stage_chunk(stage + 4096 * c, d, g, li, (o[8 * c + d] * inv) * exp2i(e));
+    if (g == c && row_raw < p.rows) p.ws_scale[(slot * p.rows + row) * 4 + c] = exp2i(-e);
   }
-  const int eg = g == 0 ? e[0] : g == 1 ? e[1] : g == 2 ? e[2] : e[3];
-  p.ws_scale[dst_row * 4 + g] = exp2i(-eg);
-  if (g == 0) p.ws_lse[dst_row] = lse2;
+  if (g == 0 && row_raw < p.rows) p.ws_lse[slot * p.rows + row] = lse2;
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int c = 0; c < 4; ++c) store_chunk(p, stage + 4096 * c, slot, first, c, g, li);
 }
 
+// 16 rows: wave w scores keys 16 w .. +15 and owns dims 128 w .. +127 of the output; the row maximum and P^T cross the
+// waves through LDS.  The work of a tile in a quarter of the time, for few rows.
 template <int FMT, bool F16>
-static void launch_format(const TreeParams& p, hipStream_t st) {
-  const dim3 grid((p.rows + 63) / 64, p.batch);
-  if (p.s_q <= 32)
-    hipLaunchKernelGGL((mla_tree_kernel<FMT, F16, 1>), grid, dim3(256), 0, st, p);
-  else
-    hipLaunchKernelGGL((mla_tree_kernel<FMT, F16, 2>), grid, dim3(256), 0, st, p);
+__global__ __launch_bounds__(256, 2) void mla_tree_keys_kernel(TreeParams p) {
+  __shared__ __attribute__((aligned(16))) uint8_t kv_sh[4 * kTileBytes];
+  __shared__ __attribute__((aligned(16))) uint8_t p_sh[2][1024];
+  __shared__ float max_sh[4][16], sum_sh[4][2][16];
+  __shared__ uint32_t spoilt_sh[4];
+  const int b = blockIdx.z;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, li = lane & 15;
+  const int first = blockIdx.x * 16;
+  Share<FMT, 16> x;
+  Tile t;
+  {
+    i32x4 qv[4], qr[1];
+    load_queries<4>(p, b, first + 4 * wave, lane, qv, qr);
+    if (!find_tile(p, b, blockIdx.y, t)) return;
+    load_tokens(p, t, 16 * wave, lane, x);
+    put_queries<4>(kv_sh + 4 * wave * kPitch, lane, qv, qr);
+  }
+  const int row_raw = first + li;
+  const int row = row_raw < p.rows ? row_raw : p.rows - 1;
+  uint64_t mask = t.known;
+  if (t.drafts) {  // uniform
+    const uint64_t nodes = p.s_q == 64 ? ~0ull : (1ull << p.s_q) - 1;
+    mask = p.mask[(int64_t)b * p.s_q + row / p.heads];
+    if ((mask & nodes & ~t.known) != 0 && p.status != nullptr) *p.status = 1;
+    mask &= t.known;
+  }
+  const int64_t slot = find_slot(p, b, blockIdx.y, t, lane);
+  __syncthreads();
+  i32x4 q[kKSteps], k[kKSteps];
+  read_fragments(kv_sh, g, li, q);
+  __syncthreads();  // the queries are read
+  spoilt_sh[wave] = put_tokens<FMT, F16, 16>(kv_sh + wave * kTileBytes, t.drafts, lane, x);
+  __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS runs its accesses in order
+  read_fragments(kv_sh + wave * kTileBytes, g, li, k);
+  f32x4 even = {0.f, 0.f, 0.f, 0.f}, odd = even;
+#pragma unroll
+  for (int kk = 0; kk < kKSteps; kk += 2) {
+    even = mfma32<F16>(k[kk], q[kk], even);
+    odd = mfma32<F16>(k[kk + 1], q[kk + 1], odd);
+  }
+  float sc[4], mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool seen = (mask >> (16 * wave + 4 * g + i)) & 1;
+    sc[i] = seen ? (even[i] + odd[i]) * p.scale_log2 : -INFINITY;
+    mx = fmaxf(mx, sc[i]);
+  }
+  max_sh[wave][li] = group_max(mx);  // four lane groups, one value
+  __syncthreads();
+  mx = fmaxf(fmaxf(max_sh[0][li], max_sh[1][li]), fmaxf(max_sh[2][li], max_sh[3][li]));
+  const float ref = mx == -INFINITY ? 0.f : mx;
+  float e[4], lx = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    e[i] = __builtin_amdgcn_exp2f(sc[i] - ref);
+    lx += e[i];
+  }
+  // P^T as it is: half of the B operand of 32 keys in the order of the transposed reads
+  const uint32_t w0 = pack2<F16>(e[0], e[1]), w1 = pack2<F16>(e[2], e[3]);
+  *(i32x2*)&p_sh[wave >> 1][16 * lane + 8 * (wave & 1)] = i32x2{(int)w0, (int)w1};
+  sum_sh[wave][0][li] = group_sum(sum2<F16>(w0) + sum2<F16>(w1));
+  sum_sh[wave][1][li] = group_sum(lx);
+  __syncthreads();
+  const i32x4 pb[2] = {*(const i32x4*)&p_sh[0][16 * lane], *(const i32x4*)&p_sh[1][16 * lane]};
+  f32x4 o[8];
+#pragma unroll
+  for (int d = 0; d < 8; ++d) {
+    o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) o[d] = mfma32<F16>(read_vt(kv_sh + 2 * u * kTileBytes, 8 * wave + d, g, li), pb[u], o[d]);
+  }
+  uint64_t spoilt = 0;
+  if (t.drafts)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) spoilt |= (uint64_t)spoilt_sh[w] << (16 * w);
+  float inv, lse2;
+  finish_row((mask & spoilt) != 0, sum_sh[0][0][li] + sum_sh[1][0][li] + sum_sh[2][0][li] + sum_sh[3][0][li],
+             sum_sh[0][1][li] + sum_sh[1][1][li] + sum_sh[2][1][li] + sum_sh[3][1][li], mx, inv, lse2);
+  float a = 0.f;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) a = largest(o[d], a);
+  const int ex = part_exp(group_max(a * inv));
+  __syncthreads();  // V is read: its place takes the rows on their way out
+  uint8_t* stage = kv_sh + 4096 * wave;
+#pragma unroll
+  for (int d = 0; d < 8; ++d) stage_chunk(stage, d, g, li, (o[d] * inv) * exp2i(ex));
+  if (g == 0 && row_raw < p.rows) {
+    p.ws_scale[(slot * p.rows + row) * 4 + wave] = exp2i(-ex);
+    if (wave == 0) p.ws_lse[slot * p.rows + row] = lse2;
+  }
+  __builtin_amdgcn_wave_barrier();
+  store_chunk(p, stage, slot, first, wave, g, li);
 }
 
-hipError_t launch_drafts(const TreeParams& p, hipStream_t st) {
-  if (p.format == MLA_KV_FP8_E4M3) launch_format<MLA_KV_FP8_E4M3, false>(p, st);
-  else if (p.format == MLA_KV_FP4_E2M1) launch_format<MLA_KV_FP4_E2M1, false>(p, st);
-  else if (p.f16) launch_format<MLA_KV_NATIVE, true>(p, st);
-  else launch_format<MLA_KV_NATIVE, false>(p, st);
+// Whether the prefixes' pages are tiles of the launch too, each its own split, instead of parts of the split-KV pass: where
+// they are few the pass is mostly start and end, a launch more, and wants a schedule.  By tiles of 16 rows x pages (the
+// table's width for all sequences; `slots`: what the workspace has), the whole decode in us, the pass -> pages:
+//   bf16  264 34.6 -> 14.7    528 36.2 -> 19.9    1056 41.7 -> 27.6    1152 31.6 -> 25.3    2112 41.4 -> 38.3, 44.1 -> 37.6
+//   fp8   264 36.5 -> 14.4    528 37.6 -> 19.7    1056 43.3 -> 28.2    1152 31.2 -> 24.5    2112 42.9 -> 37.3, 46.2 -> 39.3
+//   fp4   264 19.9 -> 14.9    528 23.3 -> 20.0    640 23.0 -> 23.6 (a form for few pages of its own)
+bool takes_pages(int64_t batch, int64_t rows, int format, int64_t bt_width, int64_t slots, int cus) {
+  const int64_t tiles = (rows + 15) / 16 * batch * bt_width;
+  return batch * (bt_width + 1) <= slots && 4 * tiles <= (format == MLA_KV_FP4_E2M1 ? 9 : 36) * (int64_t)cus;
+}
+
+// 16 rows a workgroup where there are few tiles for the CUs, else 64; the whole decode in us, 16 -> 64 (bf16):
+//   72 tiles 12.0 -> 15.5    136 12.4 -> 15.6    264 (272 with the drafted tokens') 14.7 -> 17.1    256 47.6 -> 48.7
+//   512 56.0 -> 56.0    528 22.0 -> 20.3    640 73.2 -> 70.5    1024 78.5 -> 73.2    2048 124 -> 108    4096 194 -> 160
+template <int FMT, bool F16>
+static void launch_format(const TreeParams& p, int cus, hipStream_t st) {
+  const int64_t rows16 = (p.rows + 15) / 16;
+  const int tiles = p.pages ? 1 + p.bt_width : 1;
+  const bool few = 4 * rows16 * tiles * p.batch <= 5 * (int64_t)cus;
+  const dim3 grid((uint32_t)(few ? rows16 : (rows16 + 3) / 4), tiles, p.batch);
+  if (few)
+    hipLaunchKernelGGL((mla_tree_keys_kernel<FMT, F16>), grid, dim3(256), 0, st, p);
+  else if (!p.pages && p.s_q <= 32)
+    hipLaunchKernelGGL((mla_tree_rows_kernel<FMT, F16, 1>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((mla_tree_rows_kernel<FMT, F16, 2>), grid, dim3(256), 0, st, p);
+}
+
+hipError_t launch_tiles(const TreeParams& p, int cus, hipStream_t st) {
+  if (p.format == MLA_KV_FP8_E4M3) launch_format<MLA_KV_FP8_E4M3, false>(p, cus, st);
+  else if (p.format == MLA_KV_FP4_E2M1) launch_format<MLA_KV_FP4_E2M1, false>(p, cus, st);
+  else if (p.f16) launch_format<MLA_KV_NATIVE, true>(p, cus, st);
+  else launch_format<MLA_KV_NATIVE, false>(p, cus, st);
   return hipGetLastError();
 }
 
