@@ -162,6 +162,13 @@ def _tree_without_schedule(batch: int, s_q: int, heads: int, fmt: int, width: in
     return parts if _lib.load().mla_tree_takes_pages(batch, s_q, heads, parts, fmt, width) else None
 
 
+@functools.lru_cache(maxsize=64)
+def _unread_schedule(parts: int, batch: int, device: torch.device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Tensors of a schedule's shape for a decode that reads none (see :func:`_tree_without_schedule`)."""
+    return (torch.empty(parts, _lib.MLA_SCHED_WORDS, dtype=torch.int32, device=device),
+            torch.empty(batch + 1, dtype=torch.int32, device=device))
+
+
 def kernel_variant(rows: int) -> dict:
     """Tile of the main kernel for ``rows`` = s_q * heads query rows (``mla_variant``)."""
     w, t, st, r = (ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32())
@@ -565,15 +572,14 @@ def mla_decode_with_kvcache(q: torch.Tensor, kv_cache, block_table: torch.Tensor
         if tree is not None:
             cache_seqlens = tree.prefix_lens
         longest = _lib.MLA_PAGE_TOKENS * block_table.shape[1] if block_table is not None and block_table.dim() == 2 else None
-        sched = None
-        if tree is not None and not forced and longest is not None:
-            sched = _tree_without_schedule(q.shape[0], q.shape[1], q.shape[2], _cache_format(kv_cache), block_table.shape[1])
-        if sched is None:
+        unread = None
+        if tree is not None and not forced and longest is not None and q.dim() == 4:
+            unread = _tree_without_schedule(q.shape[0], q.shape[1], q.shape[2], _cache_format(kv_cache), block_table.shape[1])
+        if unread is not None:
+            sched, splits = _unread_schedule(unread, q.shape[0], q.device)
+        else:
             sched, splits = get_mla_metadata(cache_seqlens, q.shape[1] * q.shape[2], 1,
                                              forced_splits=forced, kv_cache=kv_cache, max_seqlen=longest)
-        else:  # of that many parts, and not read
-            sched = torch.empty(sched, _lib.MLA_SCHED_WORDS, dtype=torch.int32, device=q.device)
-            splits = torch.empty(q.shape[0] + 1, dtype=torch.int32, device=q.device)
         if forced == 1:
             return _decode(q, kv_cache, block_table, cache_seqlens, sched, splits, sm_scale, causal,
                            out, lse, status=status, single_split=True, tree=tree)
@@ -678,16 +684,16 @@ class TreePlan(NamedTuple):
 
 def _check_tree(tree: TreePlan, B: int, s_q: int, device: torch.device) -> torch.Tensor:
     """The prefix lengths of a plan for ``[B, s_q]`` query tokens, checked with its masks."""
-    mask, lens = tree.mask, tree.prefix_lens
+    mask, _, _, lens = tree
     if s_q > _lib.MLA_TREE_MAX_NODES:
         raise ValueError(f"a tree decode takes s_q <= {_lib.MLA_TREE_MAX_NODES}")
     for t, name in ((mask, "tree.mask"), (lens, "tree.prefix_lens")):
-        _require_gpu(t, name)
-        if t.device != device:
+        if t.get_device() != device.index:
+            _require_gpu(t, name)
             raise ValueError(f"{name} is on {t.device}, q on {device}")
-    if mask.dtype != torch.int64 or mask.shape != (B, s_q) or not mask.is_contiguous():
+    if mask.dtype is not torch.int64 or mask.shape != (B, s_q) or not mask.is_contiguous():
         raise ValueError("tree.mask must be a contiguous int64 [B, s_q] tensor")
-    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+    if lens.dtype is not torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
         raise ValueError("tree.prefix_lens must be a contiguous int32 [B] tensor")
     return lens
 

@@ -22,11 +22,14 @@ import torch
 
 from . import _lib
 from ._lib import MlaTreePlanArgs
-from .api import TreePlan, _check_tree, _launch
-from .serving import _cache_struct, _require, _require_int32
+from .api import TreePlan, _launch
+from .serving import _cache_struct, _require
 
 _PLAN = struct.Struct("=4Q4i4Q")
 assert _PLAN.size == ctypes.sizeof(MlaTreePlanArgs)
+
+_INT32 = (torch.int32,)
+_INTS = (torch.int32, torch.int64)
 
 
 class Accepted(NamedTuple):
@@ -39,13 +42,27 @@ class Accepted(NamedTuple):
     keep_lens: torch.Tensor
 
 
-def _grid(t: torch.Tensor, name: str, dtypes, shape=None, device: Optional[torch.device] = None) -> None:
-    _require(t, name, device)
-    if t.dtype not in dtypes or t.dim() != 2 or (shape is not None and t.shape != shape) or not t.is_contiguous():
+def _grid(t: torch.Tensor, name: str, dtype: torch.dtype, shape, index: int) -> None:
+    """A contiguous ``shape`` tensor of ``dtype`` on GPU ``index``; what it is not, said in full only where it is not."""
+    if t.get_device() == index and t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return
+    _require(t, name)
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the other tensors on cuda:{index}")
+    raise ValueError(f"{name} must be a contiguous {str(dtype).replace('torch.', '')} tensor {list(shape)}")
+
+
+def _first_grid(t: torch.Tensor, name: str, dtypes) -> int:
+    """Checks the ``[B, s_q]`` tensor that gives a call its shape; its GPU's index."""
+    index = t.get_device()
+    if index < 0:
+        _require(t, name)
+    if t.dtype not in dtypes or t.dim() != 2 or not t.is_contiguous():
         kinds = " or ".join(str(d).replace("torch.", "") for d in dtypes)
-        raise ValueError(f"{name} must be a contiguous {kinds} tensor [B, s_q]" + (f" = {list(shape)}" if shape is not None else ""))
+        raise ValueError(f"{name} must be a contiguous {kinds} tensor [B, s_q]")
     if not 1 <= t.shape[1] <= _lib.MLA_TREE_MAX_NODES:
         raise ValueError(f"s_q must be in [1, {_lib.MLA_TREE_MAX_NODES}]")
+    return index
 
 
 def tree_plan(parents: torch.Tensor, cache_seqlens: torch.Tensor, block_table: torch.Tensor,
@@ -56,27 +73,29 @@ def tree_plan(parents: torch.Tensor, cache_seqlens: torch.Tensor, block_table: t
     Any other value drops the node: it sees nothing and nothing sees it, and neither does what hangs below it; so do
     nodes past ``tree_lens`` (int32 ``[B]``, by default all are s_q long).  A dropped node within the tree's length still
     has its row in the cache.  A sequence shorter than its tree has none of it."""
-    _grid(parents, "parents", (torch.int32,))
+    index = _first_grid(parents, "parents", _INT32)
     device = parents.device
-    B, s_q = parents.shape
-    _require_int32(cache_seqlens, "cache_seqlens", B, device)
+    B, s_q = shape = parents.shape
+    _grid(cache_seqlens, "cache_seqlens", torch.int32, (B,), index)
     if tree_lens is not None:
-        _require_int32(tree_lens, "tree_lens", B, device)
-    _require(block_table, "block_table", device)
+        _grid(tree_lens, "tree_lens", torch.int32, (B,), index)
+    if block_table.get_device() != index:
+        _require(block_table, "block_table", device)
     if block_table.dtype is not torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B:
         raise ValueError("block_table must be a [B, P] int32 tensor with unit column stride")
     (_, P), (stride, unit) = block_table.shape, block_table.stride()
     if P < 1 or (P > 1 and unit != 1) or (B > 1 and stride < P) or (B > 1 and stride >= 2 ** 31):
         raise ValueError("block_table must have columns of unit stride, and rows below 2^31 apart that do not overlap")
-    mask = torch.empty(B, s_q, dtype=torch.int64, device=device)
-    buf = torch.empty(2 * B * s_q + B, dtype=torch.int32, device=device)
-    positions, slots, prefix = buf.split_with_sizes((B * s_q, B * s_q, B))
-    at = buf.data_ptr()
+    mask = torch.empty(shape, dtype=torch.int64, device=device)
+    positions = torch.empty(shape, dtype=torch.int32, device=device)
+    slots = torch.empty(shape, dtype=torch.int32, device=device)
+    prefix = torch.empty(B, dtype=torch.int32, device=device)
     a = MlaTreePlanArgs.from_buffer_copy(_PLAN.pack(
         parents.data_ptr(), cache_seqlens.data_ptr(), tree_lens.data_ptr() if tree_lens is not None else 0,
-        block_table.data_ptr(), stride if B > 1 else P, P, B, s_q, mask.data_ptr(), at, at + 4 * B * s_q, at + 8 * B * s_q))
+        block_table.data_ptr(), stride if B > 1 else P, P, B, s_q, mask.data_ptr(), positions.data_ptr(),
+        slots.data_ptr(), prefix.data_ptr()))
     _launch("mla_tree_plan", _lib.load().mla_tree_plan, device, ctypes.byref(a))
-    return TreePlan(mask, positions.view(B, s_q), slots.view(B, s_q), prefix)
+    return TreePlan(mask, positions, slots, prefix)
 
 
 def tree_accept(plan: TreePlan, tokens: torch.Tensor, targets: torch.Tensor) -> Accepted:
@@ -86,19 +105,21 @@ def tree_accept(plan: TreePlan, tokens: torch.Tensor, targets: torch.Tensor) -> 
     or both int64).  Node 0 is the token that the step before decided (its ``next_tokens``): it is kept.  From there the
     path goes on, while there is one, to the child whose token is the target of the node before; of several with that
     token to the lowest.  Where node 0 is no root nothing is kept."""
-    _grid(tokens, "tokens", (torch.int32, torch.int64))
-    device, shape = tokens.device, tokens.shape
-    _grid(targets, "targets", (tokens.dtype,), shape, device)
+    index = _first_grid(tokens, "tokens", _INTS)
+    device, dtype, shape = tokens.device, tokens.dtype, tokens.shape
     B, s_q = shape
-    _check_tree(plan, B, s_q, device)
-    buf = torch.empty(B * s_q + 2 * B, dtype=torch.int32, device=device)
-    path, counts, keep = buf.split_with_sizes((B * s_q, B, B))
-    after = torch.empty(B, dtype=tokens.dtype, device=device)
-    at = buf.data_ptr()
-    _launch("mla_tree_accept", _lib.load().mla_tree_accept, device, plan.mask.data_ptr(), plan.prefix_lens.data_ptr(),
-            tokens.data_ptr(), targets.data_ptr(), int(tokens.dtype is torch.int64), B, s_q, at, at + 4 * B * s_q,
-            after.data_ptr(), at + 4 * B * (s_q + 1))
-    return Accepted(path.view(B, s_q), counts, after, keep)
+    mask, _, _, prefix = plan
+    _grid(targets, "targets", dtype, shape, index)
+    _grid(mask, "plan.mask", torch.int64, shape, index)
+    _grid(prefix, "plan.prefix_lens", torch.int32, (B,), index)
+    path = torch.empty(shape, dtype=torch.int32, device=device)
+    counts = torch.empty(B, dtype=torch.int32, device=device)
+    keep = torch.empty(B, dtype=torch.int32, device=device)
+    after = torch.empty(B, dtype=dtype, device=device)
+    _launch("mla_tree_accept", _lib.load().mla_tree_accept, device, mask.data_ptr(), prefix.data_ptr(), tokens.data_ptr(),
+            targets.data_ptr(), int(dtype is torch.int64), B, s_q, path.data_ptr(), counts.data_ptr(), after.data_ptr(),
+            keep.data_ptr())
+    return Accepted(path, counts, after, keep)
 
 
 def kv_keep_path(kv_cache, slots: torch.Tensor, path: torch.Tensor) -> None:
@@ -107,7 +128,9 @@ def kv_keep_path(kv_cache, slots: torch.Tensor, path: torch.Tensor) -> None:
     every cache format.  ``slots`` is the plan's.  Entries below their own place k and slots outside the cache name
     nothing.  A drafted token's position is its depth's, so what is moved needs no new rotation."""
     c, _, device = _cache_struct(kv_cache, None)
-    _grid(path, "path", (torch.int32,), None, device)
-    _grid(slots, "slots", (torch.int32,), path.shape, device)
+    if path.get_device() != device.index:
+        _require(path, "path", device)
+    _first_grid(path, "path", _INT32)
+    _grid(slots, "slots", torch.int32, path.shape, device.index)
     _launch("mla_kv_keep_path", _lib.load().mla_kv_keep_path, device, ctypes.byref(c), slots.data_ptr(), path.data_ptr(),
             *path.shape)
