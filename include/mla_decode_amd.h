@@ -568,6 +568,35 @@ int mla_tree_accept(const uint64_t* mask, const int32_t* prefix_lens, const void
  */
 int mla_kv_keep_path(const mla_kv_cache* cache, const int32_t* slots, const int32_t* path, int32_t batch, int32_t s_q, void* stream);
 
+/* ---- around the attention in a layer (no counterpart in the reference) --------------------- */
+
+/*
+ * Root-mean-square norm with the residual's addition: h = x + residual (residual NULL: h = x),
+ *   residual_out = h,   out = h / sqrt(mean(h^2) + eps) * weight,
+ * of rows of `dim` values.  Sums in fp32 (a row whose squares add up past fp32's range gives zeros), the norm of h before it
+ * is rounded, one rounding each.  With `scale` not NULL, out is 8-bit rows: e4m3 codes (out_stride in bytes) and a byte
+ * per 32 dims, scale [tokens, dim / 32] contiguous: the value is e4m3(code) * 2^(byte - 127), 2^(byte - 127) the smallest
+ * power of two with max|y| <= 448 * 2^(byte - 127) (byte 1 at least; 127 of zeros), rounded to nearest even; a block that
+ * holds a NaN or an infinity gets byte 255 and NaN codes (0x7F).
+ * Strides in elements; inputs may be rows of stride 0.  out and residual_out may each be x or residual themselves, row
+ * for row, and may not overlap them otherwise, nor each other.  tokens below 2^24, dim at most 2^24.
+ */
+typedef struct mla_rms_norm_args {
+  const void* x;
+  const void* residual;
+  const void* weight;  /* [dim] in dtype or fp32 */
+  void* out;
+  uint8_t* scale;
+  void* residual_out;
+  int64_t x_stride, residual_stride, out_stride, residual_out_stride;
+  int32_t tokens, dim;
+  int32_t dtype;        /* of x, residual, residual_out and 16-bit (or fp32) out: MLA_DTYPE_BF16, _F16 or _F32 */
+  int32_t weight_dtype; /* dtype, or MLA_DTYPE_F32 */
+  float eps;
+  int32_t reserved; /* must be 0 */
+} mla_rms_norm_args;
+int mla_rms_norm(const mla_rms_norm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -60,6 +60,7 @@ EXPORTED = (
     "mla_tree_takes_pages",
     "mla_tree_accept",
     "mla_kv_keep_path",
+    "mla_rms_norm",
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -250,6 +251,29 @@ class MlaTreePlanArgs(ctypes.Structure):
     ]
 
 
+class MlaRmsNormArgs(ctypes.Structure):
+    """Layout of ``mla_rms_norm_args`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("x", _vp),
+        ("residual", _vp),
+        ("weight", _vp),
+        ("out", _vp),
+        ("scale", _vp),
+        ("residual_out", _vp),
+        ("x_stride", _i64),
+        ("residual_stride", _i64),
+        ("out_stride", _i64),
+        ("residual_out_stride", _i64),
+        ("tokens", _i32),
+        ("dim", _i32),
+        ("dtype", _i32),
+        ("weight_dtype", _i32),
+        ("eps", _f32),
+        ("reserved", _i32),
+    ]
+
+
 class MlaError(RuntimeError):
     """A nonzero status from the C ABI, carrying the library's message."""
 
@@ -340,6 +364,8 @@ def load() -> ctypes.CDLL:
         lib.mla_tree_accept.restype = ctypes.c_int
         lib.mla_kv_keep_path.argtypes = [ctypes.POINTER(MlaKvCache), _vp, _vp, _i32, _i32, _vp]
         lib.mla_kv_keep_path.restype = ctypes.c_int
+        lib.mla_rms_norm.argtypes = [ctypes.POINTER(MlaRmsNormArgs), _vp]
+        lib.mla_rms_norm.restype = ctypes.c_int
         _lib = lib
         return lib
 

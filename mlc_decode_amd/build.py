@@ -5,7 +5,7 @@ of ``include/mla_decode_amd.h`` into a shared library that ``mlc_decode_amd._lib
 ctypes.  Runs without a GPU (hipcc cross-compiles).  ``csrc/mla_decode_ws.hip`` (the dense
 wave-split kernel) is compiled with LLVM's iterative ILP machine scheduler, every other
 translation unit (``mla_fp4.hip``: the decode over the 4-bit cache; ``mla_serving.hip``: rotary
-positions, appends, gather, pages; ``mla_tree.hip``: drafted tokens) with the default one.
+positions, appends, gather, pages; ``mla_tree.hip``: drafted tokens; ``mla_layer.hip``: norm and projections) with the default one.
 """
 from __future__ import annotations
 
@@ -28,6 +28,7 @@ SOURCES = [
     (os.path.join(CSRC, "mla_fp4.hip"), []),
     (os.path.join(CSRC, "mla_serving.hip"), []),
     (os.path.join(CSRC, "mla_tree.hip"), []),
+    (os.path.join(CSRC, "mla_layer.hip"), []),
 ]
 # bench.py's MFMA-rate and shader-clock probe (a measurement helper, not the decode's ABI)
 PROBE_PATH = os.path.join(LIB_DIR, "libmla_probe.so")

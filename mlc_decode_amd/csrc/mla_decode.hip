@@ -4295,6 +4295,7 @@ int launch_tree(const mla_decode_args* args, const uint64_t* mask, mla::KParams*
 }  // namespace
 
 int mla_srv::set_error(int code, const std::string& msg) { return fail(code, msg); }
+int mla_srv::cu_count() { return cu_count_current(); }
 
 extern "C" {
 

@@ -10,6 +10,9 @@ namespace mla_srv {
 // Leaves `msg` for mla_last_error() on this thread and returns `code`.
 int set_error(int code, const std::string& msg);
 
+// Compute units of the GPU (queried once).
+int cu_count();
+
 // A paged cache as the kernels take it.
 struct Cache {
   int32_t format;
