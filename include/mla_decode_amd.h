@@ -597,6 +597,36 @@ typedef struct mla_rms_norm_args {
 } mla_rms_norm_args;
 int mla_rms_norm(const mla_rms_norm_args* args, void* stream);
 
+/*
+ * Projection of few rows by 4-bit weights: y[t, m] = sum_j x[t, j] * w[m, j], m < n, j < k, with
+ * w[m, j] = e2m1(code) * 2^(s - 127), a scale byte s (1 .. 254; 255 makes output m NaN) per output and 32 inputs.
+ * Sums in fp32, one rounding to y_dtype.  Rows are 16-bit (x_dtype), or with x_scale e4m3 codes whose scales, a byte per
+ * 32 values, are at x_scale + t * x_scale_stride (mla_rms_norm's).  bf16 and 8-bit rows take the weights exactly; with fp16
+ * rows, weights below 2^-35 of the largest of their output are lost.
+ * The weights are laid out in tiles of 16 outputs (T = ceil(n / 16)) and chunks of 128 inputs (C = ceil(k / 128)): lane
+ * 16 g + i of a tile and chunk holds output i's codes of inputs 32 g .. 32 g + 31 (two a byte, the lower input in the low
+ * half), and their scale byte; outputs and inputs past the end are codes 0, scale 127:
+ *   codes [T][C][64][16] (16-byte aligned),  scale [T][C][64],  top [16 T]: the largest scale byte of each output.
+ * tokens at most 2^20, n at most 2^22, k a multiple of 32, at most 2^22.  Strides in elements (x's a multiple of 16 bytes,
+ * x 16-byte aligned); workspace: mla_linear_workspace_bytes (0: none), 16-byte aligned, of this call alone while it runs.
+ */
+typedef struct mla_linear_args {
+  const void* x;
+  const uint8_t* x_scale; /* NULL: 16-bit rows */
+  const void* codes;
+  const uint8_t* scale;
+  const uint8_t* top;
+  void* y;
+  int64_t x_stride, x_scale_stride, y_stride;
+  int32_t tokens, n, k;
+  int32_t x_dtype, y_dtype; /* MLA_DTYPE_BF16 or MLA_DTYPE_F16; x_dtype is not read with x_scale */
+  int32_t reserved;
+  void* workspace;
+  int64_t workspace_bytes;
+} mla_linear_args;
+int mla_linear_fp4(const mla_linear_args* args, void* stream);
+int64_t mla_linear_workspace_bytes(int32_t tokens, int32_t n, int32_t k);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,7 +7,7 @@ from .api import (Fp4KVCache, Fp8KVCache, TreePlan, flash_mla_with_kvcache, fp4_
                   get_mla_metadata, get_mla_metadata_host, kv_append, merge_partials, mla_decode_absorbed,
                   mla_decode_with_kvcache, num_parts_for, prepare_w_uv, quantize_kv_cache)
 from .drafts import Accepted, kv_keep_path, tree_accept, tree_plan
-from .layer import Fp8Rows, rms_norm
+from .layer import Fp4Weight, Fp8Rows, linear_fp4, pack_w_fp4, quantize_w_fp4, rms_norm
 from .legacy import MlaKernel
 from .serving import (PagePool, Reservation, Rope, apply_rope, kv_append_slots, kv_gather, page_pool,
                       release_pages, reserve_pages, rope_plan)
@@ -32,7 +32,11 @@ __all__ = [
     "kv_keep_path",
     "tree_accept",
     "tree_plan",
+    "Fp4Weight",
     "Fp8Rows",
+    "linear_fp4",
+    "pack_w_fp4",
+    "quantize_w_fp4",
     "rms_norm",
     "MlaKernel",
     "PagePool",

@@ -61,6 +61,8 @@ EXPORTED = (
     "mla_tree_accept",
     "mla_kv_keep_path",
     "mla_rms_norm",
+    "mla_linear_fp4",
+    "mla_linear_workspace_bytes",
 )
 
 _i32, _i64, _f32, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -274,6 +276,30 @@ class MlaRmsNormArgs(ctypes.Structure):
     ]
 
 
+class MlaLinearArgs(ctypes.Structure):
+    """Layout of ``mla_linear_args`` (include/mla_decode_amd.h)."""
+
+    _fields_ = [
+        ("x", _vp),
+        ("x_scale", _vp),
+        ("codes", _vp),
+        ("scale", _vp),
+        ("top", _vp),
+        ("y", _vp),
+        ("x_stride", _i64),
+        ("x_scale_stride", _i64),
+        ("y_stride", _i64),
+        ("tokens", _i32),
+        ("n", _i32),
+        ("k", _i32),
+        ("x_dtype", _i32),
+        ("y_dtype", _i32),
+        ("reserved", _i32),
+        ("workspace", _vp),
+        ("workspace_bytes", _i64),
+    ]
+
+
 class MlaError(RuntimeError):
     """A nonzero status from the C ABI, carrying the library's message."""
 
@@ -366,6 +392,10 @@ def load() -> ctypes.CDLL:
         lib.mla_kv_keep_path.restype = ctypes.c_int
         lib.mla_rms_norm.argtypes = [ctypes.POINTER(MlaRmsNormArgs), _vp]
         lib.mla_rms_norm.restype = ctypes.c_int
+        lib.mla_linear_fp4.argtypes = [ctypes.POINTER(MlaLinearArgs), _vp]
+        lib.mla_linear_fp4.restype = ctypes.c_int
+        lib.mla_linear_workspace_bytes.argtypes = [_i32] * 3
+        lib.mla_linear_workspace_bytes.restype = ctypes.c_int64
         _lib = lib
         return lib
 

@@ -510,7 +510,7 @@ def prepare_w_uv(w_uv: torch.Tensor) -> torch.Tensor:
 
 def mla_decode_absorbed(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tensor],
                         cache_seqlens: Optional[torch.Tensor], tile_scheduler_metadata: torch.Tensor,
-                        num_splits: torch.Tensor, w_uv_blk: torch.Tensor, w_o: Optional[torch.Tensor] = None,
+                        num_splits: torch.Tensor, w_uv_blk: torch.Tensor, w_o: Union[None, torch.Tensor, "Fp4Weight"] = None,
                         softmax_scale: Optional[float] = None, causal: bool = False,
                         lse: Optional[torch.Tensor] = None, indices: Optional[torch.Tensor] = None,
                         tree: Optional["TreePlan"] = None):
@@ -520,7 +520,8 @@ def mla_decode_absorbed(q: torch.Tensor, kv_cache, block_table: Optional[torch.T
     into the per-head product ``v[b, s, h] = o[b, s, h] . W_UV[h]`` (``mla_combine_absorb``,
     ``w_uv_blk`` from ``prepare_w_uv``), so the merged latent output is never written.  ``y`` is
     ``v [B, s_q, H, 128]``, or with ``w_o [H * 128, D]`` the output projection
-    ``v.reshape(B, s_q, H * 128) @ w_o`` (a plain GEMM, done by torch).  No counterpart in the
+    ``v.reshape(B, s_q, H * 128) @ w_o`` (a plain GEMM, done by torch; or by ``linear_fp4`` with 4-bit weights, an
+    ``Fp4Weight`` of ``[D, H * 128]``).  No counterpart in the
     reference; the step that consumes the decode's ``out [B, s_q, H, 512]`` in DeepSeek MLA.
     """
     if softmax_scale is None:
@@ -543,6 +544,9 @@ def mla_decode_absorbed(q: torch.Tensor, kv_cache, block_table: Optional[torch.T
     del keep
     if w_o is None:
         return v, lse
+    if isinstance(w_o, tuple):
+        from .layer import linear_fp4
+        return linear_fp4(v.view(B, s_q, H * 128), w_o), lse
     if w_o.dim() != 2 or w_o.shape[0] != H * 128 or w_o.dtype != q.dtype:
         raise ValueError("w_o must be [H * 128, D] in q's dtype")
     return torch.matmul(v.reshape(B, s_q, H * 128), w_o), lse

@@ -274,6 +274,377 @@ static void launch_norm_type(const NormParams& p, bool vec, int cus, hipStream_t
     launch_norm<E, 1>(p, cus, st);
 }
 
+// ---------------------------------------------------------------------------------------
+// projections by 4-bit weights
+// ---------------------------------------------------------------------------------------
+// y[t, n] = sum_k x[t, k] w[n, k], w[n, k] = e2m1(code) * 2^(s[n, k / 32] - 127), for few rows t: the weights are read
+// once, 17 bits for 32 of them, and that is what bounds it.  They are laid out as the operand of the matrix unit: of
+// 16 outputs x 128 inputs (a chunk), lane (g, i) holds inputs 32 g .. +31 of output i, 16 bytes; the scale bytes alike.
+//   16-bit rows: 8 codes become 8 bf16 (exact) or fp16, four 16x16x32 MFMAs a chunk.  fp16 has no room for a scale's
+//     range: a row's scales are taken relative to its largest, 2^11, and the output is multiplied back; what lies 2^-35
+//     below the largest of its row is lost there.
+//   8-bit rows: one block-scaled 16x16x128 MFMA a chunk, codes and scales as they are.
+// A lane of a result holds outputs 4 g .. +3 of row i.  Everything is summed in fp32.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((__vector_size__(8 * sizeof(__bf16))));
+typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
+
+enum { kRowsBf16 = 0, kRowsF16 = 1, kRowsFp8 = 2 };
+
+struct LinearParams {
+  const uint8_t* x;        // rows
+  const uint8_t* x_scale;  // of 8-bit rows
+  int64_t x_st, xs_st;     // bytes
+  const uint8_t* codes;    // [tiles][chunks][64][16]
+  const uint8_t* scale;    // [tiles][chunks][64]
+  const uint8_t* top;      // [16 tiles] the largest scale byte of an output's weights
+  uint8_t* y;
+  int64_t y_st;            // bytes
+  float* part;             // [splits][tokens][16 tiles] partial sums
+  int32_t tokens, n, k, tiles, chunks, per_split;  // per_split: chunks of a split
+  int32_t y_f16, y_vec;    // y_vec: rows of y take 8-byte stores
+};
+
+template <int XT>
+constexpr int kChunkBytes = XT == kRowsFp8 ? 128 : 256;  // of a row
+template <int XT>
+constexpr int kTileX = 16 * kChunkBytes<XT>;  // 16 rows of a chunk in LDS
+
+// A piece of 16 bytes of a row's chunk (p of 16 or 8): its place in the 16 rows' chunk in LDS.  Blocks of 256 bytes hold
+// what one lane group of an operand reads, the rows' order in them turned by the piece, so that both the writes (pieces of
+// one row or two) and the reads (16 rows) go over all banks.
+template <int XT>
+__device__ __forceinline__ int piece_place(int p, int row) {
+  if constexpr (XT == kRowsFp8)
+    return p * 256 + ((row ^ (2 * p)) << 4);  // operand half p / 4 (inputs 64 h + 16 g), lane group p % 4
+  else
+    return (p & 3) * 1024 + (p >> 2) * 256 + ((row ^ p) << 4);  // MFMA p % 4, lane group p / 4 (inputs 32 g + 8 j)
+}
+// The operand of MFMA j (of half j) for lane (g, i).
+template <int XT>
+__device__ __forceinline__ i32x4 read_piece(const uint8_t* tile, int j, int g, int i) {
+  const int p = XT == kRowsFp8 ? 4 * j + g : 4 * g + j;
+  return *(const i32x4*)(tile + piece_place<XT>(p, i));
+}
+
+// Registers of a 16-row chunk by one wave: 64 / pieces rows a load.
+template <int XT>
+struct RowsChunk {
+  static constexpr int kPieces = kChunkBytes<XT> / 16, kLoads = 16 * kPieces / 64;
+  i32x4 v[kLoads];
+  int sc;  // 8-bit rows: lane (g, i)'s scale byte
+};
+template <int XT>
+__device__ __forceinline__ void load_rows(const LinearParams& p, int first, int chunk, int lane, RowsChunk<XT>& c) {
+  constexpr int kPieces = RowsChunk<XT>::kPieces, kEach = 64 / kPieces;
+#pragma unroll
+  for (int q = 0; q < RowsChunk<XT>::kLoads; ++q) {
+    const int row = first + kEach * q + lane / kPieces, piece = lane % kPieces;
+    c.v[q] = i32x4{0, 0, 0, 0};
+    if (row < p.tokens && (chunk * kPieces + piece) * (XT == kRowsFp8 ? 16 : 8) < p.k)
+      c.v[q] = *(const i32x4*)(p.x + row * p.x_st + (int64_t)chunk * kChunkBytes<XT> + 16 * piece);
+  }
+  if constexpr (XT == kRowsFp8) {
+    const int row = first + (lane & 15), block = 4 * chunk + (lane >> 4);
+    c.sc = 127;
+    if (row < p.tokens && 32 * block < p.k) c.sc = p.x_scale[row * p.xs_st + block];
+  }
+}
+template <int XT>
+__device__ __forceinline__ void put_rows(uint8_t* tile, int lane, const RowsChunk<XT>& c) {
+  constexpr int kPieces = RowsChunk<XT>::kPieces, kEach = 64 / kPieces;
+#pragma unroll
+  for (int q = 0; q < RowsChunk<XT>::kLoads; ++q)
+    *(i32x4*)(tile + piece_place<XT>(lane % kPieces, kEach * q + lane / kPieces)) = c.v[q];
+}
+
+struct WeightChunk {
+  i32x4 codes;
+  int sc;
+};
+__device__ __forceinline__ void load_weights(const LinearParams& p, int64_t tile, int chunk, int lane, WeightChunk& w) {
+  const int64_t at = (tile * p.chunks + chunk) * 64 + lane;
+  w.codes = *(const i32x4*)(p.codes + at * 16);
+  w.sc = p.scale[at];
+}
+// The weights of one chunk as operands.
+template <int XT>
+struct Operand {
+  i32x4 a[XT == kRowsFp8 ? 1 : 4];
+  int sc;
+};
+template <int XT>
+__device__ __forceinline__ void widen(const WeightChunk& w, int up, Operand<XT>& o) {
+  if constexpr (XT == kRowsFp8) {
+    o.a[0] = w.codes;
+    o.sc = w.sc;
+  } else if constexpr (XT == kRowsBf16) {
+    const float sc = __uint_as_float((uint32_t)w.sc << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = w.codes[j];
+      o.a[j] = i32x4{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 0)),
+                     __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 1)),
+                     __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 2)),
+                     __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3))};
+    }
+  } else {
+    // up = 138 - the row's largest byte: that one becomes 2^11; 255 stays (a NaN)
+    const int e = w.sc == 255 ? 255 : w.sc + up > 1 ? w.sc + up : 1;
+    const float sc = __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = w.codes[j];
+      o.a[j] = i32x4{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 0)),
+                     __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 1)),
+                     __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 2)),
+                     __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, sc, 3))};
+    }
+  }
+}
+template <int XT>
+__device__ __forceinline__ f32x4 multiply(const Operand<XT>& w, const uint8_t* tile, int x_sc, int g, int i, f32x4 acc) {
+  if constexpr (XT == kRowsFp8) {
+    const i32x4 lo = read_piece<XT>(tile, 0, g, i), hi = read_piece<XT>(tile, 1, g, i);
+    const i32x8 a = {w.a[0][0], w.a[0][1], w.a[0][2], w.a[0][3], 0, 0, 0, 0};
+    const i32x8 b = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 0, 0, w.sc, 0, x_sc);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const i32x4 b = read_piece<XT>(tile, j, g, i);
+      if constexpr (XT == kRowsBf16)
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.a[j]), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+      else
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.a[j]), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+    }
+    return acc;
+  }
+}
+
+// Four outputs n .. n + 3 of a row.
+__device__ __forceinline__ void store_outputs(const LinearParams& p, int row, int n, f32x4 v) {
+  if (row >= p.tokens || n >= p.n) return;
+  uint16_t* dst = (uint16_t*)(p.y + row * p.y_st) + n;
+  float x[8] = {v[0], v[1], v[2], v[3], 0.f, 0.f, 0.f, 0.f};
+  const i32x4 w = p.y_f16 ? pack<F16>(x) : pack<Bf16>(x);
+  if (p.y_vec && n + 4 <= p.n) {
+    *(i32x2*)dst = i32x2{w[0], w[1]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.n) dst[j] = (uint16_t)((uint32_t)w[j >> 1] >> (16 * (j & 1)));
+  }
+}
+// fp16 rows: back from the scales that the products were made with.
+template <int XT>
+__device__ __forceinline__ f32x4 scale_back(const LinearParams& p, int n, f32x4 v) {
+  if constexpr (XT == kRowsF16)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __builtin_ldexpf(v[j], (int)p.top[n + j] - 138);
+  return v;
+}
+
+// Up to 16 rows.  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no barrier in the loop),
+// weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.
+template <int XT, int WK>
+__global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void mla_linear_few_kernel(LinearParams p) {
+  constexpr int WN = WK == 1 ? 4 : 1, kDepth = WK == 16 ? 2 : 4;  // of registers for 16 waves there are half
+  __shared__ __attribute__((aligned(16))) uint8_t x_sh[WN * WK][kTileX<XT>];
+  __shared__ f32x4 sum_sh[WK][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, i = lane & 15;
+  const int wk = WK == 1 ? 0 : wave;
+  const int64_t tile = (int64_t)blockIdx.x * WN + (WK == 1 ? wave : 0);
+  if (WK == 1 && tile >= p.tiles) return;
+  uint8_t* xt = x_sh[wave];
+  const int up = XT == kRowsF16 ? 138 - (int)p.top[tile * 16 + i] : 0;
+  WeightChunk w[kDepth];
+  RowsChunk<XT> x[kDepth];
+  auto fetch = [&](int chunk, int s) __attribute__((always_inline)) {
+    const int c = chunk < p.chunks ? chunk : p.chunks - 1;  // past the end: the last one again, not used
+    load_weights(p, tile, c, lane, w[s]);
+    load_rows<XT>(p, 0, c, lane, x[s]);
+  };
+#pragma unroll
+  for (int s = 0; s < kDepth; ++s) fetch(wk + s * WK, s);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int c0 = wk; c0 < p.chunks; c0 += kDepth * WK) {
+#pragma unroll
+    for (int s = 0; s < kDepth; ++s) {
+      const int c = c0 + s * WK;
+      if (c >= p.chunks) break;  // uniform
+      Operand<XT> o;
+      widen<XT>(w[s], up, o);
+      put_rows<XT>(xt, lane, x[s]);
+      const int x_sc = x[s].sc;
+      if (c + kDepth * WK < p.chunks) fetch(c + kDepth * WK, s);  // uniform
+      __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS runs its accesses in order
+      acc = multiply<XT>(o, xt, x_sc, g, i, acc);
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+  if constexpr (WK > 1) {
+    sum_sh[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int k = 1; k < WK; ++k) acc += sum_sh[k][lane];
+  }
+  const int n = (int)tile * 16 + 4 * g;
+  store_outputs(p, i, n, scale_back<XT>(p, n, acc));
+}
+
+// More rows: a workgroup takes 128 outputs (a wave 32) for 16 RT rows and a split of the chunks; the rows of kStep chunks
+// at a time go through LDS for all waves, the next ones on the way meanwhile.
+template <int XT, int RT>
+__global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p) {
+  constexpr int kStep = 2, NT = 2;
+  constexpr int kParts = kStep * RT;           // 16-row chunks of a step
+  constexpr int kMine = (kParts + 3) / 4;      // of a wave
+  __shared__ __attribute__((aligned(16))) uint8_t x_sh[2][kParts][kTileX<XT>];
+  __shared__ int sc_sh[2][kParts][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int g = lane >> 4, i = lane & 15;
+  const int first = blockIdx.z * 16 * RT;
+  const int c_begin = blockIdx.y * p.per_split;
+  const int c_end = c_begin + p.per_split < p.chunks ? c_begin + p.per_split : p.chunks;
+  int64_t tile[NT];
+  int up[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int64_t at = (int64_t)blockIdx.x * 8 + 2 * wave + t;
+    tile[t] = at < p.tiles ? at : p.tiles - 1;  // past the end: the last one again, not stored
+    up[t] = XT == kRowsF16 ? 138 - (int)p.top[tile[t] * 16 + i] : 0;
+  }
+  RowsChunk<XT> x[kMine];
+  WeightChunk w[2][kStep][NT];
+  auto fetch_rows = [&](int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int part = 4 * m + wave, chunk = c + part / RT;  // uniform
+      if (kParts % 4 == 0 || part < kParts) load_rows<XT>(p, first + 16 * (part % RT), chunk < c_end ? chunk : c_end - 1, lane, x[m]);
+    }
+  };
+  auto fetch_weights = [&](int c, WeightChunk (&v)[kStep][NT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < kStep; ++s)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) load_weights(p, tile[t], c + s < c_end ? c + s : c_end - 1, lane, v[s][t]);
+  };
+  f32x4 acc[NT][RT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+  fetch_rows(c_begin);
+  fetch_weights(c_begin, w[0]);
+  auto step = [&](int c, int b, WeightChunk (&now)[kStep][NT], WeightChunk (&next)[kStep][NT]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < kMine; ++m) {
+      const int part = 4 * m + wave;
+      if (kParts % 4 == 0 || part < kParts) {
+        put_rows<XT>(x_sh[b][part], lane, x[m]);
+        if constexpr (XT == kRowsFp8) sc_sh[b][part][lane] = x[m].sc;
+      }
+    }
+    if (c + kStep < c_end) {  // uniform
+      fetch_rows(c + kStep);
+      fetch_weights(c + kStep, next);
+    }
+    __syncthreads();  // a buffer is written again two steps on, behind the next step's barrier
+#pragma unroll
+    for (int s = 0; s < kStep; ++s) {
+      if (c + s >= c_end) break;  // uniform
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        Operand<XT> o;
+        widen<XT>(now[s][t], up[t], o);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int x_sc = XT == kRowsFp8 ? sc_sh[b][s * RT + r][lane] : 0;
+          acc[t][r] = multiply<XT>(o, x_sh[b][s * RT + r], x_sc, g, i, acc[t][r]);
+        }
+      }
+    }
+  };
+  for (int c = c_begin; c < c_end; c += 2 * kStep) {
+    step(c, 0, w[0], w[1]);
+    if (c + kStep < c_end) step(c + kStep, 1, w[1], w[0]);  // uniform
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if ((int64_t)blockIdx.x * 8 + 2 * wave + t >= p.tiles) continue;
+    const int n = (int)tile[t] * 16 + 4 * g;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = first + 16 * r + i;
+      const f32x4 v = scale_back<XT>(p, n, acc[t][r]);
+      if (p.part != nullptr) {  // uniform
+        if (row < p.tokens) *(f32x4*)(p.part + ((int64_t)blockIdx.y * p.tokens + row) * (16 * (int64_t)p.tiles) + n) = v;
+      } else {
+        store_outputs(p, row, n, v);
+      }
+    }
+  }
+}
+
+// The splits' sums, in order.
+__global__ __launch_bounds__(256) void mla_linear_sum_kernel(LinearParams p, int splits) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int quads = 4 * p.tiles;
+  const int row = (int)(at / quads), n = (int)(at % quads) * 4;
+  if (row >= p.tokens) return;
+  const int64_t stride = (int64_t)p.tokens * 16 * p.tiles;
+  const float* src = p.part + (int64_t)row * 16 * p.tiles + n;
+  f32x4 acc = *(const f32x4*)src;
+  for (int s = 1; s < splits; ++s) acc += *(const f32x4*)(src + s * stride);
+  store_outputs(p, row, n, acc);
+}
+
+// Splits of the chunks for more than 16 rows: as many workgroups as two to a CU, but four chunks each at least.
+static int linear_splits(int64_t tokens, int64_t tiles, int64_t chunks, int cus) {
+  if (tokens <= 16) return 1;
+  const int rt = tokens <= 32 ? 2 : 4;
+  const int64_t groups = (tiles + 7) / 8 * ((tokens + 16 * rt - 1) / (16 * rt));
+  int64_t s = 2 * cus / groups;
+  s = s < 1 ? 1 : s > 16 ? 16 : s;
+  const int64_t most = chunks / 4 > 1 ? chunks / 4 : 1;
+  return (int)(s < most ? s : most);
+}
+
+template <int XT>
+static void launch_linear(LinearParams p, int splits, int cus, hipStream_t st) {
+  if (p.tokens <= 16) {
+    const int wk = getenv("LIN_WK") ? atoi(getenv("LIN_WK")) : 4;
+    if (wk == 1)
+      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 1>), dim3((p.tiles + 3) / 4), dim3(256), 0, st, p);
+    else if (wk == 4)
+      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 4>), dim3(p.tiles), dim3(256), 0, st, p);
+    else if (wk == 8)
+      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 8>), dim3(p.tiles), dim3(512), 0, st, p);
+    else
+      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 16>), dim3(p.tiles), dim3(1024), 0, st, p);
+    return;
+  }
+  // whole steps of two chunks, so that the last split is the short one
+  p.per_split = (p.chunks + splits - 1) / splits;
+  p.per_split += p.per_split & 1;
+  splits = (p.chunks + p.per_split - 1) / p.per_split;
+  if (splits == 1) p.part = nullptr;
+  const int rt = p.tokens <= 32 ? 2 : 4;
+  const dim3 grid((p.tiles + 7) / 8, splits, (p.tokens + 16 * rt - 1) / (16 * rt));
+  if (rt == 2)
+    hipLaunchKernelGGL((mla_linear_rows_kernel<XT, 2>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((mla_linear_rows_kernel<XT, 4>), grid, dim3(256), 0, st, p);
+  if (splits > 1) {
+    const int64_t quads = (int64_t)p.tokens * 4 * p.tiles;
+    hipLaunchKernelGGL(mla_linear_sum_kernel, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, p, splits);
+  }
+}
+
 static bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
 static int refuse(const char* what, int code = MLA_ERR_INVALID) { return mla_srv::set_error(code, what); }
 static int launched(const char* what) {
@@ -332,6 +703,62 @@ int mla_rms_norm(const mla_rms_norm_args* a, void* stream) {
   else if (a->dtype == MLA_DTYPE_F16) launch_norm_type<F16>(k, vec, cus, st);
   else launch_norm_type<F32>(k, vec, cus, st);
   return launched("rms norm");
+}
+
+static bool linear_shape(int32_t tokens, int32_t n, int32_t k) {
+  return tokens >= 0 && tokens <= (1 << 20) && n >= 1 && n <= (1 << 22) && k >= 32 && k <= (1 << 22) && k % 32 == 0;
+}
+
+int64_t mla_linear_workspace_bytes(int32_t tokens, int32_t n, int32_t k) {
+  if (!linear_shape(tokens, n, k)) return 0;
+  const int64_t tiles = (n + 15) / 16, chunks = (k + 127) / 128;
+  const int splits = linear_splits(tokens, tiles, chunks, mla_srv::cu_count());
+  return splits > 1 ? (int64_t)splits * tokens * tiles * 64 : 0;
+}
+
+int mla_linear_fp4(const mla_linear_args* a, void* stream) {
+  if (!a) return refuse("args is NULL");
+  if (!linear_shape(a->tokens, a->n, a->k))
+    return refuse("tokens must be in [0, 2^20], n in [1, 2^22], k a multiple of 32 in [32, 2^22]");
+  if (a->y_dtype != MLA_DTYPE_BF16 && a->y_dtype != MLA_DTYPE_F16) return refuse("y_dtype must be MLA_DTYPE_BF16 or MLA_DTYPE_F16");
+  if (!a->x_scale && a->x_dtype != MLA_DTYPE_BF16 && a->x_dtype != MLA_DTYPE_F16)
+    return refuse("x_dtype must be MLA_DTYPE_BF16 or MLA_DTYPE_F16 (or 8-bit rows with x_scale)");
+  if (a->tokens == 0) return MLA_OK;
+  if (!a->x || !a->codes || !a->scale || !a->top || !a->y) return refuse("a required pointer is NULL");
+  if (!aligned(a->x, 16) || !aligned(a->codes, 16) || !aligned(a->y, 2)) return refuse("x and codes must be 16-byte aligned");
+  const int es = a->x_scale ? 1 : 2;
+  if (a->x_stride < 0 || a->x_stride * es % 16 || a->x_scale_stride < 0 || a->y_stride < 0)
+    return refuse("strides must be non-negative, x's a multiple of 16 bytes");
+  LinearParams k{};
+  k.x = (const uint8_t*)a->x;
+  k.x_scale = a->x_scale;
+  k.x_st = a->x_stride * es;
+  k.xs_st = a->x_scale_stride;
+  k.codes = (const uint8_t*)a->codes;
+  k.scale = a->scale;
+  k.top = a->top;
+  k.y = (uint8_t*)a->y;
+  k.y_st = a->y_stride * 2;
+  k.tokens = a->tokens;
+  k.n = a->n;
+  k.k = a->k;
+  k.tiles = (a->n + 15) / 16;
+  k.chunks = (a->k + 127) / 128;
+  k.y_f16 = a->y_dtype == MLA_DTYPE_F16;
+  k.y_vec = aligned(a->y, 8) && k.y_st % 8 == 0;
+  const int cus = mla_srv::cu_count();
+  const int splits = linear_splits(k.tokens, k.tiles, k.chunks, cus);
+  if (splits > 1) {
+    if (!a->workspace || a->workspace_bytes < mla_linear_workspace_bytes(a->tokens, a->n, a->k))
+      return refuse("workspace missing or smaller than mla_linear_workspace_bytes()", MLA_ERR_WORKSPACE);
+    if (!aligned(a->workspace, 16)) return refuse("workspace must be 16-byte aligned", MLA_ERR_WORKSPACE);
+    k.part = (float*)a->workspace;
+  }
+  const hipStream_t st = (hipStream_t)stream;
+  if (a->x_scale) launch_linear<kRowsFp8>(k, splits, cus, st);
+  else if (a->x_dtype == MLA_DTYPE_F16) launch_linear<kRowsF16>(k, splits, cus, st);
+  else launch_linear<kRowsBf16>(k, splits, cus, st);
+  return launched("linear");
 }
 
 }  // extern "C"

@@ -2,6 +2,9 @@
 
 * ``rms_norm(x, weight, eps, residual)``: the residual's addition and the root-mean-square norm, to rows in x's dtype or
   to 8-bit rows with scales (``Fp8Rows``).
+* ``linear_fp4(x, w)``: a projection of few rows, 16-bit or 8-bit ones, by 4-bit weights (``Fp4Weight``) that
+  ``quantize_w_fp4(w)`` makes from a matrix and ``pack_w_fp4(codes, scale)`` from codes at hand; ``mla_decode_absorbed``
+  takes one as its ``w_o``.
 
 Calls are queued on torch's current stream of the tensors' device, synchronise nothing, and can be captured in a HIP graph.
 The reference starts at rotated, projected inputs and has no counterpart of these.
@@ -9,6 +12,7 @@ The reference starts at rotated, projected inputs and has no counterpart of thes
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import struct
 from typing import NamedTuple, Optional, Tuple, Union
@@ -16,13 +20,14 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import _lib
-from ._lib import MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_DTYPE_F32, MlaRmsNormArgs
-from .api import _launch
+from ._lib import MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_DTYPE_F32, MlaLinearArgs, MlaRmsNormArgs
+from .api import _launch, _stream_ptr, _workspace
 from .serving import _apart_or_same, _require, _rows_meet
 
 _DTYPES = {torch.bfloat16: MLA_DTYPE_BF16, torch.float16: MLA_DTYPE_F16, torch.float32: MLA_DTYPE_F32}
 _NORM = struct.Struct("=6Q4q4ifi")
-assert _NORM.size == ctypes.sizeof(MlaRmsNormArgs)
+_LINEAR = struct.Struct("@6Q3q6iQq")
+assert _NORM.size == ctypes.sizeof(MlaRmsNormArgs) and _LINEAR.size == ctypes.sizeof(MlaLinearArgs)
 GROUP = 32  # dims that share a scale
 
 
@@ -146,3 +151,149 @@ def _norm_overlaps(x, residual, out, residual_out, rows, strides) -> None:
         if out.data_ptr() == residual_out.data_ptr() or not _apart_or_same(
                 out.data_ptr(), (y_t, 0), residual_out.data_ptr(), (h_t, 0), counts, D, es):
             raise ValueError("out and residual_out overlap")
+
+
+# ---------------------------------------------------------------------------------------
+# projections by 4-bit weights
+# ---------------------------------------------------------------------------------------
+class Fp4Weight(NamedTuple):
+    """Weights ``[n, k]`` in 4 bits, as ``linear_fp4`` reads them: ``codes`` uint8 ``[ceil(n / 16), ceil(k / 128), 64, 16]``
+    (OCP e2m1), ``scale`` uint8 ``[ceil(n / 16), ceil(k / 128), 64]`` (a power of two per output and 32 inputs) and ``top``
+    uint8 ``[16 * ceil(n / 16)]``, each output's largest scale.  Made by :func:`quantize_w_fp4` or :func:`pack_w_fp4`."""
+    codes: torch.Tensor
+    scale: torch.Tensor
+    top: torch.Tensor
+    n: int
+    k: int
+
+
+def pack_w_fp4(codes: torch.Tensor, scale: torch.Tensor) -> Fp4Weight:
+    """The weights ``codes`` uint8 ``[n, k / 2]`` (OCP e2m1, two a byte, the lower input in the low half) with ``scale`` uint8
+    ``[n, k / 32]`` (value ``e2m1(code) * 2**(scale - 127)``, bytes 1 .. 254, 0 taken as 1, 255 a NaN), laid out for the
+    matrix unit.  Done once per weight."""
+    if codes.dim() != 2 or scale.dim() != 2 or codes.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        raise ValueError("codes and scale must be 2-D uint8 tensors")
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    if n < 1 or k < GROUP or k % GROUP or scale.shape != (n, k // GROUP) or scale.device != codes.device:
+        raise ValueError(f"codes must be [n, k / 2] and scale [n, k / {GROUP}] on one device, k a multiple of {GROUP}")
+    tiles, chunks = -(-n // 16), -(-k // 128)
+    c = torch.zeros(16 * tiles, 64 * chunks, dtype=torch.uint8, device=codes.device)
+    c[:n, :k // 2] = codes
+    s = torch.full((16 * tiles, 4 * chunks), 127, dtype=torch.uint8, device=codes.device)
+    s[:n, :k // GROUP] = scale.clamp(min=1)
+    top = torch.where(s == 255, 1, s).amax(1)
+    return Fp4Weight(c.view(tiles, 16, chunks, 4, 16).permute(0, 2, 3, 1, 4).contiguous().view(tiles, chunks, 64, 16),
+                     s.view(tiles, 16, chunks, 4).permute(0, 2, 3, 1).contiguous().view(tiles, chunks, 64), top.contiguous(), n, k)
+
+
+def quantize_w_fp4(w: torch.Tensor) -> Fp4Weight:
+    """A weight matrix ``[n, k]`` (any float type, k a multiple of 32) in 4 bits: per output and 32 inputs the smallest power
+    of two that brings them to 6 at most, values to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6, ties to the even code, as
+    the 4-bit cache holds its latents (a block with a NaN or an infinity becomes NaN).  Done once per weight."""
+    if w.dim() != 2 or not w.is_floating_point() or w.shape[0] < 1 or w.shape[1] < GROUP or w.shape[1] % GROUP:
+        raise ValueError(f"w must be a float [n, k] tensor, k a multiple of {GROUP}")
+    parts = [_to_fp4(p) for p in w.split(4096)]
+    return pack_w_fp4(torch.cat([c for c, _ in parts]), torch.cat([s for _, s in parts]))
+
+
+def _to_fp4(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``(codes [n, k / 2], scale bytes [n, k / 32])`` of float rows."""
+    b = w.float().unflatten(-1, (-1, GROUP))
+    amax = b.abs().amax(-1)
+    bad = ~torch.isfinite(amax)
+    b = torch.where(bad[..., None], 0, b.clamp(-1.5 * 2.0 ** 127, 1.5 * 2.0 ** 127))
+    m, e = torch.frexp(b.abs().amax(-1))  # amax = m * 2^e, m in [0.5, 1); 6 = 0.75 * 2^3
+    k = torch.where(m == 0, torch.zeros_like(e), torch.where(m <= 0.75, e - 3, e - 2).clamp(-126, 127))
+    v = torch.ldexp(b, -k[..., None])
+    a = v.abs()
+    n = (a > 0.25).to(torch.uint8) + (a >= 0.75) + (a > 1.25) + (a >= 1.75) + (a > 2.5) + (a >= 3.5) + (a > 5)
+    n = (n | torch.signbit(v).to(torch.uint8) << 3).flatten(-2).unflatten(-1, (-1, 2))
+    return n[..., 0] | n[..., 1] << 4, torch.where(bad, 255, k + 127).to(torch.uint8)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_workspace(tokens: int, n: int, k: int) -> int:
+    return _lib.load().mla_linear_workspace_bytes(tokens, n, k)
+
+
+def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torch.Tensor] = None,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``y [..., n] = x [..., k] . w^T`` for few rows: decode steps, drafted tokens.
+
+    ``x`` in bf16 or fp16, or :class:`Fp8Rows` (from :func:`rms_norm`).  Sums are fp32, rounded once to ``dtype`` (bf16 or
+    fp16; x's by default, bf16 of 8-bit rows).  bf16 and 8-bit rows take the weights exactly; with fp16 rows weights
+    below ``2**-35`` of the largest of their output are lost.  The leading dims must be one stride apart; rows that do not
+    start on 16 bytes are copied first.  ``out`` (unit stride in its rows) may not overlap ``x``.  The weights are read
+    once for up to 64 rows, so a few rows cost what one does; it takes any number."""
+    coded = isinstance(x, Fp8Rows)
+    rows = x.codes if coded else x
+    index = rows.get_device()
+    if index < 0:
+        _require(rows, "x")
+    device, shape, n, k = rows.device, rows.shape, w.n, w.k
+    if len(shape) < 2 or shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}]")
+    if coded:
+        if rows.dtype not in (torch.uint8, torch.float8_e4m3fn):
+            raise ValueError("8-bit rows have uint8 (or float8_e4m3fn) codes")
+        kind = MLA_DTYPE_BF16
+        if dtype is None:
+            dtype = torch.bfloat16 if out is None else out.dtype
+    else:
+        kind = _DTYPES.get(rows.dtype)
+        if kind is None or kind == MLA_DTYPE_F32:
+            raise ValueError("x must be bfloat16 or float16, or 8-bit rows")
+        if dtype is None:
+            dtype = rows.dtype if out is None else out.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError("dtype must be bfloat16 or float16")
+    codes, scale, top = w.codes, w.scale, w.top
+    tiles, chunks = -(-n // 16), -(-k // 128)
+    for t, name, want in ((codes, "w.codes", (tiles, chunks, 64, 16)), (scale, "w.scale", (tiles, chunks, 64)), (top, "w.top", (16 * tiles,))):
+        if t.get_device() != index:
+            _require(t, name, device)
+        if t.dtype is not torch.uint8 or t.shape != want or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous uint8 {list(want)} tensor (see pack_w_fp4)")
+    if codes.data_ptr() % 16:
+        raise ValueError("w.codes must be 16-byte aligned")
+    at = _token_rows(rows)
+    if at is None or rows.stride(-1) != 1:
+        raise ValueError("x must have unit stride in its rows and token dims one stride apart")
+    tokens, x_t = at
+    size = rows.element_size()
+    if rows.data_ptr() % 16 or x_t * size % 16:
+        rows = rows.contiguous().clone()
+        x_t = k
+    s_ptr, s_t = 0, 0
+    if coded:
+        xs = x.scale
+        if xs.get_device() != index:
+            _require(xs, "x.scale", device)
+        s_at = _token_rows(xs)
+        if xs.dtype is not torch.uint8 or xs.shape != (*shape[:-1], k // GROUP) or s_at is None or (k > GROUP and xs.stride(-1) != 1):
+            raise ValueError(f"x.scale must be a uint8 [..., {k // GROUP}] tensor with unit stride in its rows")
+        s_ptr, s_t = xs.data_ptr(), s_at[1]
+    if out is None:
+        y, y_t = torch.empty(*shape[:-1], n, dtype=dtype, device=device), n
+    else:
+        y = out
+        if y.get_device() != index:
+            _require(y, "out", device)
+        y_at = _token_rows(y)
+        if y.shape != (*shape[:-1], n) or y.dtype is not dtype or y_at is None or (n > 1 and y.stride(-1) != 1):
+            raise ValueError(f"out must be a {dtype} [..., {n}] tensor with unit stride in its rows")
+        y_t = y_at[1]
+        if tokens and _rows_meet((y_t, 0), (tokens, 1), n):
+            raise ValueError("out's rows overlap")
+        y_ptr, x_ptr = y.data_ptr(), rows.data_ptr()
+        if tokens and y_ptr < x_ptr + size * ((tokens - 1) * x_t + k) and x_ptr < y_ptr + 2 * ((tokens - 1) * y_t + n):
+            raise ValueError("out overlaps x")
+    need = _linear_workspace(tokens, n, k)
+    ws_ptr = ws = 0
+    if need:
+        _, ws_ptr, ws = _workspace(device, _stream_ptr(device), need)
+    a = MlaLinearArgs.from_buffer_copy(_LINEAR.pack(
+        rows.data_ptr(), s_ptr, codes.data_ptr(), scale.data_ptr(), top.data_ptr(), y.data_ptr(), x_t, s_t, y_t,
+        tokens, n, k, kind, _DTYPES[dtype], 0, ws_ptr, ws))
+    _launch("mla_linear_fp4", _lib.load().mla_linear_fp4, device, ctypes.byref(a))
+    return y

@@ -232,3 +232,244 @@ def test_norm_in_a_graph(gpu):
             side.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(res, want))
             f()
+
+
+# ---------------------------------------------------------------------------------------
+# projections by 4-bit weights
+# ---------------------------------------------------------------------------------------
+E2M1 = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
+
+
+def weights(n, k, seed, spread=8, bias=-4):
+    """(codes, scale, values in 64 bits): random codes, scales 2^(bias - spread .. bias + spread)."""
+    g = torch.Generator().manual_seed(seed)
+    c = torch.randint(0, 16, (n, k), generator=g)
+    s = torch.randint(127 + bias - spread, 128 + bias + spread, (n, k // 32), generator=g)
+    v = E2M1[c] * torch.exp2(s.double() - 127).repeat_interleave(32, 1)
+    return (c[:, 0::2] | c[:, 1::2] << 4).to(torch.uint8), s.to(torch.uint8), v
+
+
+def rows_of(kind, T, k, seed):
+    """(what linear_fp4 takes, its values in 64 bits)."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, k, generator=g) * torch.exp2(torch.randint(-3, 4, (T, 1), generator=g).float())
+    if kind != "fp8":
+        x = x.to(DT[kind])
+        return x.cuda(), x.double()
+    s = torch.randint(120, 130, (T, k // 32), generator=g)
+    codes = x.clamp(-448, 448).to(torch.float8_e4m3fn)
+    return M.Fp8Rows(codes.view(torch.uint8).cuda(), s.to(torch.uint8).cuda()), codes.double() * torch.exp2(s.double() - 127).repeat_interleave(32, 1)
+
+
+def check_linear(got, x, w, kind, what):
+    """Products are exact; their sum is of k terms in fp32, whatever the order, below k 2^-24 of the sum of their sizes.  The
+    block-scaled MFMA (8-bit rows) may drop what lies 13 bits below the largest product of each group of eight: 8 times
+    2^-13 of that largest at most, 2^-10 of the sum of sizes.  fp16 rows: weights below 2^-35 of their output's largest
+    vanish, those near it round, each by 2^-36 of it.  Then one rounding, and half a smallest step of fp16."""
+    y, size = x @ w.T, x.abs() @ w.abs().T
+    slack = x.shape[1] * 2.0 ** -24 + (2.0 ** -10 if kind == "fp8" else 0.0)
+    tol = EPS[got.dtype] * (1 + slack) * y.abs() + slack * size
+    if kind == "f16":
+        tol = tol + 2.0 ** -36 * x.abs().sum(1, keepdim=True) * 2 * w.abs().amax(1)
+    if got.dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    off = ((got.double().cpu() - y).abs() / tol.clamp(min=1e-300)).max().item()
+    say(f"{what}: {off:.3f} of the bound, {((got.double().cpu() - y).norm() / y.norm()).item():.2e} off")
+    assert off <= 1, what
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8"])
+@pytest.mark.parametrize("n,k", [(1, 32), (5, 64), (16, 96), (17, 128), (100, 160), (40, 544), (576, 1536), (130, 4128), (1000, 2048)])
+def test_linear(gpu, n, k, kind):
+    codes, scale, w = weights(n, k, n + k, spread=3 if kind == "f16" else 8)
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    for T in (1, 2, 7, 15, 16, 17, 32, 33, 64, 65, 130):
+        x, xv = rows_of(kind, T, k, T)
+        say(f"linear {kind} T={T} n={n} k={k}")
+        got = M.linear_fp4(x, p)
+        torch.cuda.synchronize()
+        assert got.shape == (T, n) and got.dtype == (torch.float16 if kind == "f16" else torch.bfloat16)
+        check_linear(got, xv, w, kind, f"{kind} T={T} n={n} k={k}")
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8"])
+def test_linear_large(gpu, kind):
+    """Many chunks a wave, every number of splits, more rows than a workgroup takes."""
+    for T, n, k in ((3, 2064, 16384), (64, 528, 16384), (40, 2048, 7168), (300, 1040, 1024), (64, 7168, 512)):
+        codes, scale, w = weights(n, k, 3, spread=2)
+        x, xv = rows_of(kind, T, k, 5)
+        say(f"linear large {kind} {T} {n} {k}")
+        got = M.linear_fp4(x, M.pack_w_fp4(codes.cuda(), scale.cuda()))
+        torch.cuda.synchronize()
+        check_linear(got, xv, w, kind, f"large {kind} {T} {n} {k}")
+
+
+def test_linear_one_hot(gpu):
+    """Every weight in its place: rows that pick one input each give the weights back exactly."""
+    n, k = 50, 416
+    codes, scale, w = weights(n, k, 9, spread=2)
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    eye = torch.eye(k, device="cuda")
+    say("one hot")
+    for x in (eye.bfloat16(), eye.half(), M.Fp8Rows(eye.to(torch.float8_e4m3fn).view(torch.uint8), torch.full((k, k // 32), 127, dtype=torch.uint8, device="cuda"))):
+        for a in range(0, k, 16):
+            part = M.Fp8Rows(x.codes[a:a + 16], x.scale[a:a + 16]) if isinstance(x, M.Fp8Rows) else x[a:a + 16]
+            assert torch.equal(M.linear_fp4(part, p).double().cpu(), w.T[a:a + 16])
+        assert torch.equal(M.linear_fp4(x, p).double().cpu(), w.T)
+
+
+def test_linear_scales_and_special_values(gpu):
+    """Scales over the type's whole range (bf16 and 8-bit rows), outputs of very different size (fp16 rows), NaN blocks,
+    infinities in the rows, zeros."""
+    n, k = 32, 256
+    codes, _, _ = weights(n, k, 11)
+    scale = torch.arange(n * 8, dtype=torch.int32).view(n, 8) % 200 + 20
+    c = torch.stack([codes & 15, codes >> 4], -1).flatten(1).long()
+    w = E2M1[c] * torch.exp2(scale.double() - 127).repeat_interleave(32, 1)
+    p = M.pack_w_fp4(codes.cuda(), scale.to(torch.uint8).cuda())
+    for kind in ("bf16", "fp8"):
+        x, xv = rows_of(kind, 5, k, 1)
+        got = M.linear_fp4(x, p)
+        torch.cuda.synchronize()
+        check_linear(got, xv, w, kind, f"scales {kind}")
+    rows = torch.arange(n, dtype=torch.int32)[:, None].expand(n, 8) % 30 + 100  # each output at a size of its own
+    w = E2M1[c] * torch.exp2(rows.double() - 127).repeat_interleave(32, 1)
+    x, xv = rows_of("f16", 4, k, 2)
+    got = M.linear_fp4(x * 2.0 ** -6, M.pack_w_fp4(codes.cuda(), rows.to(torch.uint8).cuda()), dtype=torch.bfloat16)
+    check_linear(got, xv * 2.0 ** -6, w, "f16", "sizes f16")
+    scale = torch.full((n, 8), 120, dtype=torch.uint8)
+    scale[7, 3] = 255
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    for kind in ("bf16", "f16", "fp8"):
+        for T in (2, 20):
+            x, _ = rows_of(kind, T, k, 3)
+            got = M.linear_fp4(x, p)
+            torch.cuda.synchronize()
+            assert torch.isnan(got[:, 7]).all() and torch.isfinite(got[:, :7]).all() and torch.isfinite(got[:, 8:]).all(), kind
+    x = torch.zeros(3, k, dtype=torch.bfloat16, device="cuda")
+    x[1, 40], x[2, 41] = float("nan"), float("inf")
+    scale[7, 3] = 120
+    got = M.linear_fp4(x, M.pack_w_fp4(codes.cuda(), scale.cuda()))
+    torch.cuda.synchronize()
+    assert (got[0] == 0).all() and torch.isnan(got[1]).all() and not torch.isfinite(got[2]).any()  # inf * 0 is a NaN
+    nan8 = M.Fp8Rows(torch.zeros(2, k, dtype=torch.uint8, device="cuda"), torch.full((2, k // 32), 127, dtype=torch.uint8, device="cuda"))
+    nan8.scale[1, 2], nan8.codes[1, 64:96] = 255, 0x7F
+    got = M.linear_fp4(nan8, p)
+    torch.cuda.synchronize()
+    assert torch.isnan(got[1]).all() and (got[0, torch.arange(n, device="cuda") != 7] == 0).all()
+
+
+@pytest.mark.parametrize("T", [3, 40])
+def test_linear_strides_and_shapes(gpu, T):
+    n, k = 100, 512
+    codes, scale, w = weights(n, k, 13)
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    x, xv = rows_of("bf16", T, k, 1)
+    want = M.linear_fp4(x, p)
+    say(f"strides T={T}")
+    wide = torch.zeros(T, 600, dtype=torch.bfloat16, device="cuda")
+    for at in (8, 3):  # rows on 16 bytes, and not
+        wide[:, at:at + k] = x
+        assert torch.equal(M.linear_fp4(wide[:, at:at + k], p), want)
+    odd = torch.zeros(T, 601, dtype=torch.bfloat16, device="cuda")[:, :k]
+    odd.copy_(x)
+    assert torch.equal(M.linear_fp4(odd, p), want)
+    assert torch.equal(M.linear_fp4(x.view(1, T, 1, k), p), want.view(1, T, 1, n))
+    buf = torch.full((T, 131), 3.0, dtype=torch.bfloat16, device="cuda")
+    for at in (4, 1):
+        buf.fill_(3.0)
+        out = buf[:, at:at + n]
+        assert M.linear_fp4(x, p, out=out) is out and torch.equal(out, want)
+        assert (buf[:, :at] == 3).all() and (buf[:, at + n:] == 3).all()
+    h = M.linear_fp4(x, p, dtype=torch.float16)
+    check_linear(h, xv, w, "bf16", "to f16")
+    assert M.linear_fp4(x[:0], p).shape == (0, n)
+    r, rv = rows_of("fp8", T, k, 2)
+    side = M.Fp8Rows(torch.zeros(T, 1024, dtype=torch.uint8, device="cuda")[:, 16:16 + k], torch.zeros(T, 40, dtype=torch.uint8, device="cuda")[:, 3:3 + k // 32])
+    side.codes.copy_(r.codes), side.scale.copy_(r.scale)
+    assert torch.equal(M.linear_fp4(side, p), M.linear_fp4(r, p))
+    off = M.Fp8Rows(torch.zeros(T, k + 8, dtype=torch.uint8, device="cuda")[:, 8:], r.scale)
+    off.codes.copy_(r.codes)
+    assert torch.equal(M.linear_fp4(off, p), M.linear_fp4(r, p))
+    one = x[:1].expand(T, k)
+    assert torch.equal(M.linear_fp4(one, p)[0], M.linear_fp4(one, p)[-1])
+
+
+def test_linear_refusals(gpu):
+    say("linear refusals")
+    codes, scale, _ = weights(20, 128, 1)
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    x = torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")
+    r = M.Fp8Rows(torch.zeros(4, 128, dtype=torch.uint8, device="cuda"), torch.zeros(4, 4, dtype=torch.uint8, device="cuda"))
+    buf = torch.zeros(4 * 128 + 200, dtype=torch.bfloat16, device="cuda")
+    for args, kw in [((x.float(), p), {}), ((x[:, :96], p), {}), ((x[0], p), {}), ((x.t(), p), {}), ((x, p._replace(codes=p.codes[:1])), {}), ((x, p._replace(top=p.top.cpu())), {}),
+                     ((x, p._replace(n=40)), {}), ((x, p), dict(dtype=torch.float32)), ((x, p), dict(out=torch.zeros(4, 21, dtype=x.dtype, device="cuda"))),
+                     ((x, p), dict(out=torch.zeros(4, 20, dtype=torch.float16, device="cuda"), dtype=torch.bfloat16)), ((r._replace(scale=r.scale[:, :3]), p), {}),
+                     ((r._replace(scale=r.scale.int()), p), {}), ((r._replace(codes=r.codes.int()), p), {}), ((x, p), dict(out=buf[:80].view(4, 20).expand(4, 20)[:1].expand(4, 20))),
+                     ((buf[:512].view(4, 128), p), dict(out=buf[480:560].view(4, 20))), ((x.expand(2, 4, 128).transpose(0, 1), p), {})]:
+        with pytest.raises(ValueError):
+            M.linear_fp4(*args, **kw)
+
+
+def test_linear_streams_and_graphs(gpu):
+    """Two captured calls that share a stream's workspace, replayed in turns, and two streams at once."""
+    k, n, T = 8192, 512, 64
+    codes, scale, _ = weights(n, k, 21)
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    xs = [rows_of("bf16", T, k, i)[0] for i in range(3)]
+    want = [M.linear_fp4(x, p) for x in xs]
+    torch.cuda.synchronize()
+    say("linear graphs")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert torch.equal(M.linear_fp4(xs[0], p), want[0])
+        graphs = []
+        for x in xs[:2]:
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                y = M.linear_fp4(x, p)
+            graphs.append((gr, y))
+        for _ in range(3):
+            for (gr, y), wt in zip(graphs, want):
+                y.zero_()
+                gr.replay()
+                assert torch.equal(M.linear_fp4(xs[2], p), want[2])
+                side.synchronize()
+                assert torch.equal(y, wt)
+    other = torch.cuda.Stream()
+    got = []
+    for i in range(6):
+        with torch.cuda.stream(side if i % 2 else other):
+            got.append(M.linear_fp4(xs[i % 3], p))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 3]) for i, y in enumerate(got))
+
+
+def test_norm_then_linear(gpu):
+    """The norm's 8-bit rows through a projection, against the same in 64 bits of what the rows hold; and the absorbed
+    decode's output projection by such weights."""
+    T, D, n = 9, 7168, 576
+    x, r, w = tensors(T, D, torch.bfloat16, D, 3)
+    codes, scale, wv = weights(n, D, 5, spread=2)
+    p = M.pack_w_fp4(codes.cuda(), scale.cuda())
+    say("norm then linear")
+    rows, _ = M.rms_norm(x, w.cuda(), residual=r, quantize=True)
+    y = M.linear_fp4(rows, p)
+    torch.cuda.synchronize()
+    check_linear(y, values8(rows).cpu(), wv, "fp8", "norm then linear")
+
+
+def test_absorbed_with_4bit_output_projection(gpu):
+    B, H, D = 3, 16, 320
+    g = torch.Generator().manual_seed(1)
+    kv = torch.randn(6, 64, 1, 576, generator=g).bfloat16().cuda()
+    table = torch.arange(6, dtype=torch.int32, device="cuda").view(B, 2)
+    lens = torch.tensor([100, 64, 7], dtype=torch.int32, device="cuda")
+    q = torch.randn(B, 1, H, 576, generator=g).bfloat16().cuda()
+    w_uv = M.prepare_w_uv((torch.randn(H, 512, 128, generator=g) * 512 ** -0.5).bfloat16().cuda())
+    w_o = M.quantize_w_fp4(torch.randn(D, H * 128, generator=g).cuda() * (H * 128) ** -0.5)
+    say("absorbed with w_o")
+    sched = M.get_mla_metadata(lens, H, 1)
+    v, _ = M.mla_decode_absorbed(q, kv, table, lens, *sched, w_uv)
+    y, _ = M.mla_decode_absorbed(q, kv, table, lens, *sched, w_uv, w_o)
+    assert y.shape == (B, 1, D) and torch.equal(y, M.linear_fp4(v.view(B, 1, H * 128), w_o))
