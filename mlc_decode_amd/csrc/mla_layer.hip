@@ -328,35 +328,48 @@ __device__ __forceinline__ i32x4 read_piece(const uint8_t* tile, int j, int g, i
   return *(const i32x4*)(tile + piece_place<XT>(p, i));
 }
 
-// Registers of a 16-row chunk by one wave: 64 / pieces rows a load.
-template <int XT>
+// Registers of the first LOADS * kEach rows of a 16-row chunk, by one wave.  Rows past the last are the last again: they are
+// columns of the product that nothing reads.
+template <int XT, int LOADS>
 struct RowsChunk {
-  static constexpr int kPieces = kChunkBytes<XT> / 16, kLoads = 16 * kPieces / 64;
-  i32x4 v[kLoads];
+  i32x4 v[LOADS];
   int sc;  // 8-bit rows: lane (g, i)'s scale byte
 };
 template <int XT>
-__device__ __forceinline__ void load_rows(const LinearParams& p, int first, int chunk, int lane, RowsChunk<XT>& c) {
-  constexpr int kPieces = RowsChunk<XT>::kPieces, kEach = 64 / kPieces;
+constexpr int kPieces = kChunkBytes<XT> / 16;  // of a row's chunk
+template <int XT>
+constexpr int kEach = 64 / kPieces<XT>;  // rows of a load
+template <int XT, int LOADS>
+__device__ __forceinline__ void load_rows(const LinearParams& p, int first, int chunk, int lane, RowsChunk<XT, LOADS>& c) {
+  const int piece = lane % kPieces<XT>;
+  const int most = p.k / (XT == kRowsFp8 ? 16 : 8) - 1;  // the last piece of a row
+  const int at = chunk * kPieces<XT> + piece;
+  const uint8_t* src = p.x + 16 * (int64_t)(at < most ? at : most);
 #pragma unroll
-  for (int q = 0; q < RowsChunk<XT>::kLoads; ++q) {
-    const int row = first + kEach * q + lane / kPieces, piece = lane % kPieces;
-    c.v[q] = i32x4{0, 0, 0, 0};
-    if (row < p.tokens && (chunk * kPieces + piece) * (XT == kRowsFp8 ? 16 : 8) < p.k)
-      c.v[q] = *(const i32x4*)(p.x + row * p.x_st + (int64_t)chunk * kChunkBytes<XT> + 16 * piece);
+  for (int q = 0; q < LOADS; ++q) {
+    int row = first + kEach<XT> * q + lane / kPieces<XT>;
+    row = row < p.tokens ? row : p.tokens - 1;
+    c.v[q] = *(const i32x4*)(src + row * p.x_st);
   }
   if constexpr (XT == kRowsFp8) {
-    const int row = first + (lane & 15), block = 4 * chunk + (lane >> 4);
-    c.sc = 127;
-    if (row < p.tokens && 32 * block < p.k) c.sc = p.x_scale[row * p.xs_st + block];
+    int row = first + (lane & 15), block = 4 * chunk + (lane >> 4);
+    row = row < p.tokens ? row : p.tokens - 1;
+    block = 32 * block < p.k ? block : p.k / 32 - 1;
+    c.sc = p.x_scale[row * p.xs_st + block];
   }
 }
-template <int XT>
-__device__ __forceinline__ void put_rows(uint8_t* tile, int lane, const RowsChunk<XT>& c) {
-  constexpr int kPieces = RowsChunk<XT>::kPieces, kEach = 64 / kPieces;
+// To LDS.  Pieces past the row's end are zeros (their weights are, but an infinity times 0 is a NaN).
+template <int XT, int LOADS>
+__device__ __forceinline__ void put_rows(const LinearParams& p, uint8_t* tile, int chunk, int lane, RowsChunk<XT, LOADS>& c) {
+  if (chunk * 128 + 128 > p.k) {  // uniform
+    if (chunk * 128 + lane % kPieces<XT> * (XT == kRowsFp8 ? 16 : 8) >= p.k)
 #pragma unroll
-  for (int q = 0; q < RowsChunk<XT>::kLoads; ++q)
-    *(i32x4*)(tile + piece_place<XT>(lane % kPieces, kEach * q + lane / kPieces)) = c.v[q];
+      for (int q = 0; q < LOADS; ++q) c.v[q] = i32x4{0, 0, 0, 0};
+    if (XT == kRowsFp8 && chunk * 128 + 32 * (lane >> 4) >= p.k) c.sc = 127;
+  }
+#pragma unroll
+  for (int q = 0; q < LOADS; ++q)
+    *(i32x4*)(tile + piece_place<XT>(lane % kPieces<XT>, kEach<XT> * q + lane / kPieces<XT>)) = c.v[q];
 }
 
 struct WeightChunk {
@@ -403,23 +416,29 @@ __device__ __forceinline__ void widen(const WeightChunk& w, int up, Operand<XT>&
     }
   }
 }
-template <int XT>
-__device__ __forceinline__ f32x4 multiply(const Operand<XT>& w, const uint8_t* tile, int x_sc, int g, int i, f32x4 acc) {
+// acc[t] += the weights of tile t times 16 rows of a chunk, each operand of the rows read once.
+template <int XT, int NT>
+__device__ __forceinline__ void multiply(const Operand<XT> (&w)[NT], const uint8_t* tile, int x_sc, int g, int i, f32x4 (&acc)[NT]) {
   if constexpr (XT == kRowsFp8) {
     const i32x4 lo = read_piece<XT>(tile, 0, g, i), hi = read_piece<XT>(tile, 1, g, i);
-    const i32x8 a = {w.a[0][0], w.a[0][1], w.a[0][2], w.a[0][3], 0, 0, 0, 0};
     const i32x8 b = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 4, 0, 0, w.sc, 0, x_sc);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const i32x8 a = {w[t].a[0][0], w[t].a[0][1], w[t].a[0][2], w[t].a[0][3], 0, 0, 0, 0};
+      acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], 4, 0, 0, w[t].sc, 0, x_sc);
+    }
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const i32x4 b = read_piece<XT>(tile, j, g, i);
-      if constexpr (XT == kRowsBf16)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.a[j]), __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
-      else
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.a[j]), __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (XT == kRowsBf16)
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[t].a[j]), __builtin_bit_cast(bf16x8, b), acc[t], 0, 0, 0);
+        else
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w[t].a[j]), __builtin_bit_cast(f16x8, b), acc[t], 0, 0, 0);
+      }
     }
-    return acc;
   }
 }
 
@@ -446,54 +465,52 @@ __device__ __forceinline__ f32x4 scale_back(const LinearParams& p, int n, f32x4 
   return v;
 }
 
-// Up to 16 rows.  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no barrier in the loop),
-// weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.
-template <int XT, int WK>
-__global__ __launch_bounds__(WK == 1 ? 256 : 64 * WK) void mla_linear_few_kernel(LinearParams p) {
-  constexpr int WN = WK == 1 ? 4 : 1, kDepth = WK == 16 ? 2 : 4;  // of registers for 16 waves there are half
-  __shared__ __attribute__((aligned(16))) uint8_t x_sh[WN * WK][kTileX<XT>];
+// Up to 16 rows (LOADS * kEach).  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no
+// barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.
+template <int XT, int LOADS, int WK>
+__global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p) {
+  constexpr int kDepth = LOADS == 4 && WK >= 8 ? 2 : 4;  // 128 registers: two workgroups of 8 waves a CU
+  __shared__ __attribute__((aligned(16))) uint8_t x_sh[WK][2][kTileX<XT>];
   __shared__ f32x4 sum_sh[WK][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, i = lane & 15;
-  const int wk = WK == 1 ? 0 : wave;
-  const int64_t tile = (int64_t)blockIdx.x * WN + (WK == 1 ? wave : 0);
-  if (WK == 1 && tile >= p.tiles) return;
-  uint8_t* xt = x_sh[wave];
-  const int up = XT == kRowsF16 ? 138 - (int)p.top[tile * 16 + i] : 0;
+  const int64_t tile = blockIdx.x;
   WeightChunk w[kDepth];
-  RowsChunk<XT> x[kDepth];
-  auto fetch = [&](int chunk, int s) __attribute__((always_inline)) {
-    const int c = chunk < p.chunks ? chunk : p.chunks - 1;  // past the end: the last one again, not used
-    load_weights(p, tile, c, lane, w[s]);
-    load_rows<XT>(p, 0, c, lane, x[s]);
+  RowsChunk<XT, LOADS> x[kDepth];
+  auto fetch = [&](int c, int s) __attribute__((always_inline)) {
+    if (c < p.chunks) {  // uniform
+      load_weights(p, tile, c, lane, w[s]);
+      load_rows<XT, LOADS>(p, 0, c, lane, x[s]);
+    }
   };
 #pragma unroll
-  for (int s = 0; s < kDepth; ++s) fetch(wk + s * WK, s);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = wk; c0 < p.chunks; c0 += kDepth * WK) {
+  for (int s = 0; s < kDepth; ++s) fetch(wave + s * WK, s);
+  const int up = XT == kRowsF16 ? 138 - (int)p.top[tile * 16 + i] : 0;
+  f32x4 acc[2][1] = {{{0.f, 0.f, 0.f, 0.f}}, {{0.f, 0.f, 0.f, 0.f}}};
+  for (int c0 = wave; c0 < p.chunks; c0 += kDepth * WK) {
 #pragma unroll
     for (int s = 0; s < kDepth; ++s) {
       const int c = c0 + s * WK;
-      if (c >= p.chunks) break;  // uniform
-      Operand<XT> o;
-      widen<XT>(w[s], up, o);
-      put_rows<XT>(xt, lane, x[s]);
-      const int x_sc = x[s].sc;
-      if (c + kDepth * WK < p.chunks) fetch(c + kDepth * WK, s);  // uniform
-      __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS runs its accesses in order
-      acc = multiply<XT>(o, xt, x_sc, g, i, acc);
-      __builtin_amdgcn_wave_barrier();
+      if (c < p.chunks) {  // uniform
+        uint8_t* xt = x_sh[wave][s & 1];
+        Operand<XT> o[1];
+        put_rows<XT, LOADS>(p, xt, c, lane, x[s]);
+        widen<XT>(w[s], up, o[0]);
+        const int x_sc = x[s].sc;
+        fetch(c + kDepth * WK, s);
+        __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS runs its accesses in order
+        multiply<XT, 1>(o, xt, x_sc, g, i, acc[s & 1]);
+      }
     }
   }
-  if constexpr (WK > 1) {
-    sum_sh[wave][lane] = acc;
-    __syncthreads();
-    if (wave != 0) return;
+  f32x4 sum = acc[0][0] + acc[1][0];
+  sum_sh[wave][lane] = sum;
+  __syncthreads();
+  if (wave != 0) return;
 #pragma unroll
-    for (int k = 1; k < WK; ++k) acc += sum_sh[k][lane];
-  }
+  for (int k = 1; k < WK; ++k) sum += sum_sh[k][lane];
   const int n = (int)tile * 16 + 4 * g;
-  store_outputs(p, i, n, scale_back<XT>(p, n, acc));
+  store_outputs(p, i, n, scale_back<XT>(p, n, sum));
 }
 
 // More rows: a workgroup takes 128 outputs (a wave 32) for 16 RT rows and a split of the chunks; the rows of kStep chunks
@@ -518,13 +535,14 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
     tile[t] = at < p.tiles ? at : p.tiles - 1;  // past the end: the last one again, not stored
     up[t] = XT == kRowsF16 ? 138 - (int)p.top[tile[t] * 16 + i] : 0;
   }
-  RowsChunk<XT> x[kMine];
+  constexpr int kLoads = 16 / kEach<XT>;
+  RowsChunk<XT, kLoads> x[kMine];
   WeightChunk w[2][kStep][NT];
   auto fetch_rows = [&](int c) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       const int part = 4 * m + wave, chunk = c + part / RT;  // uniform
-      if (kParts % 4 == 0 || part < kParts) load_rows<XT>(p, first + 16 * (part % RT), chunk < c_end ? chunk : c_end - 1, lane, x[m]);
+      if (kParts % 4 == 0 || part < kParts) load_rows<XT, kLoads>(p, first + 16 * (part % RT), chunk < c_end ? chunk : c_end - 1, lane, x[m]);
     }
   };
   auto fetch_weights = [&](int c, WeightChunk (&v)[kStep][NT]) __attribute__((always_inline)) {
@@ -533,11 +551,11 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
 #pragma unroll
       for (int t = 0; t < NT; ++t) load_weights(p, tile[t], c + s < c_end ? c + s : c_end - 1, lane, v[s][t]);
   };
-  f32x4 acc[NT][RT];
+  f32x4 acc[RT][NT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int r = 0; r < RT; ++r) acc[t][r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   fetch_rows(c_begin);
   fetch_weights(c_begin, w[0]);
   auto step = [&](int c, int b, WeightChunk (&now)[kStep][NT], WeightChunk (&next)[kStep][NT]) __attribute__((always_inline)) {
@@ -545,7 +563,7 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
     for (int m = 0; m < kMine; ++m) {
       const int part = 4 * m + wave;
       if (kParts % 4 == 0 || part < kParts) {
-        put_rows<XT>(x_sh[b][part], lane, x[m]);
+        put_rows<XT, kLoads>(p, x_sh[b][part], c + part / RT, lane, x[m]);
         if constexpr (XT == kRowsFp8) sc_sh[b][part][lane] = x[m].sc;
       }
     }
@@ -557,16 +575,12 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
 #pragma unroll
     for (int s = 0; s < kStep; ++s) {
       if (c + s >= c_end) break;  // uniform
+      Operand<XT> o[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        Operand<XT> o;
-        widen<XT>(now[s][t], up[t], o);
+      for (int t = 0; t < NT; ++t) widen<XT>(now[s][t], up[t], o[t]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int x_sc = XT == kRowsFp8 ? sc_sh[b][s * RT + r][lane] : 0;
-          acc[t][r] = multiply<XT>(o, x_sh[b][s * RT + r], x_sc, g, i, acc[t][r]);
-        }
-      }
+      for (int r = 0; r < RT; ++r)
+        multiply<XT, NT>(o, x_sh[b][s * RT + r], XT == kRowsFp8 ? sc_sh[b][s * RT + r][lane] : 0, g, i, acc[r]);
     }
   };
   for (int c = c_begin; c < c_end; c += 2 * kStep) {
@@ -580,7 +594,7 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int row = first + 16 * r + i;
-      const f32x4 v = scale_back<XT>(p, n, acc[t][r]);
+      const f32x4 v = scale_back<XT>(p, n, acc[r][t]);
       if (p.part != nullptr) {  // uniform
         if (row < p.tokens) *(f32x4*)(p.part + ((int64_t)blockIdx.y * p.tokens + row) * (16 * (int64_t)p.tiles) + n) = v;
       } else {
@@ -614,19 +628,27 @@ static int linear_splits(int64_t tokens, int64_t tiles, int64_t chunks, int cus)
   return (int)(s < most ? s : most);
 }
 
+// Waves that share a tile of 16 outputs; us for 4, 8, 16 of them (one bf16 row unless said):
+//   n x k  576 x 7168 5.0, 4.0, 4.0    2048 x 16384 13.2, 8.2, 6.7    4096 x 2048 3.0, 2.9, 3.1    8192 x 8192 9.3, 8.6, 10.1
+//   7168 x 16384 15.0, 12.3, 14.6 (16 rows 18.9, 17.8, 19.2)    12288 x 4096 (8 rows) 8.2, 8.3, 10.3    24576 x 1536 6.8, 7.6, 11.5
+//   32768 x 7168 25.9, 27.9, 33.2
+template <int XT, int LOADS>
+static void launch_few(const LinearParams& p, int cus, hipStream_t st) {
+  if (2 * (int64_t)p.tiles > 5 * (int64_t)cus)
+    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 4>), dim3(p.tiles), dim3(256), 0, st, p);
+  else if (2 * p.tiles <= cus && p.chunks >= 96)
+    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 16>), dim3(p.tiles), dim3(1024), 0, st, p);
+  else
+    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 8>), dim3(p.tiles), dim3(512), 0, st, p);
+}
+
 template <int XT>
 static void launch_linear(LinearParams p, int splits, int cus, hipStream_t st) {
   if (p.tokens <= 16) {
-    const int wk = getenv("LIN_WK") ? atoi(getenv("LIN_WK")) : 4;
-    if (wk == 1)
-      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 1>), dim3((p.tiles + 3) / 4), dim3(256), 0, st, p);
-    else if (wk == 4)
-      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 4>), dim3(p.tiles), dim3(256), 0, st, p);
-    else if (wk == 8)
-      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 8>), dim3(p.tiles), dim3(512), 0, st, p);
-    else
-      hipLaunchKernelGGL((mla_linear_few_kernel<XT, 16>), dim3(p.tiles), dim3(1024), 0, st, p);
-    return;
+    constexpr int kFew = kEach<XT>;  // rows of one load
+    if (p.tokens <= kFew) return launch_few<XT, 1>(p, cus, st);
+    if (p.tokens <= 2 * kFew) return launch_few<XT, 2>(p, cus, st);
+    if constexpr (4 * kFew <= 16) return launch_few<XT, 4>(p, cus, st);
   }
   // whole steps of two chunks, so that the last split is the short one
   p.per_split = (p.chunks + splits - 1) / splits;
