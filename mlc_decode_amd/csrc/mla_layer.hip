@@ -465,7 +465,7 @@ __device__ __forceinline__ f32x4 scale_back(const LinearParams& p, int n, f32x4 
   return v;
 }
 
-// Up to 16 rows (LOADS * kEach).  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no
+// 16 rows (the first LOADS * kEach of them).  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no
 // barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.
 template <int XT, int LOADS, int WK>
 __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p) {
@@ -475,12 +475,13 @@ __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p)
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, i = lane & 15;
   const int64_t tile = blockIdx.x;
+  const int first = 16 * blockIdx.y;
   WeightChunk w[kDepth];
   RowsChunk<XT, LOADS> x[kDepth];
   auto fetch = [&](int c, int s) __attribute__((always_inline)) {
     if (c < p.chunks) {  // uniform
       load_weights(p, tile, c, lane, w[s]);
-      load_rows<XT, LOADS>(p, 0, c, lane, x[s]);
+      load_rows<XT, LOADS>(p, first, c, lane, x[s]);
     }
   };
 #pragma unroll
@@ -510,7 +511,7 @@ __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p)
 #pragma unroll
   for (int k = 1; k < WK; ++k) sum += sum_sh[k][lane];
   const int n = (int)tile * 16 + 4 * g;
-  store_outputs(p, i, n, scale_back<XT>(p, n, sum));
+  store_outputs(p, first + i, n, scale_back<XT>(p, n, sum));
 }
 
 // More rows: a workgroup takes 128 outputs (a wave 32) for 16 RT rows and a split of the chunks; the rows of kStep chunks
@@ -617,14 +618,26 @@ __global__ __launch_bounds__(256) void mla_linear_sum_kernel(LinearParams p, int
   store_outputs(p, row, n, acc);
 }
 
-// Splits of the chunks for more than 16 rows: as many workgroups as two to a CU, but four chunks each at least.
+// Whether every 16 rows go by themselves: up to 16 rows, and more where the work is small, where a launch for the splits'
+// sums costs more than reading the weights from L2 for each 16.  us by themselves, and together (bf16, rows x n x k):
+//   17 x 576 x 7168 5.3, 8.4    64 x 2048 x 2048 4.2, 8.4    100 x 512 x 16384 9.8, 15.6    32 x 4096 x 4096 6.5, 9.7
+//   64 x 4096 x 4096 11.8, 13.4    32 x 7168 x 7168 16.9, 13.6    20 x 16384 x 2048 11.1, 9.9    32 x 12288 x 512 4.5, 4.0
+static bool linear_few(int64_t tokens, int64_t tiles, int64_t chunks, int cus) {
+  const int64_t all = (tokens + 15) / 16 * tiles;
+  return tokens <= 16 || (all <= 4 * (int64_t)cus && all * chunks <= 128 * (int64_t)cus);
+}
+
+// Splits of the chunks where rows go together: as many workgroups as two to a CU, but eight chunks each at least, four
+// where there are few of both.  us for at least 4, 8, 12 chunks (bf16): 64 x 24576 x 1536 18.3, 12.6, 12.7    64 x 16384 x
+// 2048 16.7, 14.7, 14.8    33 x 1536 x 7168 11.4, 11.4, 14.3    64 x 4096 x 4096 13.6, 13.2, 17.0    64 x 2048 x 2048 8.4, 9.7, 12.4
 static int linear_splits(int64_t tokens, int64_t tiles, int64_t chunks, int cus) {
-  if (tokens <= 16) return 1;
+  if (linear_few(tokens, tiles, chunks, cus)) return 1;
   const int rt = tokens <= 32 ? 2 : 4;
   const int64_t groups = (tiles + 7) / 8 * ((tokens + 16 * rt - 1) / (16 * rt));
   int64_t s = 2 * cus / groups;
   s = s < 1 ? 1 : s > 16 ? 16 : s;
-  const int64_t most = chunks / 4 > 1 ? chunks / 4 : 1;
+  const int each = 8 * groups <= cus && chunks <= 16 ? 4 : 8;
+  const int64_t most = chunks / each > 1 ? chunks / each : 1;
   return (int)(s < most ? s : most);
 }
 
@@ -634,20 +647,22 @@ static int linear_splits(int64_t tokens, int64_t tiles, int64_t chunks, int cus)
 //   32768 x 7168 25.9, 27.9, 33.2
 template <int XT, int LOADS>
 static void launch_few(const LinearParams& p, int cus, hipStream_t st) {
-  if (2 * (int64_t)p.tiles > 5 * (int64_t)cus)
-    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 4>), dim3(p.tiles), dim3(256), 0, st, p);
-  else if (2 * p.tiles <= cus && p.chunks >= 96)
-    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 16>), dim3(p.tiles), dim3(1024), 0, st, p);
+  const dim3 grid(p.tiles, (p.tokens + 15) / 16);
+  const int64_t all = (int64_t)p.tiles * grid.y;
+  if (2 * all > 5 * (int64_t)cus)
+    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 4>), grid, dim3(256), 0, st, p);
+  else if (2 * all <= cus && p.chunks >= 96)
+    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 16>), grid, dim3(1024), 0, st, p);
   else
-    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 8>), dim3(p.tiles), dim3(512), 0, st, p);
+    hipLaunchKernelGGL((mla_linear_few_kernel<XT, LOADS, 8>), grid, dim3(512), 0, st, p);
 }
 
 template <int XT>
 static void launch_linear(LinearParams p, int splits, int cus, hipStream_t st) {
-  if (p.tokens <= 16) {
+  if (linear_few(p.tokens, p.tiles, p.chunks, cus)) {
     constexpr int kFew = kEach<XT>;  // rows of one load
     if (p.tokens <= kFew) return launch_few<XT, 1>(p, cus, st);
-    if (p.tokens <= 2 * kFew) return launch_few<XT, 2>(p, cus, st);
+    if (p.tokens <= 2 * kFew || 2 * kFew == 16) return launch_few<XT, 2>(p, cus, st);
     if constexpr (4 * kFew <= 16) return launch_few<XT, 4>(p, cus, st);
   }
   // whole steps of two chunks, so that the last split is the short one

@@ -413,7 +413,7 @@ def test_linear_refusals(gpu):
 
 def test_linear_streams_and_graphs(gpu):
     """Two captured calls that share a stream's workspace, replayed in turns, and two streams at once."""
-    k, n, T = 8192, 512, 64
+    k, n, T = 16384, 4096, 64
     codes, scale, _ = weights(n, k, 21)
     p = M.pack_w_fp4(codes.cuda(), scale.cuda())
     xs = [rows_of("bf16", T, k, i)[0] for i in range(3)]

@@ -68,13 +68,14 @@ def test_linear_refusals(lib):
             (dict(k=0), 1, b"multiple of 32"), (dict(k=48), 1, b"multiple of 32"), (dict(y_dtype=2), 1, b"y_dtype"), (dict(x_dtype=2), 1, b"x_dtype"),
             (dict(x=None), 1, b"NULL"), (dict(top=None), 1, b"NULL"), (dict(y=None), 1, b"NULL"), (dict(x=BASE + 8), 1, b"16-byte"), (dict(codes=BASE + 8), 1, b"16-byte"),
             (dict(x_stride=260), 1, b"strides"), (dict(x_scale=BASE, x_stride=264), 1, b"strides"), (dict(x_scale_stride=-1), 1, b"strides"), (dict(y_stride=-2), 1, b"strides"),
-            (dict(tokens=64, k=8192, n=512), 2, b"workspace"), (dict(tokens=64, k=8192, n=512, workspace=BASE, workspace_bytes=100), 2, b"workspace"),
-            (dict(tokens=64, k=8192, n=512, workspace=BASE + 8, workspace_bytes=1 << 40), 2, b"aligned")]:
+            (dict(tokens=64, k=16384, n=4096), 2, b"workspace"), (dict(tokens=64, k=16384, n=4096, workspace=BASE, workspace_bytes=100, x_stride=16384), 2, b"workspace"),
+            (dict(tokens=64, k=16384, n=4096, workspace=BASE + 8, workspace_bytes=1 << 40), 2, b"aligned")]:
         rc, msg = linear(**kw)
         assert rc == code and needle in msg, (kw, rc, msg)
     assert linear(tokens=0)[0] == 0 and lib.mla_linear_fp4(None, None) == 1
     assert lib.mla_linear_workspace_bytes(16, 512, 8192) == 0 and lib.mla_linear_workspace_bytes(64, 512, 48) == 0
-    assert lib.mla_linear_workspace_bytes(64, 512, 8192) % (64 * 512 * 4) == 0
+    n = lib.mla_linear_workspace_bytes(64, 4096, 16384)
+    assert n > 0 and n % (64 * 4096 * 4) == 0 and lib.mla_linear_workspace_bytes(64, 512, 2048) == 0
 
 
 def test_weights_against_the_format():
