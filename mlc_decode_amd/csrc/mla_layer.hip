@@ -736,9 +736,18 @@ int mla_rms_norm(const mla_rms_norm_args* a, void* stream) {
                    (a->scale || (aligned(a->out, 16) && k.o_st % 16 == 0));
   const int cus = mla_srv::cu_count();
   const hipStream_t st = (hipStream_t)stream;
-  if (a->dtype == MLA_DTYPE_BF16) launch_norm_type<Bf16>(k, vec, cus, st);
-  else if (a->dtype == MLA_DTYPE_F16) launch_norm_type<F16>(k, vec, cus, st);
-  else launch_norm_type<F32>(k, vec, cus, st);
+  constexpr int32_t kMost = 1 << 21;  // rows of a launch: it holds less than 2^32 threads, a row up to 1024
+  for (int32_t left = a->tokens; left > 0; left -= kMost) {
+    k.tokens = left < kMost ? left : kMost;
+    if (a->dtype == MLA_DTYPE_BF16) launch_norm_type<Bf16>(k, vec, cus, st);
+    else if (a->dtype == MLA_DTYPE_F16) launch_norm_type<F16>(k, vec, cus, st);
+    else launch_norm_type<F32>(k, vec, cus, st);
+    k.x += kMost * k.x_st;
+    if (k.residual) k.residual += kMost * k.r_st;
+    k.out += kMost * k.o_st;
+    if (k.residual_out) k.residual_out += kMost * k.ro_st;
+    if (k.scale) k.scale += (int64_t)kMost * (k.dim / 32);
+  }
   return launched("rms norm");
 }
 

@@ -78,7 +78,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     and summed in fp32; y is of h as added, and both are rounded once, to x's dtype.  With ``quantize`` y is
     :class:`Fp8Rows`, rounded from fp32 (D a multiple of 32), what ``linear_fp4`` reads.  ``out`` and ``residual_out``
     default to new tensors; each may be ``x`` or ``residual`` itself (in place), and may not overlap them otherwise, nor
-    each other.  Rows may be strided (the latent part of ``kv [T, 576]`` before it is appended); the token dims of each
+    each other, nor ``weight``.  Rows may be strided (the latent part of ``kv [T, 576]`` before it is appended); the token dims of each
     tensor must be one stride apart."""
     index = x.get_device()
     if index < 0:
@@ -92,6 +92,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     D = shape[-1]
     x_t = _norm_rows(x, "x", x)
     tokens = x.numel() // D
+    if tokens >= 2 ** 24:
+        raise ValueError("x must have fewer than 2**24 rows")
     if weight.get_device() != index:
         _require(weight, "weight", device)
     if weight.shape != (D,) or not weight.is_contiguous() or weight.dtype not in (dtype, torch.float32):
@@ -125,7 +127,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
         y, y_t = out, _norm_rows(out, "out", x)
     y_ptr = y.data_ptr()
     if tokens and (out is not None or residual_out is not None):
-        _norm_overlaps(x, residual, out, h if residual_out is not None else None, (tokens, D), (x_t, r_t, y_t, h_t))
+        _norm_overlaps(x, residual, weight, out, h if residual_out is not None else None, (tokens, D), (x_t, r_t, y_t, h_t))
     a = MlaRmsNormArgs.from_buffer_copy(_NORM.pack(
         x.data_ptr(), r_ptr, weight.data_ptr(), y_ptr, scale_ptr, h_ptr, x_t, r_t, y_t, h_t, tokens, D, kind,
         _DTYPES[weight.dtype], eps, 0))
@@ -135,7 +137,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     return y if residual is None else (y, h)
 
 
-def _norm_overlaps(x, residual, out, residual_out, rows, strides) -> None:
+def _norm_overlaps(x, residual, weight, out, residual_out, rows, strides) -> None:
     """Refuses outputs of the caller's own whose rows overlap each other's, or an input's without being it."""
     (tokens, D), (x_t, r_t, y_t, h_t), es = rows, strides, x.element_size()
     counts = (tokens, 1)
@@ -144,6 +146,9 @@ def _norm_overlaps(x, residual, out, residual_out, rows, strides) -> None:
             continue
         if _rows_meet((o_t, 0), counts, D):
             raise ValueError(f"{name}'s rows overlap")
+        w_ptr, o_ptr = weight.data_ptr(), o.data_ptr()
+        if w_ptr < o_ptr + es * ((tokens - 1) * o_t + D) and o_ptr < w_ptr + weight.element_size() * D:
+            raise ValueError(f"{name} overlaps weight")
         for t, other, t_t in ((x, "x", x_t), (residual, "residual", r_t)):
             if t is not None and not _apart_or_same(t.data_ptr(), (t_t, 0), o.data_ptr(), (o_t, 0), counts, D, es):
                 raise ValueError(f"{name} overlaps {other} without being it")
@@ -223,8 +228,8 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
     ``x`` in bf16 or fp16, or :class:`Fp8Rows` (from :func:`rms_norm`).  Sums are fp32, rounded once to ``dtype`` (bf16 or
     fp16; x's by default, bf16 of 8-bit rows).  bf16 and 8-bit rows take the weights exactly; with fp16 rows weights
     below ``2**-35`` of the largest of their output are lost.  The leading dims must be one stride apart; rows that do not
-    start on 16 bytes are copied first.  ``out`` (unit stride in its rows) may not overlap ``x``.  The weights are read
-    once for up to 64 rows, so a few rows cost what one does; it takes any number."""
+    start on 16 bytes are copied first.  ``out`` (unit stride in its rows) may not overlap ``x``.  Memory gives the weights
+    once for up to 64 rows, so a few rows cost little more than one; it takes up to 2**20."""
     coded = isinstance(x, Fp8Rows)
     rows = x.codes if coded else x
     index = rows.get_device()
@@ -260,6 +265,8 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
     if at is None or rows.stride(-1) != 1:
         raise ValueError("x must have unit stride in its rows and token dims one stride apart")
     tokens, x_t = at
+    if tokens > 2 ** 20:
+        raise ValueError("x must have at most 2**20 rows")
     size = rows.element_size()
     if rows.data_ptr() % 16 or x_t * size % 16:
         rows = rows.contiguous().clone()
@@ -286,8 +293,11 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
         if tokens and _rows_meet((y_t, 0), (tokens, 1), n):
             raise ValueError("out's rows overlap")
         y_ptr, x_ptr = y.data_ptr(), rows.data_ptr()
-        if tokens and y_ptr < x_ptr + size * ((tokens - 1) * x_t + k) and x_ptr < y_ptr + 2 * ((tokens - 1) * y_t + n):
+        y_end = y_ptr + 2 * ((tokens - 1) * y_t + n)
+        if tokens and y_ptr < x_ptr + size * ((tokens - 1) * x_t + k) and x_ptr < y_end:
             raise ValueError("out overlaps x")
+        if tokens and coded and y_ptr < s_ptr + (tokens - 1) * s_t + k // GROUP and s_ptr < y_end:
+            raise ValueError("out overlaps x.scale")
     need = _linear_workspace(tokens, n, k)
     ws_ptr = ws = 0
     if need:

@@ -250,6 +250,27 @@ def test_decode(gpu, fmt, H, s):
     check_decode(q, cache, rows, table, plan, mask, fmt, got, f"{fmt} H={H} s={s}")
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("H,s", [(1, 1), (2, 3), (16, 5), (3, 33), (8, 64), (128, 8), (100, 8), (40, 33), (16, 64)])
+def test_decode_behind_a_wide_table(gpu, fmt, H, s):
+    """A table too wide for the decode of pages by themselves: the split-KV pass over the schedule, then the drafted
+    tokens, by 16 rows and by 64."""
+    prefixes = [0, 1, 63, 64, 65, 200, 130]
+    q, cache, rows, table, plan, mask = problem(fmt, H, s, prefixes, 2000 + 10 * H + s)
+    wide = table.repeat(1, -(-600 // table.shape[1]))[:, :600]
+    code = {"fp8": 1, "fp4": 2}.get(fmt, 0)
+    sched = M.get_mla_metadata(plan.prefix_lens, H * s, 1, kv_cache=cache)
+    lib = M._lib.load()
+    assert not lib.mla_tree_takes_pages(7, s, H, sched[0].shape[0], code, 600) and api._tree_without_schedule(7, s, H, code, 600) is None
+    say(f"wide table {fmt} H={H} s={s}")
+    got = decode(q, cache, wide, plan)
+    torch.cuda.synchronize()
+    check_decode(q, cache, rows, table, plan, mask, fmt, got, f"wide {fmt} H={H} s={s}")
+    auto = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan)
+    torch.cuda.synchronize()
+    check_decode(q, cache, rows, table, plan, mask, fmt, auto, f"wide auto {fmt} H={H} s={s}")
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
 def test_decode_ragged_trees(gpu, fmt):
     prefixes, n = [0, 0, 40, 60, 300, 5, 128], [0, 3, 12, 1, 7, 0, 12]

@@ -213,6 +213,46 @@ def test_norm_refusals(gpu):
             M.rms_norm(*args, **kw)
 
 
+def test_norm_of_millions_of_rows(gpu):
+    """More rows than a launch holds threads for at 1024 a row; inputs whose token dim has stride 0, and memory past 2^32
+    elements in the output."""
+    T, D = 2 ** 22 + 5, 1026
+    say("norm millions of rows")
+    g = torch.Generator().manual_seed(3)
+    pair = torch.randn(2, D, generator=g).bfloat16().cuda()
+    w = torch.ones(D, dtype=torch.bfloat16, device="cuda")
+    few = M.rms_norm(pair, w)
+    y = M.rms_norm(pair[:1].expand(T, D), w)
+    torch.cuda.synchronize()
+    for part in y.split(2 ** 20):
+        assert (part == few[0]).all()
+    rows = pair[None].expand(2 ** 11, 2, D).reshape(-1, D)  # [2^12, D], the two in turns
+    assert torch.equal(M.rms_norm(rows, w), few.repeat(2 ** 11, 1))
+    x = torch.empty(2 ** 24, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        M.rms_norm(x, w[:1])
+    assert (M.rms_norm(x.fill_(-3)[1:], w[:1]) == -1).all()
+
+
+def test_outputs_apart_from_the_other_inputs(gpu):
+    say("overlaps")
+    buf = torch.zeros(64 * 40, dtype=torch.bfloat16, device="cuda")
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        M.rms_norm(x, buf[:64], out=buf[32:].as_strided((4, 64), (64, 1)))
+    with pytest.raises(ValueError):
+        M.rms_norm(x, buf[200:264], residual=x, residual_out=buf.as_strided((4, 64), (64, 1)))
+    w = M.quantize_w_fp4(torch.zeros(16, 64, device="cuda"))
+    raw = buf.view(torch.uint8)
+    rows = M.Fp8Rows(raw[:256].view(4, 64), raw[256:264].view(4, 2))
+    with pytest.raises(ValueError):
+        M.linear_fp4(rows, w, out=buf[131:131 + 64].view(4, 16))
+    M.linear_fp4(rows, w, out=buf[132:132 + 64].view(4, 16))
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError):
+        M.linear_fp4(x[:1, :32].expand(2 ** 20 + 1, 32), M.quantize_w_fp4(torch.zeros(16, 32, device="cuda")))
+
+
 def test_norm_in_a_graph(gpu):
     say("norm graph")
     x, r, w = tensors(9, 7168, torch.bfloat16, 7168, 5)
