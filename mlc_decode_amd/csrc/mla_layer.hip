@@ -31,7 +31,8 @@ using mla_srv::unpack;
 //
 // A piece is 16 bytes of x (8 values, 4 of fp32), or one value where rows, strides or dims do not fall on such pieces;
 // thread t of a row holds pieces t, t + threads, ...  P of them.
-// Bound by memory for many rows, by latency for few: row, sum, two barriers.
+// Bound by memory for many rows, by latency for few (row, sum, barrier): 1 x 7168 with the residual 2.9 us, 256 rows 4.1,
+// 1024 rows 11.0 (5.3 TB/s), 8192 rows 96 (4.9; to 16 bits without a residual 42.7, 5.5), 65536 x 512 40 us, 6.7 TB/s.
 struct NormParams {
   const uint8_t* x;
   const uint8_t* residual;  // may be NULL
@@ -255,6 +256,8 @@ static void launch_norm(const NormParams& p, int cus, hipStream_t st) {
   if (pieces <= 128) return launch_norm_as<E, V, 64, 2>(p, st);
   if (pieces <= 256) return launch_norm_as<E, V, 256, 1>(p, st);
   if (pieces <= 512) return launch_norm_as<E, V, 256, 2>(p, st);
+  // Few rows take threads, many rows workgroups that fit a CU in numbers; us for 1024 and 256 threads a row of 7168 with the
+  // residual: 1 row 2.9, 4.2    128 3.5, 4.9    256 4.2, 5.5    512 5.8, 7.0    768 9.0, 9.0    1024 11.8, 11.0
   if (pieces <= 1024) {
     if (p.tokens <= 2 * cus) return launch_norm_as<E, V, 1024, 1>(p, st);
     return launch_norm_as<E, V, 256, 4>(p, st);

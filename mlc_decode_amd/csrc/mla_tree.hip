@@ -552,7 +552,8 @@ hipError_t launch_tiles(const TreeParams& p, int cus, hipStream_t st) {
 // ---------------------------------------------------------------------------------------
 // A wave a sequence, a lane a node.  A node's mask is its own bit and its parent's mask.  Each of six rounds takes
 // over the mask of the node that the lane points at and then points where that one does: 2, 4, .. 64 generations.
-// Bound by latency: two loads, six rounds of lane reads, a table lookup: a step's 128 trees of 16 nodes 2.7 us.
+// Bound by latency: two loads, six rounds of lane reads, a table lookup: 128 trees of 16 nodes 2.7 us,
+// 4096 of them 3.2.
 struct PlanParams {
   const int32_t* parents;
   const int32_t* seqlens;
@@ -664,10 +665,13 @@ __global__ __launch_bounds__(256) void mla_tree_accept_kernel(AcceptParams p) {
 // keep: the path's rows together
 // ---------------------------------------------------------------------------------------
 // Row slots[k] <- row slots[path[k]] for the entries of the path, as if all were read before any is written.  A thread
-// takes one 16-byte piece of the rows (4 bytes of the fp8 cache's scales) and walks the path in order, kAhead rows
+// takes one 16-byte piece of the rows (4 bytes of the fp8 cache's scales) and walks the path in order, 16 rows
 // read ahead of their writes.  No read can meet an earlier write: an entry is at least its own place (others are
-// passed over), so the rows written before it lie below the one that it reads.  Bound by latency: rows read in turns
-// of kAhead; paths are a few nodes long.
+// passed over), so the rows written before it lie below the one that it reads.  Lane k of each wave holds entry k, its
+// row and that of path[k]: what a round moves is known without another load.  Bound by latency, a read and a write per 16
+// rows: 128 sequences that move 15 rows each 3.9 us (bf16; with the rows' indices loaded for every item 8.6, and in the
+// fp8 cache, whose parts went one after the other, 21.7 -> 3.7), 256 that move 63 10.9 us (32.1); 4096 that move 15 24 us,
+// 5.9 TB/s, a large copy's rate.
 struct KeepParams {
   uint8_t* nope;
   uint8_t* rope;
@@ -678,49 +682,61 @@ struct KeepParams {
   const int32_t* path;
   int32_t s_q, format;
 };
-constexpr int kAhead = 8;
 
-template <class V>
-__device__ __forceinline__ void keep_pieces(uint8_t* base, int64_t page_stride, int64_t row_stride, const int32_t* slots,
-                                            const int32_t* path, int s_q, int64_t tokens) {
-  for (int k0 = 0; k0 < s_q; k0 += kAhead) {
-    V v[kAhead];
-    int64_t to[kAhead];
-    bool more = false;
+// The next N moves, all read, then all written; where fewer are left, the last of them again, the same bytes (a branch an
+// item would have each write wait for the one before it).  from, to: lane k's rows.  The strides are the thread's own; the
+// moves are uniform.
+template <class V, int N>
+__device__ __forceinline__ uint64_t keep_some(uint8_t* base, int64_t page_stride, int64_t row_stride, int from, int to, uint64_t moves) {
+  V v[N];
+  uint8_t* dst[N];
+  int k = 0;
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int k = k0 + u;
-      to[u] = -1;
-      if (k >= s_q) continue;
-      const int j = path[k];
-      more = j >= 0;
-      if (j <= k || j >= s_q) continue;
-      const int64_t src = slots[j], dst = slots[k];
-      if (src < 0 || dst < 0 || src >= tokens || dst >= tokens) continue;
-      to[u] = dst / kPage * page_stride + dst % kPage * row_stride;
-      v[u] = *(const V*)(base + src / kPage * page_stride + src % kPage * row_stride);
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-      if (to[u] >= 0) *(V*)(base + to[u]) = v[u];
-    if (!more) break;  // the path's end
+  for (int u = 0; u < N; ++u) {
+    k = moves ? __builtin_ctzll(moves) : k;
+    moves &= moves - 1;
+    const int i = __builtin_amdgcn_readlane(from, k), o = __builtin_amdgcn_readlane(to, k);
+    v[u] = *(const V*)(base + i / kPage * page_stride + i % kPage * row_stride);
+    dst[u] = base + o / kPage * page_stride + o % kPage * row_stride;
   }
+#pragma unroll
+  for (int u = 0; u < N; ++u) *(V*)dst[u] = v[u];
+  return moves;
+}
+template <class V>
+__device__ __forceinline__ void keep_pieces(uint8_t* base, int64_t page_stride, int64_t row_stride, int from, int to, uint64_t moves) {
+  while (__builtin_popcountll(moves) > 4) moves = keep_some<V, 16>(base, page_stride, row_stride, from, to, moves);
+  if (moves) keep_some<V, 4>(base, page_stride, row_stride, from, to, moves);
 }
 
 __global__ __launch_bounds__(128) void mla_keep_path_kernel(KeepParams p) {
-  const int t = threadIdx.x;
-  const int32_t* slots = p.slots + (int64_t)blockIdx.x * p.s_q;
-  const int32_t* path = p.path + (int64_t)blockIdx.x * p.s_q;
+  const int t = threadIdx.x, lane = t & 63;
+  const int64_t at = (int64_t)blockIdx.x * p.s_q + lane;
+  const bool in = lane < p.s_q;
+  const int slot = in ? p.slots[at] : -1, j = in ? p.path[at] : -1;
+  const bool goes = j > lane && j < p.s_q;
+  const int from = __shfl(slot, goes ? j : lane);
+  const bool moved = goes && slot >= 0 && from >= 0 && slot < p.tokens && from < p.tokens;
+  const uint64_t moves = __builtin_amdgcn_ballot_w64(moved);
   const int pieces = p.format == MLA_KV_NATIVE ? 64 : p.format == MLA_KV_FP8_E4M3 ? 32 : 16;  // of the latent
-  if (t < pieces) {
-    keep_pieces<i32x4>(p.nope + 16 * t, p.sp, p.st, slots, path, p.s_q, p.tokens);
-  } else if (t < pieces + 8) {
-    keep_pieces<i32x4>(p.rope + 16 * (t - pieces), p.rp, p.rt, slots, path, p.s_q, p.tokens);
-  } else if (p.format == MLA_KV_FP8_E4M3 && t < pieces + 12) {
-    keep_pieces<int32_t>(p.scale + (t - pieces - 8) * p.ct, p.cp, 4, slots, path, p.s_q, p.tokens);
-  } else if (p.format == MLA_KV_FP4_E2M1 && t == pieces + 8) {
-    keep_pieces<i32x4>(p.scale, p.cp, p.ct, slots, path, p.s_q, p.tokens);
+  if (p.format == MLA_KV_FP8_E4M3 && t >= 64) {
+    if (t < 68) keep_pieces<int32_t>(p.scale + (t - 64) * p.ct, p.cp, 4, from, slot, moves);
+    return;
   }
+  uint8_t* base = p.nope + 16 * t;
+  int64_t page_stride = p.sp, row_stride = p.st;
+  if (t >= pieces) {
+    base = p.rope + 16 * (t - pieces);
+    page_stride = p.rp;
+    row_stride = p.rt;
+  }
+  if (t >= pieces + 8) {
+    base = p.scale;
+    page_stride = p.cp;
+    row_stride = p.ct;
+  }
+  if (t < pieces + 8 || (p.format == MLA_KV_FP4_E2M1 && t == pieces + 8))
+    keep_pieces<i32x4>(base, page_stride, row_stride, from, slot, moves);
 }
 
 static bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }
