@@ -126,7 +126,7 @@ def kv_keep_path(kv_cache, slots: torch.Tensor, path: torch.Tensor) -> None:
     """Move the tokens of ``path [B, s_q]`` (int32, from :func:`tree_accept`) together: cache row ``slots[b, k]`` takes
     the token of row ``slots[b, path[b, k]]``, as if all were read before any is written; in place, bit for bit, in
     every cache format.  ``slots`` is the plan's.  Entries below their own place k and slots outside the cache name
-    nothing.  A drafted token's position is its depth's, so what is moved needs no new rotation."""
+    nothing; a row that slots name twice holds one of its values afterwards.  A drafted token's position is its depth's, so what is moved needs no new rotation."""
     c, _, device = _cache_struct(kv_cache, None)
     if path.get_device() != device.index:
         _require(path, "path", device)

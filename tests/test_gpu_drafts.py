@@ -448,6 +448,61 @@ def test_absorbed(gpu, fmt, H, s):
     assert torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("fmt", ["bf16", "fp8"])
+def test_many_pages_by_themselves(gpu, fmt):
+    """Pages in one launch, more of them than the merge holds at once (a schedule of more parts makes the room)."""
+    q, cache, rows, table, plan, mask = problem(fmt, 8, 2, [64 * 700 + 3], 53)
+    sched = M.get_mla_metadata(plan.prefix_lens, 16, 1, num_parts=1000, fixed_overhead=0)
+    code = 1 if fmt == "fp8" else 0
+    assert M._lib.load().mla_tree_takes_pages(1, 2, 8, 1000, code, table.shape[1])
+    say(f"many pages {fmt}")
+    got = M.flash_mla_with_kvcache(q, cache, table, None, 512, *sched, tree=plan)
+    torch.cuda.synchronize()
+    check_decode(q, cache, rows, table, plan, mask, fmt, got, f"many pages {fmt}")
+
+
+@pytest.mark.parametrize("width", [0, 900])
+def test_absorbed_of_many_splits(gpu, width):
+    """Merges past 64 splits, from pages by themselves and from the schedule's: whole rows first, then the projection."""
+    H, s = 2, 4
+    q, cache, rows, table, plan, mask = problem("bf16", H, s, [64 * 200 + 9], 59)
+    if width:
+        table = table.repeat(1, -(-width // table.shape[1]))[:, :width]
+    g = torch.Generator().manual_seed(7)
+    w = (torch.randn(H, 512, 128, generator=g) * 512 ** -0.5).to(q.dtype).cuda()
+    sched = M.get_mla_metadata(plan.prefix_lens, s * H, 1, num_parts=256, fixed_overhead=0)
+    assert bool(M._lib.load().mla_tree_takes_pages(1, s, H, 256, 0, table.shape[1])) == (not width)
+    say(f"absorbed of many splits, width {width}")
+    out, lse = M.flash_mla_with_kvcache(q, cache, table, None, 512, *sched, tree=plan)
+    v, lse2 = M.mla_decode_absorbed(q, cache, table, None, *sched, M.prepare_w_uv(w), tree=plan)
+    torch.cuda.synchronize()
+    check_decode(q, cache, rows, table, plan, mask, "bf16", (out, lse), f"absorbed, width {width}")
+    rows_ = out.double().transpose(1, 2).transpose(0, 1).reshape(H, -1, 512)
+    want = (rows_ @ w.double()).view(H, 1, s, 128).permute(1, 2, 0, 3)
+    size = (rows_.abs() @ w.double().abs()).view(H, 1, s, 128).permute(1, 2, 0, 3)
+    # as in test_absorbed
+    assert ((v.double() - want).abs() <= (2.0 ** -7 + 2.0 ** -14) * size + 2.0 ** -8 * want.abs()).all()
+    assert torch.equal(lse, lse2)
+
+
+def test_tiny_latents(gpu):
+    """One key in sight and latents near the smallest normal number: the output is the key's latent, rounded twice (the
+    partial to 2^-11 of its chunk's largest, at worst as subnormals of 16 bits)."""
+    q, cache, rows, table, plan, _ = problem("bf16", 4, 3, [0, 0], 61)
+    plan = plan._replace(mask=ints([[1, 2, 4]] * 2, torch.int64))
+    for e in (-100, -113, -118):
+        tiny = (cache.float().clamp(-4, 4) * 2.0 ** e).bfloat16()
+        say(f"tiny 2^{e}")
+        out, _ = decode(q, tiny, table, plan)
+        torch.cuda.synchronize()
+        for b in range(2):
+            for i in range(3):
+                page, row = divmod(int(plan.slots[b, i]) if int(plan.slots[b, i]) >= 0 else int(table[b, 0]) * 64 + i, 64)
+                want = tiny[page, row, 0, :512].double()
+                got = out[b, i].double()
+                assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -11 * want.abs().max()).all()
+
+
 def test_decode_refusals(gpu):
     q, cache, rows, table, plan, mask = problem("bf16", 4, 5, [10, 20], 43)
     say("decode refusals")
