@@ -1,7 +1,8 @@
 """MI355X (gfx950) split-KV MLA decode behind the reference's Python entry points.
 
 The hot path is hand-written HIP (``csrc/mla_decode.hip``) reached through the C ABI of
-``include/mla_decode_amd.h``; this package is the torch-side host code around it.
+``include/mla_decode_amd.h``; this package is the torch-side host code around it.  Around the decode: the serving step
+(``serving``), trees of drafted tokens (``drafts``), norm and projections by 4-bit weights (``layer``).
 """
 from .api import (Fp4KVCache, Fp8KVCache, TreePlan, flash_mla_with_kvcache, fp4_kv_cache, fp8_kv_cache,
                   get_mla_metadata, get_mla_metadata_host, kv_append, merge_partials, mla_decode_absorbed,
