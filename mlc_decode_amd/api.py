@@ -77,6 +77,17 @@ def _launch(name: str, fn, device: torch.device, *args) -> None:
         check(name, status)
 
 
+def new_tensor(shape: Tuple[int, ...], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """``torch.empty(shape)`` at the host's price of one with given strides (1.3 us against 1.7 to 2.1)."""
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1] or 1, 1), dtype=dtype, device=device)
+    strides, n = [], 1
+    for d in reversed(shape):
+        strides.append(n)
+        n *= d if d > 1 else 1
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
 def _require_gpu(t: torch.Tensor, name: str) -> None:
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor (the decode runs only as HIP kernels)")
@@ -410,9 +421,9 @@ def make_decode_args(q: torch.Tensor, kv_cache, block_table: Optional[torch.Tens
         if status.dtype != torch.int32 or status.numel() < 1:
             raise ValueError("status must be an int32 tensor of at least one element")
     if out is None:
-        out = torch.empty(B, s_q, H, MLA_DIM_V, dtype=q.dtype, device=q.device)
+        out = new_tensor((B, s_q, H, MLA_DIM_V), dtype, q.device)
     if lse is None:
-        lse = torch.empty(B, H, s_q, dtype=torch.float32, device=q.device)
+        lse = new_tensor((B, H, s_q), torch.float32, q.device)
     if lse.shape != (B, H, s_q) or not lse.is_contiguous() or lse.dtype != torch.float32:
         raise ValueError("lse must be a contiguous fp32 [B, H, s_q] tensor")
     if out.shape != (B, s_q, H, MLA_DIM_V) or out.dtype != q.dtype or out.stride(-1) != 1:
@@ -715,8 +726,9 @@ def _check_coded_cache(c):
 
 def _check_fp4_cache(c: Fp4KVCache):
     latent, scale, rope = c
-    for t, n in ((latent, "fp4 latent"), (scale, "fp4 scale"), (rope, "fp4 rope")):
-        _require_gpu(t, n)
+    if not (latent.is_cuda and scale.is_cuda and rope.is_cuda):
+        for t, n in ((latent, "fp4 latent"), (scale, "fp4 scale"), (rope, "fp4 rope")):
+            _require_gpu(t, n)
     nb, page = latent.shape[0], _lib.MLA_PAGE_TOKENS
     if latent.dtype != torch.uint8 or latent.shape != (nb, page, MLA_DIM_V // 2) or latent.stride(-1) != 1:
         raise ValueError("fp4 latent must be a uint8 [num_blocks, 64, 256] tensor")
@@ -728,12 +740,12 @@ def _check_fp4_cache(c: Fp4KVCache):
 
 
 def _check_fp8_cache(c: Fp8KVCache):
-    latent, scale, rope = c.latent, c.scale, c.rope
-    for t, n in ((latent, "fp8 latent"), (scale, "fp8 scale"), (rope, "fp8 rope")):
-        _require_gpu(t, n)
+    latent, scale, rope = c
+    if not (latent.is_cuda and scale.is_cuda and rope.is_cuda):
+        for t, n in ((latent, "fp8 latent"), (scale, "fp8 scale"), (rope, "fp8 rope")):
+            _require_gpu(t, n)
     nb, page = latent.shape[0], _lib.MLA_PAGE_TOKENS
-    if latent.dtype not in (torch.uint8, torch.float8_e4m3fn) or latent.dim() != 3 or \
-            latent.shape[1:] != (page, MLA_DIM_V) or latent.stride(-1) != 1:
+    if latent.dtype not in (torch.uint8, torch.float8_e4m3fn) or latent.shape != (nb, page, MLA_DIM_V) or latent.stride(-1) != 1:
         raise ValueError("fp8 latent must be a uint8 / float8_e4m3fn [num_blocks, 64, 512] tensor")
     if scale.dtype != torch.float32 or scale.shape != (nb, 4, page) or scale.stride(-1) != 1:
         raise ValueError("fp8 scale must be a float32 [num_blocks, 4, 64] tensor")

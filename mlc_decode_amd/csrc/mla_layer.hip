@@ -469,7 +469,9 @@ __device__ __forceinline__ f32x4 scale_back(const LinearParams& p, int n, f32x4 
 }
 
 // 16 rows (the first LOADS * kEach of them).  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no
-// barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.
+// barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.  Bound by
+// the weights: 8 x 24576 x 1536 (8-bit rows) 5.6 us, 3.6 TB/s; 1 x 7168 x 16384 12.3 us, 5.1 TB/s; one of 576 x 7168 4.0, a
+// load's latency over and over.
 template <int XT, int LOADS, int WK>
 __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p) {
   constexpr int kDepth = LOADS == 4 && WK >= 8 ? 2 : 4;  // 128 registers: two workgroups of 8 waves a CU
@@ -518,7 +520,10 @@ __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p)
 }
 
 // More rows: a workgroup takes 128 outputs (a wave 32) for 16 RT rows and a split of the chunks; the rows of kStep chunks
-// at a time go through LDS for all waves, the next ones on the way meanwhile.
+// at a time go through LDS for all waves, the next ones on the way meanwhile.  64 x 7168 x 16384 (bf16, 62 MB of weights)
+// 23 us and 3 to 4 of sums.  Products and the reads of their rows from LDS, which want the whole of both units, are 11 of
+// them, loads 3, the rows' way into LDS 2, the splits' partial sums 3.  Eight waves of 256 outputs (half the rows'
+// traffic) 27.8 us in all against 27.3, that with twice as much on the way 30.8; four splits 30.9, sixteen 33.6.
 template <int XT, int RT>
 __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p) {
   constexpr int kStep = 2, NT = 2;

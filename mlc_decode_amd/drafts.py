@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import MlaTreePlanArgs
-from .api import TreePlan, _launch
+from .api import TreePlan, _launch, new_tensor
 from .serving import _cache_struct, _require
 
 _PLAN = struct.Struct("=4Q4i4Q")
@@ -86,10 +86,8 @@ def tree_plan(parents: torch.Tensor, cache_seqlens: torch.Tensor, block_table: t
     (_, P), (stride, unit) = block_table.shape, block_table.stride()
     if P < 1 or (P > 1 and unit != 1) or (B > 1 and stride < P) or (B > 1 and stride >= 2 ** 31):
         raise ValueError("block_table must have columns of unit stride, and rows below 2^31 apart that do not overlap")
-    mask = torch.empty(shape, dtype=torch.int64, device=device)
-    positions = torch.empty(shape, dtype=torch.int32, device=device)
-    slots = torch.empty(shape, dtype=torch.int32, device=device)
-    prefix = torch.empty(B, dtype=torch.int32, device=device)
+    mask = new_tensor(shape, torch.int64, device)
+    positions, slots, prefix = torch.empty_like(parents), torch.empty_like(parents), torch.empty_like(cache_seqlens)
     a = MlaTreePlanArgs.from_buffer_copy(_PLAN.pack(
         parents.data_ptr(), cache_seqlens.data_ptr(), tree_lens.data_ptr() if tree_lens is not None else 0,
         block_table.data_ptr(), stride if B > 1 else P, P, B, s_q, mask.data_ptr(), positions.data_ptr(),
@@ -112,10 +110,8 @@ def tree_accept(plan: TreePlan, tokens: torch.Tensor, targets: torch.Tensor) -> 
     _grid(targets, "targets", dtype, shape, index)
     _grid(mask, "plan.mask", torch.int64, shape, index)
     _grid(prefix, "plan.prefix_lens", torch.int32, (B,), index)
-    path = torch.empty(shape, dtype=torch.int32, device=device)
-    counts = torch.empty(B, dtype=torch.int32, device=device)
-    keep = torch.empty(B, dtype=torch.int32, device=device)
-    after = torch.empty(B, dtype=dtype, device=device)
+    path, after = new_tensor(shape, torch.int32, device), new_tensor((B,), dtype, device)
+    counts, keep = torch.empty_like(prefix), torch.empty_like(prefix)
     _launch("mla_tree_accept", _lib.load().mla_tree_accept, device, mask.data_ptr(), prefix.data_ptr(), tokens.data_ptr(),
             targets.data_ptr(), int(dtype is torch.int64), B, s_q, path.data_ptr(), counts.data_ptr(), after.data_ptr(),
             keep.data_ptr())

@@ -21,7 +21,7 @@ import torch
 
 from . import _lib
 from ._lib import MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_DTYPE_F32, MlaLinearArgs, MlaRmsNormArgs
-from .api import _launch, _stream_ptr, _workspace
+from .api import _launch, _stream_ptr, _workspace, new_tensor
 from .serving import _apart_or_same, _require, _rows_meet
 
 _DTYPES = {torch.bfloat16: MLA_DTYPE_BF16, torch.float16: MLA_DTYPE_F16, torch.float32: MLA_DTYPE_F32}
@@ -44,6 +44,8 @@ def _token_rows(t: torch.Tensor) -> Optional[Tuple[int, int]]:
     if t.dim() == 2:
         n = t.shape[0]
         return n, t.stride(0) if n > 1 else 0
+    if 0 in t.shape:
+        return 0, 0
     tokens, stride = 1, 0
     for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if n == 1:
@@ -90,8 +92,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     if len(shape) < 2 or shape[-1] < 1:
         raise ValueError("x must be [..., D], D at least 1")
     D = shape[-1]
-    x_t = _norm_rows(x, "x", x)
-    tokens = x.numel() // D
+    rows = _token_rows(x)
+    if rows is None or (D > 1 and x.stride(-1) != 1):
+        raise ValueError("x must have unit stride in its rows, and token dims one stride apart")
+    tokens, x_t = rows
     if tokens >= 2 ** 24:
         raise ValueError("x must have fewer than 2**24 rows")
     if weight.get_device() != index:
@@ -106,7 +110,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
         r_ptr, r_t = residual.data_ptr(), _norm_rows(residual, "residual", x)
         h = residual_out
         if h is None:
-            h, h_t = torch.empty(shape, dtype=dtype, device=device), D
+            h, h_t = torch.empty_like(x, memory_format=torch.contiguous_format), D
         else:
             h_t = _norm_rows(h, "residual_out", x)
         h_ptr = h.data_ptr()
@@ -118,11 +122,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
             raise ValueError("8-bit rows are new tensors: no out")
         if D % GROUP:
             raise ValueError(f"8-bit rows take a D that is a multiple of {GROUP}")
-        y = torch.empty(shape, dtype=torch.uint8, device=device)
-        scale = torch.empty(*shape[:-1], D // GROUP, dtype=torch.uint8, device=device)
+        y = new_tensor(shape, torch.uint8, device)
+        scale = new_tensor((*shape[:-1], D // GROUP), torch.uint8, device)
         y_t, scale_ptr = D, scale.data_ptr()
     elif out is None:
-        y, y_t = torch.empty(shape, dtype=dtype, device=device), D
+        y, y_t = torch.empty_like(x, memory_format=torch.contiguous_format), D
     else:
         y, y_t = out, _norm_rows(out, "out", x)
     y_ptr = y.data_ptr()
@@ -250,15 +254,20 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
             raise ValueError("x must be bfloat16 or float16, or 8-bit rows")
         if dtype is None:
             dtype = rows.dtype if out is None else out.dtype
-    if dtype not in (torch.bfloat16, torch.float16):
+    y_kind = _DTYPES.get(dtype)
+    if y_kind is None or y_kind == MLA_DTYPE_F32:
         raise ValueError("dtype must be bfloat16 or float16")
     codes, scale, top = w.codes, w.scale, w.top
     tiles, chunks = -(-n // 16), -(-k // 128)
-    for t, name, want in ((codes, "w.codes", (tiles, chunks, 64, 16)), (scale, "w.scale", (tiles, chunks, 64)), (top, "w.top", (16 * tiles,))):
-        if t.get_device() != index:
-            _require(t, name, device)
-        if t.dtype is not torch.uint8 or t.shape != want or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous uint8 {list(want)} tensor (see pack_w_fp4)")
+    u8 = torch.uint8
+    if not (codes.get_device() == scale.get_device() == top.get_device() == index and codes.dtype is scale.dtype is top.dtype is u8
+            and codes.shape == (tiles, chunks, 64, 16) and scale.shape == (tiles, chunks, 64) and top.shape == (16 * tiles,)
+            and codes.is_contiguous() and scale.is_contiguous() and top.is_contiguous()):
+        for t, name, want in ((codes, "w.codes", (tiles, chunks, 64, 16)), (scale, "w.scale", (tiles, chunks, 64)), (top, "w.top", (16 * tiles,))):
+            if t.get_device() != index:
+                _require(t, name, device)
+            if t.dtype is not u8 or t.shape != want or not t.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous uint8 {list(want)} tensor (see pack_w_fp4)")
     if codes.data_ptr() % 16:
         raise ValueError("w.codes must be 16-byte aligned")
     at = _token_rows(rows)
@@ -281,7 +290,7 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
             raise ValueError(f"x.scale must be a uint8 [..., {k // GROUP}] tensor with unit stride in its rows")
         s_ptr, s_t = xs.data_ptr(), s_at[1]
     if out is None:
-        y, y_t = torch.empty(*shape[:-1], n, dtype=dtype, device=device), n
+        y, y_t = new_tensor((*shape[:-1], n), dtype, device), n
     else:
         y = out
         if y.get_device() != index:
@@ -304,6 +313,6 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
         _, ws_ptr, ws = _workspace(device, _stream_ptr(device), need)
     a = MlaLinearArgs.from_buffer_copy(_LINEAR.pack(
         rows.data_ptr(), s_ptr, codes.data_ptr(), scale.data_ptr(), top.data_ptr(), y.data_ptr(), x_t, s_t, y_t,
-        tokens, n, k, kind, _DTYPES[dtype], 0, ws_ptr, ws))
+        tokens, n, k, kind, y_kind, 0, ws_ptr, ws))
     _launch("mla_linear_fp4", _lib.load().mla_linear_fp4, device, ctypes.byref(a))
     return y

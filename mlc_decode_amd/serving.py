@@ -246,36 +246,39 @@ def _cache_struct(kv_cache, device: Optional[torch.device]) -> tuple:
     """``(mla_kv_cache, dtype, device)`` of a cache in any of its forms."""
     fmt = _cache_format(kv_cache)
     rope_offset, scale_args = 0, (0, 0, 0)
+    others = ()
     if fmt != MLA_KV_NATIVE:
         latent, scale, rope = _check_coded_cache(kv_cache)
         dtype = torch.bfloat16
-        scale_args = (scale.data_ptr(), *scale.stride()[:2])
+        page, block, _ = scale.stride()
+        scale_args = (scale.data_ptr(), page, block)
         others = (scale, rope)
     else:
         if isinstance(kv_cache, (tuple, list)):
             latent, rope = _split_kv(kv_cache)
+            others = (rope,)
         else:
             latent = rope = kv_cache
             if kv_cache.shape[-1] != MLA_DIM_QK:
                 raise ValueError(f"kv_cache last dim must be {MLA_DIM_QK}")
             rope_offset = 2 * MLA_DIM_V
         dtype = latent.dtype
-        for t in (latent, rope):
+        for t in (latent, *others):
             if t.dtype not in (torch.bfloat16, torch.float16) or t.dtype != dtype:
                 raise ValueError("the cache must be bfloat16 or float16")
             if t.dim() != 4 or t.shape[1] != _PAGE or t.shape[2] != 1 or t.stride(-1) != 1:
                 raise ValueError("kv cache must be [num_blocks, 64, 1, D] with unit stride in D")
         if latent.shape[0] != rope.shape[0]:
             raise ValueError("the cache's halves have different page counts")
-        others = (rope,)
     if device is None:
         device = latent.device
-    _require(latent, "kv_cache", device)
-    for t in others:
-        _require(t, "kv_cache", device)
+    for t in (latent, *others):
+        if t.get_device() != device.index or device.index is None:
+            _require(t, "kv_cache", device)
+    (sp, st, *_), (rp, rt, *_) = latent.stride(), rope.stride()
     c = MlaKvCache.from_buffer_copy(_CACHE.pack(
         fmt, _DTYPES[dtype], latent.shape[0], 0, latent.data_ptr(), rope.data_ptr() + rope_offset, scale_args[0],
-        latent.stride(0), latent.stride(1), rope.stride(0), rope.stride(1), scale_args[1], scale_args[2]))
+        sp, st, rp, rt, scale_args[1], scale_args[2]))
     return c, dtype, device
 
 

@@ -234,6 +234,19 @@ def test_norm_of_millions_of_rows(gpu):
     assert (M.rms_norm(x.fill_(-3)[1:], w[:1]) == -1).all()
 
 
+def test_empty_batches(gpu):
+    say("empty batches")
+    w, packed = torch.ones(64, dtype=torch.bfloat16, device="cuda"), M.quantize_w_fp4(torch.ones(17, 64, device="cuda"))
+    for shape in ((0, 64), (3, 0, 64), (0, 3, 64), (2, 3, 0, 64)):
+        x = torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+        y, h = M.rms_norm(x, w, residual=x)
+        assert y.shape == h.shape == shape
+        q = M.rms_norm(x, w, quantize=True)
+        assert q.codes.shape == shape and q.scale.shape == (*shape[:-1], 2)
+        for rows in (x, q):
+            assert M.linear_fp4(rows, packed).shape == (*shape[:-1], 17)
+
+
 def test_outputs_apart_from_the_other_inputs(gpu):
     say("overlaps")
     buf = torch.zeros(64 * 40, dtype=torch.bfloat16, device="cuda")
