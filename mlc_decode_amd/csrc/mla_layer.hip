@@ -519,19 +519,23 @@ __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p)
   store_outputs(p, first + i, n, scale_back<XT>(p, n, sum));
 }
 
-// More rows: a workgroup takes 128 outputs (a wave 32) for 16 RT rows and a split of the chunks; the rows of kStep chunks
-// at a time go through LDS for all waves, the next ones on the way meanwhile.  64 x 7168 x 16384 (bf16, 62 MB of weights)
-// 23 us and 3 to 4 of sums.  Products and the reads of their rows from LDS, which want the whole of both units, are 11 of
-// them, loads 3, the rows' way into LDS 2, the splits' partial sums 3.  Eight waves of 256 outputs (half the rows'
-// traffic) 27.8 us in all against 27.3, that with twice as much on the way 30.8; four splits 30.9, sixteen 33.6.
+// More rows: a workgroup takes 128 outputs for 16 RT rows and a split of the chunks.  Its two halves take the steps of two
+// chunks in turns, each with its own rows in LDS, a wave 32 outputs, the next step's on the way meanwhile; the halves
+// add up through LDS.  64 x 7168 x 16384 (bf16, 62 MB of weights) 23 us and 3 to 4 of sums.  Products and the reads of
+// their rows from LDS, which want the whole of both units, are 11 of them, loads 3, the rows' way into LDS 2, the splits'
+// partial sums 2 to 3.  Two workgroups of one half each and twice the splits: 27.9 us in all against 27.2, 16384 x 2048 15.0
+// against 12.7; one workgroup of 256 outputs 27.8, that with twice as much on the way 30.8.
 template <int XT, int RT>
-__global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p) {
+__global__ __launch_bounds__(512, 1) void mla_linear_rows_kernel(LinearParams p) {
   constexpr int kStep = 2, NT = 2;
   constexpr int kParts = kStep * RT;           // 16-row chunks of a step
   constexpr int kMine = (kParts + 3) / 4;      // of a wave
-  __shared__ __attribute__((aligned(16))) uint8_t x_sh[2][kParts][kTileX<XT>];
-  __shared__ int sc_sh[2][kParts][64];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  __shared__ __attribute__((aligned(16))) uint8_t rows_sh[2][2][kParts][kTileX<XT>];
+  __shared__ int scales_sh[2][2][kParts][64];
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3), lane = threadIdx.x & 63;
+  auto& x_sh = rows_sh[half];
+  auto& sc_sh = scales_sh[half];
   const int g = lane >> 4, i = lane & 15;
   const int first = blockIdx.z * 16 * RT;
   const int c_begin = blockIdx.y * p.per_split;
@@ -565,8 +569,9 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  fetch_rows(c_begin);
-  fetch_weights(c_begin, w[0]);
+  const int c_first = c_begin + half * kStep;  // steps in turns
+  fetch_rows(c_first);
+  fetch_weights(c_first, w[0]);
   auto step = [&](int c, int b, WeightChunk (&now)[kStep][NT], WeightChunk (&next)[kStep][NT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
@@ -576,9 +581,9 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
         if constexpr (XT == kRowsFp8) sc_sh[b][part][lane] = x[m].sc;
       }
     }
-    if (c + kStep < c_end) {  // uniform
-      fetch_rows(c + kStep);
-      fetch_weights(c + kStep, next);
+    if (c + 2 * kStep < c_end) {  // uniform
+      fetch_rows(c + 2 * kStep);
+      fetch_weights(c + 2 * kStep, next);
     }
     __syncthreads();  // a buffer is written again two steps on, behind the next step's barrier
 #pragma unroll
@@ -592,10 +597,25 @@ __global__ __launch_bounds__(256, 2) void mla_linear_rows_kernel(LinearParams p)
         multiply<XT, NT>(o, x_sh[b][s * RT + r], XT == kRowsFp8 ? sc_sh[b][s * RT + r][lane] : 0, g, i, acc[r]);
     }
   };
-  for (int c = c_begin; c < c_end; c += 2 * kStep) {
+  for (int c = c_first; c - half * kStep < c_end; c += 4 * kStep) {  // as often for both halves
     step(c, 0, w[0], w[1]);
-    if (c + kStep < c_end) step(c + kStep, 1, w[1], w[0]);  // uniform
+    if (c - half * kStep + 2 * kStep < c_end) step(c + 2 * kStep, 1, w[1], w[0]);  // uniform
   }
+  // the halves' sums, in order
+  f32x4* sum_sh = (f32x4*)&rows_sh[0][0][0][0];
+  __syncthreads();
+  if (half == 1) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sum_sh[((wave * RT + r) * NT + t) * 64 + lane] = acc[r][t];
+  }
+  __syncthreads();
+  if (half == 1) return;
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[r][t] += sum_sh[((wave * RT + r) * NT + t) * 64 + lane];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if ((int64_t)blockIdx.x * 8 + 2 * wave + t >= p.tiles) continue;
@@ -628,25 +648,24 @@ __global__ __launch_bounds__(256) void mla_linear_sum_kernel(LinearParams p, int
 
 // Whether every 16 rows go by themselves: up to 16 rows, and more where the work is small, where a launch for the splits'
 // sums costs more than reading the weights from L2 for each 16.  us by themselves, and together (bf16, rows x n x k):
-//   17 x 576 x 7168 5.3, 8.4    64 x 2048 x 2048 4.2, 8.4    100 x 512 x 16384 9.8, 15.6    32 x 4096 x 4096 6.5, 9.7
-//   64 x 4096 x 4096 11.8, 13.4    32 x 7168 x 7168 16.9, 13.6    20 x 16384 x 2048 11.1, 9.9    32 x 12288 x 512 4.5, 4.0
+//   17 x 576 x 7168 5.3, 9.6    64 x 2048 x 2048 4.4, 10.8    100 x 512 x 16384 10.3, 15.8    32 x 4096 x 4096 6.6, 10.3
+//   64 x 4096 x 4096 11.9, 14.4    32 x 8192 x 4096 11.6, 11.5    32 x 7168 x 7168 16.7, 12.5    20 x 16384 x 2048 11.1, 8.3
+//   32 x 12288 x 512 4.5, 4.1    64 x 8192 x 1024 7.0, 7.5
 static bool linear_few(int64_t tokens, int64_t tiles, int64_t chunks, int cus) {
   const int64_t all = (tokens + 15) / 16 * tiles;
   return tokens <= 16 || (all <= 4 * (int64_t)cus && all * chunks <= 128 * (int64_t)cus);
 }
 
-// Splits of the chunks where rows go together: as many workgroups as two to a CU, but eight chunks each at least, four
-// where there are few of both.  us for at least 4, 8, 12 chunks (bf16): 64 x 24576 x 1536 18.3, 12.6, 12.7    64 x 16384 x
-// 2048 16.7, 14.7, 14.8    33 x 1536 x 7168 11.4, 11.4, 14.3    64 x 4096 x 4096 13.6, 13.2, 17.0    64 x 2048 x 2048 8.4, 9.7, 12.4
+// Splits of the chunks where rows go together: as many workgroups as CUs, but twelve chunks each at least, below which the
+// splits' sums cost more than the CUs give.  us for 1, 2, 3, 4, 6 splits (bf16, rows x n x k; a workgroup is 128 outputs):
+//   64 x 7168 x 16384 63.4, 38.2, 30.7, 27.2, 34.2    64 x 7168 x 7168 30.7, 21.1, 18.5, 17.0, 23.2    256 x 4096 x 4096 19.8,
+//   19.2, 24.4    64 x 16384 x 2048 12.7, 14.9    64 x 8192 x 1024 7.3, 9.3    64 x 24576 x 1536 11.8, 20.0
 static int linear_splits(int64_t tokens, int64_t tiles, int64_t chunks, int cus) {
   if (linear_few(tokens, tiles, chunks, cus)) return 1;
   const int rt = tokens <= 32 ? 2 : 4;
   const int64_t groups = (tiles + 7) / 8 * ((tokens + 16 * rt - 1) / (16 * rt));
-  int64_t s = 2 * cus / groups;
-  s = s < 1 ? 1 : s > 16 ? 16 : s;
-  const int each = 8 * groups <= cus && chunks <= 16 ? 4 : 8;
-  const int64_t most = chunks / each > 1 ? chunks / each : 1;
-  return (int)(s < most ? s : most);
+  const int64_t s = cus / groups < chunks / 12 ? cus / groups : chunks / 12;
+  return s < 1 ? 1 : s > 16 ? 16 : (int)s;
 }
 
 // Waves that share a tile of 16 outputs; us for 4, 8, 16 of them (one bf16 row unless said):
@@ -673,17 +692,16 @@ static void launch_linear(LinearParams p, int splits, int cus, hipStream_t st) {
     if (p.tokens <= 2 * kFew || 2 * kFew == 16) return launch_few<XT, 2>(p, cus, st);
     if constexpr (4 * kFew <= 16) return launch_few<XT, 4>(p, cus, st);
   }
-  // whole steps of two chunks, so that the last split is the short one
-  p.per_split = (p.chunks + splits - 1) / splits;
-  p.per_split += p.per_split & 1;
+  // whole steps of two chunks for both halves, so that the last split is the short one
+  p.per_split = ((p.chunks + splits - 1) / splits + 3) / 4 * 4;
   splits = (p.chunks + p.per_split - 1) / p.per_split;
   if (splits == 1) p.part = nullptr;
   const int rt = p.tokens <= 32 ? 2 : 4;
   const dim3 grid((p.tiles + 7) / 8, splits, (p.tokens + 16 * rt - 1) / (16 * rt));
   if (rt == 2)
-    hipLaunchKernelGGL((mla_linear_rows_kernel<XT, 2>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((mla_linear_rows_kernel<XT, 2>), grid, dim3(512), 0, st, p);
   else
-    hipLaunchKernelGGL((mla_linear_rows_kernel<XT, 4>), grid, dim3(256), 0, st, p);
+    hipLaunchKernelGGL((mla_linear_rows_kernel<XT, 4>), grid, dim3(512), 0, st, p);
   if (splits > 1) {
     const int64_t quads = (int64_t)p.tokens * 4 * p.tiles;
     hipLaunchKernelGGL(mla_linear_sum_kernel, dim3((uint32_t)((quads + 255) / 256)), dim3(256), 0, st, p, splits);

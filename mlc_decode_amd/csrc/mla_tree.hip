@@ -313,8 +313,8 @@ __device__ __forceinline__ void store_chunk(const TreeParams& p, const uint8_t* 
 
 // 64 rows, a wave 16 of them: few synchronisations, for many rows.  The waves read their own 16 queries and a quarter of
 // the keys; the queries become operands in the place that the keys take afterwards.  Drafted tokens alone are bound by latency
-// (length, table, tokens, LDS, products, store, one after the other): 32 x 256 rows 12 us (fp8), 8 x 4096 rows 19 us (bf16, 69 MB
-// in and out, 3.6 TB/s).
+// (length, table, tokens, LDS, products, store, one after the other): 32 x 256 rows 12 us (fp8), 8 x 4096 rows 19 us (bf16, 71 MB
+// in and out, 3.7 TB/s).
 template <int FMT, bool F16, int KT>
 __global__ __launch_bounds__(256, 2) void mla_tree_rows_kernel(TreeParams p) {
   constexpr int kTok = 32 * KT, kShare = kTok / 4;

@@ -357,6 +357,22 @@ def test_linear_large(gpu, kind):
         check_linear(got, xv, w, kind, f"large {kind} {T} {n} {k}")
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8"])
+@pytest.mark.parametrize("T,n,k,splits", [(17, 8200, 32, 1), (33, 6000, 160, 1), (40, 5500, 96, 1), (64, 7175, 288, 1), (100, 4112, 1696, 1), (32, 9000, 3200, 2),
+                                          (20, 3000, 16384, 10), (64, 2200, 16384, 10), (130, 1500, 16384, 7), (64, 1040, 32768, 16)])
+def test_linear_rows_together(gpu, T, n, k, splits, kind):
+    """More rows and outputs than go by themselves: both halves of a workgroup, one of them without a chunk, splits that end
+    inside a step, outputs past the last tile."""
+    ws = M._lib.load().mla_linear_workspace_bytes(T, n, k)
+    assert ws == (splits * T * -(-n // 16) * 64 if splits > 1 else 0)
+    codes, scale, w = weights(n, k, T + n + k, spread=2)
+    x, xv = rows_of(kind, T, k, T)
+    say(f"linear together {kind} T={T} n={n} k={k}")
+    got = M.linear_fp4(x, M.pack_w_fp4(codes.cuda(), scale.cuda()))
+    torch.cuda.synchronize()
+    check_linear(got, xv, w, kind, f"together {kind} T={T} n={n} k={k}")
+
+
 def test_linear_one_hot(gpu):
     """Every weight in its place: rows that pick one input each give the weights back exactly."""
     n, k = 50, 416
