@@ -620,7 +620,7 @@ typedef struct mla_linear_args {
   int64_t x_stride, x_scale_stride, y_stride;
   int32_t tokens, n, k;
   int32_t x_dtype, y_dtype; /* MLA_DTYPE_BF16 or MLA_DTYPE_F16; x_dtype is not read with x_scale */
-  int32_t reserved;
+  int32_t reserved; /* must be 0 */
   void* workspace;
   int64_t workspace_bytes;
 } mla_linear_args;

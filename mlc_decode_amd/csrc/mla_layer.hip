@@ -793,6 +793,7 @@ int mla_linear_fp4(const mla_linear_args* a, void* stream) {
   if (!linear_shape(a->tokens, a->n, a->k))
     return refuse("tokens must be in [0, 2^20], n in [1, 2^22], k a multiple of 32 in [32, 2^22]");
   if (a->y_dtype != MLA_DTYPE_BF16 && a->y_dtype != MLA_DTYPE_F16) return refuse("y_dtype must be MLA_DTYPE_BF16 or MLA_DTYPE_F16");
+  if (a->reserved != 0) return refuse("reserved must be 0");
   if (!a->x_scale && a->x_dtype != MLA_DTYPE_BF16 && a->x_dtype != MLA_DTYPE_F16)
     return refuse("x_dtype must be MLA_DTYPE_BF16 or MLA_DTYPE_F16 (or 8-bit rows with x_scale)");
   if (a->tokens == 0) return MLA_OK;

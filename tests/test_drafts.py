@@ -57,6 +57,16 @@ def test_absorb_refusals(lib):
     assert lib.mla_tree_decode_fwd(None, BASE, None) == 1 and b"NULL" in lib.mla_last_error()
 
 
+def test_takes_pages(lib):
+    """Few pages and rows, room in the workspace; nothing of a call that the decode would refuse."""
+    f = lib.mla_tree_takes_pages
+    for fmt in (0, 1, 4):
+        assert f(1, 8, 16, 256, fmt, 33) == 1 and f(1, 1, 1, 256, fmt, 1) == 1
+        assert f(1, 8, 16, 256, fmt, 258) == 0 and f(64, 8, 128, 256, fmt, 2) == 0  # slots; tiles
+        assert f(1, 8, 16, 256, fmt, 2 ** 24) == 0 and f(65535, 64, 1024, 256, fmt, 2 ** 24) == 0
+    assert f(1, 1, 1, 256, 2, 1) == 0 and f(0, 1, 1, 256, 0, 1) == 0 and f(1, 1, 1, 256, 0, 0) == 0 and f(1, 1, 1, 0, 0, 1) == 0
+
+
 def test_plan_accept_keep_refusals(lib):
     def plan(**kw):
         a = _lib.MlaTreePlanArgs()

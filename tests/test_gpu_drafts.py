@@ -258,7 +258,7 @@ def test_decode_behind_a_wide_table(gpu, fmt, H, s):
     prefixes = [0, 1, 63, 64, 65, 200, 130]
     q, cache, rows, table, plan, mask = problem(fmt, H, s, prefixes, 2000 + 10 * H + s)
     wide = table.repeat(1, -(-600 // table.shape[1]))[:, :600]
-    code = {"fp8": 1, "fp4": 2}.get(fmt, 0)
+    code = {"fp8": 1, "fp4": 4}.get(fmt, 0)
     sched = M.get_mla_metadata(plan.prefix_lens, H * s, 1, kv_cache=cache)
     lib = M._lib.load()
     assert not lib.mla_tree_takes_pages(7, s, H, sched[0].shape[0], code, 600) and api._tree_without_schedule(7, s, H, code, 600) is None

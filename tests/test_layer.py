@@ -65,7 +65,7 @@ def test_linear_refusals(lib):
 
     for kw, code, needle in [
             (dict(tokens=-1), 1, b"tokens"), (dict(tokens=(1 << 20) + 1), 1, b"tokens"), (dict(n=0), 1, b"n in"), (dict(n=(1 << 22) + 1), 1, b"n in"),
-            (dict(k=0), 1, b"multiple of 32"), (dict(k=48), 1, b"multiple of 32"), (dict(y_dtype=2), 1, b"y_dtype"), (dict(x_dtype=2), 1, b"x_dtype"),
+            (dict(k=0), 1, b"multiple of 32"), (dict(k=48), 1, b"multiple of 32"), (dict(y_dtype=2), 1, b"y_dtype"), (dict(x_dtype=2), 1, b"x_dtype"), (dict(reserved=1), 1, b"reserved"),
             (dict(x=None), 1, b"NULL"), (dict(top=None), 1, b"NULL"), (dict(y=None), 1, b"NULL"), (dict(x=BASE + 8), 1, b"16-byte"), (dict(codes=BASE + 8), 1, b"16-byte"),
             (dict(x_stride=260), 1, b"strides"), (dict(x_scale=BASE, x_stride=264), 1, b"strides"), (dict(x_scale_stride=-1), 1, b"strides"), (dict(y_stride=-2), 1, b"strides"),
             (dict(tokens=64, k=16384, n=4096), 2, b"workspace"), (dict(tokens=64, k=16384, n=4096, workspace=BASE, workspace_bytes=100, x_stride=16384), 2, b"workspace"),
