@@ -32,7 +32,7 @@ using mla_srv::unpack;
 // A piece is 16 bytes of x (8 values, 4 of fp32), or one value where rows, strides or dims do not fall on such pieces;
 // thread t of a row holds pieces t, t + threads, ...  P of them.
 // Bound by memory for many rows, by latency for few (row, sum, barrier): 1 x 7168 with the residual 2.9 us, 256 rows 4.1,
-// 1024 rows 11.0 (5.3 TB/s), 8192 rows 96 (4.9; to 16 bits without a residual 42.7, 5.5), 65536 x 512 40 us, 6.7 TB/s.
+// 1024 rows 11.0 (5.3 TB/s), 8192 rows 96 (4.9; to 16 bits without a residual 42.7, 5.5), 65536 x 512 39 us, 6.9 TB/s; 65536 x 128 12.8, 5.2.
 struct NormParams {
   const uint8_t* x;
   const uint8_t* residual;  // may be NULL
@@ -122,13 +122,13 @@ __device__ __forceinline__ void store_codes(const NormParams& p, int64_t row, in
   if (dim % 32 == 0) p.scale[row * (p.dim / 32) + dim / 32] = bad ? 255 : (uint8_t)(k + 127);
 }
 
-// One row by T threads; 256 / T rows a workgroup where T < 256.
+// One row by T threads; 256 / T rows a workgroup where T < 256, 64 / T rows a wave where T < 64.
 template <class E, int V, int T, int P>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void mla_rms_norm_kernel(NormParams p) {
   constexpr int kRows = T < 256 ? 256 / T : 1;
-  constexpr int kWaves = T / 64;
+  constexpr int kWaves = T > 64 ? T / 64 : 1;
   __shared__ float sum_sh[kRows][kWaves];
-  const int sub = kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0;
+  const int sub = T < 64 ? (int)threadIdx.x / T : kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0;
   const int t = kRows > 1 ? threadIdx.x % T : threadIdx.x;
   const int64_t row = (int64_t)blockIdx.x * kRows + sub;
   const bool on = row < p.tokens;  // uniform over a row's threads
@@ -168,7 +168,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void mla_rms_norm_kernel(NormPar
 #pragma unroll
     for (int j = 0; j < V; ++j) sum += h[i][j] * h[i][j];
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+  for (int d = T < 64 ? T / 2 : 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
   if constexpr (kWaves > 1) {
     if ((t & 63) == 0) sum_sh[sub][t >> 6] = sum;
     __syncthreads();
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void mla_rms_norm_kernel(NormPar
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) sum += sum_sh[sub][i];
   }
-  if (!on) return;  // a wave belongs to one row
+  if (!on) return;  // a row's threads together
   const float f = 1.f / sqrtf(sum * p.inv_dim + p.eps);
 #pragma unroll
   for (int i = 0; i < P; ++i) {
@@ -252,6 +252,10 @@ static void launch_norm_as(const NormParams& p, hipStream_t st) {
 template <class E, int V>
 static void launch_norm(const NormParams& p, int cus, hipStream_t st) {
   const int pieces = p.dim / V;
+  // Short rows share a wave; us for a wave a row and so (bf16): 65536 x 64 14.2, 4.2    x 128 14.6, 6.3    x 256 18.1, 13.0
+  if (pieces <= 8) return launch_norm_as<E, V, 8, 1>(p, st);
+  if (pieces <= 16) return launch_norm_as<E, V, 16, 1>(p, st);
+  if (pieces <= 32) return launch_norm_as<E, V, 32, 1>(p, st);
   if (pieces <= 64) return launch_norm_as<E, V, 64, 1>(p, st);
   if (pieces <= 128) return launch_norm_as<E, V, 64, 2>(p, st);
   if (pieces <= 256) return launch_norm_as<E, V, 256, 1>(p, st);

@@ -114,6 +114,31 @@ def check_norm8(x, w, eps, residual, got, what):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [3, 16, 25, 36, 64, 65, 72, 128, 130, 160, 256, 264])
+def test_norm_of_short_rows(gpu, D, dt):
+    """Several rows a wave, the last wave with fewer; heads of a token, rows out of wider ones; a row of NaN beside others."""
+    for T, pitch in ((7, D), (33, D), (129, D + 5), (1000, D + 64)):
+        x, r, w = tensors(T, D, DT[dt], pitch, D + T)
+        ww = w.to(DT[dt]).cuda()
+        say(f"norm of short rows D={D} {dt} T={T} pitch={pitch}")
+        a, b = M.rms_norm(x, ww), M.rms_norm(x, ww, 1e-3, residual=r)
+        torch.cuda.synchronize()
+        check_norm(x, ww, 1e-6, None, a, "plain")
+        check_norm(x, ww, 1e-3, r, b, "residual")
+        if D % 32 == 0:
+            c, d = M.rms_norm(x, ww, quantize=True), M.rms_norm(x, ww, residual=r, quantize=True)
+            torch.cuda.synchronize()
+            check_norm8(x, ww, 1e-6, None, c, "plain")
+            check_norm8(x, ww, 1e-6, r, d, "residual")
+            check_sum(exact_norm(x, ww, 1e-6, r)[0], d[1], "residual")
+        spoilt = x.clone()
+        spoilt[5, D // 2] = float("nan")
+        e, f = M.rms_norm(spoilt, ww), M.rms_norm(x.clone(), ww)  # in one layout: the order of a row's sum is the layout's
+        torch.cuda.synchronize()
+        assert e[5].isnan().all() and torch.equal(e[:5], f[:5]) and torch.equal(e[6:], f[6:])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("D", [32, 64, 96, 512, 544, 1536, 2048, 2080, 4096, 7168, 8192, 8224, 16384, 20000 // 32 * 32, 40000])
 def test_norm_8bit(gpu, D, dt):
     for T, pitch in ((1, D), (6, D), (3, D + 5)):
