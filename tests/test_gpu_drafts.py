@@ -558,6 +558,30 @@ def test_other_streams_and_graphs(gpu):
             assert all(torch.equal(t, u) for t, u in zip(again, want[0]))
 
 
+@pytest.mark.parametrize("width", [0, 600])
+def test_two_streams_at_once(gpu, width):
+    """Decodes of different problems queued on two streams without a wait between them: each its own workspace, whether
+    pages go by themselves or the schedule is followed."""
+    jobs = []
+    for seed, (H, s) in ((67, (16, 6)), (71, (32, 9))):
+        q, cache, rows, table, plan, mask = problem("bf16", H, s, [300, 64, 5, 0], seed)
+        if width:
+            table = table.repeat(1, -(-width // table.shape[1]))[:, :width]
+        jobs.append((q, cache, table, plan))
+    want = [[t.clone() for t in M.mla_decode_with_kvcache(q, c, t, None, tree=p)] for q, c, t, p in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[], []]
+    say(f"two streams, width {width}")
+    for _ in range(20):
+        for st, (q, c, t, p), res in zip(streams, jobs, got):
+            with torch.cuda.stream(st):
+                res.append(M.mla_decode_with_kvcache(q, c, t, None, tree=p))
+    torch.cuda.synchronize()
+    for res, w in zip(got, want):
+        assert all(torch.equal(x, y) for r in res for x, y in zip(r, w))
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
 def test_whole_step(gpu, fmt):
     """Reserve, plan, append, decode, accept, keep, release: afterwards the cache holds the prefix and the kept tokens, in
