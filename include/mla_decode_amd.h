@@ -601,8 +601,9 @@ int mla_rms_norm(const mla_rms_norm_args* args, void* stream);
  * Projection of few rows by 4-bit weights: y[t, m] = sum_j x[t, j] * w[m, j], m < n, j < k, with
  * w[m, j] = e2m1(code) * 2^(s - 127), a scale byte s (1 .. 254; 255 makes output m NaN) per output and 32 inputs.
  * Sums in fp32, one rounding to y_dtype.  Rows are 16-bit (x_dtype), or with x_scale e4m3 codes whose scales, a byte per
- * 32 values, are at x_scale + t * x_scale_stride (mla_rms_norm's).  bf16 and 8-bit rows take the weights exactly; with fp16
- * rows, weights below 2^-35 of the largest of their output are lost.
+ * 32 values, are at x_scale + t * x_scale_stride (mla_rms_norm's); they are taken as the bf16 values that they stand for, all
+ * exact but for what bf16 has no room for (2^128 and more: an infinity; bits below 2^-133: lost).  bf16 and 8-bit rows take
+ * the weights exactly; with fp16 rows, weights below 2^-35 of the largest of their output are lost.
  * The weights are laid out in tiles of 16 outputs (T = ceil(n / 16)) and chunks of 128 inputs (C = ceil(k / 128)): lane
  * 16 g + i of a tile and chunk holds output i's codes of inputs 32 g .. 32 g + 31 (two a byte, the lower input in the low
  * half), and their scale byte; outputs and inputs past the end are codes 0, scale 127:

@@ -287,13 +287,15 @@ static void launch_norm_type(const NormParams& p, bool vec, int cus, hipStream_t
 // y[t, n] = sum_k x[t, k] w[n, k], w[n, k] = e2m1(code) * 2^(s[n, k / 32] - 127), for few rows t: the weights are read
 // once, 17 bits for 32 of them, and that is what bounds it.  They are laid out as the operand of the matrix unit: of
 // 16 outputs x 128 inputs (a chunk), lane (g, i) holds inputs 32 g .. +31 of output i, 16 bytes; the scale bytes alike.
-//   16-bit rows: 8 codes become 8 bf16 (exact) or fp16, four 16x16x32 MFMAs a chunk.  fp16 has no room for a scale's
-//     range: a row's scales are taken relative to its largest, 2^11, and the output is multiplied back; what lies 2^-35
-//     below the largest of its row is lost there.
-//   8-bit rows: one block-scaled 16x16x128 MFMA a chunk, codes and scales as they are.
+//   8 codes become 8 bf16 (exact) or fp16, four 16x16x32 MFMAs a chunk.  fp16 has no room for a scale's range: a row's
+//     scales are taken relative to its largest, 2^11, and the output is multiplied back; what lies 2^-35 below the
+//     largest of its row is lost there.
+//   8-bit rows become bf16 rows on their way into LDS: e4m3 has 4 significant bits, so every value inside bf16's range is
+//     exact.  The block-scaled 16x16x128 MFMA would take both sides' codes and scales as they are, but it adds its products
+//     in groups of eight within about 13 bits below the largest: 448 * 6 less itself beside six products of 2^-8 gives 0.
+//     Faster it is: 8 x 24576 x 1536 4.6 us against 6.0, 64 x 7168 x 16384 20.4 against 25.8.
 // A lane of a result holds outputs 4 g .. +3 of row i.  Everything is summed in fp32.
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((__vector_size__(8 * sizeof(__bf16))));
 typedef _Float16 f16x8 __attribute__((__vector_size__(8 * sizeof(_Float16))));
 
@@ -313,70 +315,73 @@ struct LinearParams {
   int32_t y_f16, y_vec;    // y_vec: rows of y take 8-byte stores
 };
 
-template <int XT>
-constexpr int kChunkBytes = XT == kRowsFp8 ? 128 : 256;  // of a row
-template <int XT>
-constexpr int kTileX = 16 * kChunkBytes<XT>;  // 16 rows of a chunk in LDS
+constexpr int kTileX = 16 * 256;  // 16 rows of a chunk in LDS, 16-bit values
 
-// A piece of 16 bytes of a row's chunk (p of 16 or 8): its place in the 16 rows' chunk in LDS.  Blocks of 256 bytes hold
-// what one lane group of an operand reads, the rows' order in them turned by the piece, so that both the writes (pieces of
-// one row or two) and the reads (16 rows) go over all banks.
-template <int XT>
-__device__ __forceinline__ int piece_place(int p, int row) {
-  if constexpr (XT == kRowsFp8)
-    return p * 256 + ((row ^ (2 * p)) << 4);  // operand half p / 4 (inputs 64 h + 16 g), lane group p % 4
-  else
-    return (p & 3) * 1024 + (p >> 2) * 256 + ((row ^ p) << 4);  // MFMA p % 4, lane group p / 4 (inputs 32 g + 8 j)
-}
-// The operand of MFMA j (of half j) for lane (g, i).
-template <int XT>
+// A piece of 16 bytes of a row's chunk in LDS (p of 16): its place in the 16 rows' chunk.  Blocks of 256 bytes hold what one
+// lane group of an operand reads, MFMA p % 4, lane group p / 4 (inputs 32 g + 8 j), the rows' order in them turned by the
+// piece, so that both the writes (pieces of a few rows) and the reads (16 rows) go over all banks.
+__device__ __forceinline__ int piece_place(int p, int row) { return (p & 3) * 1024 + (p >> 2) * 256 + ((row ^ p) << 4); }
+// The operand of MFMA j for lane (g, i).
 __device__ __forceinline__ i32x4 read_piece(const uint8_t* tile, int j, int g, int i) {
-  const int p = XT == kRowsFp8 ? 4 * j + g : 4 * g + j;
-  return *(const i32x4*)(tile + piece_place<XT>(p, i));
+  return *(const i32x4*)(tile + piece_place(4 * g + j, i));
 }
 
-// Registers of the first LOADS * kEach rows of a 16-row chunk, by one wave.  Rows past the last are the last again: they are
-// columns of the product that nothing reads.
+// Registers of the first LOADS * kEach rows of a 16-row chunk, by one wave, 16 bytes a lane and load.  Rows past the last are
+// the last again: they are columns of the product that nothing reads.
 template <int XT, int LOADS>
 struct RowsChunk {
   i32x4 v[LOADS];
-  int sc;  // 8-bit rows: lane (g, i)'s scale byte
+  int sc[XT == kRowsFp8 ? LOADS : 1];  // 8-bit rows: the scale byte of v's 16 codes
 };
 template <int XT>
-constexpr int kPieces = kChunkBytes<XT> / 16;  // of a row's chunk
+constexpr int kPieces = XT == kRowsFp8 ? 8 : 16;  // of 16 bytes, of a row's chunk in memory
 template <int XT>
 constexpr int kEach = 64 / kPieces<XT>;  // rows of a load
 template <int XT, int LOADS>
 __device__ __forceinline__ void load_rows(const LinearParams& p, int first, int chunk, int lane, RowsChunk<XT, LOADS>& c) {
   const int piece = lane % kPieces<XT>;
   const int most = p.k / (XT == kRowsFp8 ? 16 : 8) - 1;  // the last piece of a row
-  const int at = chunk * kPieces<XT> + piece;
-  const uint8_t* src = p.x + 16 * (int64_t)(at < most ? at : most);
+  int at = chunk * kPieces<XT> + piece;
+  at = at < most ? at : most;
+  const uint8_t* src = p.x + 16 * (int64_t)at;
 #pragma unroll
   for (int q = 0; q < LOADS; ++q) {
     int row = first + kEach<XT> * q + lane / kPieces<XT>;
     row = row < p.tokens ? row : p.tokens - 1;
     c.v[q] = *(const i32x4*)(src + row * p.x_st);
-  }
-  if constexpr (XT == kRowsFp8) {
-    int row = first + (lane & 15), block = 4 * chunk + (lane >> 4);
-    row = row < p.tokens ? row : p.tokens - 1;
-    block = 32 * block < p.k ? block : p.k / 32 - 1;
-    c.sc = p.x_scale[row * p.xs_st + block];
+    if constexpr (XT == kRowsFp8) c.sc[q] = p.x_scale[row * p.xs_st + at / 2];
   }
 }
 // To LDS.  Pieces past the row's end are zeros (their weights are, but an infinity times 0 is a NaN).
 template <int XT, int LOADS>
 __device__ __forceinline__ void put_rows(const LinearParams& p, uint8_t* tile, int chunk, int lane, RowsChunk<XT, LOADS>& c) {
-  if (chunk * 128 + 128 > p.k) {  // uniform
-    if (chunk * 128 + lane % kPieces<XT> * (XT == kRowsFp8 ? 16 : 8) >= p.k)
+  const int piece = lane % kPieces<XT>;
+  const bool past = chunk * 128 + piece * (XT == kRowsFp8 ? 16 : 8) >= p.k;
+  if (chunk * 128 + 128 > p.k)  // uniform
 #pragma unroll
-      for (int q = 0; q < LOADS; ++q) c.v[q] = i32x4{0, 0, 0, 0};
-    if (XT == kRowsFp8 && chunk * 128 + 32 * (lane >> 4) >= p.k) c.sc = 127;
+    for (int q = 0; q < LOADS; ++q) {
+      if (past) c.v[q] = i32x4{0, 0, 0, 0};
+      if (XT == kRowsFp8 && past) c.sc[q] = 127;
+    }
+#pragma unroll
+  for (int q = 0; q < LOADS; ++q) {
+    const int row = kEach<XT> * q + lane / kPieces<XT>;
+    if constexpr (XT == kRowsFp8) {
+      const float sc = __uint_as_float((uint32_t)c.sc[q] << 23);  // the conversion takes its exponent alone
+      const int nan = c.sc[q] == 255 ? 0x7F7F7F7F : 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int a = c.v[q][2 * h] | nan, b = c.v[q][2 * h + 1] | nan;
+        *(i32x4*)(tile + piece_place(2 * piece + h, row)) =
+            i32x4{__builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, false)),
+                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, sc, true)),
+                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, false)),
+                  __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, sc, true))};
+      }
+    } else {
+      *(i32x4*)(tile + piece_place(piece, row)) = c.v[q];
+    }
   }
-#pragma unroll
-  for (int q = 0; q < LOADS; ++q)
-    *(i32x4*)(tile + piece_place<XT>(lane % kPieces<XT>, kEach<XT> * q + lane / kPieces<XT>)) = c.v[q];
 }
 
 struct WeightChunk {
@@ -389,17 +394,12 @@ __device__ __forceinline__ void load_weights(const LinearParams& p, int64_t tile
   w.sc = p.scale[at];
 }
 // The weights of one chunk as operands.
-template <int XT>
 struct Operand {
-  i32x4 a[XT == kRowsFp8 ? 1 : 4];
-  int sc;
+  i32x4 a[4];
 };
 template <int XT>
-__device__ __forceinline__ void widen(const WeightChunk& w, int up, Operand<XT>& o) {
-  if constexpr (XT == kRowsFp8) {
-    o.a[0] = w.codes;
-    o.sc = w.sc;
-  } else if constexpr (XT == kRowsBf16) {
+__device__ __forceinline__ void widen(const WeightChunk& w, int up, Operand& o) {
+  if constexpr (XT != kRowsF16) {
     const float sc = __uint_as_float((uint32_t)w.sc << 23);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -425,26 +425,16 @@ __device__ __forceinline__ void widen(const WeightChunk& w, int up, Operand<XT>&
 }
 // acc[t] += the weights of tile t times 16 rows of a chunk, each operand of the rows read once.
 template <int XT, int NT>
-__device__ __forceinline__ void multiply(const Operand<XT> (&w)[NT], const uint8_t* tile, int x_sc, int g, int i, f32x4 (&acc)[NT]) {
-  if constexpr (XT == kRowsFp8) {
-    const i32x4 lo = read_piece<XT>(tile, 0, g, i), hi = read_piece<XT>(tile, 1, g, i);
-    const i32x8 b = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+__device__ __forceinline__ void multiply(const Operand (&w)[NT], const uint8_t* tile, int g, int i, f32x4 (&acc)[NT]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const i32x4 b = read_piece(tile, j, g, i);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const i32x8 a = {w[t].a[0][0], w[t].a[0][1], w[t].a[0][2], w[t].a[0][3], 0, 0, 0, 0};
-      acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[t], 4, 0, 0, w[t].sc, 0, x_sc);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const i32x4 b = read_piece<XT>(tile, j, g, i);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        if constexpr (XT == kRowsBf16)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[t].a[j]), __builtin_bit_cast(bf16x8, b), acc[t], 0, 0, 0);
-        else
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w[t].a[j]), __builtin_bit_cast(f16x8, b), acc[t], 0, 0, 0);
-      }
+      if constexpr (XT == kRowsF16)
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w[t].a[j]), __builtin_bit_cast(f16x8, b), acc[t], 0, 0, 0);
+      else
+        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w[t].a[j]), __builtin_bit_cast(bf16x8, b), acc[t], 0, 0, 0);
     }
   }
 }
@@ -474,12 +464,12 @@ __device__ __forceinline__ f32x4 scale_back(const LinearParams& p, int n, f32x4 
 
 // 16 rows (the first LOADS * kEach of them).  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no
 // barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.  Bound by
-// the weights: 8 x 24576 x 1536 (8-bit rows) 5.6 us, 3.6 TB/s; 1 x 7168 x 16384 12.3 us, 5.1 TB/s; one of 576 x 7168 4.0, a
+// the weights: 8 x 24576 x 1536 (8-bit rows) 6.0 us, 3.3 TB/s; 1 x 7168 x 16384 12.3 us, 5.1 TB/s; one of 576 x 7168 4.0, a
 // load's latency over and over.
 template <int XT, int LOADS, int WK>
 __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p) {
   constexpr int kDepth = LOADS == 4 && WK >= 8 ? 2 : 4;  // 128 registers: two workgroups of 8 waves a CU
-  __shared__ __attribute__((aligned(16))) uint8_t x_sh[WK][2][kTileX<XT>];
+  __shared__ __attribute__((aligned(16))) uint8_t x_sh[WK][2][kTileX];
   __shared__ f32x4 sum_sh[WK][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int g = lane >> 4, i = lane & 15;
@@ -503,13 +493,12 @@ __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p)
       const int c = c0 + s * WK;
       if (c < p.chunks) {  // uniform
         uint8_t* xt = x_sh[wave][s & 1];
-        Operand<XT> o[1];
+        Operand o[1];
         put_rows<XT, LOADS>(p, xt, c, lane, x[s]);
         widen<XT>(w[s], up, o[0]);
-        const int x_sc = x[s].sc;
         fetch(c + kDepth * WK, s);
         __builtin_amdgcn_wave_barrier();  // the wave's own rows: LDS runs its accesses in order
-        multiply<XT, 1>(o, xt, x_sc, g, i, acc[s & 1]);
+        multiply<XT, 1>(o, xt, g, i, acc[s & 1]);
       }
     }
   }
@@ -534,12 +523,10 @@ __global__ __launch_bounds__(512, 1) void mla_linear_rows_kernel(LinearParams p)
   constexpr int kStep = 2, NT = 2;
   constexpr int kParts = kStep * RT;           // 16-row chunks of a step
   constexpr int kMine = (kParts + 3) / 4;      // of a wave
-  __shared__ __attribute__((aligned(16))) uint8_t rows_sh[2][2][kParts][kTileX<XT>];
-  __shared__ int scales_sh[2][2][kParts][64];
+  __shared__ __attribute__((aligned(16))) uint8_t rows_sh[2][2][kParts][kTileX];
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
   const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) & 3), lane = threadIdx.x & 63;
   auto& x_sh = rows_sh[half];
-  auto& sc_sh = scales_sh[half];
   const int g = lane >> 4, i = lane & 15;
   const int first = blockIdx.z * 16 * RT;
   const int c_begin = blockIdx.y * p.per_split;
@@ -580,10 +567,7 @@ __global__ __launch_bounds__(512, 1) void mla_linear_rows_kernel(LinearParams p)
 #pragma unroll
     for (int m = 0; m < kMine; ++m) {
       const int part = 4 * m + wave;
-      if (kParts % 4 == 0 || part < kParts) {
-        put_rows<XT, kLoads>(p, x_sh[b][part], c + part / RT, lane, x[m]);
-        if constexpr (XT == kRowsFp8) sc_sh[b][part][lane] = x[m].sc;
-      }
+      if (kParts % 4 == 0 || part < kParts) put_rows<XT, kLoads>(p, x_sh[b][part], c + part / RT, lane, x[m]);
     }
     if (c + 2 * kStep < c_end) {  // uniform
       fetch_rows(c + 2 * kStep);
@@ -593,12 +577,12 @@ __global__ __launch_bounds__(512, 1) void mla_linear_rows_kernel(LinearParams p)
 #pragma unroll
     for (int s = 0; s < kStep; ++s) {
       if (c + s >= c_end) break;  // uniform
-      Operand<XT> o[NT];
+      Operand o[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) widen<XT>(now[s][t], up[t], o[t]);
 #pragma unroll
       for (int r = 0; r < RT; ++r)
-        multiply<XT, NT>(o, x_sh[b][s * RT + r], XT == kRowsFp8 ? sc_sh[b][s * RT + r][lane] : 0, g, i, acc[r]);
+        multiply<XT, NT>(o, x_sh[b][s * RT + r], g, i, acc[r]);
     }
   };
   for (int c = c_first; c - half * kStep < c_end; c += 4 * kStep) {  // as often for both halves

@@ -230,8 +230,8 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
     """``y [..., n] = x [..., k] . w^T`` for few rows: decode steps, drafted tokens.
 
     ``x`` in bf16 or fp16, or :class:`Fp8Rows` (from :func:`rms_norm`).  Sums are fp32, rounded once to ``dtype`` (bf16 or
-    fp16; x's by default, bf16 of 8-bit rows).  bf16 and 8-bit rows take the weights exactly; with fp16 rows weights
-    below ``2**-35`` of the largest of their output are lost.  The leading dims must be one stride apart; rows that do not
+    fp16; x's by default, bf16 of 8-bit rows).  8-bit rows are taken as bf16 values, exactly inside bf16's range; bf16 and
+    8-bit rows take the weights exactly; with fp16 rows weights below ``2**-35`` of the largest of their output are lost.  The leading dims must be one stride apart; rows that do not
     start on 16 bytes are copied first.  ``out`` (unit stride in its rows) may not overlap ``x``.  Memory gives the weights
     once for up to 64 rows, so a few rows cost little more than one; it takes up to 2**20."""
     coded = isinstance(x, Fp8Rows)

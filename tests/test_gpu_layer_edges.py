@@ -1,0 +1,117 @@
+"""GPU tests of the operators around the attention where every sum is exact: no tolerance hides a term that is lost, taken
+twice or in another's place."""
+import sys
+
+import pytest
+import torch
+
+import mlc_decode_amd as M
+
+pytestmark = pytest.mark.gpu
+
+E2M1 = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, -0.0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
+DT = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def say(msg):
+    print(f"[gpu-layer-edges] {msg}", flush=True)
+    sys.stdout.flush()
+
+
+def packed(codes, scale):
+    """Weights from codes 0 .. 15 [n, k] and scale bytes [n, k / 32], and their values in 64 bits."""
+    w = E2M1[codes] * torch.exp2(scale.double() - 127).repeat_interleave(32, 1)
+    return M.pack_w_fp4((codes[:, 0::2] | codes[:, 1::2] << 4).to(torch.uint8).cuda(), scale.to(torch.uint8).cuda()), w
+
+
+def given(x, kind):
+    """Rows of 64-bit values as linear_fp4 takes them; 8-bit ones with scales 2^-1 .. 2^1 in turns."""
+    if kind != "fp8":
+        assert torch.equal(x.to(DT[kind]).double(), x)
+        return x.to(DT[kind]).cuda()
+    s = 126 + torch.arange(x.shape[0] * x.shape[1] // 32).view(x.shape[0], -1) % 3
+    v = x * torch.exp2(127 - s.double()).repeat_interleave(32, 1)
+    codes = v.to(torch.float8_e4m3fn)
+    assert torch.equal(codes.double(), v)
+    return M.Fp8Rows(codes.view(torch.uint8).cuda(), s.to(torch.uint8).cuda())
+
+
+def exactly(T, n, k, kind, seed):
+    """(rows, weights, y in 64 bits).  Values of the rows are multiples of 1/2 up to 3 and pairs of +-224 eight inputs apart or
+    fewer, those of the weights multiples of 1/4 up to 12 of one size in a pair's places, so that what is left of 224 * 12 less
+    itself is the small products'.  All products are multiples of 2^-3 and their sizes add up to less than 2^21: every sum of some of them, in any order, is exact in fp32."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randint(-6, 7, (T, k), generator=g).double() / 2
+    codes = torch.randint(0, 16, (n, k), generator=g)
+    for a in range(0, k - 8, max(32, k // 24 // 8 * 8)):  # a pair in each of some groups of eight
+        i, j = a + int(torch.randint(0, 4, (1,), generator=g)), a + int(torch.randint(4, 8, (1,), generator=g))
+        x[:, i], x[:, j] = 224.0, -224.0
+        codes[:, i] = codes[:, j]
+    scale = torch.randint(126, 129, (n, k // 32), generator=g)
+    p, w = packed(codes, scale)
+    assert (x.abs() @ w.abs().T).max() < 2 ** 21
+    return given(x, kind), p, x @ w.T
+
+
+SHAPES = [(1, 576, 7168), (3, 2064, 16384), (16, 100, 7168), (8, 25600, 160), (17, 576, 7168),     # by themselves, 4, 8 and 16 waves
+          (32, 12288, 512), (17, 8200, 32), (33, 6000, 160), (40, 5500, 96), (64, 7175, 288),        # together, one split
+          (32, 9000, 3200), (20, 3000, 16384), (64, 2200, 16384), (130, 1500, 16384), (64, 1040, 32768), (200, 2100, 7168 + 96)]
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16", "fp8"])
+@pytest.mark.parametrize("T,n,k", SHAPES)
+def test_linear_exact(gpu, T, n, k, kind):
+    """Outputs are the exact sums, rounded once: every product in its place, none lost beside larger ones."""
+    rows, p, y = exactly(T, n, k, kind, T + n + k)
+    for dtype in (torch.bfloat16, torch.float16):
+        say(f"exact {kind} T={T} n={n} k={k} to {dtype}")
+        got = M.linear_fp4(rows, p, dtype=dtype)
+        torch.cuda.synchronize()
+        want = y.to(dtype)
+        assert torch.equal(got.cpu(), want), f"{(got.cpu() != want).sum().item()} of {want.numel()} differ"
+
+
+@pytest.mark.parametrize("T", [1, 5, 9, 16, 40])
+def test_linear_8bit_small_products_beside_large_ones(gpu, T):
+    """An outlier's products cancel and leave those of its neighbours, 2^19 times smaller, whole: 448 * 6 and 2^-8."""
+    k, n = 64, 16 if T <= 16 else 16 * 1100
+    x = torch.zeros(T, k, dtype=torch.float64)
+    codes = torch.zeros(n, k, dtype=torch.long)
+    for j in range(0, k, 8):
+        x[:, j], x[:, j + 3], x[:, j + 1:j + 3], x[:, j + 4:j + 8] = 448.0, -448.0, 2.0 ** -7, 2.0 ** -7
+        codes[:, [j, j + 3]], codes[:, j + 1:j + 3], codes[:, j + 4:j + 8] = 7, 1, 1  # 6, and 0.5
+    p, w = packed(codes, torch.full((n, k // 32), 127))
+    rows = M.Fp8Rows(x.to(torch.float8_e4m3fn).view(torch.uint8).cuda(), torch.full((T, k // 32), 127, dtype=torch.uint8, device="cuda"))
+    y = x @ w.T
+    assert (y == 48 * 2.0 ** -8).all()
+    say(f"outliers T={T}")
+    got = M.linear_fp4(rows, p)
+    torch.cuda.synchronize()
+    assert (got.double().cpu() == y).all(), got[0, :4]
+
+
+@pytest.mark.parametrize("T", [4, 40])
+def test_linear_8bit_scales_one_hot(gpu, T):
+    """A code of each size at scales over bf16's range, in every block of a row: rows that pick one input each; a scale byte
+    of 255 is a NaN whatever its codes, and of its own row alone."""
+    k, n = 160, 64 if T <= 16 else 16 * 1100
+    p, w = packed(torch.full((n, k), 2), torch.full((n, k // 32), 127))
+    x = torch.zeros(T, k, dtype=torch.uint8)
+    s = torch.full((T, k // 32), 127, dtype=torch.uint8)
+    g = torch.Generator().manual_seed(T)
+    codes = torch.randint(1, 127, (T,), generator=g)
+    at = torch.randint(0, k, (T,), generator=g)
+    for t in range(T):
+        x[t, at[t]] = codes[t]
+        s[t, at[t] // 32] = 12 + (t * 37) % 230  # 2^-115 .. 2^114: with codes of 2^-9 .. 448 inside bf16's normal numbers
+    want = x.view(torch.float8_e4m3fn).double() * torch.exp2(s.double() - 127).repeat_interleave(32, 1)
+    want = want.sum(1, keepdim=True).expand(T, n)
+    rows = M.Fp8Rows(x.cuda(), s.cuda())
+    say(f"scales T={T}")
+    got = M.linear_fp4(rows, p)
+    torch.cuda.synchronize()
+    assert torch.equal(got.double().cpu(), want)
+    rows.scale[1, 4] = 255  # its codes are zeros, or one
+    bad = M.linear_fp4(rows, p)
+    torch.cuda.synchronize()
+    assert bad[1].isnan().all() and torch.equal(bad[0], got[0]) and torch.equal(bad[2:], got[2:])
