@@ -607,7 +607,8 @@ int mla_rms_norm(const mla_rms_norm_args* args, void* stream);
  * The weights are laid out in tiles of 16 outputs (T = ceil(n / 16)) and chunks of 128 inputs (C = ceil(k / 128)): lane
  * 16 g + i of a tile and chunk holds output i's codes of inputs 32 g .. 32 g + 31 (two a byte, the lower input in the low
  * half), and their scale byte; outputs and inputs past the end are codes 0, scale 127:
- *   codes [T][C][64][16] (16-byte aligned),  scale [T][C][64],  top [16 T]: the largest scale byte of each output.
+ *   codes [T][C][64][16] (16-byte aligned),  scale [T][C][64],  top [16 T]: the largest scale byte of each output (of its
+ *   k inputs; 255 as 1; outputs past the end: any).
  * tokens at most 2^20, n at most 2^22, k a multiple of 32, at most 2^22.  Strides in elements (x's a multiple of 16 bytes,
  * x 16-byte aligned); workspace: mla_linear_workspace_bytes (0: none), 16-byte aligned, of this call alone while it runs.
  */

@@ -410,8 +410,10 @@ __device__ __forceinline__ void widen(const WeightChunk& w, int up, Operand& o) 
                      __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, sc, 3))};
     }
   } else {
-    // up = 138 - the row's largest byte: that one becomes 2^11; 255 stays (a NaN)
-    const int e = w.sc == 255 ? 255 : w.sc + up > 1 ? w.sc + up : 1;
+    // up = 138 - the row's largest byte: that one becomes 2^11; 255 stays (a NaN).  Inputs past the end, zeros of a scale
+    // that has no part in that largest, stay zeros.
+    const int to = w.sc + up < 254 ? w.sc + up : 254;
+    const int e = w.sc == 255 ? 255 : to > 1 ? to : 1;
     const float sc = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -168,7 +168,7 @@ def _norm_overlaps(x, residual, weight, out, residual_out, rows, strides) -> Non
 class Fp4Weight(NamedTuple):
     """Weights ``[n, k]`` in 4 bits, as ``linear_fp4`` reads them: ``codes`` uint8 ``[ceil(n / 16), ceil(k / 128), 64, 16]``
     (OCP e2m1), ``scale`` uint8 ``[ceil(n / 16), ceil(k / 128), 64]`` (a power of two per output and 32 inputs) and ``top``
-    uint8 ``[16 * ceil(n / 16)]``, each output's largest scale.  Made by :func:`quantize_w_fp4` or :func:`pack_w_fp4`."""
+    uint8 ``[16 * ceil(n / 16)]``, each output's largest scale (255, a NaN block's, as 1).  Made by :func:`quantize_w_fp4` or :func:`pack_w_fp4`."""
     codes: torch.Tensor
     scale: torch.Tensor
     top: torch.Tensor
@@ -190,9 +190,10 @@ def pack_w_fp4(codes: torch.Tensor, scale: torch.Tensor) -> Fp4Weight:
     c[:n, :k // 2] = codes
     s = torch.full((16 * tiles, 4 * chunks), 127, dtype=torch.uint8, device=codes.device)
     s[:n, :k // GROUP] = scale.clamp(min=1)
-    top = torch.where(s == 255, 1, s).amax(1)
+    top = torch.full((16 * tiles,), 127, dtype=torch.uint8, device=codes.device)
+    top[:n] = torch.where(s == 255, 1, s)[:n, :k // GROUP].amax(1)
     return Fp4Weight(c.view(tiles, 16, chunks, 4, 16).permute(0, 2, 3, 1, 4).contiguous().view(tiles, chunks, 64, 16),
-                     s.view(tiles, 16, chunks, 4).permute(0, 2, 3, 1).contiguous().view(tiles, chunks, 64), top.contiguous(), n, k)
+                     s.view(tiles, 16, chunks, 4).permute(0, 2, 3, 1).contiguous().view(tiles, chunks, 64), top, n, k)
 
 
 def quantize_w_fp4(w: torch.Tensor) -> Fp4Weight:

@@ -1,0 +1,83 @@
+"""GPU tests of the tree decode in every one of its forms: what cache rows hold that a query row does not see reaches no bit of
+it, whether the rows are drafted tokens or lie behind the last one."""
+import pytest
+import torch
+
+import mlc_decode_amd as M
+from test_gpu_drafts import INF, NAN, ints, problem, say
+
+pytestmark = pytest.mark.gpu
+
+# (heads, drafted tokens, columns of the table, 64 rows a workgroup): pages by themselves, and the schedule's pass before
+# the drafted tokens, which are one tile of 32 or 64 keys there
+FORMS = [(16, 9, 0, False), (64, 9, 0, True), (16, 9, 600, False), (128, 14, 600, True), (16, 40, 600, False), (48, 40, 600, True)]
+
+
+def spoil(cache, fmt, slot, n):
+    """An infinity or a NaN in a cached token, of the n-th kind of its format."""
+    page, row = divmod(slot, 64)
+    if fmt == "fp4":
+        cache.scale[page, row, (5 * n) % 16] = 255
+    elif fmt == "fp8" and n % 2:
+        cache.scale[page, n % 4, row] = (INF, NAN)[n // 2 % 2]
+        cache.latent[page, row, 128 * (n % 4):128 * (n % 4) + 128] = 0x38  # 1.0: a NaN times a zero would do as well
+    elif fmt == "fp8":
+        cache.latent[page, row, (97 * n) % 512] = 0x7F
+    else:
+        cache[page, row, 0, (97 * n + 5) % 512] = (INF, NAN, -INF)[n % 3]
+        if n % 4 == 1:
+            cache[page, row, 0, 512:] = NAN
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16", "fp8", "fp4"])
+@pytest.mark.parametrize("H,s,width,rows64", FORMS)
+def test_hidden_tokens_in_every_form(gpu, fmt, H, s, width, rows64):
+    """Of prefixes that end inside a page, with it, and of none; the tokens behind the last one are spoilt too."""
+    prefixes = [60, 0, 64]
+    q, cache, rows, table, plan, mask = problem(fmt, H, s, prefixes, 100 + H + s, drop=0.1)
+    B = len(prefixes)
+    slot = lambda b, t: int(pages[b][t // 64]) * 64 + t % 64  # noqa: E731
+    pages = table.tolist()
+    wide = table.repeat(1, -(-width // table.shape[1]))[:, :width] if width else table
+    sched = M.get_mla_metadata(plan.prefix_lens, H * s, 1, kv_cache=cache)
+    code = {"fp8": 1, "fp4": 4}.get(fmt, 0)
+    lone = M._lib.load().mla_tree_takes_pages(B, s, H, sched[0].shape[0], code, wide.shape[1])
+    assert bool(lone) == (not width)
+    tiles = -(-H * s // 16) * B * (1 + wide.shape[1] if lone else 1)
+    assert (4 * tiles > 5 * 256) == rows64
+    say(f"hidden {fmt} H={H} s={s} columns {wide.shape[1]}")
+    run = lambda: M.flash_mla_with_kvcache(q, cache, wide, None, 512, *sched, tree=plan)  # noqa: E731
+    clean = [t.clone() for t in run()]
+    for b, p in enumerate(prefixes):  # what is behind the trees
+        for t in range(p + s, 64 * table.shape[1]):
+            spoil(cache, fmt, slot(b, t), t)
+    got = run()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, clean)), "rows behind the trees"
+    spoilt = [(0, 3), (0, s - 1), (1, 1), (1, s // 2), (2, s - 2), (0, 33 % s), (2, 2)]
+    for n, (b, j) in enumerate(spoilt):
+        spoil(cache, fmt, slot(b, prefixes[b] + j), n)
+    got = run()
+    torch.cuda.synchronize()
+    seen = torch.tensor([[any(x == b and j in mask[b][i] for x, j in spoilt) for i in range(s)] for b in range(B)], device="cuda")
+    assert seen.any() and not seen.all()
+    assert torch.isnan(got[0][seen]).all() and (got[1].transpose(1, 2)[seen] == -INF).all()
+    assert torch.equal(got[0][~seen], clean[0][~seen]) and torch.equal(got[1].transpose(1, 2)[~seen], clean[1].transpose(1, 2)[~seen])
+
+
+@pytest.mark.parametrize("width", [0, 600])
+def test_dropped_nodes_still_see_the_prefix(gpu, width):
+    """A node that is none has no drafted token in sight, itself neither: its row is the prefix's attention, and empty only
+    where there is no prefix."""
+    q, cache, rows, table, plan, _ = problem("bf16", 16, 5, [70, 0], 5)
+    plan = M.tree_plan(ints([[-1, 0, -2, 2, 9]] * 2), ints([75, 5]), table)
+    wide = table.repeat(1, -(-width // table.shape[1]))[:, :width] if width else table
+    say(f"dropped nodes, columns {wide.shape[1]}")
+    out, lse = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan)
+    alone, alse = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan._replace(mask=torch.zeros_like(plan.mask)))
+    torch.cuda.synchronize()
+    none = plan.mask == 0
+    assert none.tolist() == [[False, False, True, True, True]] * 2 and torch.equal(none, plan.positions == -1)
+    assert torch.equal(out[none], alone[none]) and torch.equal(lse.transpose(1, 2)[none], alse.transpose(1, 2)[none])
+    assert torch.isfinite(lse[0]).all() and (out[0].abs().amax(-1) > 0).all()
+    assert (out[1, 2:] == 0).all() and (lse[1, :, 2:] == -INF).all() and torch.isfinite(lse[1, :, :2]).all()

@@ -115,3 +115,25 @@ def test_linear_8bit_scales_one_hot(gpu, T):
     bad = M.linear_fp4(rows, p)
     torch.cuda.synchronize()
     assert bad[1].isnan().all() and torch.equal(bad[0], got[0]) and torch.equal(bad[2:], got[2:])
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("k", [96, 128, 416])
+@pytest.mark.parametrize("top", [3, 10, 80, 140, 250])
+def test_linear_f16_rows_by_weights_of_any_size(gpu, T, k, top):
+    """fp16 rows take weights relative to their output's largest, whether or not the last chunk has inputs past the end: exact
+    sums of eight products a row, rounded once to bf16."""
+    n = 50 if T <= 16 else 16 * 1100
+    g = torch.Generator().manual_seed(k + top)
+    p, w = packed(torch.randint(0, 16, (n, k), generator=g), torch.randint(top - 2, top + 1, (n, k // 32), generator=g))
+    assert (p.top[:n].cpu() == p.scale.cpu().view(-1, p.scale.shape[1], 4, 16).permute(0, 3, 1, 2).reshape(-1, 4 * p.scale.shape[1])[:n, :k // 32].amax(1)).all()
+    x = torch.zeros(T, k, dtype=torch.float64)
+    x[:, k - 32:] = torch.randint(1, 5, (T, 32), generator=g).double()
+    x[:, k - 24:] = 0
+    x[:, 0] = 4
+    say(f"f16 rows T={T} k={k} top={top}")
+    got = M.linear_fp4(x.half().cuda(), p, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    want = (x @ w.T).to(torch.bfloat16)  # top 250: of up to 2^130, some past bf16's range
+    assert want.abs().max() > 0
+    assert (got.cpu() == want).all()
