@@ -512,6 +512,8 @@ int mla_release_pages(const mla_page_pool* pool, const int32_t* keep_lens, void*
  *   slots [batch, s_q]        the cache row (page * 64 + row) of token prefix + i, i < tree_lens; -1 past it, or where
  *                             the table's row has no column or no page (a negative id) for it
  * A sequence shorter than its tree has none of it: prefix 0, no nodes, slots -1.
+ * tree_lens must be what the step's mla_reserve_pages added to cache_seqlens, 0 where it granted nothing: a sequence that did
+ * not grow has its last tokens taken for the tree otherwise.
  */
 typedef struct mla_tree_plan_args {
   const int32_t* parents; /* [batch, s_q] */

@@ -6,8 +6,8 @@
   the model's own choices agree with.
 * ``kv_keep_path(kv_cache, slots, path)``: that path's rows together at the front of the tree, in place.
 
-A step that verifies trees is ``reserve_pages`` -> ``tree_plan`` -> ``kv_append_slots`` (the plan's slots and positions) ->
-``get_mla_metadata`` over the plan's ``prefix_lens`` -> ``flash_mla_with_kvcache(..., tree=plan)`` -> ``tree_accept`` ->
+A step that verifies trees is ``reserve_pages`` -> ``tree_plan`` (with ``tree_lens`` the nodes reserved times the
+reservation's ``granted``) -> ``kv_append_slots`` (the plan's slots and positions) -> ``get_mla_metadata`` over the plan's ``prefix_lens`` -> ``flash_mla_with_kvcache(..., tree=plan)`` -> ``tree_accept`` ->
 ``kv_keep_path`` (each layer's cache) -> ``release_pages`` (to ``keep_lens``).  Calls are queued on torch's current stream
 of the tensors' device, synchronise nothing, and can be captured in a HIP graph.  The reference decodes one token or a
 causal run of them and has no counterpart of these.
@@ -71,7 +71,9 @@ def tree_plan(parents: torch.Tensor, cache_seqlens: torch.Tensor, block_table: t
 
     ``parents [B, s_q]`` (int32, s_q <= 64): node i's parent, a lower node, or -1 for a root, which follows the prefix.
     Any other value drops the node: it sees nothing and nothing sees it, and neither does what hangs below it; so do
-    nodes past ``tree_lens`` (int32 ``[B]``, by default all are s_q long).  A dropped node within the tree's length still
+    nodes past ``tree_lens`` (int32 ``[B]``, by default all are s_q long).  ``tree_lens`` is what the step's
+    ``reserve_pages`` added to ``cache_seqlens``: 0 for a request that it did not grant, whose last tokens would be taken
+    for the tree otherwise, overwritten by the append and released.  A dropped node within the tree's length still
     has its row in the cache.  A sequence shorter than its tree has none of it."""
     index = _first_grid(parents, "parents", _INT32)
     device = parents.device

@@ -1,5 +1,8 @@
 """GPU tests of the tree decode in every one of its forms: what cache rows hold that a query row does not see reaches no bit of
 it, whether the rows are drafted tokens or lie behind the last one."""
+import os
+import re
+
 import pytest
 import torch
 
@@ -65,19 +68,38 @@ def test_hidden_tokens_in_every_form(gpu, fmt, H, s, width, rows64):
     assert torch.equal(got[0][~seen], clean[0][~seen]) and torch.equal(got[1].transpose(1, 2)[~seen], clean[1].transpose(1, 2)[~seen])
 
 
-@pytest.mark.parametrize("width", [0, 600])
-def test_dropped_nodes_still_see_the_prefix(gpu, width):
-    """A node that is none has no drafted token in sight, itself neither: its row is the prefix's attention, and empty only
-    where there is no prefix."""
-    q, cache, rows, table, plan, _ = problem("bf16", 16, 5, [70, 0], 5)
-    plan = M.tree_plan(ints([[-1, 0, -2, 2, 9]] * 2), ints([75, 5]), table)
-    wide = table.repeat(1, -(-width // table.shape[1]))[:, :width] if width else table
-    say(f"dropped nodes, columns {wide.shape[1]}")
-    out, lse = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan)
-    alone, alse = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan._replace(mask=torch.zeros_like(plan.mask)))
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
+def test_documented_step_when_pages_run_out(gpu, fmt):
+    """The step that the README shows, as it stands there: requests that got no pages (one longer than its tree, one empty)
+    and one with nothing to verify keep every cached row, their length and their pages; the others, trees of their own
+    sizes, go on."""
+    readme = open(os.path.join(os.path.dirname(__file__), "..", "README.md")).read()
+    code, = [c for c in re.findall(r"```python\n(.*?)```", readme, re.S) if "tree_plan" in c]
+    B, s, H, D, nb = 5, 6, 16, 64, 7
+    start, each = [62, 200, 0, 40, 64], [6, 6, 6, 3, 0]  # pages 1, 4, 0, 1, 1: all; sequences 0 and 2 want one that is not there
+    g = torch.Generator().manual_seed(3)
+    rand = lambda *shape: torch.randn(*shape, generator=g).bfloat16().cuda()  # noqa: E731
+    cache = {"fp4": M.fp4_kv_cache, "fp8": M.fp8_kv_cache}[fmt](nb) if fmt != "bf16" else torch.zeros(nb, 64, 1, 576, dtype=torch.bfloat16, device="cuda")
+    pool, table, lens = M.page_pool(nb), torch.zeros(B, 6, dtype=torch.int32, device="cuda"), ints([0] * B)
+    rope = M.rope_plan(64)
+    r = M.reserve_pages(pool, table, lens, ints(start), sum(start))
+    assert r.granted.tolist() == [1] * B and pool.count.item() == 0
+    M.kv_append_slots(rand(sum(start), 576), cache, r.slots, r.positions, rope)
+    every = torch.arange(nb * 64, dtype=torch.int32, device="cuda")
+    before = M.kv_gather(cache, every).clone()
+    names = dict(M=M, torch=torch, pool=pool, table=table, lens=lens, cache=cache, rope=rope, B=B, s=s, H=H, s_each=ints(each),
+                 parents=ints([[-1, 0, 0, 1, 2, 2]] * B), tokens=ints([[9, 1, 2, 3, 4, 5]] * B), targets=ints([[2, 0, 5, 0, 0, 7]] * B),
+                 w_o_matrix=rand(D, H * 128), w_norm=rand(D), x=rand(B * s, D), h=rand(B * s, D), kv_new=rand(B * s, 576), q_pe=rand(B * s, H, 64),
+                 q=rand(B * s, H, 576), w_uv=M.prepare_w_uv(rand(H, 512, 128)))
+    say(f"documented step {fmt}")
+    exec(code, names)
     torch.cuda.synchronize()
-    none = plan.mask == 0
-    assert none.tolist() == [[False, False, True, True, True]] * 2 and torch.equal(none, plan.positions == -1)
-    assert torch.equal(out[none], alone[none]) and torch.equal(lse.transpose(1, 2)[none], alse.transpose(1, 2)[none])
-    assert torch.isfinite(lse[0]).all() and (out[0].abs().amax(-1) > 0).all()
-    assert (out[1, 2:] == 0).all() and (lse[1, :, 2:] == -INF).all() and torch.isfinite(lse[1, :, :2]).all()
+    a = names["a"]
+    counts = [0, 3, 0, 2, 0]
+    assert a.counts.tolist() == counts and a.next_tokens.tolist() == [-1, 7, -1, 5, -1]
+    assert lens.tolist() == [p + c for p, c in zip(start, counts)] and pool.count.item() == 0
+    after = M.kv_gather(cache, every)
+    rows = table.tolist()
+    for b in range(B):
+        at = [rows[b][t // 64] * 64 + t % 64 for t in range(start[b])]
+        assert torch.equal(after[at].view(torch.int16), before[at].view(torch.int16)), f"sequence {b}"
