@@ -505,7 +505,8 @@ int mla_release_pages(const mla_page_pool* pool, const int32_t* keep_lens, void*
 /*
  * The plan of a step whose last tree_lens[b] (at most s_q; NULL: s_q) cached tokens are a tree of drafted ones, from
  * each one's parent: -1 for a root, whose parent is the prefix's last token, or a lower node of the same tree.  Any other
- * value, and a node below such a one or past tree_lens, is no node: it sees nothing and nothing sees it.
+ * value, and a node below such a one or past tree_lens, is no node: no node sees it, and it sees none, itself neither.  (Its
+ * query row still sees the prefix in the decode.)
  *   prefix_lens [batch]       cache_seqlens - tree_lens
  *   mask [batch, s_q]         bit j of node i: j is i or an ancestor of it; 0 for no node
  *   positions [batch, s_q]    prefix + the node's depth; -1 for no node

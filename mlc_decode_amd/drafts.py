@@ -70,11 +70,12 @@ def tree_plan(parents: torch.Tensor, cache_seqlens: torch.Tensor, block_table: t
     """Plan of a step in which the last ``tree_lens[b]`` tokens of ``cache_seqlens[b]`` are a tree of drafted ones.
 
     ``parents [B, s_q]`` (int32, s_q <= 64): node i's parent, a lower node, or -1 for a root, which follows the prefix.
-    Any other value drops the node: it sees nothing and nothing sees it, and neither does what hangs below it; so do
-    nodes past ``tree_lens`` (int32 ``[B]``, by default all are s_q long).  ``tree_lens`` is what the step's
+    Any other value drops the node, and with it what hangs below it: no node sees it and it sees none, itself neither;
+    so do nodes past ``tree_lens`` (int32 ``[B]``, by default all are s_q long).  ``tree_lens`` is what the step's
     ``reserve_pages`` added to ``cache_seqlens``: 0 for a request that it did not grant, whose last tokens would be taken
-    for the tree otherwise, overwritten by the append and released.  A dropped node within the tree's length still
-    has its row in the cache.  A sequence shorter than its tree has none of it."""
+    for the tree otherwise, overwritten by the append and released.  A dropped node is known by its mask, 0, and its
+    position, -1: the decode still gives it a row, the attention of the prefix alone (lse -inf only where that is empty),
+    and within the tree's length it still has its row in the cache.  A sequence shorter than its tree has none of it."""
     index = _first_grid(parents, "parents", _INT32)
     device = parents.device
     B, s_q = shape = parents.shape

@@ -68,6 +68,24 @@ def test_hidden_tokens_in_every_form(gpu, fmt, H, s, width, rows64):
     assert torch.equal(got[0][~seen], clean[0][~seen]) and torch.equal(got[1].transpose(1, 2)[~seen], clean[1].transpose(1, 2)[~seen])
 
 
+@pytest.mark.parametrize("width", [0, 600])
+def test_dropped_nodes_still_see_the_prefix(gpu, width):
+    """A node that is none has no drafted token in sight, itself neither: its row is the prefix's attention, and empty only
+    where there is no prefix."""
+    q, cache, rows, table, plan, _ = problem("bf16", 16, 5, [70, 0], 5)
+    plan = M.tree_plan(ints([[-1, 0, -2, 2, 9]] * 2), ints([75, 5]), table)
+    wide = table.repeat(1, -(-width // table.shape[1]))[:, :width] if width else table
+    say(f"dropped nodes, columns {wide.shape[1]}")
+    out, lse = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan)
+    alone, alse = M.mla_decode_with_kvcache(q, cache, wide, None, tree=plan._replace(mask=torch.zeros_like(plan.mask)))
+    torch.cuda.synchronize()
+    none = plan.mask == 0
+    assert none.tolist() == [[False, False, True, True, True]] * 2 and torch.equal(none, plan.positions == -1)
+    assert torch.equal(out[none], alone[none]) and torch.equal(lse.transpose(1, 2)[none], alse.transpose(1, 2)[none])
+    assert torch.isfinite(lse[0]).all() and (out[0].abs().amax(-1) > 0).all()
+    assert (out[1, 2:] == 0).all() and (lse[1, :, 2:] == -INF).all() and torch.isfinite(lse[1, :, :2]).all()
+
+
 @pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
 def test_documented_step_when_pages_run_out(gpu, fmt):
     """The step that the README shows, as it stands there: requests that got no pages (one longer than its tree, one empty)
