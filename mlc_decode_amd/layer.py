@@ -13,7 +13,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 import struct
 from typing import NamedTuple, Optional, Tuple, Union
 
@@ -22,7 +21,7 @@ import torch
 from . import _lib
 from ._lib import MLA_DTYPE_BF16, MLA_DTYPE_F16, MLA_DTYPE_F32, MlaLinearArgs, MlaRmsNormArgs
 from .api import _launch, _stream_ptr, _workspace, new_tensor
-from .serving import _apart_or_same, _require, _rows_meet
+from .serving import _FLT_MAX, _apart_or_same, _require, _rows_meet
 
 _DTYPES = {torch.bfloat16: MLA_DTYPE_BF16, torch.float16: MLA_DTYPE_F16, torch.float32: MLA_DTYPE_F32}
 _NORM = struct.Struct("=6Q4q4ifi")
@@ -103,8 +102,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     if weight.shape != (D,) or not weight.is_contiguous() or weight.dtype not in (dtype, torch.float32):
         raise ValueError(f"weight must be a contiguous [{D}] tensor in x's dtype or float32")
     eps = float(eps)
-    if not 0.0 <= eps < math.inf:
-        raise ValueError("eps must be finite and at least 0")
+    if not 0.0 <= eps <= _FLT_MAX:
+        raise ValueError("eps must be finite in fp32 and at least 0")
     r_ptr, r_t, h, h_ptr, h_t = 0, 0, None, 0, 0
     if residual is not None:
         r_ptr, r_t = residual.data_ptr(), _norm_rows(residual, "residual", x)

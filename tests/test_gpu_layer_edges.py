@@ -137,3 +137,12 @@ def test_linear_f16_rows_by_weights_of_any_size(gpu, T, k, top):
     want = (x @ w.T).to(torch.bfloat16)  # top 250: of up to 2^130, some past bf16's range
     assert want.abs().max() > 0
     assert (got.cpu() == want).all()
+
+
+def test_norm_refuses_an_eps_that_fp32_does_not_hold(gpu):
+    say("extreme eps")
+    x, w = torch.ones(4, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(64, dtype=torch.bfloat16, device="cuda")
+    for eps in (1e39, 3.4028235677973366e38):
+        with pytest.raises(ValueError):
+            M.rms_norm(x, w, eps)
+    assert (M.rms_norm(x, w, 3.4028234e38) == 2.0 ** -64).all()
