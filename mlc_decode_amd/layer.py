@@ -232,7 +232,7 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
     ``x`` in bf16 or fp16, or :class:`Fp8Rows` (from :func:`rms_norm`).  Sums are fp32, rounded once to ``dtype`` (bf16 or
     fp16; x's by default, bf16 of 8-bit rows).  8-bit rows are taken as bf16 values, exactly inside bf16's range; bf16 and
     8-bit rows take the weights exactly; with fp16 rows weights below ``2**-35`` of the largest of their output are lost.  The leading dims must be one stride apart; rows that do not
-    start on 16 bytes are copied first.  ``out`` (unit stride in its rows) may not overlap ``x``.  Memory gives the weights
+    start on 16 bytes are copied first.  ``out`` (unit stride in its rows) may not overlap ``x`` or ``w``.  Memory gives the weights
     once for up to 64 rows, so a few rows cost little more than one; it takes up to 2**20."""
     coded = isinstance(x, Fp8Rows)
     rows = x.codes if coded else x
@@ -307,6 +307,8 @@ def linear_fp4(x: Union[torch.Tensor, Fp8Rows], w: Fp4Weight, out: Optional[torc
             raise ValueError("out overlaps x")
         if tokens and coded and y_ptr < s_ptr + (tokens - 1) * s_t + k // GROUP and s_ptr < y_end:
             raise ValueError("out overlaps x.scale")
+        if tokens and any(y_ptr < t.data_ptr() + t.numel() and t.data_ptr() < y_end for t in (codes, scale, top)):
+            raise ValueError("out overlaps w")
     need = _linear_workspace(tokens, n, k)
     ws_ptr = ws = 0
     if need:

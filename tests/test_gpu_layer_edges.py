@@ -146,3 +146,20 @@ def test_norm_refuses_an_eps_that_fp32_does_not_hold(gpu):
         with pytest.raises(ValueError):
             M.rms_norm(x, w, eps)
     assert (M.rms_norm(x, w, 3.4028234e38) == 2.0 ** -64).all()
+
+
+def test_linear_refuses_outputs_in_the_weights(gpu):
+    """Projections that would write over the weights that they read: codes, scales, largest scales."""
+    say("outputs in the weights")
+    x = torch.ones(4, 64, dtype=torch.bfloat16, device="cuda")
+    buf = torch.zeros(2048, dtype=torch.uint8, device="cuda")
+    p = M.quantize_w_fp4(torch.zeros(16, 64, device="cuda"))
+    for name, at in (("codes", 0), ("scale", 1024), ("top", 1024 + 64)):
+        buf[at:at + getattr(p, name).numel()].copy_(getattr(p, name).flatten())
+    p = p._replace(codes=buf[:1024].view(p.codes.shape), scale=buf[1024:1088].view(p.scale.shape), top=buf[1088:1104])
+    half = buf.view(torch.bfloat16)
+    for at in (0, 449, 511, 540, 551):
+        with pytest.raises(ValueError):
+            M.linear_fp4(x, p, out=half[at:at + 64].view(4, 16))
+    assert M.linear_fp4(x, p, out=half[552:616].view(4, 16)).data_ptr() == half[552:].data_ptr()
+    torch.cuda.synchronize()
