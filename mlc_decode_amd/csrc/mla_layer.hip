@@ -32,7 +32,8 @@ using mla_srv::unpack;
 // A piece is 16 bytes of x (8 values, 4 of fp32), or one value where rows, strides or dims do not fall on such pieces;
 // thread t of a row holds pieces t, t + threads, ...  P of them.
 // Bound by memory for many rows, by latency for few (row, sum, barrier): 1 x 7168 with the residual 2.9 us, 256 rows 4.1,
-// 1024 rows 11.0 (5.3 TB/s), 8192 rows 96 (4.9; to 16 bits without a residual 42.7, 5.5), 65536 x 512 39 us, 6.9 TB/s; 65536 x 128 12.8, 5.2.
+// 1024 rows 11.0 (5.3 TB/s), 8192 rows 96 (4.9; to 16 bits without a residual 42.7, 5.5), 65536 x 512 39 us, 65536 x 128 12.8 (in
+// the last-level cache: 6.9 and 5.2).
 struct NormParams {
   const uint8_t* x;
   const uint8_t* residual;  // may be NULL
@@ -319,7 +320,8 @@ constexpr int kTileX = 16 * 256;  // 16 rows of a chunk in LDS, 16-bit values
 
 // A piece of 16 bytes of a row's chunk in LDS (p of 16): its place in the 16 rows' chunk.  Blocks of 256 bytes hold what one
 // lane group of an operand reads, MFMA p % 4, lane group p / 4 (inputs 32 g + 8 j), the rows' order in them turned by the
-// piece, so that both the writes (pieces of a few rows) and the reads (16 rows) go over all banks.
+// piece, so that a write's pieces of a few rows and a lane group's read of 16 rows each go over all banks.  (Lane groups meet
+// in some: conflicts are 25 to 39% of LDS's busy cycles with 16-bit rows, 47% with 8-bit ones.)
 __device__ __forceinline__ int piece_place(int p, int row) { return (p & 3) * 1024 + (p >> 2) * 256 + ((row ^ p) << 4); }
 // The operand of MFMA j for lane (g, i).
 __device__ __forceinline__ i32x4 read_piece(const uint8_t* tile, int j, int g, int i) {
@@ -465,9 +467,12 @@ __device__ __forceinline__ f32x4 scale_back(const LinearParams& p, int n, f32x4 
 }
 
 // 16 rows (the first LOADS * kEach of them).  A wave takes 16 outputs and every WK-th chunk, its rows through LDS of its own (no
-// barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.  Bound by
-// the weights: 8 x 24576 x 1536 (8-bit rows) 6.0 us, 3.3 TB/s; 1 x 7168 x 16384 12.3 us, 5.1 TB/s; one of 576 x 7168 4.0, a
-// load's latency over and over.
+// barrier in the loop), weights and rows kDepth chunks ahead; the waves of a tile add up through LDS, in order.
+// us where the weights are in the last-level cache (the same ones again and again), and where they come from memory (others
+// in turns, as a model's layers are): 1 x 7168 x 16384 12.1, 14.5 (4.3 TB/s: bound by the weights)    16 x 7168 x 16384 17.6,
+// 25.1 (2.5)    8 x 24576 x 1536 (8-bit rows) 5.7, 8.0 (2.5)    1 x 576 x 7168 3.8, 5.3, a load's latency over and over.
+// Where rows are several, the waves wait for LDS and loads in turn: of the CU's cycles LDS is busy 38 to 47%, the matrix
+// units 9 to 18%.
 template <int XT, int LOADS, int WK>
 __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p) {
   constexpr int kDepth = LOADS == 4 && WK >= 8 ? 2 : 4;  // 128 registers: two workgroups of 8 waves a CU
@@ -516,10 +521,11 @@ __global__ __launch_bounds__(64 * WK) void mla_linear_few_kernel(LinearParams p)
 
 // More rows: a workgroup takes 128 outputs for 16 RT rows and a split of the chunks.  Its two halves take the steps of two
 // chunks in turns, each with its own rows in LDS, a wave 32 outputs, the next step's on the way meanwhile; the halves
-// add up through LDS.  64 x 7168 x 16384 (bf16, 62 MB of weights) 23 us and 3 to 4 of sums.  Products and the reads of
-// their rows from LDS, which want the whole of both units, are 11 of them, loads 3, the rows' way into LDS 2, the splits'
-// partial sums 2 to 3.  Two workgroups of one half each and twice the splits: 27.9 us in all against 27.2, 16384 x 2048 15.0
-// against 12.7; one workgroup of 256 outputs 27.8, that with twice as much on the way 30.8.
+// add up through LDS.  64 x 7168 x 16384 (bf16, 62 MB of weights) 25 us with the splits' sums, 27 where the weights come from
+// memory; in a trace, which runs one kernel after the other, 24 and 4 of sums.  Of the CU's cycles the matrix units are busy
+// 37% and LDS 47% (two fifths of that bank conflicts); the waves wait 35% of theirs and queue to issue 38%: no unit is
+// full, and two waves a SIMD do not cover each other.  Two workgroups of one half each and twice the splits: 27.9 us in all
+// against 27.2, 16384 x 2048 15.0 against 12.7; one workgroup of 256 outputs 27.8, that with twice as much on the way 30.8.
 template <int XT, int RT>
 __global__ __launch_bounds__(512, 1) void mla_linear_rows_kernel(LinearParams p) {
   constexpr int kStep = 2, NT = 2;

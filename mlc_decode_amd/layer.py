@@ -76,7 +76,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     ``residual`` ``(y, h)``.
 
     ``x [..., D]`` in bf16, fp16 or fp32, ``residual`` like it, ``weight [D]`` in x's dtype or fp32.  ``h`` is added, squared
-    and summed in fp32; y is of h as added, and both are rounded once, to x's dtype.  With ``quantize`` y is
+    and summed in fp32 (a row whose squares add up past its range gives zeros); y is of h as added, and both are rounded once, to x's dtype.  With ``quantize`` y is
     :class:`Fp8Rows`, rounded from fp32 (D a multiple of 32), what ``linear_fp4`` reads.  ``out`` and ``residual_out``
     default to new tensors; each may be ``x`` or ``residual`` itself (in place), and may not overlap them otherwise, nor
     each other, nor ``weight``.  Rows may be strided (the latent part of ``kv [T, 576]`` before it is appended); the token dims of each
