@@ -163,3 +163,39 @@ def test_linear_refuses_outputs_in_the_weights(gpu):
             M.linear_fp4(x, p, out=half[at:at + 64].view(4, 16))
     assert M.linear_fp4(x, p, out=half[552:616].view(4, 16)).data_ptr() == half[552:].data_ptr()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("kind", ["f16", "fp8"])
+@pytest.mark.parametrize("T,n,k", [(5, 576, 7168), (64, 2200, 16384)])
+def test_linear_of_every_kind_in_a_graph(gpu, T, n, k, kind):
+    """Captured once and replayed beside eager calls of the same stream, with rows that change in place, and on two streams at
+    once."""
+    rows, p, y = exactly(T, n, k, kind, 7)
+    other, _, _ = exactly(T, n, k, kind, 7)
+    parts = lambda r: list(r) if isinstance(r, M.Fp8Rows) else [r]  # noqa: E731
+    for t in parts(other):
+        t.copy_(t.flip(0))
+    want, flipped = y.to(torch.bfloat16), M.linear_fp4(other, p, dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    say(f"graph {kind} T={T}")
+    side, third = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        assert torch.equal(M.linear_fp4(rows, p, dtype=torch.bfloat16).cpu(), want)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            got = M.linear_fp4(rows, p, dtype=torch.bfloat16)
+        first = [t.clone() for t in parts(rows)]
+        for i in range(4):
+            for t, a, b in zip(parts(rows), first, parts(other)):
+                t.copy_(b if i % 2 else a)
+            got.zero_()
+            gr.replay()
+            eager = M.linear_fp4(other, p, dtype=torch.bfloat16)
+            side.synchronize()
+            assert torch.equal(got.cpu(), flipped.cpu() if i % 2 else want) and torch.equal(eager, flipped)
+    results = []
+    for i in range(6):
+        with torch.cuda.stream(side if i % 2 else third):
+            results.append(M.linear_fp4(other, p, dtype=torch.bfloat16))
+    torch.cuda.synchronize()
+    assert all(torch.equal(r, flipped) for r in results)
