@@ -500,7 +500,7 @@ def flash_mla_with_kvcache(q: torch.Tensor, k_cache, block_table: torch.Tensor,
     sees the sequence's prefix and, of the drafted ones, its ancestors and itself, as the plan's masks say.
     ``cache_seqlens`` is not read (the plan has the lengths) and ``causal`` has no part in it; the schedule must come
     from ``get_mla_metadata(tree.prefix_lens, ...)``.  Every cache format; no ``indices``.  The drafted tokens are one more
-    split of their sequence, so outputs are as exact as those of a decode in several splits.
+    split of their sequence: outputs are at least as exact as those of a decode in several splits.
     """
     if head_dim_v != MLA_DIM_V:
         raise ValueError(f"head_dim_v must be {MLA_DIM_V}")

@@ -46,13 +46,14 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   else
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
 }
+// What pack2 left of a and b.
 template <bool F16>
-__device__ __forceinline__ float sum2(uint32_t w) {
+__device__ __forceinline__ uint32_t pack2_rest(float a, float b, uint32_t w) {
   if constexpr (F16) {
     const f16x2 h = __builtin_bit_cast(f16x2, w);
-    return (float)h[0] + (float)h[1];
+    return pack2<true>(a - (float)h[0], b - (float)h[1]);
   } else {
-    return __uint_as_float(w << 16) + __uint_as_float(w & 0xFFFF0000u);
+    return pack2<false>(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xFFFF0000u));
   }
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
@@ -90,11 +91,12 @@ __device__ __forceinline__ bool non_finite(i32x4 v) {
 // and leaves a partial: S^T = K Q^T (16x16x32 MFMA), softmax over the visible keys, O^T = V^T P^T with V^T from
 // transposed LDS reads.  All keys are in the tile, so the softmax is one pass.
 //
-// Fewer bits, as in the split-KV pass whose partials these are merged with.  P is rounded to 16 bits, the type that the
-// matrix unit takes beside V, and the sum that divides the output is of the rounded weights, so that what they have in common
-// cancels.  A partial output is fp16 with a power of two per 128 dims, half of fp32's bytes to write and merge.  Error of a
-// chain of 5 behind 300 tokens, of the outputs' norm: bf16 2.0e-3, fp16 3.2e-4; the causal decode 2.1e-3, 3.3e-4; the exact
-// result rounded once 1.7e-3, 2.1e-4.  Scores, maxima, sums and lse are fp32.
+// P goes as two 16-bit halves, its rounding and the rest, in two products beside the same V: 16 bits and more of each weight
+// (one half alone: 0.1 to 0.4 us less of 17 to 27, and outputs 20% further off).  A partial output is fp16 with a power of two
+// per 128 dims, half of fp32's bytes to write and merge, as the split-KV pass writes the partials that these are merged
+// with; that pass rounds P to one half.  Scores, maxima, sums and lse are fp32.  Error of a chain of 5 behind 300 tokens against
+// 64 bits, of the outputs' norm: pages by themselves bf16 1.7e-3, fp16 2.8e-4; behind the pass 2.1e-3, 3.3e-4, as the causal decode;
+// the exact result rounded once 1.7e-3, 2.1e-4.
 //
 // Tokens and queries are read row by row, a wave's lanes side by side, and become operands through LDS.  Loaded in operand
 // order, 16 rows a quarter wave, each load took the address unit 64 cycles instead of 16: 36 of them 4.2 us.
@@ -295,10 +297,10 @@ __device__ __forceinline__ float largest(f32x4 v, float a) {
   return fmaxf(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))), a);
 }
 // A row's divisor and lse.  A NaN in the lse makes the merged one -inf, as any NaN row's is.
-__device__ __forceinline__ void finish_row(bool spoilt, float l, float lx, float ref, float& inv, float& lse2) {
+__device__ __forceinline__ void finish_row(bool spoilt, float l, float ref, float& inv, float& lse2) {
   const float nan = __builtin_nanf("");
   inv = spoilt ? nan : l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-  lse2 = spoilt ? nan : lx > 0.f ? ref + __log2f(lx) : lx == 0.f ? -INFINITY : lx;
+  lse2 = spoilt ? nan : l > 0.f ? ref + __log2f(l) : l == 0.f ? -INFINITY : l;
 }
 
 // The rows of one 128-dim chunk on their way out: 16 rows of 256 bytes in LDS, 16-byte pieces swizzled by the row, so
@@ -379,30 +381,35 @@ __global__ __launch_bounds__(256, 2) void mla_tree_rows_kernel(TreeParams p) {
     }
   mx = group_max(mx);
   const float ref = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, lx = 0.f;
-  i32x4 pb[KT];  // P^T as it is: the B operand in the key order of the transposed reads
+  float l = 0.f;
+  i32x4 pb[KT], pr[KT];  // P^T as it is: the B operand in the key order of the transposed reads, and its rest
 #pragma unroll
   for (int u = 0; u < 2 * KT; ++u) {
     float e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       e[i] = __builtin_amdgcn_exp2f(sc[u][i] - ref);
-      lx += e[i];
+      l += e[i];
     }
     const uint32_t w0 = pack2<F16>(e[0], e[1]), w1 = pack2<F16>(e[2], e[3]);
-    l += sum2<F16>(w0) + sum2<F16>(w1);
     pb[u >> 1][2 * (u & 1)] = (int)w0;
     pb[u >> 1][2 * (u & 1) + 1] = (int)w1;
+    pr[u >> 1][2 * (u & 1)] = (int)pack2_rest<F16>(e[0], e[1], w0);
+    pr[u >> 1][2 * (u & 1) + 1] = (int)pack2_rest<F16>(e[2], e[3], w1);
   }
   f32x4 o[kDV / 16];
 #pragma unroll
   for (int d = 0; d < kDV / 16; ++d) {
     o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < KT; ++u) o[d] = mfma32<F16>(read_vt(kv_sh + 2 * u * kTileBytes, d, g, li), pb[u], o[d]);
+    for (int u = 0; u < KT; ++u) {
+      const i32x4 vt = read_vt(kv_sh + 2 * u * kTileBytes, d, g, li);
+      o[d] = mfma32<F16>(vt, pb[u], o[d]);
+      o[d] = mfma32<F16>(vt, pr[u], o[d]);
+    }
   }
   float inv, lse2;
-  finish_row((mask & spoilt) != 0, group_sum(l), group_sum(lx), mx, inv, lse2);
+  finish_row((mask & spoilt) != 0, group_sum(l), mx, inv, lse2);
   __syncthreads();  // V is read: its place takes the rows on their way out
   uint8_t* stage = kv_sh + wave * kTileBytes;  // 4 KiB a chunk
 #pragma unroll
@@ -426,8 +433,8 @@ __global__ __launch_bounds__(256, 2) void mla_tree_rows_kernel(TreeParams p) {
 template <int FMT, bool F16>
 __global__ __launch_bounds__(256, 2) void mla_tree_keys_kernel(TreeParams p) {
   __shared__ __attribute__((aligned(16))) uint8_t kv_sh[4 * kTileBytes];
-  __shared__ __attribute__((aligned(16))) uint8_t p_sh[2][1024];
-  __shared__ float max_sh[4][16], sum_sh[4][2][16];
+  __shared__ __attribute__((aligned(16))) uint8_t p_sh[2][2][1024];  // P^T, and its rest
+  __shared__ float max_sh[4][16], sum_sh[4][16];
   __shared__ uint32_t spoilt_sh[4];
   const int b = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -476,33 +483,38 @@ __global__ __launch_bounds__(256, 2) void mla_tree_keys_kernel(TreeParams p) {
   __syncthreads();
   mx = fmaxf(fmaxf(max_sh[0][li], max_sh[1][li]), fmaxf(max_sh[2][li], max_sh[3][li]));
   const float ref = mx == -INFINITY ? 0.f : mx;
-  float e[4], lx = 0.f;
+  float e[4], l = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     e[i] = __builtin_amdgcn_exp2f(sc[i] - ref);
-    lx += e[i];
+    l += e[i];
   }
   // P^T as it is: half of the B operand of 32 keys in the order of the transposed reads
   const uint32_t w0 = pack2<F16>(e[0], e[1]), w1 = pack2<F16>(e[2], e[3]);
-  *(i32x2*)&p_sh[wave >> 1][16 * lane + 8 * (wave & 1)] = i32x2{(int)w0, (int)w1};
-  sum_sh[wave][0][li] = group_sum(sum2<F16>(w0) + sum2<F16>(w1));
-  sum_sh[wave][1][li] = group_sum(lx);
+  *(i32x2*)&p_sh[0][wave >> 1][16 * lane + 8 * (wave & 1)] = i32x2{(int)w0, (int)w1};
+  *(i32x2*)&p_sh[1][wave >> 1][16 * lane + 8 * (wave & 1)] =
+      i32x2{(int)pack2_rest<F16>(e[0], e[1], w0), (int)pack2_rest<F16>(e[2], e[3], w1)};
+  sum_sh[wave][li] = group_sum(l);
   __syncthreads();
-  const i32x4 pb[2] = {*(const i32x4*)&p_sh[0][16 * lane], *(const i32x4*)&p_sh[1][16 * lane]};
+  const i32x4 pb[2] = {*(const i32x4*)&p_sh[0][0][16 * lane], *(const i32x4*)&p_sh[0][1][16 * lane]};
+  const i32x4 pr[2] = {*(const i32x4*)&p_sh[1][0][16 * lane], *(const i32x4*)&p_sh[1][1][16 * lane]};
   f32x4 o[8];
 #pragma unroll
   for (int d = 0; d < 8; ++d) {
     o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < 2; ++u) o[d] = mfma32<F16>(read_vt(kv_sh + 2 * u * kTileBytes, 8 * wave + d, g, li), pb[u], o[d]);
+    for (int u = 0; u < 2; ++u) {
+      const i32x4 vt = read_vt(kv_sh + 2 * u * kTileBytes, 8 * wave + d, g, li);
+      o[d] = mfma32<F16>(vt, pb[u], o[d]);
+      o[d] = mfma32<F16>(vt, pr[u], o[d]);
+    }
   }
   uint64_t spoilt = 0;
   if (t.drafts)
 #pragma unroll
     for (int w = 0; w < 4; ++w) spoilt |= (uint64_t)spoilt_sh[w] << (16 * w);
   float inv, lse2;
-  finish_row((mask & spoilt) != 0, sum_sh[0][0][li] + sum_sh[1][0][li] + sum_sh[2][0][li] + sum_sh[3][0][li],
-             sum_sh[0][1][li] + sum_sh[1][1][li] + sum_sh[2][1][li] + sum_sh[3][1][li], mx, inv, lse2);
+  finish_row((mask & spoilt) != 0, sum_sh[0][li] + sum_sh[1][li] + sum_sh[2][li] + sum_sh[3][li], mx, inv, lse2);
   float a = 0.f;
 #pragma unroll
   for (int d = 0; d < 8; ++d) a = largest(o[d], a);

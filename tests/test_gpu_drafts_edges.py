@@ -1,5 +1,6 @@
 """GPU tests of the tree decode in every one of its forms: what cache rows hold that a query row does not see reaches no bit of
-it, whether the rows are drafted tokens or lie behind the last one."""
+it, whether the rows are drafted tokens or lie behind the last one; weights keep more bits than the cache's type has; and the
+documented step."""
 import os
 import re
 
@@ -7,7 +8,8 @@ import pytest
 import torch
 
 import mlc_decode_amd as M
-from test_gpu_drafts import INF, NAN, ints, problem, say
+from oracle import mla_tree_ref as T
+from test_gpu_drafts import INF, NAN, SCALE, ints, problem, say
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +123,30 @@ def test_documented_step_when_pages_run_out(gpu, fmt):
     for b in range(B):
         at = [rows[b][t // 64] * 64 + t % 64 for t in range(start[b])]
         assert torch.equal(after[at].view(torch.int16), before[at].view(torch.int16)), f"sequence {b}"
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "fp8", "fp4"])
+@pytest.mark.parametrize("H,s,width,rows64", FORMS)
+def test_weights_keep_their_bits(gpu, fmt, H, s, width, rows64):
+    """Softmax weights are held past 16 bits.  Queries have one dim that is not zero, a power of two, so that scores have one
+    product each: off by their scaling, the fast exponential and its argument, 2^-20 (1 + |score|) together, as is the sum of
+    the weights.  Two 16-bit halves hold a weight to 2^-16.  Then the partials' rounding, 2^-11 of each, and the output's,
+    2^-8.  (Of the schedule's form the drafted tokens alone are looked at, without a prefix.)"""
+    prefixes = [0, 0, 0] if width else [10, 60, 70]
+    q, cache, rows, table, plan, mask = problem(fmt, H, s, prefixes, 300 + H + s, drop=0.1)
+    q = torch.zeros_like(q)
+    q[..., 512] = 64.0
+    wide = table.repeat(1, -(-width // table.shape[1]))[:, :width] if width else table
+    sched = M.get_mla_metadata(plan.prefix_lens, H * s, 1, kv_cache=cache)
+    code = {"fp8": 1, "fp4": 4}.get(fmt, 0)
+    lone = M._lib.load().mla_tree_takes_pages(3, s, H, sched[0].shape[0], code, wide.shape[1])
+    assert bool(lone) == (not width)
+    say(f"weights {fmt} H={H} s={s} columns {wide.shape[1]}")
+    out, _ = M.flash_mla_with_kvcache(q, cache, wide, None, 512, *sched, tree=plan)
+    torch.cuda.synchronize()
+    ro, rl, size, reach = T.attend(q.double().cpu(), rows, table.cpu(), plan.prefix_lens.tolist(), mask, SCALE)
+    d = 2.0 ** -20 * (1 + reach + rl.abs().nan_to_num(0, 0, 0)).transpose(1, 2)[..., None]
+    tol = (2.0 ** -16 + torch.expm1(2 * d) + 2.0 ** -11) * size * (1 + 2.0 ** -8) + 2.0 ** -8 * ro.abs() + 2.0 ** -24
+    off = ((out.double().cpu() - ro).abs() / tol).max().item()
+    say(f"  {off:.3f} of the bound")
+    assert off <= 1
